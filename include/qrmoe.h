@@ -260,6 +260,101 @@ int  qrm_ffn_forward(qrm_ffn* ffn, const float* xn_dev, const float* x_dev, int 
  * Nothing needs to start at zero: every table byte read is written first. */
 int  qrm_matrix_gemv_static(qrm_matrix* m, const float* x_dev, int T, float* y_dev, void* stream);
 
+/* ---- experts in 8-bit floating point: tokens sorted by expert and back,
+ * block-scaled products, SwiGLU, with their gradients (no counterpart in the
+ * reference, whose formats are the QuantFormat ids above) ----
+ * 8-bit rows: e4m3 codes with one f32 scale for each 128 columns,
+ * scale = max(max|v| / 448, 2^-126), code = e4m3(v / scale) to nearest even;
+ * a matrix has one scale for each 128 x 128 block.  The last block of a row or
+ * matrix may be short.  A block that holds a NaN or an infinity stands for NaN
+ * throughout; other blocks are untouched.
+ * type: QRM_F32, QRM_F16 or QRM_BF16, of every activation array of the call;
+ * sums, scales and weights w are f32.  ld_*: elements from row to row, 0 for
+ * dense rows.  Everything is asynchronous on `stream` (NULL: the default
+ * stream) and may be captured in a graph.  The calls without a handle run on
+ * the calling thread's current device and keep nothing.  Arrays must be
+ * aligned to their own values; 16-byte rows (8-byte for codes) are faster.
+ *
+ * qrm_sort_tokens: the n = T k assignments a = t k + j, in order of their
+ * expert topk_idx[a] - first, stable.  perm [n] lists them, pos [n] is its
+ * inverse, offsets [n_experts + 1] delimits each expert's run.  An assignment
+ * whose index is outside [first, first + n_experts) (another rank's, or -1)
+ * gets pos -1, and perm ends with as many -1.  At most 1024 experts
+ * (QRM_E_CAPACITY).
+ * qrm_gather_rows: rows[pos[a]] = x[t]; rows that no assignment has stay as
+ * they are, and positions outside [0, n_rows) are passed over (here and
+ * below).  qrm_gather_rows_fp8 writes them in 8 bits.
+ * qrm_combine_rows: out[t] = add[t] + sum_j w[a] rows[pos[a]], in slot order
+ * (w NULL: weights 1, which is the gradient of qrm_gather_rows; add NULL: 0).
+ * out may be add.
+ * qrm_combine_rows_grad: its gradient, drows[pos[a]] = w[a] dout[t] and
+ * dw[a] = <dout[t], rows[pos[a]]> (0 without a row; dw NULL: not wanted, and
+ * rows not read); _fp8 writes drows in 8 bits. */
+int qrm_sort_tokens(const int32_t* topk_idx_dev, int64_t T, int k, int first, int n_experts, int32_t* perm_dev,
+                    int32_t* pos_dev, int32_t* offsets_dev, void* stream);
+int qrm_gather_rows(int type, const void* x_dev, int64_t ld_x, const int32_t* pos_dev, int64_t T, int k, int64_t d,
+                    void* rows_dev, int64_t n_rows, int64_t ld_rows, void* stream);
+int qrm_gather_rows_fp8(int type, const void* x_dev, int64_t ld_x, const int32_t* pos_dev, int64_t T, int k, int64_t d,
+                        uint8_t* codes_dev, int64_t n_rows, int64_t ld_codes, float* scales_dev, int64_t ld_scales,
+                        void* stream);
+int qrm_combine_rows(int type, const void* rows_dev, int64_t n_rows, int64_t ld_rows, const int32_t* pos_dev,
+                     const float* w_dev, int64_t T, int k, int64_t d, const void* add_dev, int64_t ld_add, void* out_dev,
+                     int64_t ld_out, void* stream);
+int qrm_combine_rows_grad(int type, const void* dout_dev, int64_t ld_dout, const void* rows_dev, int64_t n_rows,
+                          int64_t ld_rows, const int32_t* pos_dev, const float* w_dev, int64_t T, int k, int64_t d,
+                          void* drows_dev, int64_t ld_drows, float* dw_dev, void* stream);
+int qrm_combine_rows_grad_fp8(int type, const void* dout_dev, int64_t ld_dout, const void* rows_dev, int64_t n_rows,
+                              int64_t ld_rows, const int32_t* pos_dev, const float* w_dev, int64_t T, int k, int64_t d,
+                              uint8_t* codes_dev, int64_t ld_codes, float* scales_dev, int64_t ld_scales, float* dw_dev,
+                              void* stream);
+/* Rows into 8 bits.  n_rows_dev (here and below; NULL: rows): only the first
+ * min(rows, *n_rows_dev) rows are done, e.g. offsets + n_experts of
+ * qrm_sort_tokens. */
+int qrm_quantize_fp8(int type, const void* x_dev, int64_t ld_x, int64_t rows, int64_t cols, const int32_t* n_rows_dev,
+                     uint8_t* codes_dev, int64_t ld_codes, float* scales_dev, int64_t ld_scales, void* stream);
+/* w [groups][rows][cols] into codes of the same layout and scales
+ * [groups][ceil(rows/128)][ceil(cols/128)], as qrm_fp8_create_device takes
+ * them. */
+int qrm_quantize_fp8_weights(int type, const void* w_dev, int groups, int64_t rows, int64_t cols, uint8_t* codes_dev,
+                             float* scales_dev, void* stream);
+/* gu [rows][2f]: the gate's f columns, then up's.  qrm_swiglu_fp8 writes
+ * h = silu(gate) up [rows][f]; qrm_swiglu_fp8_grad, given dh [rows][f], the
+ * gradients of gate and up [rows][2f] (f a multiple of 128, else
+ * QRM_E_INVALID: a block would hold both).  limit > 0: gate is cut off above
+ * it and up to [-limit, limit] first, as Glm5Ops.LimitedSwiglu does. */
+int qrm_swiglu_fp8(int type, const void* gu_dev, int64_t ld_gu, int64_t rows, int64_t f, const int32_t* n_rows_dev,
+                   float limit, uint8_t* codes_dev, int64_t ld_codes, float* scales_dev, int64_t ld_scales, void* stream);
+int qrm_swiglu_fp8_grad(int type, const void* gu_dev, int64_t ld_gu, const void* dh_dev, int64_t ld_dh, int64_t rows,
+                        int64_t f, const int32_t* n_rows_dev, float limit, uint8_t* codes_dev, int64_t ld_codes,
+                        float* scales_dev, int64_t ld_scales, void* stream);
+
+/* groups matrices [rows x cols] in 8 bits, kept in HBM: codes
+ * [groups][rows][cols] (code_bytes = their number) and scales
+ * [groups][ceil(rows/128)][ceil(cols/128)] are copied, from the host or
+ * (_device, after a device synchronise) from the device.  At most 1024 groups
+ * (QRM_E_CAPACITY).
+ * qrm_fp8_product: y[t] = W_g x[t] for the rows t in [offsets[g],
+ * offsets[g+1]) of each group g (offsets NULL: one group, all T rows), x
+ * [T][cols] and y [T][rows]; rows outside every group are not written.
+ * qrm_fp8_product_t: x[t] = W_g^T y[t], the gradient of the product's input,
+ * from the same stored matrix.  Rows of codes start on 16 bytes (pitch
+ * included).  type is the result's.  Products on one handle must not overlap:
+ * they share its workspace (128 KiB for each SM).  qrm_fp8_sync waits for the
+ * device and reports what the products met: QRM_E_INVALID for offsets that do
+ * not ascend within [0, T] (such a group counts as empty), QRM_E_TIMEOUT for a
+ * wait that gave up (QRM_WAIT_LIMIT_US in the environment at creation). */
+typedef struct qrm_fp8 qrm_fp8;
+int  qrm_fp8_create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes,
+                    const float* scales, size_t scale_bytes, qrm_fp8** out);
+int  qrm_fp8_create_device(int device, int groups, int64_t rows, int64_t cols, const void* codes_dev, size_t code_bytes,
+                           const float* scales_dev, size_t scale_bytes, qrm_fp8** out);
+void qrm_fp8_destroy(qrm_fp8* m);
+int  qrm_fp8_product(qrm_fp8* m, const void* x_codes_dev, int64_t ld_x, const float* x_scales_dev, int64_t ld_xs,
+                     const int32_t* offsets_dev, int64_t T, int type, void* y_dev, int64_t ld_y, void* stream);
+int  qrm_fp8_product_t(qrm_fp8* m, const void* y_codes_dev, int64_t ld_y, const float* y_scales_dev, int64_t ld_ys,
+                       const int32_t* offsets_dev, int64_t T, int type, void* x_dev, int64_t ld_x, void* stream);
+int  qrm_fp8_sync(qrm_fp8* m);
+
 /* ---- expert parallelism (no counterpart in the reference, whose MoE layer
  * runs in one process) ----
  * world ranks, one process and GPU each; rank r holds the routed experts

@@ -127,6 +127,29 @@ _SIGS = {
     "qrm_ffn_create": (C.c_int, [P, P, P, C.c_int, C.POINTER(P)]),
     "qrm_ffn_destroy": (None, [P]),
     "qrm_ffn_forward": (C.c_int, [P, P, P, C.c_int, C.c_float, P, P]),
+    "qrm_sort_tokens": (C.c_int, [P, C.c_int64, C.c_int, C.c_int, C.c_int, P, P, P, P]),
+    "qrm_gather_rows": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int, C.c_int64, P, C.c_int64, C.c_int64, P]),
+    "qrm_gather_rows_fp8": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int, C.c_int64, P, C.c_int64, C.c_int64,
+                                      P, C.c_int64, P]),
+    "qrm_combine_rows": (C.c_int, [C.c_int, P, C.c_int64, C.c_int64, P, P, C.c_int64, C.c_int, C.c_int64, P, C.c_int64,
+                                   P, C.c_int64, P]),
+    "qrm_combine_rows_grad": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int64, P, P, C.c_int64, C.c_int,
+                                        C.c_int64, P, C.c_int64, P, P]),
+    "qrm_combine_rows_grad_fp8": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int64, P, P, C.c_int64, C.c_int,
+                                            C.c_int64, P, C.c_int64, P, C.c_int64, P, P]),
+    "qrm_quantize_fp8": (C.c_int, [C.c_int, P, C.c_int64, C.c_int64, C.c_int64, P, P, C.c_int64, P, C.c_int64, P]),
+    "qrm_quantize_fp8_weights": (C.c_int, [C.c_int, P, C.c_int, C.c_int64, C.c_int64, P, P, P]),
+    "qrm_swiglu_fp8": (C.c_int, [C.c_int, P, C.c_int64, C.c_int64, C.c_int64, P, C.c_float, P, C.c_int64, P, C.c_int64,
+                                 P]),
+    "qrm_swiglu_fp8_grad": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int64, C.c_int64, P, C.c_float, P,
+                                      C.c_int64, P, C.c_int64, P]),
+    "qrm_fp8_create": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, P, C.c_size_t, P, C.c_size_t, C.POINTER(P)]),
+    "qrm_fp8_create_device": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, P, C.c_size_t, P, C.c_size_t,
+                                        C.POINTER(P)]),
+    "qrm_fp8_destroy": (None, [P]),
+    "qrm_fp8_product": (C.c_int, [P, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int, P, C.c_int64, P]),
+    "qrm_fp8_product_t": (C.c_int, [P, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int, P, C.c_int64, P]),
+    "qrm_fp8_sync": (C.c_int, [P]),
     "qrm_nccl_unique_id": (C.c_int, [P]),
     "qrm_create_ep": (C.c_int, [C.POINTER(LayerDesc), C.c_int, C.c_int, P, C.POINTER(P)]),
     "qrm_expert_range": (C.c_int, [P, P, P]),
@@ -462,6 +485,127 @@ class DenseFfn:
     def close(self):
         if getattr(self, "_h", None):
             lib().qrm_ffn_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# ---- experts in 8-bit floating point (include/qrmoe.h: 8-bit rows, order of
+# the tokens, types, pitches).  Arrays are device pointers or objects with
+# data_ptr(); `type` is QuantFormat.F32, F16 or BF16; ld_* are pitches in
+# elements, 0 for dense rows.
+
+
+def sort_tokens(topk_idx, T, k, n_experts, perm, pos, offsets, first=0, stream=None):
+    """The T k assignments in order of their expert: perm, its inverse pos (-1:
+    an expert outside [first, first + n_experts)) and the experts' offsets."""
+    _check(lib().qrm_sort_tokens(_ptr(topk_idx), T, k, first, n_experts, _ptr(perm), _ptr(pos), _ptr(offsets), stream))
+
+
+def gather_rows(type, x, pos, T, k, d, rows, n_rows, ld_x=0, ld_rows=0, stream=None):
+    """rows[pos[t, j]] = x[t]."""
+    _check(lib().qrm_gather_rows(int(type), _ptr(x), ld_x, _ptr(pos), T, k, d, _ptr(rows), n_rows, ld_rows, stream))
+
+
+def gather_rows_fp8(type, x, pos, T, k, d, codes, scales, n_rows, ld_x=0, ld_codes=0, ld_scales=0, stream=None):
+    """gather_rows into 8-bit rows (codes, scales)."""
+    _check(lib().qrm_gather_rows_fp8(int(type), _ptr(x), ld_x, _ptr(pos), T, k, d, _ptr(codes), n_rows, ld_codes,
+                                     _ptr(scales), ld_scales, stream))
+
+
+def combine_rows(type, rows, n_rows, pos, w, T, k, d, out, add=None, ld_rows=0, ld_add=0, ld_out=0, stream=None):
+    """out[t] = add[t] + sum_j w[t, j] rows[pos[t, j]] (w None: 1)."""
+    _check(lib().qrm_combine_rows(int(type), _ptr(rows), n_rows, ld_rows, _ptr(pos), _ptr(w), T, k, d, _ptr(add), ld_add,
+                                  _ptr(out), ld_out, stream))
+
+
+def combine_rows_grad(type, dout, rows, n_rows, pos, w, T, k, d, drows, dw=None, ld_dout=0, ld_rows=0, ld_drows=0,
+                      stream=None):
+    """drows[pos[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], rows[pos[t, j]]>."""
+    _check(lib().qrm_combine_rows_grad(int(type), _ptr(dout), ld_dout, _ptr(rows), n_rows, ld_rows, _ptr(pos), _ptr(w),
+                                       T, k, d, _ptr(drows), ld_drows, _ptr(dw), stream))
+
+
+def combine_rows_grad_fp8(type, dout, rows, n_rows, pos, w, T, k, d, codes, scales, dw=None, ld_dout=0, ld_rows=0,
+                          ld_codes=0, ld_scales=0, stream=None):
+    """combine_rows_grad with the rows' gradient in 8 bits (codes, scales)."""
+    _check(lib().qrm_combine_rows_grad_fp8(int(type), _ptr(dout), ld_dout, _ptr(rows), n_rows, ld_rows, _ptr(pos),
+                                           _ptr(w), T, k, d, _ptr(codes), ld_codes, _ptr(scales), ld_scales, _ptr(dw),
+                                           stream))
+
+
+def quantize_fp8(type, x, rows, cols, codes, scales, n_rows=None, ld_x=0, ld_codes=0, ld_scales=0, stream=None):
+    """Rows into 8 bits; n_rows: how many of them, on the device."""
+    _check(lib().qrm_quantize_fp8(int(type), _ptr(x), ld_x, rows, cols, _ptr(n_rows), _ptr(codes), ld_codes,
+                                  _ptr(scales), ld_scales, stream))
+
+
+def quantize_fp8_weights(type, w, rows, cols, codes, scales, groups=1, stream=None):
+    """Matrices into 8 bits, one scale for each 128 x 128 block."""
+    _check(lib().qrm_quantize_fp8_weights(int(type), _ptr(w), groups, rows, cols, _ptr(codes), _ptr(scales), stream))
+
+
+def swiglu_fp8(type, gu, rows, f, codes, scales, limit=0.0, n_rows=None, ld_gu=0, ld_codes=0, ld_scales=0, stream=None):
+    """silu(gate) up of gu [rows][2f] (gate's columns, then up's) into 8-bit rows."""
+    _check(lib().qrm_swiglu_fp8(int(type), _ptr(gu), ld_gu, rows, f, _ptr(n_rows), limit, _ptr(codes), ld_codes,
+                                _ptr(scales), ld_scales, stream))
+
+
+def swiglu_fp8_grad(type, gu, dh, rows, f, codes, scales, limit=0.0, n_rows=None, ld_gu=0, ld_dh=0, ld_codes=0,
+                    ld_scales=0, stream=None):
+    """The gradients of gate and up [rows][2f], given dh [rows][f], into 8-bit rows."""
+    _check(lib().qrm_swiglu_fp8_grad(int(type), _ptr(gu), ld_gu, _ptr(dh), ld_dh, rows, f, _ptr(n_rows), limit,
+                                     _ptr(codes), ld_codes, _ptr(scales), ld_scales, stream))
+
+
+class Fp8Matrix:
+    """`groups` matrices [rows x cols] in 8-bit floating point with a scale for
+    each 128 x 128 block, kept in HBM (qrm_fp8_*).  codes [groups][rows][cols]
+    (one byte each) and scales [groups][ceil(rows/128)][ceil(cols/128)] are
+    NumPy arrays or tensors, on the host or the device, and are copied."""
+
+    def __init__(self, rows, cols, codes, scales, groups=1, device=0):
+        on_device = [bool(getattr(a, "is_cuda", False)) for a in (codes, scales)]
+        if on_device[0] != on_device[1]:
+            raise ValueError("codes and scales must both be on the host or both on the device")
+        if on_device[0]:
+            codes, scales = codes.contiguous(), scales.contiguous()
+            if codes.element_size() != 1 or str(scales.dtype) != "torch.float32":
+                raise ValueError("codes of one byte and scales of float32 are needed")
+        else:
+            if hasattr(codes, "data_ptr"):
+                import torch
+                codes = codes.view(torch.uint8)
+            codes = np.ascontiguousarray(codes)
+            scales = np.ascontiguousarray(scales, dtype=np.float32)
+            if codes.itemsize != 1:
+                raise ValueError("codes of one byte are needed")
+        create = lib().qrm_fp8_create_device if on_device[0] else lib().qrm_fp8_create
+        h = P()
+        _check(create(device, groups, rows, cols, _ptr(codes), codes.nbytes, _ptr(scales), scales.nbytes, C.byref(h)))
+        self._h, self.rows, self.cols, self.groups = h, rows, cols, groups
+
+    def product(self, type, x, x_scales, T, y, offsets=None, ld_x=0, ld_scales=0, ld_y=0, stream=None):
+        """y[t] = W_g x[t] for the 8-bit rows x of each group g (offsets)."""
+        _check(lib().qrm_fp8_product(self._h, _ptr(x), ld_x, _ptr(x_scales), ld_scales, _ptr(offsets), T, int(type),
+                                     _ptr(y), ld_y, stream))
+
+    def product_t(self, type, y, y_scales, T, x, offsets=None, ld_y=0, ld_scales=0, ld_x=0, stream=None):
+        """x[t] = W_g^T y[t]: the gradient of the product's input."""
+        _check(lib().qrm_fp8_product_t(self._h, _ptr(y), ld_y, _ptr(y_scales), ld_scales, _ptr(offsets), T, int(type),
+                                       _ptr(x), ld_x, stream))
+
+    def sync(self):
+        """Waits for the device and raises what the products met."""
+        _check(lib().qrm_fp8_sync(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().qrm_fp8_destroy(self._h)
             self._h = None
 
     def __del__(self):

@@ -22,7 +22,8 @@ LIB = os.path.join(PKG, "lib", "libqrmoe.so")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-I", os.path.join(ROOT, "include"),
           "--expt-relaxed-constexpr"]
-UNITS = [("qrmoe.cu", []), ("umma.cu", []), ("qwfile.cu", []), ("synth.cu", ["-fmad=false"])]
+UNITS = [("qrmoe.cu", []), ("umma.cu", []), ("qwfile.cu", []), ("rows.cu", []), ("fp8.cu", []),
+         ("synth.cu", ["-fmad=false"])]
 
 
 def nvcc():
@@ -42,7 +43,7 @@ def sources_newer(target, deps):
 def build(ptxas_verbose=False, force=False, quiet=False):
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
-    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cuh")]
+    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     headers.append(os.path.join(ROOT, "include", "qrmoe.h"))
     objs = []
     for src, extra in UNITS:

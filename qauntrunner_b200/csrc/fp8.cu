@@ -1,0 +1,225 @@
+// fp8.cu -- matrices in 8-bit floating point with a scale for each 128 x 128
+// block, resident in HBM, and their products (kernels: fp8.cuh).
+#include <stdlib.h>
+
+#include <algorithm>
+#include <climits>
+#include <new>
+
+#include "fp8.cuh"
+#include "host_util.h"
+#include "umma_host.h"
+
+using namespace qrm;
+
+struct qrm_fp8 {
+    int device = 0, sms = 0, groups = 0;
+    int64_t rows = 0, cols = 0, pitch = 0;   // of one matrix; pitch: bytes of a stored row
+    uint8_t* codes = nullptr;                // [groups][rows][pitch]
+    float* scales = nullptr;                 // [groups][row blocks][column blocks]
+    float* part = nullptr;                   // partial tiles of the CTAs
+    int32_t* arrivals = nullptr;
+    int32_t* err = nullptr;
+    CUtensorMap map;
+};
+
+namespace {
+
+int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
+
+void release(qrm_fp8* m) {
+    if (!m) return;
+    cudaSetDevice(m->device);
+    cudaDeviceSynchronize();
+    cudaFree(m->codes);
+    cudaFree(m->scales);
+    cudaFree(m->part);
+    cudaFree(m->arrivals);
+    cudaFree(m->err);
+    delete m;
+}
+
+// 8-bit tensor of up to three dimensions, innermost first, as a TMA map with
+// 128-byte swizzle; what lies outside reads as zero
+bool encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+            const cuuint32_t* box) {
+    auto fn = tensor_map_encoder();
+    if (!fn) return false;
+    const cuuint32_t step[3] = {1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, step,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int kSmemMost = 227 * 1024;
+int stage_bytes(int x_rows) { return kFp8Tile + x_rows * 128; }
+int stages_for(int groups, int x_rows) {
+    return std::min(kFp8MaxStages, (kSmemMost - 1024 - fp8_stage_off(groups)) / stage_bytes(x_rows));
+}
+size_t smem_for(int groups, int x_rows) {
+    return 1024 + (size_t)fp8_stage_off(groups) + (size_t)stages_for(groups, x_rows) * stage_bytes(x_rows);
+}
+
+int create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes, const float* scales,
+           size_t scale_bytes, cudaMemcpyKind kind, qrm_fp8** out) {
+    const char* what = "qrm_fp8_create";
+    if (!out) return failf(QRM_E_INVALID, "%s: out is NULL", what);
+    *out = nullptr;
+    if (!codes || !scales) return failf(QRM_E_INVALID, "%s: NULL argument", what);
+    if (groups <= 0 || rows <= 0 || cols <= 0 || rows > (1 << 24) || cols > (1 << 24))
+        return failf(QRM_E_INVALID, "%s: %d matrices of %lld x %lld", what, groups, (long long)rows, (long long)cols);
+    if (groups > kFp8MaxGroups) return failf(QRM_E_CAPACITY, "%s: %d matrices, at most %d", what, groups, kFp8MaxGroups);
+    const int64_t nb = (int64_t)groups * blocks_of(rows) * blocks_of(cols);
+    if (code_bytes != (size_t)(groups * rows * cols))
+        return failf(QRM_E_SIZE, "%s: %zu bytes of codes, %d x %lld x %lld = %lld", what, code_bytes, groups,
+                     (long long)rows, (long long)cols, (long long)(groups * rows * cols));
+    if (scale_bytes != (size_t)nb * sizeof(float))
+        return failf(QRM_E_SIZE, "%s: %zu bytes of scales, one f32 for each of %lld blocks is %lld", what, scale_bytes,
+                     (long long)nb, (long long)nb * 4);
+    int count = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) return failf(QRM_E_CUDA, "%s: no CUDA device", what);
+    if (device < 0 || device >= count) return failf(QRM_E_INVALID, "%s: device %d out of range", what, device);
+    int sms;
+    if (cudaSetDevice(device) != cudaSuccess) return failf(QRM_E_CUDA, "%s: device %d", what, device);
+    if (int rc = current_device(&device, &sms)) return rc;
+    if (const char* e = getenv("QRM_WAIT_LIMIT_US"))
+        if (set_wait_limit_here((uint64_t)std::max(1LL, atoll(e)) * 1000ull) != cudaSuccess)
+            return failf(QRM_E_CUDA, "%s: wait limit", what);
+    qrm_fp8* m = new (std::nothrow) qrm_fp8();
+    if (!m) return failf(QRM_E_NOMEM, "%s: host memory", what);
+    auto bail = [&](int rc) {
+        release(m);
+        return rc;
+    };
+    m->device = device;
+    m->sms = sms;
+    m->groups = groups;
+    m->rows = rows;
+    m->cols = cols;
+    m->pitch = (cols + 15) / 16 * 16;
+    const size_t part = sizeof(float) * (size_t)sms * 2 * kFp8MaxRows * 128;
+    const size_t arrivals = sizeof(int32_t) * (size_t)sms * kFp8EpiWarps;
+    if (cudaMalloc(&m->codes, (size_t)groups * rows * m->pitch) != cudaSuccess ||
+        cudaMalloc(&m->scales, scale_bytes) != cudaSuccess || cudaMalloc(&m->part, part) != cudaSuccess ||
+        cudaMalloc(&m->arrivals, arrivals) != cudaSuccess || cudaMalloc(&m->err, sizeof(int32_t)) != cudaSuccess) {
+        cudaGetLastError();
+        return bail(failf(QRM_E_NOMEM, "%s: cannot allocate %lld bytes", what, (long long)(groups * rows * m->pitch)));
+    }
+    // device sources: what any stream still writes there is awaited, as in qrm_upload_expert_device
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess)
+        e = cudaMemcpy2D(m->codes, m->pitch, codes, cols, cols, (size_t)groups * rows, kind);
+    if (e == cudaSuccess) e = cudaMemcpy(m->scales, scales, scale_bytes, kind);
+    if (e == cudaSuccess) e = cudaMemset(m->arrivals, 0, arrivals);
+    if (e == cudaSuccess) e = cudaMemset(m->err, 0, sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    if (e != cudaSuccess) return bail(failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e)));
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)groups};
+    const cuuint64_t strides[2] = {(cuuint64_t)m->pitch, (cuuint64_t)(m->pitch * rows)};
+    const cuuint32_t box[3] = {128, 128, 1};
+    if (!encode(&m->map, m->codes, 3, dims, strides, box)) return bail(failf(QRM_E_CUDA, "%s: tensor map", what));
+    *out = m;
+    return QRM_OK;
+}
+
+int product(const char* what, qrm_fp8* m, bool back, const void* x, int64_t ld_x, const float* xs, int64_t ld_xs,
+            const int32_t* offsets, int64_t T, int type, void* out, int64_t ld_out, void* stream) {
+    if (!m) return failf(QRM_E_INVALID, "%s: NULL matrix", what);
+    const int64_t in = back ? m->rows : m->cols, M = back ? m->cols : m->rows;
+    const int b = type_bytes(type);
+    if (!b) return failf(QRM_E_FORMAT, "%s: type %d is not F32, F16 or BF16", what, type);
+    if (T < 0 || T > INT_MAX) return failf(QRM_E_INVALID, "%s: %lld rows", what, (long long)T);
+    const int64_t mb = blocks_of(M), kb = blocks_of(in);
+    // (at most one partly filled tile for each group)
+    if ((T / kFp8MaxRows + m->groups) * mb > INT_MAX)
+        return failf(QRM_E_CAPACITY, "%s: %lld rows in %d groups are too many tiles", what, (long long)T, m->groups);
+    if (T == 0) return QRM_OK;
+    if (!x || !xs || !out) return failf(QRM_E_INVALID, "%s: NULL argument", what);
+    if (!offsets && m->groups > 1) return failf(QRM_E_INVALID, "%s: %d matrices need offsets", what, m->groups);
+    if (!pitch_ok(&ld_x, in) || !pitch_ok(&ld_xs, kb) || !pitch_ok(&ld_out, M))
+        return failf(QRM_E_INVALID, "%s: a pitch is below its row (x %lld, scales %lld, out %lld)", what, (long long)ld_x,
+                     (long long)ld_xs, (long long)ld_out);
+    if (!aligned(x, 16) || ld_x % 16)
+        return failf(QRM_E_INVALID, "%s: rows of codes must start on 16 bytes (pitch %lld)", what, (long long)ld_x);
+    if (!aligned(xs, 4) || !aligned(out, b) || (offsets && !aligned(offsets, 4)))
+        return failf(QRM_E_INVALID, "%s: a pointer is not aligned to its values", what);
+    cudaError_t e = cudaSetDevice(m->device);
+    if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    CUtensorMap x_map;
+    const cuuint64_t dims[2] = {(cuuint64_t)in, (cuuint64_t)T};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld_x};
+    const cuuint32_t box[2] = {128, 16};
+    if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
+    const int wkb = (int)blocks_of(m->cols), wnb = (int)blocks_of(m->rows);
+    Fp8Params p{};
+    p.w_scales = m->scales;
+    p.x_scales = xs;
+    p.offsets = offsets;
+    p.out = out;
+    p.part = m->part;
+    p.arrivals = m->arrivals;
+    p.err = m->err;
+    p.ld_xs = ld_xs;
+    p.ld_out = ld_out;
+    p.T = (int)T;
+    p.groups = m->groups;
+    p.M = (int)M;
+    p.mb = (int)mb;
+    p.kb = (int)kb;
+    p.s_group = wnb * wkb;
+    p.s_m = back ? 1 : wkb;
+    p.s_k = back ? wkb : 1;
+    p.back = back;
+    p.type = type;
+    const int x_rows = (int)std::min<int64_t>(kFp8MaxRows, (T + 15) / 16 * 16);
+    fp8_stream_kernel<<<m->sms, kFp8Warps * 32, smem_for(m->groups, x_rows), (cudaStream_t)stream>>>(
+        m->map, x_map, p, stages_for(m->groups, x_rows), x_rows);
+    return launched(what);
+}
+
+}  // namespace
+
+extern "C" int qrm_fp8_create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes,
+                              const float* scales, size_t scale_bytes, qrm_fp8** out) {
+    return create(device, groups, rows, cols, codes, code_bytes, scales, scale_bytes, cudaMemcpyHostToDevice, out);
+}
+
+extern "C" int qrm_fp8_create_device(int device, int groups, int64_t rows, int64_t cols, const void* codes_dev,
+                                     size_t code_bytes, const float* scales_dev, size_t scale_bytes, qrm_fp8** out) {
+    return create(device, groups, rows, cols, codes_dev, code_bytes, scales_dev, scale_bytes, cudaMemcpyDeviceToDevice, out);
+}
+
+extern "C" void qrm_fp8_destroy(qrm_fp8* m) { release(m); }
+
+extern "C" int qrm_fp8_product(qrm_fp8* m, const void* x_codes_dev, int64_t ld_x, const float* x_scales_dev,
+                               int64_t ld_xs, const int32_t* offsets_dev, int64_t T, int type, void* y_dev, int64_t ld_y,
+                               void* stream) {
+    return product("qrm_fp8_product", m, false, x_codes_dev, ld_x, x_scales_dev, ld_xs, offsets_dev, T, type, y_dev, ld_y,
+                   stream);
+}
+
+extern "C" int qrm_fp8_product_t(qrm_fp8* m, const void* y_codes_dev, int64_t ld_y, const float* y_scales_dev,
+                                 int64_t ld_ys, const int32_t* offsets_dev, int64_t T, int type, void* x_dev,
+                                 int64_t ld_x, void* stream) {
+    return product("qrm_fp8_product_t", m, true, y_codes_dev, ld_y, y_scales_dev, ld_ys, offsets_dev, T, type, x_dev, ld_x,
+                   stream);
+}
+
+extern "C" int qrm_fp8_sync(qrm_fp8* m) {
+    if (!m) return failf(QRM_E_INVALID, "qrm_fp8_sync: NULL matrix");
+    cudaError_t e = cudaSetDevice(m->device);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    int32_t err = 0;
+    if (e == cudaSuccess) e = cudaMemcpy(&err, m->err, sizeof err, cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && err) {
+        // a product that gave up may have left counts behind
+        e = cudaMemset(m->arrivals, 0, sizeof(int32_t) * (size_t)m->sms * kFp8EpiWarps);
+        if (e == cudaSuccess) e = cudaMemset(m->err, 0, sizeof err);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    }
+    if (e != cudaSuccess) return failf(QRM_E_CUDA, "qrm_fp8_sync: %s", cudaGetErrorString(e));
+    if (err & ERR_TIMEOUT) return failf(QRM_E_TIMEOUT, "qrm_fp8_sync: a device wait timed out");
+    if (err) return failf(QRM_E_INVALID, "qrm_fp8_sync: offsets do not ascend within the rows (flags 0x%x)", err);
+    return QRM_OK;
+}

@@ -1,7 +1,5 @@
 // umma.cu -- host side of the tcgen05 grouped expert path (umma.cuh): tensor
 // maps, the gather and planning kernels, the grouped kernel launches.
-#include <cudaTypedefs.h>
-
 #include <algorithm>
 #include <mutex>
 
@@ -16,8 +14,7 @@ cudaError_t umma_set_wait_limit(uint64_t ns) { return set_wait_limit_here(ns); }
 
 bool umma_format(int fmt) { return fmt == Q4_K || fmt == Q8_0 || fmt == Q4_0 || fmt == Q6_K || fmt == TRI; }
 
-// cuTensorMapEncodeTiled from the driver (no link-time dependency on libcuda)
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static std::once_flag once;
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     std::call_once(once, [] {
@@ -31,7 +28,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 int umma_encode_map(CUtensorMap* map, const void* base, long long rows, int K) {
-    auto fn = encode_fn();
+    auto fn = tensor_map_encoder();
     if (!fn) return -1;
     const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)K * 2};

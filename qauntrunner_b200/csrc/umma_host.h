@@ -2,6 +2,7 @@
 // (umma.cu), used by the forward in qrmoe.cu.
 #pragma once
 #include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -17,6 +18,9 @@ struct UmmaItem {
     int n;        // tokens (1..256)
 };
 
+// cuTensorMapEncodeTiled from the driver (no link-time dependency on libcuda);
+// NULL when it has none
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 // the grouped kernel's wait limit on the current device (QRM_WAIT_LIMIT_US)
 cudaError_t umma_set_wait_limit(uint64_t ns);
 // true when matrices of format fmt in the tiled layout can take the path
