@@ -93,6 +93,62 @@ __device__ __forceinline__ void store_typed(void* out, long long i, float v, int
     else reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
 }
 
+// ------------------------------------------------------------ waits
+// A ready barrier costs one try_wait and a vote; the bounded loop is out of
+// line.  (The single-lane waits with an integer division for the ring's slot
+// that this kernel began with cost some 300 cycles each, ready or not, and
+// were what bounded it: 710 TFLOP/s at 4096 x 28672 x 4096.)
+struct Fp8Ctl {
+    volatile int* abort_flag;
+    int32_t* err;
+};
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+    const uint64_t t0 = global_ns(), lim = wait_limit_ns();
+    bool ok = false;
+    for (;;) {
+        for (int i = 0; i < 8 && !ok; i++) ok = bar_try(bar, parity);
+        if (ok || *abort_flag || global_ns() - t0 > lim) break;
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && (threadIdx.x & 31) == 0) {
+        *abort_flag = 1;
+        atomicOr(err, (int)ERR_TIMEOUT);
+    }
+    return ok;
+}
+// all lanes; false for all of them when the wait gave up
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const Fp8Ctl& c) {
+    if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
+    return bar_wait_slow(bar, parity, c.abort_flag, c.err);
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
+}
+// position in a ring: slot and the parity of its current phase
+struct Ring {
+    uint32_t i = 0, phase = 0;
+    __device__ __forceinline__ void next(uint32_t n) {
+        if (++i == n) {
+            i = 0;
+            phase ^= 1;
+        }
+    }
+};
+
 // ------------------------------------------------------------ weights on the MMA's M side
 // A tile is 128 outputs (one block row of the matrix, the MMA's M) x up to 128
 // rows of x (its N, rounded up to 16 only), so a group of a few rows costs
@@ -114,10 +170,11 @@ constexpr int kFp8EpiWarps = 8;
 constexpr int kFp8Tile = 128 * 128;     // bytes of a weight tile
 constexpr int kFp8MaxRows = 128;        // rows of x in a tile
 constexpr int kFp8Acc = 4;              // accumulators in tensor memory
-constexpr int kFp8ScaleRing = 16;
+constexpr int kFp8ScaleRing = 4;        // slots of four blocks' scales
 constexpr int kFp8MaxStages = 12;
 constexpr int kFp8ScaleOff = 1024;                                       // after the barriers
-constexpr int kFp8TableOff = kFp8ScaleOff + kFp8ScaleRing * kFp8MaxRows * 4;
+constexpr int kFp8ScaleSlot = 4 * kFp8MaxRows;                           // floats
+constexpr int kFp8TableOff = kFp8ScaleOff + kFp8ScaleRing * kFp8ScaleSlot * 4;
 __host__ __device__ inline int fp8_stage_off(int groups) { return (kFp8TableOff + 12 * (groups + 1) + 1023) / 1024 * 1024; }
 
 // What a CTA does: blocks [q, q_end) of the sequence (tile, block).
@@ -203,10 +260,10 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
                   int stages, int x_rows /* room for rows of x in a stage */) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm);          // [stages]
-    uint64_t* empty = full + kFp8MaxStages;
-    uint64_t* acc_full = empty + kFp8MaxStages;                // [kFp8Acc]
-    uint64_t* acc_empty = acc_full + kFp8Acc;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm);
+    uint64_t* full = bars;                                     // [stages] tiles are there
+    uint64_t* done = full + kFp8MaxStages;                     // [stages] their MMAs are done
+    uint64_t* acc_empty = done + kFp8MaxStages;                // [kFp8Acc]
     uint64_t* sc_full = acc_empty + kFp8Acc;                   // [kFp8ScaleRing]
     uint64_t* sc_empty = sc_full + kFp8ScaleRing;
     uint64_t* done_bar = sc_empty + kFp8ScaleRing;
@@ -216,19 +273,16 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp8TableOff);
     int32_t* start = first_tile + p.groups + 1;
     int32_t* rows = start + p.groups + 1;
-    const int stage_off = fp8_stage_off(p.groups), stage_bytes = kFp8Tile + x_rows * 128;
-    uint8_t* ring = sm + stage_off;
+    const uint32_t stage_bytes = kFp8Tile + x_rows * 128;
+    uint8_t* ring = sm + fp8_stage_off(p.groups);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; i++) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&done[i], 1);
         }
-        for (int i = 0; i < kFp8Acc; i++) {
-            mbar_init(&acc_full[i], 1);
-            mbar_init(&acc_empty[i], kFp8EpiWarps);
-        }
+        for (int i = 0; i < kFp8Acc; i++) mbar_init(&acc_empty[i], kFp8EpiWarps);
         for (int i = 0; i < kFp8ScaleRing; i++) {
             mbar_init(&sc_full[i], 1);
             mbar_init(&sc_empty[i], kFp8EpiWarps);
@@ -243,6 +297,9 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    const Fp8Ctl ctl{abort_flag, p.err};
+    const uint32_t full0 = smem_u32(full), done0 = smem_u32(done), acc_empty0 = smem_u32(acc_empty);
+    const uint32_t sc_full0 = smem_u32(sc_full), sc_empty0 = smem_u32(sc_empty);
     Fp8Plan plan{first_tile, start, rows, p.groups, p.mb, p.kb, (long long)first_tile[p.groups] * p.kb, 0};
     plan.ctas = (int)min((long long)gridDim.x, plan.total);   // each has a block at least
     const bool idle = (int)blockIdx.x >= plan.ctas;
@@ -251,95 +308,93 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     if (warp == 0) {
         // ------------------------------------------------ tiles
         bool ok = true;
-        uint32_t i = 0;
+        Ring r;
+        uint32_t issued = 0;
         for (long long q = q0; q < q1 && ok;) {
             const Fp8Piece t = plan.piece(q, q1);
             const int boxes = (t.n + 15) >> 4;
-            for (int kb = t.k0; kb < t.k1; kb++, i++) {
-                const int s = i % stages;
-                if (i >= (uint32_t)stages) {
-                    const bool w = lane == 0 ? mbar_wait_abort(&empty[s], ((i / stages) & 1u) ^ 1u, abort_flag) : true;
-                    if (!__shfl_sync(0xffffffffu, (int)w, 0)) { ok = false; break; }
-                }
-                uint8_t* st = ring + (size_t)s * stage_bytes;
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&full[s], (uint32_t)(kFp8Tile + boxes * 2048));
-                    if (p.back) tma_load_3d(st, &w_map, t.m * 128, kb * 128, t.group, &full[s]);
-                    else tma_load_3d(st, &w_map, kb * 128, t.m * 128, t.group, &full[s]);
+            for (int kb = t.k0; kb < t.k1; kb++) {
+                if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                uint8_t* st = ring + r.i * stage_bytes;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(&full[r.i], (uint32_t)(kFp8Tile + boxes * 2048));
+                    if (p.back) tma_load_3d(st, &w_map, t.m * 128, kb * 128, t.group, &full[r.i]);
+                    else tma_load_3d(st, &w_map, kb * 128, t.m * 128, t.group, &full[r.i]);
+                    for (int b = 0; b < boxes; b++)
+                        tma_load_2d(st + kFp8Tile + b * 2048, &x_map, kb * 128, t.pos + 16 * b, &full[r.i]);
                 }
                 __syncwarp();
-                if (lane < boxes) tma_load_2d(st + kFp8Tile + lane * 2048, &x_map, kb * 128, t.pos + 16 * lane, &full[s]);
+                r.next(stages);
+                issued++;
             }
             q += t.k1 - t.k0;
         }
-        if (!ok && lane == 0) {
-            *abort_flag = 1;
-            atomicOr(p.err, (int)ERR_TIMEOUT);
-            // copies already issued must land before the CTA exits
-            for (uint32_t j = i > (uint32_t)stages ? i - stages : 0; j < i; j++) mbar_wait(&full[j % stages], (j / stages) & 1u);
-        }
+        if (!ok && lane == 0)   // copies already issued must land before the CTA exits
+            for (uint32_t j = issued > (uint32_t)stages ? issued - stages : 0; j < issued; j++)
+                mbar_wait(&full[j % stages], (j / stages) & 1u);
     } else if (warp == 1) {
-        // ------------------------------------------------ MMAs (one thread)
-        if (lane == 0) {
-            bool ok = true;
-            uint32_t i = 0;
-            for (long long q = q0; q < q1 && ok;) {
-                const Fp8Piece t = plan.piece(q, q1);
-                const uint32_t idesc = umma_idesc_e4m3((t.n + 15) & ~15, p.back, false);
-                for (int kb = t.k0; kb < t.k1; kb++, i++) {
-                    const int s = i % stages, b = i % kFp8Acc;
-                    if ((i >= kFp8Acc && !mbar_wait_abort(&acc_empty[b], ((i / kFp8Acc) & 1u) ^ 1u, abort_flag)) ||
-                        !mbar_wait_abort(&full[s], (i / stages) & 1u, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t a = smem_u32(ring + (size_t)s * stage_bytes), x = a + kFp8Tile;
-#pragma unroll
-                    for (int c = 0; c < 4; c++)   // 32 contracted values: 32 bytes along K, or 32 rows of 128 bytes
-                        umma_f8(tmem + 128 * b, p.back ? sw128_desc_mn(a + 4096 * c, kFp8Tile) : sw128_desc(a + 32 * c),
-                                sw128_desc(x + 32 * c), idesc, c ? 1u : 0u);
-                    umma_commit(&empty[s]);
-                    umma_commit(&acc_full[b]);
+        // ------------------------------------------------ MMAs (one thread issues)
+        bool ok = true;
+        Ring r, a;
+        // 32 contracted values are 32 bytes along K, or 32 rows of 128 bytes
+        const uint32_t ring0 = smem_u32(ring), step = p.back ? 4096 >> 4 : 32 >> 4;
+        const uint64_t w_desc = p.back ? sw128_desc_mn(ring0, kFp8Tile) : sw128_desc(ring0), x_desc = sw128_desc(ring0 + kFp8Tile);
+        for (long long q = q0; q < q1 && ok;) {
+            const Fp8Piece t = plan.piece(q, q1);
+            const uint32_t idesc = umma_idesc_e4m3((t.n + 15) & ~15, p.back, false);
+            for (int kb = t.k0; kb < t.k1; kb++) {
+                if (!bar_wait(acc_empty0 + 8 * a.i, a.phase ^ 1u, ctl) || !bar_wait(full0 + 8 * r.i, r.phase, ctl)) {
+                    ok = false;
+                    break;
                 }
-                q += t.k1 - t.k0;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint32_t at = r.i * stage_bytes >> 4, d = tmem + 128 * a.i;
+                    umma_f8(d, w_desc + at, x_desc + at, idesc, 0u);
+                    umma_f8(d, w_desc + at + step, x_desc + at + 2, idesc, 1u);
+                    umma_f8(d, w_desc + at + 2 * step, x_desc + at + 4, idesc, 1u);
+                    umma_f8(d, w_desc + at + 3 * step, x_desc + at + 6, idesc, 1u);
+                    umma_commit(&done[r.i]);
+                }
+                __syncwarp();
+                r.next(stages);
+                a.next(kFp8Acc);
             }
-            if (!ok) {
-                *abort_flag = 1;
-                atomicOr(p.err, (int)ERR_TIMEOUT);
-            }
-            // every MMA of this CTA has completed before tensor memory is released
+            q += t.k1 - t.k0;
+        }
+        // every MMA of this CTA has completed before tensor memory is released
+        if (elect_one()) {
             umma_commit(done_bar);
             mbar_wait(done_bar, 0u);
         }
         __syncwarp();
     } else if (warp == 2) {
-        // ------------------------------------------------ scales, four blocks' loads at a time
+        // ------------------------------------------------ scales, four blocks at a time
         bool ok = true;
-        uint32_t i = 0;
+        Ring r;
         for (long long q = q0; q < q1 && ok;) {
             const Fp8Piece t = plan.piece(q, q1);
             const float* ws = p.w_scales + (long long)t.group * p.s_group + (long long)t.m * p.s_m;
             const float* xs = p.x_scales + (long long)t.pos * p.ld_xs;
-            for (int k4 = t.k0; k4 < t.k1 && ok; k4 += 4) {
+            for (int k4 = t.k0; k4 < t.k1; k4 += 4) {
                 float v[4][4], w[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int kb = k4 + j;
                     w[j] = kb < t.k1 ? __ldg(ws + (long long)kb * p.s_k) : 0.f;
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        v[j][r] = kb < t.k1 && lane + 32 * r < t.n ? __ldg(xs + (lane + 32 * r) * p.ld_xs + kb) : 0.f;
+                    for (int c = 0; c < 4; c++)
+                        v[j][c] = kb < t.k1 && lane + 32 * c < t.n ? __ldg(xs + (lane + 32 * c) * p.ld_xs + kb) : 0.f;
                 }
+                if (!bar_wait(sc_empty0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (k4 + j >= t.k1) break;
-                    const int s = i % kFp8ScaleRing;
-                    if (i >= kFp8ScaleRing &&
-                        !warp_wait(&sc_empty[s], ((i / kFp8ScaleRing) & 1u) ^ 1u, abort_flag, p.err)) { ok = false; break; }
+                for (int j = 0; j < 4; j++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) sc_ring[s * kFp8MaxRows + lane + 32 * r] = v[j][r] * w[j];
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sc_full[s]);
-                    i++;
-                }
+                    for (int c = 0; c < 4; c++)
+                        sc_ring[r.i * kFp8ScaleSlot + j * kFp8MaxRows + lane + 32 * c] = v[j][c] * w[j];
+                __syncwarp();
+                if (lane == 0) bar_arrive(sc_full0 + 8 * r.i);
+                r.next(kFp8ScaleRing);
             }
             q += t.k1 - t.k0;
         }
@@ -349,24 +404,27 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
         const int lane_row = 32 * (warp & 3) + lane;             // output inside the tile
         const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c0;
         bool ok = true;
-        uint32_t i = 0;
+        Ring r, a, sr;
         for (long long q = q0; q < q1 && ok;) {
             const Fp8Piece t = plan.piece(q, q1);
             const int n = t.n - c0;   // rows of x of this warp (none: it only keeps the hand-overs going)
             float2 acc[32];
 #pragma unroll
             for (int c = 0; c < 32; c++) acc[c] = make_float2(0.f, 0.f);
-            for (int kb = t.k0; kb < t.k1; kb++, i++) {
-                const int b = i % kFp8Acc, s = i % kFp8ScaleRing;
-                if (!warp_wait(&acc_full[b], (i / kFp8Acc) & 1u, abort_flag, p.err) ||
-                    !warp_wait(&sc_full[s], (i / kFp8ScaleRing) & 1u, abort_flag, p.err)) { ok = false; break; }
+            for (int kb = t.k0; kb < t.k1; kb++) {
+                const int j = (kb - t.k0) & 3;
+                if ((j == 0 && !bar_wait(sc_full0 + 8 * sr.i, sr.phase, ctl)) || !bar_wait(done0 + 8 * r.i, r.phase, ctl)) {
+                    ok = false;
+                    break;
+                }
                 tc_fence_after();
-                const float4* sc = reinterpret_cast<const float4*>(sc_ring + s * kFp8MaxRows + c0);
+                const float4* sc = reinterpret_cast<const float4*>(sc_ring + sr.i * kFp8ScaleSlot + j * kFp8MaxRows + c0);
+                const uint32_t from = taddr + 128 * a.i;
                 if (n > 32) {
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         float v[32];
-                        tmem_ld32(taddr + 128 * b + 32 * h, v);
+                        tmem_ld32(from + 32 * h, v);
 #pragma unroll
                         for (int c = 0; c < 8; c++) {
                             const float4 w = sc[8 * h + c];
@@ -374,21 +432,20 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
                             acc[16 * h + 2 * c + 1] = ffma2(make_float2(v[4 * c + 2], v[4 * c + 3]), make_float2(w.z, w.w), acc[16 * h + 2 * c + 1]);
                         }
                     }
-                } else if (n > 0) {
+                } else if (n > 16) {
                     float v[32];
-                    if (n > 16) {
-                        tmem_ld32(taddr + 128 * b, v);
-                    } else {
-                        float u[16];
-                        tmem_ld16(taddr + 128 * b, u);
-#pragma unroll
-                        for (int c = 0; c < 16; c++) {
-                            v[c] = u[c];
-                            v[16 + c] = 0.f;
-                        }
-                    }
+                    tmem_ld32(from, v);
 #pragma unroll
                     for (int c = 0; c < 8; c++) {
+                        const float4 w = sc[c];
+                        acc[2 * c] = ffma2(make_float2(v[4 * c], v[4 * c + 1]), make_float2(w.x, w.y), acc[2 * c]);
+                        acc[2 * c + 1] = ffma2(make_float2(v[4 * c + 2], v[4 * c + 3]), make_float2(w.z, w.w), acc[2 * c + 1]);
+                    }
+                } else if (n > 0) {
+                    float v[16];
+                    tmem_ld16(from, v);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
                         const float4 w = sc[c];
                         acc[2 * c] = ffma2(make_float2(v[4 * c], v[4 * c + 1]), make_float2(w.x, w.y), acc[2 * c]);
                         acc[2 * c + 1] = ffma2(make_float2(v[4 * c + 2], v[4 * c + 3]), make_float2(w.z, w.w), acc[2 * c + 1]);
@@ -396,10 +453,14 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
                 }
                 tc_fence_before();
                 __syncwarp();
+                const bool last = j == 3 || kb + 1 == t.k1;   // of the scales' slot
                 if (lane == 0) {
-                    mbar_arrive(&acc_empty[b]);
-                    mbar_arrive(&sc_empty[s]);
+                    bar_arrive(acc_empty0 + 8 * a.i);
+                    if (last) bar_arrive(sc_empty0 + 8 * sr.i);
                 }
+                r.next(stages);
+                a.next(kFp8Acc);
+                if (last) sr.next(kFp8ScaleRing);
             }
             if (!ok) break;
             const bool whole = t.k0 == 0 && t.k1 == p.kb;
