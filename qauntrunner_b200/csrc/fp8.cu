@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <new>
 
 #include "fp8.cuh"
@@ -14,13 +15,16 @@ using namespace qrm;
 
 struct qrm_fp8 {
     int device = 0, sms = 0, groups = 0;
+    int form = -1;                           // QRM_FP8_PAIR: 1 always / 0 never rows of x on the MMA's M side
     int64_t rows = 0, cols = 0, pitch = 0;   // of one matrix; pitch: bytes of a stored row
     uint8_t* codes = nullptr;                // [groups][rows][pitch]
     float* scales = nullptr;                 // [groups][row blocks][column blocks]
     float* part = nullptr;                   // partial tiles of the CTAs
     int32_t* arrivals = nullptr;
     int32_t* err = nullptr;
-    CUtensorMap map;
+    // the stored codes in boxes of 128 x 128, and, for a pair's CTA, of half a block of outputs: 64 outputs of
+    // the product x 128 contracted, 64 of the transposed product x 128
+    CUtensorMap map, pair_map, pair_map_t;
 };
 
 namespace {
@@ -39,15 +43,15 @@ void release(qrm_fp8* m) {
     delete m;
 }
 
-// 8-bit tensor of up to three dimensions, innermost first, as a TMA map with
-// 128-byte swizzle; what lies outside reads as zero
+// 8-bit tensor of up to three dimensions, innermost first, as a TMA map; what
+// lies outside reads as zero
 bool encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
-            const cuuint32_t* box) {
+            const cuuint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     auto fn = tensor_map_encoder();
     if (!fn) return false;
     const cuuint32_t step[3] = {1, 1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box, step,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -59,6 +63,8 @@ int stages_for(int groups, int x_rows) {
 size_t smem_for(int groups, int x_rows) {
     return 1024 + (size_t)fp8_stage_off(groups) + (size_t)stages_for(groups, x_rows) * stage_bytes(x_rows);
 }
+
+size_t pair_smem(int groups) { return 1024 + (size_t)fp8_pair_stage_off(groups) + (size_t)kFp8PairStages * kFp8PairStage; }
 
 int create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes, const float* scales,
            size_t scale_bytes, cudaMemcpyKind kind, qrm_fp8** out) {
@@ -91,6 +97,7 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
         release(m);
         return rc;
     };
+    if (const char* e = getenv("QRM_FP8_PAIR")) m->form = atoi(e) != 0;
     m->device = device;
     m->sms = sms;
     m->groups = groups;
@@ -114,13 +121,35 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     if (e == cudaSuccess) e = cudaMemset(m->err, 0, sizeof(int32_t));
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e != cudaSuccess) return bail(failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e)));
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)groups};
     const cuuint64_t strides[2] = {(cuuint64_t)m->pitch, (cuuint64_t)(m->pitch * rows)};
     const cuuint32_t box[3] = {128, 128, 1};
-    if (!encode(&m->map, m->codes, 3, dims, strides, box)) return bail(failf(QRM_E_CUDA, "%s: tensor map", what));
+    const cuuint32_t pair_box[3] = {128, 64, 1}, pair_box_t[3] = {64, 128, 1};
+    if (!encode(&m->map, m->codes, 3, dims, strides, box) || !encode(&m->pair_map, m->codes, 3, dims, strides, pair_box) ||
+        !encode(&m->pair_map_t, m->codes, 3, dims, strides, pair_box_t, CU_TENSOR_MAP_SWIZZLE_64B))
+        return bail(failf(QRM_E_CUDA, "%s: tensor map", what));
     *out = m;
     return QRM_OK;
+}
+
+// Which kernel a product takes, by what both would cost with the rows spread
+// evenly over the groups.  Measured (us; weights on the M side / rows of x on
+// the M side, K and N of the product):
+//   1 x 4096 x 7168:  1 row 15 / 32, 64 rows 23 / 33, 128 rows 28 / 35, 512 rows 48 / 39, 1024 rows 72 / 42
+//   1 x 28672 x 4096: 1 row 31 / 46, 128 rows 48 / 44, 256 rows 86 / 47, 4096 rows 877 / 530
+//   32 x 4096 x 7168: 16 rows each 179 / 253, 96 rows each 253 / 280, 128 rows each 315 / 306, 256 rows each 561 / 389
+//   8 x 5632 x 1024:  16 rows each 21 / 20, 64 rows each 27 / 23; 1 x 1024 x 2816: 1 row 12 / 15, 16 rows 13 / 15
+// The first shares all blocks out to all SMs; a block costs it 0.38 us (the
+// weights' bytes) and 2 ns a row.  The second does whole tiles, 0.55 us a
+// block of 256 rows x 256 outputs, in waves over the pairs of SMs.
+bool pair_is_faster(int64_t T, int groups, int64_t M, int64_t mb, int64_t kb, int sms) {
+    const double used = (double)std::min<int64_t>(T, groups), rows = T / used;   // groups with rows, rows of each
+    const double tiles = used * mb * std::ceil(rows / kFp8MaxRows), pairs = used * ((M + 255) / 256) * std::ceil(rows / 256);
+    const double in_tile = rows / std::ceil(rows / kFp8MaxRows);
+    const double one = 10 + (0.38 + 0.002 * in_tile) * std::ceil(tiles * kb / sms), two = 6 + 0.55 * std::ceil(pairs / (sms / 2)) * kb;
+    return two < one;
 }
 
 int product(const char* what, qrm_fp8* m, bool back, const void* x, int64_t ld_x, const float* xs, int64_t ld_xs,
@@ -149,8 +178,6 @@ int product(const char* what, qrm_fp8* m, bool back, const void* x, int64_t ld_x
     CUtensorMap x_map;
     const cuuint64_t dims[2] = {(cuuint64_t)in, (cuuint64_t)T};
     const cuuint64_t strides[1] = {(cuuint64_t)ld_x};
-    const cuuint32_t box[2] = {128, 16};
-    if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
     const int wkb = (int)blocks_of(m->cols), wnb = (int)blocks_of(m->rows);
     Fp8Params p{};
     p.w_scales = m->scales;
@@ -172,6 +199,15 @@ int product(const char* what, qrm_fp8* m, bool back, const void* x, int64_t ld_x
     p.s_k = back ? wkb : 1;
     p.back = back;
     p.type = type;
+    const bool pair = m->form >= 0 ? m->form : pair_is_faster(T, m->groups, M, mb, kb, m->sms);
+    const cuuint32_t box[2] = {128, pair ? 128u : 16u};
+    if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
+    if (pair) {
+        const int wide_out = aligned(out, 32) && ld_out * b % 32 == 0, wide_xs = aligned(xs, 16) && ld_xs % 4 == 0;
+        fp8_pair_kernel<<<m->sms / 2 * 2, kFp8Warps * 32, pair_smem(m->groups), (cudaStream_t)stream>>>(
+            back ? m->pair_map_t : m->pair_map, x_map, p, wide_out, wide_xs);
+        return launched(what);
+    }
     const int x_rows = (int)std::min<int64_t>(kFp8MaxRows, (T + 15) / 16 * 16);
     fp8_stream_kernel<<<m->sms, kFp8Warps * 32, smem_for(m->groups, x_rows), (cudaStream_t)stream>>>(
         m->map, x_map, p, stages_for(m->groups, x_rows), x_rows);

@@ -47,6 +47,11 @@ __device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t wide_
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(wide_stride >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// The same with the 64-byte swizzle: 64 values a row, atoms of 512 bytes.
+__device__ __forceinline__ uint64_t sw64_desc_mn(uint32_t saddr, uint32_t wide_stride) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(wide_stride >> 4) << 16) | ((uint64_t)(512 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)4 << 61);
+}
 // Instruction descriptor of kind::f8f6f4: f32 accumulators, e4m3 A and B,
 // M = 128; a_mn / b_mn: the operand is contiguous along M / N, not K.
 __device__ __forceinline__ uint32_t umma_idesc_e4m3(int n, bool a_mn, bool b_mn) {
@@ -87,12 +92,36 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
 }
 
-__device__ __forceinline__ void store_typed(void* out, long long i, float v, int type) {
-    if (type == 0) reinterpret_cast<float*>(out)[i] = v;
-    else if (type == 1) reinterpret_cast<__half*>(out)[i] = __float2half_rn(v);
-    else reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+// 32 columns of this warp's 32 tensor-memory lanes, in two steps: the load goes
+// on while other work is done, and the wait names the registers, so nothing
+// that uses them can move before it (it waits for all loads of the warp)
+__device__ __forceinline__ void tmem_ld32_begin(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+          "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_end(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
 }
 
+template <typename T> __device__ __forceinline__ T round_to(float v);
+template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 // ------------------------------------------------------------ waits
 // A ready barrier costs one try_wait and a vote; the bounded loop is out of
 // line.  (The single-lane waits with an integer division for the ring's slot
@@ -111,7 +140,7 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
     const uint64_t t0 = global_ns(), lim = wait_limit_ns();
     bool ok = false;
     for (;;) {
@@ -172,6 +201,7 @@ constexpr int kFp8MaxRows = 128;        // rows of x in a tile
 constexpr int kFp8Acc = 4;              // accumulators in tensor memory
 constexpr int kFp8ScaleRing = 4;        // slots of four blocks' scales
 constexpr int kFp8MaxStages = 12;
+constexpr int kFp8MinRun = 4;           // blocks a CTA has at least
 constexpr int kFp8ScaleOff = 1024;                                       // after the barriers
 constexpr int kFp8ScaleSlot = 4 * kFp8MaxRows;                           // floats
 constexpr int kFp8TableOff = kFp8ScaleOff + kFp8ScaleRing * kFp8ScaleSlot * 4;
@@ -222,7 +252,9 @@ struct Fp8Plan {
 // The groups' tables in shared memory, by one warp; the caller synchronises.
 // Offsets that do not ascend within [0, T] make a group empty and raise an
 // error: no row outside x or out is ever touched.
-__device__ inline void fp8_tables(const Fp8Params& p, int32_t* first_tile, int32_t* start, int32_t* rows, bool report) {
+// tile_rows rows of x a tile, `across` tiles along the outputs.
+__device__ inline void fp8_tables(const Fp8Params& p, int32_t* first_tile, int32_t* start, int32_t* rows, int tile_rows,
+                                  int across, bool report) {
     const int lane = threadIdx.x & 31;
     int before = 0;
     bool bad = false;
@@ -237,7 +269,7 @@ __device__ inline void fp8_tables(const Fp8Params& p, int32_t* first_tile, int32
                 a = b = 0;
             }
         }
-        const int tiles = (b - a + kFp8MaxRows - 1) / kFp8MaxRows * p.mb;
+        const int tiles = (b - a + tile_rows - 1) / tile_rows * across;
         int scan = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -253,6 +285,34 @@ __device__ inline void fp8_tables(const Fp8Params& p, int32_t* first_tile, int32
     }
     if (lane == 0) first_tile[p.groups] = before;
     if (__any_sync(0xffffffffu, bad) && report && lane == 0) atomicOr(p.err, (int)ERR_BOUNDS);
+}
+
+// f(0) ... f(n - 1), n <= 64, by constant indices (the columns are registers),
+// 16 at a time: what is not needed is jumped over.  This code runs once or
+// twice in a launch, cold, and straight through all 64 it took 2.5 us for one.
+template <typename F>
+__device__ __forceinline__ void for_columns(int n, F f) {
+#pragma unroll
+    for (int h = 0; h < 4; h++) {
+        if (n <= 16 * h) return;
+#pragma unroll
+        for (int c = 0; c < 16; c++)
+            if (16 * h + c < n) f(16 * h + c);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_columns_as(T* to, long long ld, const float2 (&acc)[32], int n) {
+    for_columns(n, [&](int c) { to[c * ld] = round_to<T>(c & 1 ? acc[c >> 1].y : acc[c >> 1].x); });
+}
+// a warp's sums to out: lane_row is the output inside the tile, c0 the first of the n rows of x
+__device__ __forceinline__ void store_columns(const Fp8Params& p, const float2 (&acc)[32], const Fp8Piece& t, int c0, int n,
+                                              int lane_row) {
+    const int m = t.m * 128 + lane_row;
+    if (m >= p.M) return;
+    const long long o = (long long)(t.pos + c0) * p.ld_out + m;
+    if (p.type == 0) store_columns_as(reinterpret_cast<float*>(p.out) + o, p.ld_out, acc, n);
+    else if (p.type == 1) store_columns_as(reinterpret_cast<__half*>(p.out) + o, p.ld_out, acc, n);
+    else store_columns_as(reinterpret_cast<__nv_bfloat16*>(p.out) + o, p.ld_out, acc, n);
 }
 
 __global__ void __launch_bounds__(kFp8Warps * 32, 1)
@@ -292,7 +352,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
         fence_barrier_init();
     }
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
-    if (warp == 2) fp8_tables(p, first_tile, start, rows, blockIdx.x == 0);
+    if (warp == 2) fp8_tables(p, first_tile, start, rows, kFp8MaxRows, p.mb, blockIdx.x == 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -301,7 +361,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     const uint32_t full0 = smem_u32(full), done0 = smem_u32(done), acc_empty0 = smem_u32(acc_empty);
     const uint32_t sc_full0 = smem_u32(sc_full), sc_empty0 = smem_u32(sc_empty);
     Fp8Plan plan{first_tile, start, rows, p.groups, p.mb, p.kb, (long long)first_tile[p.groups] * p.kb, 0};
-    plan.ctas = (int)min((long long)gridDim.x, plan.total);   // each has a block at least
+    // a CTA has kFp8MinRun blocks at least, unless there are fewer in all
+    plan.ctas = (int)min((long long)gridDim.x, (plan.total + kFp8MinRun - 1) / kFp8MinRun);
     const bool idle = (int)blockIdx.x >= plan.ctas;
     const long long q0 = idle ? 0 : plan.cut(blockIdx.x), q1 = idle ? 0 : plan.cut(blockIdx.x + 1);
 
@@ -404,6 +465,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
         const int lane_row = 32 * (warp & 3) + lane;             // output inside the tile
         const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c0;
         bool ok = true;
+        const size_t slot = (size_t)x_rows * 128;   // floats of a part
         Ring r, a, sr;
         for (long long q = q0; q < q1 && ok;) {
             const Fp8Piece t = plan.piece(q, q1);
@@ -463,49 +525,64 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
                 if (last) sr.next(kFp8ScaleRing);
             }
             if (!ok) break;
-            const bool whole = t.k0 == 0 && t.k1 == p.kb;
-            bool mine = true;   // this warp writes the tile's sums out
-            if (!whole && n > 0) {
-                const long long tq = (long long)t.tile * p.kb;
-                const int c_first = plan.owner(tq), c_last = plan.owner(tq + p.kb - 1);
+            if (t.k0 == 0 && t.k1 == p.kb) {
+                store_columns(p, acc, t, c0, n, lane_row);
+            } else {
                 // slot 0: the CTA did not begin the tile; slot 1: it began and left it
-                const size_t slot = (size_t)x_rows * 128;
                 float* to = p.part + ((size_t)blockIdx.x * 2 + (t.k0 == 0 ? 1 : 0)) * slot + (size_t)c0 * 128 + lane_row;
+                for_columns(n, [&](int c) { __stcg(to + c * 128, c & 1 ? acc[c >> 1].y : acc[c >> 1].x); });
+            }
+            q += t.k1 - t.k0;
+        }
+        // Parts of tiles: the CTA's first and its last piece, if they are.  Both
+        // are announced here, when their stores have long landed, and not
+        // between the pieces, where the fence stopped the sums for 1.5 us.
+        __threadfence();
+        __syncwarp();
+#pragma unroll 1
+        for (int w = 0; w < 2 && ok && q0 < q1; w++) {
+            const int last_tile = (int)((q1 - 1) / p.kb);
+            if (w == 1 && (long long)last_tile * p.kb <= q0) break;   // one piece only
+            const Fp8Piece t = plan.piece(w == 0 ? q0 : (long long)last_tile * p.kb, q1);
+            const int n = t.n - c0;
+            if ((t.k0 == 0 && t.k1 == p.kb) || n <= 0) continue;
+            const long long tq = (long long)t.tile * p.kb;
+            const int c_first = plan.owner(tq), c_last = plan.owner(tq + p.kb - 1);
+            int arrived = 0;
+            if (lane == 0) arrived = atomicAdd(&p.arrivals[c_first * kFp8EpiWarps + e], 1);
+            arrived = __shfl_sync(0xffffffffu, arrived, 0);
+            if (arrived != c_last - c_first) continue;
+            // the last to arrive adds the parts up, in the CTAs' order
+            if (lane == 0) p.arrivals[c_first * kFp8EpiWarps + e] = 0;   // as the next launch finds it
+            __threadfence();
+            float2 acc[32];
 #pragma unroll
-                for (int c = 0; c < 64; c++)
-                    if (c < n) __stcg(to + c * 128, c & 1 ? acc[c >> 1].y : acc[c >> 1].x);
-                __threadfence();
-                __syncwarp();
-                int arrived = 0;
-                if (lane == 0) arrived = atomicAdd(&p.arrivals[c_first * kFp8EpiWarps + e], 1);
-                arrived = __shfl_sync(0xffffffffu, arrived, 0);
-                mine = arrived == c_last - c_first;
-                if (mine) {
-                    if (lane == 0) p.arrivals[c_first * kFp8EpiWarps + e] = 0;   // as the next launch finds it
-                    __threadfence();
+            for (int c = 0; c < 32; c++) acc[c] = make_float2(0.f, 0.f);
+            const float* from = p.part + (size_t)c0 * 128 + lane_row;
+#pragma unroll 1
+            for (int k = c_first; k <= c_last; k += 4) {   // of up to 16 columns, four parts' loads in flight
+                const float* part[4];
 #pragma unroll
-                    for (int c = 0; c < 32; c++) acc[c] = make_float2(0.f, 0.f);
-                    for (int k = c_first; k <= c_last; k++) {
-                        const float* from = p.part + ((size_t)k * 2 + (k == c_first ? 1 : 0)) * slot + (size_t)c0 * 128 + lane_row;
+                for (int u = 0; u < 4; u++) part[u] = from + ((size_t)min(k + u, c_last) * 2 + (k + u == c_first ? 1 : 0)) * slot;
 #pragma unroll
-                        for (int c = 0; c < 64; c++)
-                            if (c < n) {
-                                const float v = __ldcg(from + c * 128);
-                                if (c & 1) acc[c >> 1].y += v;
-                                else acc[c >> 1].x += v;
-                            }
-                    }
+                for (int h = 0; h < 4; h++) {
+                    if (n <= 16 * h) break;
+                    float v[4][16];
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int c = 0; c < 16; c++)
+                            v[u][c] = 16 * h + c < n && k + u <= c_last ? __ldcg(part[u] + (16 * h + c) * 128) : 0.f;
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int c = 0; c < 8; c++) {
+                            acc[8 * h + c].x += v[u][2 * c];
+                            acc[8 * h + c].y += v[u][2 * c + 1];
+                        }
                 }
             }
-            const int m = t.m * 128 + lane_row;
-            if (mine && m < p.M) {
-                const long long o = (long long)(t.pos + c0) * p.ld_out + m;
-#pragma unroll
-                for (int c = 0; c < 64; c++)
-                    if (c < n) store_typed(p.out, o + c * p.ld_out, c & 1 ? acc[c >> 1].y : acc[c >> 1].x, p.type);
-            }
-            __syncwarp();
-            q += t.k1 - t.k0;
+            store_columns(p, acc, t, c0, n, lane_row);
         }
     }
     // ---------------- teardown: every role is done (or gave up); free tensor memory
@@ -513,6 +590,371 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------ rows of x on the MMA's M side
+// For groups of many rows, which the tensor cores bound.  A pair of SMs
+// (cta_group::2) shares a tile of 256 rows of x times 256 outputs: each CTA
+// loads 128 rows of x and 128 outputs' weights for a block (32 KB) and the MMA
+// reads both halves of the weights, so a block costs each SM 64 bytes of L2
+// traffic a cycle at the full MMA rate, half of what a tile of its own would
+// cost.  A thread of the epilogue owns one row of x and 128 outputs (128 f32 in
+// registers): the two scales are one product for all 128.
+//
+// What bounds it is the way around an accumulator: MMAs, hand-over, the
+// epilogue's loads out of tensor memory, hand-over back.  So the tile's two
+// blocks of 128 outputs have MMAs, accumulators (two each) and epilogue warps
+// of their own, and take turns on the tensor cores.
+//
+// Warps: 0 loads tiles, 1 issues the MMAs (in the pair's first CTA), 2 brings
+// the scales, 4-11 add up: lane quarter (warp & 3), outputs 128 (warp >= 8).
+constexpr int kFp8PairStages = 6;
+constexpr int kFp8PairStage = 2 * kFp8Tile;   // rows of x, weights
+constexpr int kFp8PairAcc = 2;                // accumulators of 128 columns for each block of outputs
+constexpr int kFp8PairScaleSlot = 4 * 2 * 128;
+constexpr int kFp8PairScaleRing = 3;
+constexpr int kFp8PairTableOff = kFp8ScaleOff + kFp8PairScaleRing * kFp8PairScaleSlot * 4;
+__host__ __device__ inline int fp8_pair_stage_off(int groups) {
+    return (kFp8PairTableOff + 12 * (groups + 1) + 1023) / 1024 * 1024;
+}
+__device__ __forceinline__ uint32_t map_to_rank0(uint32_t addr) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+    return r;
+}
+// (What it hands over was read from tensor memory and is ordered by the
+// tcgen05 fence before it; with cluster scope here a full memory barrier came
+// with every block: 1010 us in place of REPLACE at 4096 x 28672 x 4096.)
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// loads of a pair's CTA that complete on a barrier of its first CTA
+__device__ __forceinline__ void tma_pair_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_pair_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4}], [%5];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// arrives on the barrier at `bar`'s offset in both CTAs once the MMAs are done
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+struct Fp8PairTile {
+    int group, n;    // matrix, first output
+    int pos, rows;   // first row of x of the tile, rows of the group from there on
+};
+
+__device__ __forceinline__ void store_32b(void* to, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+// 128 outputs of one row, 32 bytes at a time; `wide`: they start on 32 bytes.
+// (A warp writes 32 rows at once, so what counts is how few stores a row takes.)
+template <typename T>
+__device__ __forceinline__ void store_row(T* out, int left, const float2 (&acc)[64], bool wide) {
+    constexpr int V = 32 / sizeof(T);   // values of one store
+#pragma unroll
+    for (int c = 0; c < 128 / V; c++) {
+        if (wide && V * c + V <= left) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if constexpr (sizeof(T) == 4) {
+                    const float2 v = acc[4 * c + i / 2];
+                    w[i] = __float_as_uint(i & 1 ? v.y : v.x);
+                } else {
+                    const T h[2] = {round_to<T>(acc[8 * c + i].x), round_to<T>(acc[8 * c + i].y)};
+                    memcpy(&w[i], h, 4);
+                }
+            }
+            store_32b(out + V * c, w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; i++) {
+                const float2 v = acc[V / 2 * c + i];
+                if (V * c + 2 * i < left) out[V * c + 2 * i] = round_to<T>(v.x);
+                if (V * c + 2 * i + 1 < left) out[V * c + 2 * i + 1] = round_to<T>(v.y);
+            }
+        }
+        asm volatile("" ::: "memory");   // one store's registers at a time
+    }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8Warps * 32, 1)
+fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, Fp8Params p,
+                int wide_out, int wide_xs) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm);
+    uint64_t* full = bars;                            // first CTA: both CTAs' tiles are there
+    uint64_t* done = full + kFp8PairStages;           // both: the stage's MMAs are done
+    uint64_t* done_first = done + kFp8PairStages;     // both: those of its first block of outputs
+    uint64_t* acc_empty = done_first + kFp8PairStages;   // first CTA: both epilogues have read; [block of outputs][acc]
+    uint64_t* sc_full = acc_empty + 2 * kFp8PairAcc;
+    uint64_t* sc_empty = sc_full + kFp8PairScaleRing;
+    uint64_t* done_bar = sc_empty + kFp8PairScaleRing;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + 768);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 776);
+    float* sc_ring = reinterpret_cast<float*>(sm + kFp8ScaleOff);
+    int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp8PairTableOff);
+    int32_t* start = first_tile + p.groups + 1;
+    int32_t* rows = start + p.groups + 1;
+    uint8_t* ring = sm + fp8_pair_stage_off(p.groups);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & 1;   // in the pair: the cluster is two CTAs along x
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kFp8PairStages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&done[i], 1);
+            mbar_init(&done_first[i], 1);
+        }
+        for (int i = 0; i < 2 * kFp8PairAcc; i++) mbar_init(&acc_empty[i], kFp8EpiWarps);
+        for (int i = 0; i < kFp8PairScaleRing; i++) {
+            mbar_init(&sc_full[i], 1);
+            mbar_init(&sc_empty[i], kFp8EpiWarps);
+        }
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    if (warp == 2) fp8_tables(p, first_tile, start, rows, 256, (p.M + 255) / 256, blockIdx.x == 0);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();   // the peer's barriers are ready
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const Fp8Ctl ctl{abort_flag, p.err};
+    const uint32_t done0 = smem_u32(done), sc_full0 = smem_u32(sc_full), sc_empty0 = smem_u32(sc_empty);
+    const int tiles = first_tile[p.groups], pairs = gridDim.x >> 1, KB = p.kb;
+
+    // tile number -> what this CTA does of it; the tiles of one block of
+    // outputs follow each other, so its weights come from HBM once
+    auto tile_at = [&](int i) {
+        int lo = 0, hi = p.groups;   // the last group with first_tile <= i has rows
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first_tile[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        const int blocks = (rows[lo] + 255) >> 8, in = i - first_tile[lo];
+        const int n = in / blocks, at = (in - n * blocks) * 256 + 128 * (int)rank;
+        return Fp8PairTile{lo, n * 256, start[lo] + at, rows[lo] - at};
+    };
+
+    if (warp < kFp8EpiWarp0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            // -------------------------------------------- tiles
+            bool ok = true;
+            Ring r;
+            uint32_t issued = 0;
+            const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
+                const Fp8PairTile t = tile_at(i);
+                const int n = t.n + 64 * (int)rank;   // half of each block of outputs
+                for (int kb = 0; kb < KB; kb++) {
+                    if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                    if (elect_one()) {
+                        const uint32_t st = ring0 + r.i * kFp8PairStage, bar = full0 + 8 * r.i;
+                        if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * kFp8PairStage);
+                        tma_pair_2d(st, &x_map, kb * 128, t.pos, bar);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const uint32_t to = st + kFp8Tile + h * (kFp8Tile / 2);
+                            if (p.back) tma_pair_3d(to, &w_map, n + 128 * h, kb * 128, t.group, bar);
+                            else tma_pair_3d(to, &w_map, kb * 128, n + 128 * h, t.group, bar);
+                        }
+                    }
+                    __syncwarp();
+                    r.next(kFp8PairStages);
+                    issued++;
+                }
+            }
+            // copies already issued must land before the CTAs exit (both CTAs' complete on the first's barriers)
+            if (!ok && rank == 0 && lane == 0)
+                for (uint32_t j = issued > (uint32_t)kFp8PairStages ? issued - kFp8PairStages : 0; j < issued; j++)
+                    mbar_wait(&full[j % kFp8PairStages], (j / kFp8PairStages) & 1u);
+        } else if (warp == 1 && rank == 0) {
+            // -------------------------------------------- MMAs (one thread issues for both CTAs)
+            bool ok = true;
+            Ring r, a;
+            const uint32_t full0 = smem_u32(full), acc_empty0 = smem_u32(acc_empty), ring0 = smem_u32(ring);
+            const uint32_t done_first0 = smem_u32(done_first);
+            // (along N: rows of 64 values, half of a block of outputs, 32 of them contracted by one MMA)
+            const uint32_t step = p.back ? 2048 >> 4 : 32 >> 4;
+            const uint64_t x_desc = sw128_desc(ring0);
+            const uint64_t w_desc = p.back ? sw64_desc_mn(ring0 + kFp8Tile, kFp8Tile / 2) : sw128_desc(ring0 + kFp8Tile);
+            const uint32_t idesc = (umma_idesc_e4m3(128, false, p.back) & ~(0x1Fu << 24)) | ((uint32_t)(256 >> 4) << 24);
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
+                for (int kb = 0; kb < KB; kb++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (!bar_wait(acc_empty0 + 8 * (kFp8PairAcc * h + a.i), a.phase ^ 1u, ctl) ||
+                            (h == 0 && !bar_wait(full0 + 8 * r.i, r.phase, ctl))) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        if (elect_one()) {
+                            const uint32_t at = r.i * (kFp8PairStage >> 4), d = tmem + 128 * (kFp8PairAcc * h + a.i);
+                            const uint64_t xd = x_desc + at, wd = w_desc + at + h * (kFp8Tile / 2 >> 4);
+                            umma_f8_pair(d, xd, wd, idesc, 0u);
+                            umma_f8_pair(d, xd + 2, wd + step, idesc, 1u);
+                            umma_f8_pair(d, xd + 4, wd + 2 * step, idesc, 1u);
+                            umma_f8_pair(d, xd + 6, wd + 3 * step, idesc, 1u);
+                            umma_commit_pair((h == 0 ? done_first0 : done0) + 8 * r.i);
+                        }
+                        __syncwarp();
+                    }
+                    if (!ok) break;
+                    r.next(kFp8PairStages);
+                    a.next(kFp8PairAcc);
+                }
+            }
+            // every MMA has completed before tensor memory is released
+            if (elect_one()) {
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done_bar)) : "memory");
+                mbar_wait(done_bar, 0u);
+            }
+            __syncwarp();
+        } else if (warp == 2) {
+            // -------------------------------------------- scales: sx sw of 128 rows x two blocks of outputs
+            bool ok = true;
+            Ring r;
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
+                const Fp8PairTile t = tile_at(i);
+                const int m = t.n >> 7, m1 = min(m + 1, p.mb - 1);   // an absent second block is not stored
+                const float* ws = p.w_scales + (long long)t.group * p.s_group;
+                const float* xs = p.x_scales + (long long)t.pos * p.ld_xs;
+                for (int k4 = 0; k4 < KB; k4 += 4) {
+                    float v[4][4], w[4][2];   // [row lane + 32 c][block j]
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int kb = k4 + j;
+                        w[j][0] = kb < KB ? __ldg(ws + (long long)m * p.s_m + (long long)kb * p.s_k) : 0.f;
+                        w[j][1] = kb < KB ? __ldg(ws + (long long)m1 * p.s_m + (long long)kb * p.s_k) : 0.f;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const bool in = lane + 32 * c < t.rows;
+                        const float* from = xs + (long long)(lane + 32 * c) * p.ld_xs + k4;
+                        if (wide_xs && k4 + 4 <= KB) {
+                            const float4 f = in ? __ldg(reinterpret_cast<const float4*>(from)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            v[c][0] = f.x; v[c][1] = f.y; v[c][2] = f.z; v[c][3] = f.w;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) v[c][j] = in && k4 + j < KB ? __ldg(from + j) : 0.f;
+                        }
+                    }
+                    if (!bar_wait(sc_empty0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                    float* to = sc_ring + r.i * kFp8PairScaleSlot + lane;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            to[j * 256 + 32 * c] = v[c][j] * w[j][0];
+                            to[j * 256 + 128 + 32 * c] = v[c][j] * w[j][1];
+                        }
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(sc_full0 + 8 * r.i);
+                    r.next(kFp8PairScaleRing);
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------ sums over the blocks
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int half = (warp - kFp8EpiWarp0) >> 2, row = 32 * (warp & 3) + lane;   // block of outputs, row of x in the tile
+        const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * kFp8PairAcc * half;
+        const uint32_t acc_empty0 = map_to_rank0(smem_u32(acc_empty + kFp8PairAcc * half));
+        const uint32_t ready0 = half ? done0 : smem_u32(done_first);
+        bool ok = true;
+        Ring r, a, sr;
+        for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
+            const Fp8PairTile t = tile_at(i);
+            float2 acc[64];
+#pragma unroll
+            for (int c = 0; c < 64; c++) acc[c] = make_float2(0.f, 0.f);
+            for (int kb = 0; kb < KB; kb++) {
+                const int j = kb & 3;
+                if ((j == 0 && !bar_wait(sc_full0 + 8 * sr.i, sr.phase, ctl)) || !bar_wait(ready0 + 8 * r.i, r.phase, ctl)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const float f = sc_ring[sr.i * kFp8PairScaleSlot + j * 256 + 128 * half + row];
+                const float2 f2 = make_float2(f, f);
+                const uint32_t from = taddr + 128 * a.i;
+                uint32_t v[2][32];
+                tmem_ld32_begin(from, v[0]);
+#pragma unroll
+                for (int h = 0; h < 4; h++) {
+                    tmem_ld32_end(v[h & 1]);
+                    if (h < 3) {
+                        tmem_ld32_begin(from + 32 * (h + 1), v[(h + 1) & 1]);
+                    } else {   // all of it is in registers
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive_cluster(acc_empty0 + 8 * a.i);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 16; c++)
+                        acc[16 * h + c] = ffma2(make_float2(__uint_as_float(v[h & 1][2 * c]), __uint_as_float(v[h & 1][2 * c + 1])), f2,
+                                                acc[16 * h + c]);
+                }
+                if (j == 3 || kb + 1 == KB) {
+                    if (lane == 0) bar_arrive(sc_empty0 + 8 * sr.i);
+                    sr.next(kFp8PairScaleRing);
+                }
+                r.next(kFp8PairStages);
+                a.next(kFp8PairAcc);
+            }
+            if (!ok) break;
+            if (row < t.rows) {
+                const long long o = (long long)(t.pos + row) * p.ld_out + t.n + 128 * half;
+                const int left = p.M - t.n - 128 * half;
+                if (p.type == 0) store_row(reinterpret_cast<float*>(p.out) + o, left, acc, wide_out);
+                else if (p.type == 1) store_row(reinterpret_cast<__half*>(p.out) + o, left, acc, wide_out);
+                else store_row(reinterpret_cast<__nv_bfloat16*>(p.out) + o, left, acc, wide_out);
+            }
+            __syncwarp();
+        }
+    }
+    // ---------------- teardown: every role of both CTAs is done (or gave up); free tensor memory
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 }  // namespace qrm

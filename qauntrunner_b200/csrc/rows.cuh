@@ -12,9 +12,13 @@
 // 8-bit rows: for each block of 128 columns scale = max(amax / 448, 2^-126),
 // code = e4m3(v / scale), round to nearest even.  448 is e4m3's largest
 // number, so no code saturates.  The lower bound keeps the scale of a block of
-// zeros (or of denormals) a normal number.  A NaN in a block makes its scale
-// NaN, an infinity makes it infinite: either way the whole block stands for
-// NaN, and its neighbours are untouched.
+// zeros (or of denormals) a normal number.  A NaN or an infinity in a block
+// makes its scale NaN: the whole block stands for NaN, and its neighbours are
+// untouched.
+//
+// Both divisions are a product with the rounded reciprocal and one correction
+// by the exact remainder (Markstein's theorem: rounded like the division), 3
+// operations a value in place of some 10 with a branch.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -42,31 +46,43 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// Eight columns as they are stored: what a thread keeps of a load in flight.
+template <typename T>
+struct Raw8 {
+    uint32_t w[2 * sizeof(T)];
+};
+
 // the n <= 8 columns at p (the others are 0); `wide`: p is on a 16-byte boundary
 template <typename T>
-__device__ __forceinline__ Vec8 load8(const T* __restrict__ p, int n, bool wide) {
-    Vec8 r;
+__device__ __forceinline__ Raw8<T> load_raw8(const T* __restrict__ p, int n, bool wide) {
+    Raw8<T> r;
     if (wide && n == 8) {
-        if constexpr (sizeof(T) == 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-            const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-            r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w;
-            r.v[4] = b.x; r.v[5] = b.y; r.v[6] = b.z; r.v[7] = b.w;
-        } else {
-            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                T h[2];
-                memcpy(h, &w[i], 4);
-                r.v[2 * i] = to_f32(h[0]);
-                r.v[2 * i + 1] = to_f32(h[1]);
-            }
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            r.w[4 * i] = a.x; r.w[4 * i + 1] = a.y; r.w[4 * i + 2] = a.z; r.w[4 * i + 3] = a.w;
         }
     } else {
+        T h[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) r.v[i] = i < n ? to_f32(p[i]) : 0.f;
+        for (int i = 0; i < 8; i++) h[i] = i < n ? p[i] : from_f32<T>(0.f);
+        memcpy(r.w, h, sizeof h);
     }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float column(const Raw8<T>& r, int i) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[i]);
+    T h[2];
+    memcpy(h, &r.w[i / 2], 4);
+    return to_f32(h[i & 1]);
+}
+template <typename T>
+__device__ __forceinline__ Vec8 load8(const T* __restrict__ p, int n, bool wide) {
+    const Raw8<T> raw = load_raw8(p, n, wide);
+    Vec8 r;
+#pragma unroll
+    for (int i = 0; i < 8; i++) r.v[i] = column(raw, i);
     return r;
 }
 
@@ -100,30 +116,40 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-__device__ __forceinline__ float block_scale(float amax) { return max_nan(amax / kFp8Max, kFp8MinScale); }
+// v / s given r = 1 / s, both rounded (in this order a zero keeps its sign)
+__device__ __forceinline__ float divided(float v, float s, float r) {
+    const float q = v * r;
+    return fmaf(-fmaf(q, s, -v), r, q);
+}
+__device__ __forceinline__ float block_scale(float amax) {
+    return max_nan(divided(amax, kFp8Max, 1.f / kFp8Max), kFp8MinScale);
+}
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
 
-// The scale of the block that this half warp's 16 threads hold (8 columns
-// each), in every one of them.  All 32 lanes take part.
-__device__ __forceinline__ float half_warp_scale(const Vec8& r) {
+// The largest magnitude of the block that this half warp's 16 threads hold (8
+// columns each), in every one of them.  All 32 lanes take part.
+__device__ __forceinline__ float half_warp_amax(const Vec8& r) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) m = max_nan(m, fabsf(r.v[i]));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return block_scale(m);
+    return m;
 }
+__device__ __forceinline__ float half_warp_scale(const Vec8& r) { return block_scale(half_warp_amax(r)); }
 
-__device__ __forceinline__ uint2 codes8(const Vec8& r, float scale) {
+// r = 1 / scale
+__device__ __forceinline__ uint2 codes8(const Vec8& v, float scale, float r) {
     uint32_t c[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) c[i] = e4m3x2(r.v[2 * i] / scale, r.v[2 * i + 1] / scale);
+    for (int i = 0; i < 4; i++) c[i] = e4m3x2(divided(v.v[2 * i], scale, r), divided(v.v[2 * i + 1], scale, r));
     return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
+__device__ __forceinline__ uint2 codes8(const Vec8& v, float scale) { return codes8(v, scale, 1.f / scale); }
 
 __device__ __forceinline__ void store_codes8(uint8_t* __restrict__ p, uint2 c, int n, bool wide) {
     if (wide && n == 8) {
@@ -311,6 +337,7 @@ __global__ void combine_rows_kernel(const T* __restrict__ rows, long long ld_row
                                     const int32_t* __restrict__ pos, const float* __restrict__ w, long long T_, int k,
                                     long long d, int segments, const T* __restrict__ add, long long ld_add,
                                     T* __restrict__ out, long long ld_out, bool wide) {
+    constexpr int S = sizeof(T) == 4 ? 4 : 8;   // rows at a time: 32 registers
     for (long long u = blockIdx.x; u < T_ * segments; u += gridDim.x) {
         const long long t = u / segments;
         const long long c = ((u - t * segments) * blockDim.x + threadIdx.x) * 8;
@@ -321,24 +348,24 @@ __global__ void combine_rows_kernel(const T* __restrict__ rows, long long ld_row
         else
 #pragma unroll
             for (int i = 0; i < 8; i++) acc.v[i] = 0.f;
-        for (int j0 = 0; j0 < k; j0 += 4) {   // four rows' loads in flight
-            Vec8 r[4];
-            float wj[4];
-            bool held[4];
+        for (int j0 = 0; j0 < k; j0 += S) {   // their loads in flight together
+            Raw8<T> r[S];
+            float wj[S];
+            uint32_t held = 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const long long p = j0 + j < k ? pos[t * k + j0 + j] : -1;
-                held[j] = p >= 0 && p < n_rows;
-                if (held[j]) {
-                    r[j] = load8(rows + p * ld_rows + c, n, wide);
-                    wj[j] = w ? w[t * k + j0 + j] : 1.f;
-                }
+            for (int j = 0; j < S; j++) {
+                if (j0 + j >= k) break;
+                const long long p = pos[t * k + j0 + j];
+                if (p < 0 || p >= n_rows) continue;
+                held |= 1u << j;
+                r[j] = load_raw8(rows + p * ld_rows + c, n, wide);
+                wj[j] = w ? w[t * k + j0 + j] : 1.f;
             }
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (held[j])
+            for (int j = 0; j < S; j++)
+                if (held >> j & 1)
 #pragma unroll
-                    for (int i = 0; i < 8; i++) acc.v[i] = fmaf(wj[j], r[j].v[i], acc.v[i]);
+                    for (int i = 0; i < 8; i++) acc.v[i] = fmaf(wj[j], column(r[j], i), acc.v[i]);
         }
         store8(out + t * ld_out + c, acc, n, wide);
     }
@@ -347,20 +374,24 @@ __global__ void combine_rows_kernel(const T* __restrict__ rows, long long ld_row
 // The gradient of combine_rows: drows[pos[t, j]] = w[t, j] dout[t] (T or 8
 // bits) and dw[t, j] = <dout[t], rows[pos[t, j]]>.  One CTA per token: dw
 // needs the whole row.  Eight slots at a time, whose sums stay in registers.
+// Rounding does not change an order, so the largest magnitude of w dout is the
+// rounded product of |w| and dout's: it is looked for once for all slots, and
+// the eight slots' scales and reciprocals are computed by eight lanes of the
+// half warp, one each, and handed round.
 template <typename T, bool FP8>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(512, 2)
 combine_grad_kernel(const T* __restrict__ dout, long long ld_dout, const T* __restrict__ rows,
                                     long long ld_rows, long long n_rows, const int32_t* __restrict__ pos,
                                     const float* __restrict__ w, long long T_, int k, long long d, T* __restrict__ drows,
                                     uint8_t* __restrict__ codes, long long ld_d, float* __restrict__ scales,
                                     long long ld_s, float* __restrict__ dw, bool wide, bool wide_d) {
-    constexpr int S = 8;
+    constexpr int S = 8, B = sizeof(T) == 4 ? 2 : 4;   // slots; rows' loads in flight
     __shared__ float part[S][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     for (long long t = blockIdx.x; t < T_; t += gridDim.x) {
         for (int j0 = 0; j0 < k; j0 += S) {
             float dot[S];
-            long long p[S];
+            int p[S];
             float wj[S];
 #pragma unroll
             for (int j = 0; j < S; j++) {
@@ -370,32 +401,46 @@ combine_grad_kernel(const T* __restrict__ dout, long long ld_dout, const T* __re
                 if (p[j] >= n_rows) p[j] = -1;
                 if (p[j] >= 0) wj[j] = w ? w[t * k + j0 + j] : 1.f;
             }
+            float w_lane = 0.f;   // slot lane & 7
+            if (FP8)
+#pragma unroll
+                for (int j = 0; j < S; j++)
+                    if ((lane & 7) == j) w_lane = fabsf(wj[j]);
             for (long long c0 = 0; c0 < d; c0 += (long long)blockDim.x * 8) {
                 const long long c = c0 + threadIdx.x * 8;
                 const int n = columns_at(c, d);
                 const Vec8 g = load8(dout + t * ld_dout + c, n, wide);
-                Vec8 r[S];
-                if (dw)
+                float s_lane = 0.f, r_lane = 0.f;
 #pragma unroll
-                    for (int j = 0; j < S; j++)
-                        if (p[j] >= 0) r[j] = load8(rows + p[j] * ld_rows + c, n, wide);
-#pragma unroll
-                for (int j = 0; j < S; j++) {
-                    if (p[j] < 0) continue;   // the same for all threads of the CTA
+                for (int jb = 0; jb < S; jb += B) {
+                    Raw8<T> r[B];
                     if (dw)
 #pragma unroll
-                        for (int i = 0; i < 8; i++) dot[j] = fmaf(g.v[i], r[j].v[i], dot[j]);
-                    Vec8 v;
+                        for (int j = 0; j < B; j++)
+                            if (p[jb + j] >= 0) r[j] = load_raw8(rows + p[jb + j] * ld_rows + c, n, wide);
+                    if (FP8 && jb == 0) {
+                        s_lane = block_scale(__fmul_rn(w_lane, half_warp_amax(g)));
+                        r_lane = 1.f / s_lane;
+                    }
 #pragma unroll
-                    for (int i = 0; i < 8; i++) v.v[i] = __fmul_rn(wj[j], g.v[i]);
-                    if constexpr (FP8) {
-                        const float s = half_warp_scale(v);
-                        if (n) {
-                            store_codes8(codes + p[j] * ld_d + c, codes8(v, s), n, wide_d);
-                            if ((threadIdx.x & 15) == 0) scales[p[j] * ld_s + c / kFp8Block] = s;
+                    for (int u = 0; u < B; u++) {
+                        const int j = jb + u;
+                        if (p[j] < 0) continue;   // the same for all threads of the CTA
+                        Vec8 v;
+#pragma unroll
+                        for (int i = 0; i < 8; i++) v.v[i] = __fmul_rn(wj[j], g.v[i]);
+                        if constexpr (FP8) {
+                            const float s = __shfl_sync(0xffffffffu, s_lane, j, 16), q = __shfl_sync(0xffffffffu, r_lane, j, 16);
+                            if (n) {
+                                store_codes8(codes + p[j] * ld_d + c, codes8(v, s, q), n, wide_d);
+                                if ((threadIdx.x & 15) == 0) scales[p[j] * ld_s + c / kFp8Block] = s;
+                            }
+                        } else if (n) {
+                            store8(drows + p[j] * ld_d + c, v, n, wide_d);
                         }
-                    } else if (n) {
-                        store8(drows + p[j] * ld_d + c, v, n, wide_d);
+                        if (dw)
+#pragma unroll
+                            for (int i = 0; i < 8; i++) dot[j] = fmaf(g.v[i], column(r[u], i), dot[j]);
                     }
                 }
             }
@@ -495,7 +540,7 @@ __device__ __forceinline__ Swiglu swiglu_parts(float gate, float up, float limit
         if (!r.u_in) r.u = copysignf(limit, up);
     }
     const float e = expf(-fabsf(r.g));   // never overflows
-    r.sig = (r.g < 0.f ? e : 1.f) / (1.f + e);
+    r.sig = __fdividef(r.g < 0.f ? e : 1.f, 1.f + e);   // the divisor is in [1, 2]: within 2 ulp
     return r;
 }
 
