@@ -9,24 +9,25 @@
 namespace qrm {
 namespace {
 
-// Columns to CTAs: eight columns a thread, at most 256 threads, the threads
-// spread evenly over the segments a row is cut into (d = 7168: 4 x 224).
+// Columns to threads, `each` of them in one, in whole blocks of 128; at most
+// 256 threads a CTA, spread evenly over the pieces that a row is cut into
+// (7168 columns: 4 x 224 threads of 8, 2 x 224 threads of 16).
 struct Cut {
-    int threads, segments;
+    int threads;
+    dim3 grid;
 };
-Cut cut_columns(int64_t cols, int64_t whole) {
-    const int64_t lanes = (cols + whole - 1) / whole * (whole / 8);
-    const int64_t segments = (lanes + 255) / 256;
-    const int64_t threads = ((lanes + segments - 1) / segments + 31) / 32 * 32;
-    return {(int)threads, (int)segments};
+Cut cut_columns(int64_t rows, int64_t cols, int each) {
+    const int64_t lanes = (cols + kFp8Block - 1) / kFp8Block * (kFp8Block / each);
+    const int64_t pieces = (lanes + 255) / 256;
+    const int64_t threads = ((lanes + pieces - 1) / pieces + 31) / 32 * 32;
+    return {(int)threads, dim3((unsigned)rows, (unsigned)pieces)};
 }
-// one unit a CTA; the kernels stride over what a grid cannot hold
-int grid_of(int64_t units) { return (int)std::min<int64_t>(units, 1 << 24); }
 
 bool wide_rows(const void* p, int64_t ld, int bytes) { return aligned(p, 16) && ld * bytes % 16 == 0; }
 bool wide_codes(const void* p, int64_t ld) { return aligned(p, 8) && ld % 8 == 0; }
+bool wide_codes16(const void* p, int64_t ld) { return aligned(p, 16) && ld % 16 == 0; }
 
-constexpr int64_t kMaxCols = 1 << 24;   // columns of a row
+constexpr int64_t kMaxCols = 1 << 24;   // columns of a row (a grid's y holds its pieces)
 
 int check_rows(const char* what, int type, int64_t rows, int64_t cols) {
     if (!type_bytes(type)) return failf(QRM_E_FORMAT, "%s: type %d is not F32, F16 or BF16", what, type);
@@ -128,10 +129,10 @@ extern "C" int qrm_gather_rows(int type, const void* x_dev, int64_t ld_x, const 
     TRY(check_ints(what, "pos", pos_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(d, 8);
+    const Cut c = cut_columns(T, d, 8);
     const bool wide = wide_rows(x_dev, ld_x, b) && wide_rows(rows_dev, ld_rows, b);
-    BY_TYPE(type, gather_rows_kernel<V><<<grid_of(T * c.segments), c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)x_dev, ld_x, pos_dev, T, k, d, c.segments, n_rows, (V*)rows_dev, ld_rows, wide));
+    BY_TYPE(type, gather_rows_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
+                      (const V*)x_dev, ld_x, pos_dev, k, (int)d, (uint32_t)n_rows, (V*)rows_dev, ld_rows, wide));
     return launched(what);
 }
 
@@ -149,10 +150,10 @@ extern "C" int qrm_gather_rows_fp8(int type, const void* x_dev, int64_t ld_x, co
     TRY(check_ints(what, "pos", pos_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(d, kFp8Block);
-    BY_TYPE(type, gather_rows_fp8_kernel<V><<<grid_of(T * c.segments), c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)x_dev, ld_x, pos_dev, T, k, d, c.segments, n_rows, codes_dev, ld_codes, scales_dev,
-                      ld_scales, wide_rows(x_dev, ld_x, b), wide_codes(codes_dev, ld_codes)));
+    const Cut c = cut_columns(T, d, 16);
+    BY_TYPE(type, gather_rows_fp8_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
+                      (const V*)x_dev, ld_x, pos_dev, k, (int)d, (uint32_t)n_rows, codes_dev, ld_codes, scales_dev,
+                      ld_scales, wide_rows(x_dev, ld_x, b), wide_codes16(codes_dev, ld_codes)));
     return launched(what);
 }
 
@@ -171,11 +172,11 @@ extern "C" int qrm_combine_rows(int type, const void* rows_dev, int64_t n_rows, 
     if (w_dev) TRY(check_ints(what, "w", w_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(d, 8);
+    const Cut c = cut_columns(T, d, 8);
     const bool wide = wide_rows(rows_dev, ld_rows, b) && wide_rows(out_dev, ld_out, b) &&
                       (!add_dev || wide_rows(add_dev, ld_add, b));
-    BY_TYPE(type, combine_rows_kernel<V><<<grid_of(T * c.segments), c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)rows_dev, ld_rows, n_rows, pos_dev, w_dev, T, k, d, c.segments, (const V*)add_dev, ld_add,
+    BY_TYPE(type, combine_rows_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
+                      (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, k, (int)d, (const V*)add_dev, ld_add,
                       (V*)out_dev, ld_out, wide));
     return launched(what);
 }
@@ -210,12 +211,12 @@ static int combine_grad(const char* what, int type, const void* dout_dev, int64_
     const bool wide = wide_rows(dout_dev, ld_dout, b) && (!dw_dev || wide_rows(rows_dev, ld_rows, b));
     const cudaStream_t s = (cudaStream_t)stream;
     if (fp8)
-        BY_TYPE(type, combine_grad_kernel<V, true><<<grid_of(T), threads, 0, s>>>(
-                          (const V*)dout_dev, ld_dout, (const V*)rows_dev, ld_rows, n_rows, pos_dev, w_dev, T, k, d,
+        BY_TYPE(type, combine_grad_kernel<V, true><<<(unsigned)T, threads, 0, s>>>(
+                          (const V*)dout_dev, ld_dout, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, k, (int)d,
                           (V*)nullptr, codes_dev, ld_d, scales_dev, ld_scales, dw_dev, wide, wide_codes(codes_dev, ld_d)));
     else
-        BY_TYPE(type, combine_grad_kernel<V, false><<<grid_of(T), threads, 0, s>>>(
-                          (const V*)dout_dev, ld_dout, (const V*)rows_dev, ld_rows, n_rows, pos_dev, w_dev, T, k, d,
+        BY_TYPE(type, combine_grad_kernel<V, false><<<(unsigned)T, threads, 0, s>>>(
+                          (const V*)dout_dev, ld_dout, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, k, (int)d,
                           (V*)drows_dev, nullptr, ld_d, nullptr, 0, dw_dev, wide, wide_rows(drows_dev, ld_d, b)));
     return launched(what);
 }
@@ -249,10 +250,10 @@ extern "C" int qrm_quantize_fp8(int type, const void* x_dev, int64_t ld_x, int64
     if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(cols, kFp8Block);
-    BY_TYPE(type, quantize_fp8_kernel<V><<<grid_of(rows * c.segments), c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)x_dev, ld_x, rows, n_rows_dev, cols, c.segments, codes_dev, ld_codes, scales_dev, ld_scales,
-                      wide_rows(x_dev, ld_x, b), wide_codes(codes_dev, ld_codes)));
+    const Cut c = cut_columns(rows, cols, 16);
+    BY_TYPE(type, quantize_fp8_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
+                      (const V*)x_dev, ld_x, n_rows_dev, (int)cols, codes_dev, ld_codes, scales_dev, ld_scales,
+                      wide_rows(x_dev, ld_x, b), wide_codes16(codes_dev, ld_codes)));
     return launched(what);
 }
 
@@ -271,7 +272,7 @@ extern "C" int qrm_quantize_fp8_weights(int type, const void* w_dev, int groups,
     TRY(current_device(&device, &sms));
     const dim3 grid((unsigned)blocks_of(cols), (unsigned)blocks_of(rows), (unsigned)groups);
     const bool wide = wide_rows(w_dev, cols, b) && wide_codes(codes_dev, cols);
-    BY_TYPE(type, quantize_fp8_weights_kernel<V><<<grid, 256, 0, (cudaStream_t)stream>>>((const V*)w_dev, rows, cols,
+    BY_TYPE(type, quantize_fp8_weights_kernel<V><<<grid, 256, 0, (cudaStream_t)stream>>>((const V*)w_dev, (int)rows, (int)cols,
                                                                                          codes_dev, scales_dev, wide));
     return launched(what);
 }
@@ -294,10 +295,10 @@ extern "C" int qrm_swiglu_fp8(int type, const void* gu_dev, int64_t ld_gu, int64
     if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(f, kFp8Block);
+    const Cut c = cut_columns(rows, f, 8);
     const bool wide = wide_rows(gu_dev, ld_gu, b) && f * b % 16 == 0;
-    BY_TYPE(type, swiglu_fp8_kernel<V><<<grid_of(rows * c.segments), c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)gu_dev, ld_gu, rows, n_rows_dev, f, c.segments, limit, codes_dev, ld_codes, scales_dev,
+    BY_TYPE(type, swiglu_fp8_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
+                      (const V*)gu_dev, ld_gu, n_rows_dev, (int)f, limit, codes_dev, ld_codes, scales_dev,
                       ld_scales, wide, wide_codes(codes_dev, ld_codes)));
     return launched(what);
 }
@@ -320,10 +321,10 @@ extern "C" int qrm_swiglu_fp8_grad(int type, const void* gu_dev, int64_t ld_gu, 
     if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(f, kFp8Block);
+    const Cut c = cut_columns(rows, f, 8);
     const bool wide = wide_rows(gu_dev, ld_gu, b) && wide_rows(dh_dev, ld_dh, b);
-    BY_TYPE(type, swiglu_fp8_grad_kernel<V><<<grid_of(rows * c.segments), c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, rows, n_rows_dev, f, c.segments, limit, codes_dev,
-                      ld_codes, scales_dev, ld_scales, wide, wide_codes(codes_dev, ld_codes)));
+    BY_TYPE(type, swiglu_fp8_grad_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
+                      (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, n_rows_dev, (int)f, limit, codes_dev, ld_codes,
+                      scales_dev, ld_scales, wide, wide_codes(codes_dev, ld_codes)));
     return launched(what);
 }

@@ -18,7 +18,7 @@
 //
 // Both divisions are a product with the rounded reciprocal and one correction
 // by the exact remainder (Markstein's theorem: rounded like the division), 3
-// operations a value in place of some 10 with a branch.
+// operations for two values in place of some 20 with branches.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -110,19 +110,45 @@ __device__ __forceinline__ void store8(T* __restrict__ p, const Vec8& r, int n, 
 
 // ------------------------------------------------------------ 8-bit blocks
 
-// max that keeps a NaN
+// largest magnitude; a NaN stays one
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// v / s given r = 1 / s, both rounded (in this order a zero keeps its sign)
-__device__ __forceinline__ float divided(float v, float s, float r) {
-    const float q = v * r;
-    return fmaf(-fmaf(q, s, -v), r, q);
+// two f32 in one operation
+typedef uint64_t Pair;
+__device__ __forceinline__ Pair pair(float x, float y) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
 }
+__device__ __forceinline__ float2 unpair(Pair p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// scale = max(amax / 448, 2^-126): the quotient by reciprocal and remainder, as below
 __device__ __forceinline__ float block_scale(float amax) {
-    return max_nan(divided(amax, kFp8Max, 1.f / kFp8Max), kFp8MinScale);
+    constexpr float r = 1.f / kFp8Max;
+    const float q = amax * r;
+    return max_nan(fmaf(-fmaf(q, kFp8Max, -amax), r, q), kFp8MinScale);
 }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     uint16_t r;
@@ -130,26 +156,73 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return r;
 }
 
-// The largest magnitude of the block that this half warp's 16 threads hold (8
-// columns each), in every one of them.  All 32 lanes take part.
-__device__ __forceinline__ float half_warp_amax(const Vec8& r) {
+// How the values of one block are turned into codes: the scale and, for pairs,
+// the scale and minus its rounded reciprocal.
+struct Quant {
+    Pair s, nr;
+};
+__device__ __forceinline__ Quant quant(float scale) {
+    const float nr = -1.f / scale;
+    return {pair(scale, scale), pair(nr, nr)};
+}
+// Codes of the pair whose negated values nv holds: v / s rounded, from
+// q = v r, e = q s - v (exact) and q - e r.  With the signs placed so, a zero
+// keeps its sign.
+__device__ __forceinline__ uint32_t codes2(Pair nv, const Quant& z) {
+    const Pair q = mul2(nv, z.nr);
+    const float2 f = unpair(fma2(fma2(q, z.s, nv), z.nr, q));
+    return e4m3x2(f.x, f.y);
+}
+struct Pairs8 {   // eight values, negated where they are to become codes
+    Pair p[4];
+};
+__device__ __forceinline__ uint2 codes8(const Pairs8& v, const Quant& z) {
+    return make_uint2(codes2(v.p[0], z) | (codes2(v.p[1], z) << 16), codes2(v.p[2], z) | (codes2(v.p[3], z) << 16));
+}
+
+// The largest magnitude among eight values, then in the block of 128 that a
+// half warp holds (8 columns a thread), in each of its threads.  All 32 lanes
+// take part.
+__device__ __forceinline__ float amax8(const Pairs8& v) {
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) m = max_nan(m, fabsf(r.v[i]));
+    for (int i = 0; i < 4; i++) {
+        const float2 f = unpair(v.p[i]);
+        m = amax3(m, f.x, f.y);
+    }
+    return m;
+}
+__device__ __forceinline__ float half_warp_max(float m) {
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     return m;
 }
-__device__ __forceinline__ float half_warp_scale(const Vec8& r) { return block_scale(half_warp_amax(r)); }
 
-// r = 1 / scale
-__device__ __forceinline__ uint2 codes8(const Vec8& v, float scale, float r) {
-    uint32_t c[4];
+// Eight stored columns, negated, as f32 (the sign bits are turned over where
+// two 16-bit values still share a word)
+template <typename T>
+__device__ __forceinline__ Pairs8 negated(const Raw8<T>& r) {
+    Pairs8 v;
 #pragma unroll
-    for (int i = 0; i < 4; i++) c[i] = e4m3x2(divided(v.v[2 * i], scale, r), divided(v.v[2 * i + 1], scale, r));
-    return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            v.p[i] = pair(-__uint_as_float(r.w[2 * i]), -__uint_as_float(r.w[2 * i + 1]));
+        } else {
+            const uint32_t w = r.w[i] ^ 0x80008000u;
+            T h[2];
+            memcpy(h, &w, 4);
+            v.p[i] = pair(to_f32(h[0]), to_f32(h[1]));
+        }
+    }
+    return v;
 }
-__device__ __forceinline__ uint2 codes8(const Vec8& v, float scale) { return codes8(v, scale, 1.f / scale); }
+template <typename T>
+__device__ __forceinline__ Pairs8 values8(const Raw8<T>& r) {
+    Pairs8 v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) v.p[i] = pair(column(r, 2 * i), column(r, 2 * i + 1));
+    return v;
+}
 
 __device__ __forceinline__ void store_codes8(uint8_t* __restrict__ p, uint2 c, int n, bool wide) {
     if (wide && n == 8) {
@@ -161,10 +234,8 @@ __device__ __forceinline__ void store_codes8(uint8_t* __restrict__ p, uint2 c, i
     }
 }
 
-// columns that a thread at column c holds of `cols`
-__device__ __forceinline__ int columns_at(long long c, long long cols) {
-    return c >= cols ? 0 : (int)(cols - c < 8 ? cols - c : 8);
-}
+// columns that a thread at column c holds of `cols`, at most `most`
+__device__ __forceinline__ int columns_at(int c, int cols, int most = 8) { return min(max(cols - c, 0), most); }
 
 // ------------------------------------------------------------ tokens sorted by expert
 // A stable counting sort of the n = T k assignments by expert in one launch:
@@ -274,101 +345,133 @@ sort_tokens_kernel(const int32_t* __restrict__ idx, long long n, int first, int 
 }
 
 // ------------------------------------------------------------ rows out and back
-// One unit of work = one token x the columns that a CTA's threads hold.
+// blockIdx.x is the token or row, blockIdx.y the piece of its columns that the
+// CTA's threads hold.  Positions are compared unsigned, so -1 is out too.
 
 // rows[pos[t, j]] = x[t] for every slot j whose row is in [0, n_rows)
 template <typename T>
-__global__ void gather_rows_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ pos, long long T_,
-                                   int k, long long d, int segments, long long n_rows, T* __restrict__ rows,
-                                   long long ld_rows, bool wide) {
-    for (long long u = blockIdx.x; u < T_ * segments; u += gridDim.x) {
-        const long long t = u / segments;
-        const long long c = ((u - t * segments) * blockDim.x + threadIdx.x) * 8;
-        const int n = columns_at(c, d);
-        if (!n) continue;
-        if (wide && n == 8) {   // the bits as they are
-            constexpr int W = sizeof(T) / 2;
-            uint4 v[W];
+__global__ void __launch_bounds__(256)
+gather_rows_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ pos, int k, int d, uint32_t n_rows,
+                   T* __restrict__ rows, long long ld_rows, bool wide) {
+    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, d);
+    if (!n) return;
+    pos += (size_t)t * k;
+    x += t * ld_x + c;
+    if (wide && n == 8) {   // the bits as they are
+        const Raw8<T> v = load_raw8(x, 8, true);
+#pragma unroll 4
+        for (int j = 0; j < k; j++) {
+            const uint32_t p = pos[j];
+            if (p >= n_rows) continue;
 #pragma unroll
-            for (int i = 0; i < W; i++) v[i] = __ldg(reinterpret_cast<const uint4*>(x + t * ld_x + c) + i);
-            for (int j = 0; j < k; j++) {
-                const long long p = pos[t * k + j];
-                if (p < 0 || p >= n_rows) continue;
-#pragma unroll
-                for (int i = 0; i < W; i++) reinterpret_cast<uint4*>(rows + p * ld_rows + c)[i] = v[i];
-            }
-        } else {
-            for (int j = 0; j < k; j++) {
-                const long long p = pos[t * k + j];
-                if (p < 0 || p >= n_rows) continue;
-                for (int i = 0; i < n; i++) rows[p * ld_rows + c + i] = x[t * ld_x + c + i];
-            }
+            for (int i = 0; i < (int)sizeof(T) / 2; i++)
+                reinterpret_cast<uint4*>(rows + p * ld_rows + c)[i] = make_uint4(v.w[4 * i], v.w[4 * i + 1], v.w[4 * i + 2], v.w[4 * i + 3]);
+        }
+    } else {
+        for (int j = 0; j < k; j++) {
+            const uint32_t p = pos[j];
+            if (p >= n_rows) continue;
+            for (int i = 0; i < n; i++) rows[p * ld_rows + c + i] = x[i];
         }
     }
 }
 
-// the same into 8 bits: a token's row is quantised once for all its slots
+// 16 columns in 8 bits: their codes, given the 8 threads' block
+struct Codes16 {
+    uint2 lo, hi;
+    float scale;
+};
 template <typename T>
-__global__ void gather_rows_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ pos,
-                                       long long T_, int k, long long d, int segments, long long n_rows,
-                                       uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales,
-                                       long long ld_s, bool wide_x, bool wide_c) {
-    for (long long u = blockIdx.x; u < T_ * segments; u += gridDim.x) {
-        const long long t = u / segments;
-        const long long c = ((u - t * segments) * blockDim.x + threadIdx.x) * 8;
-        const int n = columns_at(c, d);
-        const Vec8 v = load8(x + t * ld_x + c, n, wide_x);
-        const float s = half_warp_scale(v);
-        if (!n) continue;
-        const uint2 q = codes8(v, s);
-        const bool lead = (threadIdx.x & 15) == 0;
-        for (int j = 0; j < k; j++) {
-            const long long p = pos[t * k + j];
-            if (p < 0 || p >= n_rows) continue;
-            store_codes8(codes + p * ld_c + c, q, n, wide_c);
-            if (lead) scales[p * ld_s + c / kFp8Block] = s;
-        }
+__device__ __forceinline__ Codes16 quantize16(const T* __restrict__ x, int n, bool wide) {
+    const Pairs8 a = negated(load_raw8(x, min(n, 8), wide)), b = negated(load_raw8(x + 8, max(n - 8, 0), wide));
+    float m = amax3(amax8(a), amax8(b), 0.f);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    Codes16 r;
+    r.scale = block_scale(m);
+    const Quant z = quant(r.scale);
+    r.lo = codes8(a, z);
+    r.hi = codes8(b, z);
+    return r;
+}
+__device__ __forceinline__ void store_codes16(uint8_t* __restrict__ p, const Codes16& q, int n, bool wide) {
+    if (wide && n == 16) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(q.lo.x, q.lo.y, q.hi.x, q.hi.y);
+    } else {
+        store_codes8(p, q.lo, min(n, 8), false);
+        store_codes8(p + 8, q.hi, n - 8, false);
+    }
+}
+
+// the same into 8 bits: a token's row is quantised once for all its slots.  A
+// thread holds 16 columns: the slots' addresses and checks were most of what
+// it did with 8.
+template <typename T>
+__global__ void __launch_bounds__(256)
+gather_rows_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ pos, int k, int d,
+                       uint32_t n_rows, uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales,
+                       long long ld_s, bool wide_x, bool wide_c) {
+    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 16, n = columns_at(c, d, 16);
+    pos += (size_t)t * k;
+    const Codes16 q = quantize16(x + t * ld_x + c, n, wide_x);
+    if (!n) return;
+    const bool lead = (threadIdx.x & 7) == 0;
+#pragma unroll 4
+    for (int j = 0; j < k; j++) {
+        const uint32_t p = pos[j];
+        if (p >= n_rows) continue;
+        store_codes16(codes + p * ld_c + c, q, n, wide_c);
+        if (lead) scales[p * ld_s + c / kFp8Block] = q.scale;
     }
 }
 
 // out[t] = add[t] + sum_j w[t, j] rows[pos[t, j]], in slot order; w NULL: 1
 template <typename T>
-__global__ void combine_rows_kernel(const T* __restrict__ rows, long long ld_rows, long long n_rows,
-                                    const int32_t* __restrict__ pos, const float* __restrict__ w, long long T_, int k,
-                                    long long d, int segments, const T* __restrict__ add, long long ld_add,
-                                    T* __restrict__ out, long long ld_out, bool wide) {
-    constexpr int S = sizeof(T) == 4 ? 4 : 8;   // rows at a time: 32 registers
-    for (long long u = blockIdx.x; u < T_ * segments; u += gridDim.x) {
-        const long long t = u / segments;
-        const long long c = ((u - t * segments) * blockDim.x + threadIdx.x) * 8;
-        const int n = columns_at(c, d);
-        if (!n) continue;
-        Vec8 acc;
-        if (add) acc = load8(add + t * ld_add + c, n, wide);
-        else
+__global__ void __launch_bounds__(256, 4)
+combine_rows_kernel(const T* __restrict__ rows, long long ld_rows, uint32_t n_rows, const int32_t* __restrict__ pos,
+                    const float* __restrict__ w, int k, int d, const T* __restrict__ add, long long ld_add,
+                    T* __restrict__ out, long long ld_out, bool wide) {
+    constexpr int S = sizeof(T) == 4 ? 4 : 8;   // rows whose loads are in flight: 32 registers
+    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, d);
+    if (!n) return;
+    pos += (size_t)t * k;
+    if (w) w += (size_t)t * k;
+    Pairs8 acc;
 #pragma unroll
-            for (int i = 0; i < 8; i++) acc.v[i] = 0.f;
-        for (int j0 = 0; j0 < k; j0 += S) {   // their loads in flight together
-            Raw8<T> r[S];
-            float wj[S];
-            uint32_t held = 0;
+    for (int i = 0; i < 4; i++) acc.p[i] = 0;
+    Raw8<T> first;
+    if (add) first = load_raw8(add + t * ld_add + c, n, wide);
+    for (int j0 = 0; j0 < k; j0 += S) {
+        Raw8<T> r[S];
+        float wj[S];
+        uint32_t held = 0;
 #pragma unroll
-            for (int j = 0; j < S; j++) {
-                if (j0 + j >= k) break;
-                const long long p = pos[t * k + j0 + j];
-                if (p < 0 || p >= n_rows) continue;
-                held |= 1u << j;
-                r[j] = load_raw8(rows + p * ld_rows + c, n, wide);
-                wj[j] = w ? w[t * k + j0 + j] : 1.f;
-            }
-#pragma unroll
-            for (int j = 0; j < S; j++)
-                if (held >> j & 1)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) acc.v[i] = fmaf(wj[j], column(r[j], i), acc.v[i]);
+        for (int j = 0; j < S; j++) {
+            if (j0 + j >= k) break;
+            const uint32_t p = pos[j0 + j];
+            if (p >= n_rows) continue;
+            held |= 1u << j;
+            r[j] = load_raw8(rows + p * ld_rows + c, n, wide);
+            wj[j] = w ? w[j0 + j] : 1.f;
         }
-        store8(out + t * ld_out + c, acc, n, wide);
+        if (add && j0 == 0) acc = values8(first);
+#pragma unroll
+        for (int j = 0; j < S; j++)
+            if (held >> j & 1) {
+                const Pair wp = pair(wj[j], wj[j]);
+                const Pairs8 v = values8(r[j]);
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc.p[i] = fma2(wp, v.p[i], acc.p[i]);
+            }
     }
+    Vec8 o;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = unpair(acc.p[i]);
+        o.v[2 * i] = f.x;
+        o.v[2 * i + 1] = f.y;
+    }
+    store8(out + t * ld_out + c, o, n, wide);
 }
 
 // The gradient of combine_rows: drows[pos[t, j]] = w[t, j] dout[t] (T or 8
@@ -380,139 +483,149 @@ __global__ void combine_rows_kernel(const T* __restrict__ rows, long long ld_row
 // half warp, one each, and handed round.
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(512, 2)
-combine_grad_kernel(const T* __restrict__ dout, long long ld_dout, const T* __restrict__ rows,
-                                    long long ld_rows, long long n_rows, const int32_t* __restrict__ pos,
-                                    const float* __restrict__ w, long long T_, int k, long long d, T* __restrict__ drows,
-                                    uint8_t* __restrict__ codes, long long ld_d, float* __restrict__ scales,
-                                    long long ld_s, float* __restrict__ dw, bool wide, bool wide_d) {
-    constexpr int S = 8, B = sizeof(T) == 4 ? 2 : 4;   // slots; rows' loads in flight
-    __shared__ float part[S][32];
+combine_grad_kernel(const T* __restrict__ dout, long long ld_dout, const T* __restrict__ rows, long long ld_rows,
+                    uint32_t n_rows, const int32_t* __restrict__ pos, const float* __restrict__ w, int k, int d,
+                    T* __restrict__ drows, uint8_t* __restrict__ codes, long long ld_d, float* __restrict__ scales,
+                    long long ld_s, float* __restrict__ dw, bool wide, bool wide_d) {
+    constexpr int S = 8, B = sizeof(T) == 4 ? 2 : 4;   // slots; rows whose loads are in flight
+    __shared__ float part[S][16];
+    __shared__ uint32_t at[S];   // the slots' rows
+    __shared__ float wn[S];      // minus their weights
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    for (long long t = blockIdx.x; t < T_; t += gridDim.x) {
-        for (int j0 = 0; j0 < k; j0 += S) {
-            float dot[S];
-            int p[S];
-            float wj[S];
+    const int t = blockIdx.x;
+    pos += (size_t)t * k;
+    if (w) w += (size_t)t * k;
+    dout += t * ld_dout;
+    for (int j0 = 0; j0 < k; j0 += S) {
+        Pair dot[S];
 #pragma unroll
-            for (int j = 0; j < S; j++) {
-                dot[j] = 0.f;
-                wj[j] = 0.f;
-                p[j] = j0 + j < k ? pos[t * k + j0 + j] : -1;
-                if (p[j] >= n_rows) p[j] = -1;
-                if (p[j] >= 0) wj[j] = w ? w[t * k + j0 + j] : 1.f;
-            }
-            float w_lane = 0.f;   // slot lane & 7
-            if (FP8)
+        for (int j = 0; j < S; j++) dot[j] = 0;
+        if (threadIdx.x < S) {
+            const int j = j0 + threadIdx.x;
+            at[threadIdx.x] = j < k ? (uint32_t)pos[j] : ~0u;
+            wn[threadIdx.x] = j >= k ? 0.f : w ? -w[j] : -1.f;
+        }
+        __syncthreads();
+        const int mine = j0 + (lane & 7);
+        const float w_lane = !FP8 || mine >= k ? 0.f : w ? fabsf(w[mine]) : 1.f;
+        for (int c0 = 0; c0 < d; c0 += blockDim.x * 8) {
+            const int c = c0 + threadIdx.x * 8, n = columns_at(c, d);
+            const Raw8<T> g_raw = load_raw8(dout + c, n, wide);
+            float s_lane = 0.f, r_lane = 0.f;
 #pragma unroll
-                for (int j = 0; j < S; j++)
-                    if ((lane & 7) == j) w_lane = fabsf(wj[j]);
-            for (long long c0 = 0; c0 < d; c0 += (long long)blockDim.x * 8) {
-                const long long c = c0 + threadIdx.x * 8;
-                const int n = columns_at(c, d);
-                const Vec8 g = load8(dout + t * ld_dout + c, n, wide);
-                float s_lane = 0.f, r_lane = 0.f;
+            for (int jb = 0; jb < S; jb += B) {
+                Raw8<T> r[B];
+                if (dw)
 #pragma unroll
-                for (int jb = 0; jb < S; jb += B) {
-                    Raw8<T> r[B];
-                    if (dw)
+                    for (int j = 0; j < B; j++)
+                        if (at[jb + j] < n_rows) r[j] = load_raw8(rows + at[jb + j] * ld_rows + c, n, wide);
+                const Pairs8 g = values8(g_raw);
+                if (FP8 && jb == 0) {
+                    s_lane = block_scale(__fmul_rn(w_lane, half_warp_max(amax8(g))));
+                    r_lane = -1.f / s_lane;
+                }
 #pragma unroll
-                        for (int j = 0; j < B; j++)
-                            if (p[jb + j] >= 0) r[j] = load_raw8(rows + p[jb + j] * ld_rows + c, n, wide);
-                    if (FP8 && jb == 0) {
-                        s_lane = block_scale(__fmul_rn(w_lane, half_warp_amax(g)));
-                        r_lane = 1.f / s_lane;
-                    }
+                for (int u = 0; u < B; u++) {
+                    const int j = jb + u;
+                    const uint32_t p = at[j];
+                    if (p >= n_rows) continue;   // the same for all threads of the CTA
+                    Pairs8 v;   // minus w dout
+                    const Pair wp = pair(wn[j], wn[j]);
 #pragma unroll
-                    for (int u = 0; u < B; u++) {
-                        const int j = jb + u;
-                        if (p[j] < 0) continue;   // the same for all threads of the CTA
-                        Vec8 v;
-#pragma unroll
-                        for (int i = 0; i < 8; i++) v.v[i] = __fmul_rn(wj[j], g.v[i]);
-                        if constexpr (FP8) {
-                            const float s = __shfl_sync(0xffffffffu, s_lane, j, 16), q = __shfl_sync(0xffffffffu, r_lane, j, 16);
-                            if (n) {
-                                store_codes8(codes + p[j] * ld_d + c, codes8(v, s, q), n, wide_d);
-                                if ((threadIdx.x & 15) == 0) scales[p[j] * ld_s + c / kFp8Block] = s;
-                            }
-                        } else if (n) {
-                            store8(drows + p[j] * ld_d + c, v, n, wide_d);
+                    for (int i = 0; i < 4; i++) v.p[i] = mul2(wp, g.p[i]);
+                    if constexpr (FP8) {
+                        const float s = __shfl_sync(0xffffffffu, s_lane, j, 16), q = __shfl_sync(0xffffffffu, r_lane, j, 16);
+                        if (n) {
+                            store_codes8(codes + p * ld_d + c, codes8(v, Quant{pair(s, s), pair(q, q)}), n, wide_d);
+                            if ((threadIdx.x & 15) == 0) scales[p * ld_s + c / kFp8Block] = s;
                         }
-                        if (dw)
+                    } else if (n) {
+                        Vec8 o;
 #pragma unroll
-                            for (int i = 0; i < 8; i++) dot[j] = fmaf(g.v[i], column(r[u], i), dot[j]);
+                        for (int i = 0; i < 4; i++) {
+                            const float2 f = unpair(v.p[i]);
+                            o.v[2 * i] = -f.x;
+                            o.v[2 * i + 1] = -f.y;
+                        }
+                        store8(drows + p * ld_d + c, o, n, wide_d);
+                    }
+                    if (dw) {
+                        const Pairs8 x = values8(r[u]);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) dot[j] = fma2(g.p[i], x.p[i], dot[j]);
                     }
                 }
             }
-            if (!dw) continue;
-#pragma unroll
-            for (int j = 0; j < S; j++) {
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
-                if (lane == 0) part[j][warp] = dot[j];
-            }
-            __syncthreads();
-            if (warp < S && j0 + warp < k) {
-                float v = lane < warps ? part[warp][lane] : 0.f;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                if (lane == 0) dw[t * k + j0 + warp] = v;   // 0 for a slot without a row
-            }
-            __syncthreads();
         }
+        if (!dw) {
+            __syncthreads();   // before the next slots' rows
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < S; j++) {
+            const float2 f = unpair(dot[j]);
+            float sum = f.x + f.y;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) part[j][warp] = sum;
+        }
+        __syncthreads();
+        if (warp < S && j0 + warp < k) {
+            float v = lane < warps ? part[warp][lane] : 0.f;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            if (lane == 0) dw[(size_t)t * k + j0 + warp] = v;   // 0 for a slot without a row
+        }
+        __syncthreads();
     }
 }
 
 // ------------------------------------------------------------ rows into 8 bits
+// (n_dev: how many of the rows there are, on the device)
 
 template <typename T>
-__global__ void quantize_fp8_kernel(const T* __restrict__ x, long long ld_x, long long rows,
-                                    const int32_t* __restrict__ n_dev, long long cols, int segments,
-                                    uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales,
-                                    long long ld_s, bool wide_x, bool wide_c) {
-    if (n_dev) rows = min(rows, (long long)max(*n_dev, 0));
-    for (long long u = blockIdx.x; u < rows * segments; u += gridDim.x) {
-        const long long t = u / segments;
-        const long long c = ((u - t * segments) * blockDim.x + threadIdx.x) * 8;
-        const int n = columns_at(c, cols);
-        const Vec8 v = load8(x + t * ld_x + c, n, wide_x);
-        const float s = half_warp_scale(v);
-        if (!n) continue;
-        store_codes8(codes + t * ld_c + c, codes8(v, s), n, wide_c);
-        if ((threadIdx.x & 15) == 0) scales[t * ld_s + c / kFp8Block] = s;
-    }
+__global__ void __launch_bounds__(256)
+quantize_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ n_dev, int cols,
+                    uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales, long long ld_s, bool wide_x,
+                    bool wide_c) {
+    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 16, n = columns_at(c, cols, 16);
+    if (n_dev && t >= *n_dev) return;
+    const Codes16 q = quantize16(x + t * ld_x + c, n, wide_x);
+    if (!n) return;
+    store_codes16(codes + t * ld_c + c, q, n, wide_c);
+    if ((threadIdx.x & 7) == 0) scales[t * ld_s + c / kFp8Block] = q.scale;
 }
 
 // One CTA of 256 threads per 128 x 128 block of a weight matrix (rows x cols,
 // dense): thread i holds 8 columns of every 16th row.
 template <typename T>
 __global__ void __launch_bounds__(256)
-quantize_fp8_weights_kernel(const T* __restrict__ w, long long rows, long long cols, uint8_t* __restrict__ codes,
+quantize_fp8_weights_kernel(const T* __restrict__ w, int rows, int cols, uint8_t* __restrict__ codes,
                             float* __restrict__ scales, bool wide) {
     __shared__ float top[8];
-    const long long r0 = (long long)blockIdx.y * kFp8Block, c = (long long)blockIdx.x * kFp8Block + (threadIdx.x & 15) * 8;
+    const int r0 = blockIdx.y * kFp8Block, c = blockIdx.x * kFp8Block + (threadIdx.x & 15) * 8;
     const long long base = (long long)blockIdx.z * rows * cols;
     const int n = columns_at(c, cols);
-    Vec8 v[8];
+    Pairs8 v[8];
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const long long r = r0 + (threadIdx.x >> 4) + 16 * i;
-        v[i] = load8(w + base + r * cols + c, r < rows ? n : 0, wide);
-#pragma unroll
-        for (int q = 0; q < 8; q++) m = max_nan(m, fabsf(v[i].v[q]));
+        const int r = r0 + (threadIdx.x >> 4) + 16 * i;
+        v[i] = negated(load_raw8(w + base + (long long)r * cols + c, r < rows ? n : 0, wide));
+        m = max_nan(m, amax8(v[i]));
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = half_warp_max(m);
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 16));
     if ((threadIdx.x & 31) == 0) top[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; i++) m = max_nan(m, top[i]);
     const float s = block_scale(m);
+    const Quant z = quant(s);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const long long r = r0 + (threadIdx.x >> 4) + 16 * i;
-        if (r < rows && n) store_codes8(codes + base + r * cols + c, codes8(v[i], s), n, wide);
+        const int r = r0 + (threadIdx.x >> 4) + 16 * i;
+        if (r < rows && n) store_codes8(codes + base + (long long)r * cols + c, codes8(v[i], z), n, wide);
     }
     if (threadIdx.x == 0)
         scales[((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = s;
@@ -545,58 +658,62 @@ __device__ __forceinline__ Swiglu swiglu_parts(float gate, float up, float limit
 }
 
 template <typename T>
-__global__ void swiglu_fp8_kernel(const T* __restrict__ gu, long long ld, long long rows,
-                                  const int32_t* __restrict__ n_dev, long long f, int segments, float limit,
-                                  uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales, long long ld_s,
-                                  bool wide, bool wide_c) {
-    if (n_dev) rows = min(rows, (long long)max(*n_dev, 0));
-    for (long long x = blockIdx.x; x < rows * segments; x += gridDim.x) {
-        const long long t = x / segments;
-        const long long c = ((x - t * segments) * blockDim.x + threadIdx.x) * 8;
-        const int n = columns_at(c, f);
-        const Vec8 g = load8(gu + t * ld + c, n, wide), u = load8(gu + t * ld + f + c, n, wide);
-        Vec8 h;
+__global__ void __launch_bounds__(256)
+swiglu_fp8_kernel(const T* __restrict__ gu, long long ld, const int32_t* __restrict__ n_dev, int f, float limit,
+                  uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales, long long ld_s, bool wide,
+                  bool wide_c) {
+    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
+    if (n_dev && t >= *n_dev) return;
+    gu += t * ld + c;
+    const Raw8<T> g = load_raw8(gu, n, wide), u = load_raw8(gu + f, n, wide);   // absent columns are 0, and so is h there
+    Pairs8 h;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const Swiglu p = swiglu_parts(g.v[i], u.v[i], limit);
-            h.v[i] = i < n ? p.g * p.sig * p.u : 0.f;
+    for (int i = 0; i < 4; i++) {
+        float v[2];
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const Swiglu p = swiglu_parts(column(g, 2 * i + q), column(u, 2 * i + q), limit);
+            v[q] = p.g * p.sig * -p.u;
         }
-        const float s = half_warp_scale(h);
-        if (!n) continue;
-        store_codes8(codes + t * ld_c + c, codes8(h, s), n, wide_c);
-        if ((threadIdx.x & 15) == 0) scales[t * ld_s + c / kFp8Block] = s;
+        h.p[i] = pair(v[0], v[1]);
     }
+    const float s = block_scale(half_warp_max(amax8(h)));
+    if (!n) return;
+    store_codes8(codes + t * ld_c + c, codes8(h, quant(s)), n, wide_c);
+    if ((threadIdx.x & 15) == 0) scales[t * ld_s + c / kFp8Block] = s;
 }
 
 // f is a multiple of 128 here, so no block of the 2f columns holds both halves
 template <typename T>
-__global__ void swiglu_fp8_grad_kernel(const T* __restrict__ gu, long long ld, const T* __restrict__ dh, long long ld_dh,
-                                       long long rows, const int32_t* __restrict__ n_dev, long long f, int segments,
-                                       float limit, uint8_t* __restrict__ codes, long long ld_c,
-                                       float* __restrict__ scales, long long ld_s, bool wide, bool wide_c) {
-    if (n_dev) rows = min(rows, (long long)max(*n_dev, 0));
-    for (long long x = blockIdx.x; x < rows * segments; x += gridDim.x) {
-        const long long t = x / segments;
-        const long long c = ((x - t * segments) * blockDim.x + threadIdx.x) * 8;
-        const int n = columns_at(c, f);
-        const Vec8 g = load8(gu + t * ld + c, n, wide), u = load8(gu + t * ld + f + c, n, wide);
-        const Vec8 d = load8(dh + t * ld_dh + c, n, wide);
-        Vec8 dg, du;
+__global__ void __launch_bounds__(256)
+swiglu_fp8_grad_kernel(const T* __restrict__ gu, long long ld, const T* __restrict__ dh, long long ld_dh,
+                       const int32_t* __restrict__ n_dev, int f, float limit, uint8_t* __restrict__ codes, long long ld_c,
+                       float* __restrict__ scales, long long ld_s, bool wide, bool wide_c) {
+    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
+    if (n_dev && t >= *n_dev) return;
+    gu += t * ld + c;
+    const Raw8<T> g = load_raw8(gu, n, wide), u = load_raw8(gu + f, n, wide), d = load_raw8(dh + t * ld_dh + c, n, wide);
+    Pairs8 dg, du;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const Swiglu p = swiglu_parts(g.v[i], u.v[i], limit);
-            const float silu = p.g * p.sig;
-            dg.v[i] = i < n && p.g_in ? d.v[i] * p.u * (p.sig * (1.f + p.g * (1.f - p.sig))) : 0.f;
-            du.v[i] = i < n && p.u_in ? d.v[i] * silu : 0.f;
+    for (int i = 0; i < 4; i++) {
+        float a[2], b[2];
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const Swiglu p = swiglu_parts(column(g, 2 * i + q), column(u, 2 * i + q), limit);
+            const float nd = -column(d, 2 * i + q);
+            a[q] = p.g_in ? nd * p.u * (p.sig * fmaf(p.g, 1.f - p.sig, 1.f)) : 0.f;
+            b[q] = p.u_in ? nd * (p.g * p.sig) : 0.f;
         }
-        const float sg = half_warp_scale(dg), su = half_warp_scale(du);
-        if (!n) continue;
-        store_codes8(codes + t * ld_c + c, codes8(dg, sg), n, wide_c);
-        store_codes8(codes + t * ld_c + f + c, codes8(du, su), n, wide_c);
-        if ((threadIdx.x & 15) == 0) {
-            scales[t * ld_s + c / kFp8Block] = sg;
-            scales[t * ld_s + (f + c) / kFp8Block] = su;
-        }
+        dg.p[i] = pair(a[0], a[1]);
+        du.p[i] = pair(b[0], b[1]);
+    }
+    const float sg = block_scale(half_warp_max(amax8(dg))), su = block_scale(half_warp_max(amax8(du)));
+    if (!n) return;
+    store_codes8(codes + t * ld_c + c, codes8(dg, quant(sg)), n, wide_c);
+    store_codes8(codes + t * ld_c + f + c, codes8(du, quant(su)), n, wide_c);
+    if ((threadIdx.x & 15) == 0) {
+        scales[t * ld_s + c / kFp8Block] = sg;
+        scales[t * ld_s + (f + c) / kFp8Block] = su;
     }
 }
 
