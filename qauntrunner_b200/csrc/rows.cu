@@ -9,6 +9,11 @@
 namespace qrm {
 namespace {
 
+// The CTAs that fit on the SMs at once, for kernels that walk the rows.
+int walkers(int64_t rows, unsigned pieces, int sms, int resident) {
+    return (int)std::min<int64_t>(rows, std::max<int64_t>(1, (int64_t)sms * resident / pieces));
+}
+
 // Columns to threads, `each` of them in one, in whole blocks of 128; at most
 // 256 threads a CTA, spread evenly over the pieces that a row is cut into
 // (7168 columns: 4 x 224 threads of 8, 2 x 224 threads of 16).
@@ -95,8 +100,10 @@ extern "C" int qrm_sort_tokens(const int32_t* topk_idx_dev, int64_t T, int k, in
     TRY(current_device(&device, &sms));
     const int64_t n = T * k;
     const bool many = n > 4096;
-    const int warps = (int)std::min<int64_t>(32, std::max<int64_t>(8, (n + 31) / 32));
+    const int warps = (int)std::min<int64_t>(32, std::max<int64_t>(8, (n + 255) / 256 * 8));
     cudaLaunchConfig_t cfg = {};
+    int bits = 1;
+    while (n_experts >> bits) bits++;   // an expert outside is all ones, which no expert is in this many bits
     cfg.gridDim = dim3(many ? kSortCluster : 1);
     cfg.blockDim = dim3(32 * warps);
     cfg.dynamicSmemBytes = sizeof(int32_t) * (size_t)(2 + warps) * n_experts;
@@ -107,13 +114,13 @@ extern "C" int qrm_sort_tokens(const int32_t* topk_idx_dev, int64_t T, int k, in
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (cfg.dynamicSmemBytes > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)(sizeof(int32_t) * 34 * kSortMaxExperts));
-        if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    }
-    cudaError_t e = cudaLaunchKernelEx(&cfg, sort_tokens_kernel, topk_idx_dev, (long long)n, first, n_experts, perm_dev,
-                                       pos_dev, offsets_dev);
+    auto kernel = many ? sort_tokens_kernel<kSortCluster> : sort_tokens_kernel<1>;
+    cudaError_t e = cudaSuccess;
+    if (cfg.dynamicSmemBytes > 48 * 1024)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (int)(sizeof(int32_t) * 34 * kSortMaxExperts));
+    if (e == cudaSuccess)
+        e = cudaLaunchKernelEx(&cfg, kernel, topk_idx_dev, (long long)n, first, n_experts, bits, perm_dev, pos_dev, offsets_dev);
     return e == cudaSuccess ? launched(what) : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
 }
 
@@ -172,11 +179,12 @@ extern "C" int qrm_combine_rows(int type, const void* rows_dev, int64_t n_rows, 
     if (w_dev) TRY(check_ints(what, "w", w_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(T, d, 8);
+    Cut c = cut_columns(T, d, 8);
+    c.grid.x = walkers(T, c.grid.y, sms, 4 * 256 / c.threads);
     const bool wide = wide_rows(rows_dev, ld_rows, b) && wide_rows(out_dev, ld_out, b) &&
                       (!add_dev || wide_rows(add_dev, ld_add, b));
     BY_TYPE(type, combine_rows_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, k, (int)d, (const V*)add_dev, ld_add,
+                      (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, (int)T, k, (int)d, (const V*)add_dev, ld_add,
                       (V*)out_dev, ld_out, wide));
     return launched(what);
 }
@@ -205,19 +213,21 @@ static int combine_grad(const char* what, int type, const void* dout_dev, int64_
     if (dw_dev) TRY(check_ints(what, "dw", dw_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    // one CTA per token; at most 512 threads, which a row's columns fill evenly
-    const int64_t lanes = blocks_of(d) * 16, rounds = (lanes + 511) / 512;
-    const int threads = (int)std::max<int64_t>(256, ((lanes + rounds - 1) / rounds + 31) / 32 * 32);
+    // one CTA per token, dout's columns in shared memory
+    const size_t smem = sizeof(float) * blocks_of(std::min<int64_t>(d, kGradCols)) * kFp8Block;   // 32 KB at most
     const bool wide = wide_rows(dout_dev, ld_dout, b) && (!dw_dev || wide_rows(rows_dev, ld_rows, b));
+    const bool wide_d = fp8 ? wide_codes(codes_dev, ld_d) : wide_rows(drows_dev, ld_d, b);
+    const bool fast = wide && wide_d && d % 8 == 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (fp8)
-        BY_TYPE(type, combine_grad_kernel<V, true><<<(unsigned)T, threads, 0, s>>>(
-                          (const V*)dout_dev, ld_dout, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, k, (int)d,
-                          (V*)nullptr, codes_dev, ld_d, scales_dev, ld_scales, dw_dev, wide, wide_codes(codes_dev, ld_d)));
-    else
-        BY_TYPE(type, combine_grad_kernel<V, false><<<(unsigned)T, threads, 0, s>>>(
-                          (const V*)dout_dev, ld_dout, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, k, (int)d,
-                          (V*)drows_dev, nullptr, ld_d, nullptr, 0, dw_dev, wide, wide_rows(drows_dev, ld_d, b)));
+#define QRM_GRAD(FP8, FAST)                                                                                             \
+    BY_TYPE(type, combine_grad_kernel<V, FP8, FAST><<<(unsigned)T, 256, smem, s>>>(                                     \
+                      (const V*)dout_dev, ld_dout, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, k, (int)d, \
+                      (V*)drows_dev, codes_dev, ld_d, scales_dev, ld_scales, dw_dev, wide, wide_d))
+    if (fp8 && fast) QRM_GRAD(true, true);
+    else if (fp8) QRM_GRAD(true, false);
+    else if (fast) QRM_GRAD(false, true);
+    else QRM_GRAD(false, false);
+#undef QRM_GRAD
     return launched(what);
 }
 
@@ -295,11 +305,17 @@ extern "C" int qrm_swiglu_fp8(int type, const void* gu_dev, int64_t ld_gu, int64
     if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(rows, f, 8);
+    Cut c = cut_columns(rows, f, 8);
+    c.grid.x = walkers(rows, c.grid.y, sms, 6 * 256 / c.threads);
     const bool wide = wide_rows(gu_dev, ld_gu, b) && f * b % 16 == 0;
-    BY_TYPE(type, swiglu_fp8_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)gu_dev, ld_gu, n_rows_dev, (int)f, limit, codes_dev, ld_codes, scales_dev,
-                      ld_scales, wide, wide_codes(codes_dev, ld_codes)));
+    const cudaStream_t s = (cudaStream_t)stream;
+    const bool wide_c = wide_codes(codes_dev, ld_codes);
+    if (limit > 0.f)
+        BY_TYPE(type, swiglu_fp8_kernel<V, true><<<c.grid, c.threads, 0, s>>>((const V*)gu_dev, ld_gu, (int)rows, n_rows_dev, (int)f,
+                          limit, codes_dev, ld_codes, scales_dev, ld_scales, wide, wide_c));
+    else
+        BY_TYPE(type, swiglu_fp8_kernel<V, false><<<c.grid, c.threads, 0, s>>>((const V*)gu_dev, ld_gu, (int)rows, n_rows_dev, (int)f,
+                          limit, codes_dev, ld_codes, scales_dev, ld_scales, wide, wide_c));
     return launched(what);
 }
 
@@ -321,10 +337,18 @@ extern "C" int qrm_swiglu_fp8_grad(int type, const void* gu_dev, int64_t ld_gu, 
     if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
-    const Cut c = cut_columns(rows, f, 8);
+    Cut c = cut_columns(rows, f, 8);
+    c.grid.x = walkers(rows, c.grid.y, sms, 4 * 256 / c.threads);
     const bool wide = wide_rows(gu_dev, ld_gu, b) && wide_rows(dh_dev, ld_dh, b);
-    BY_TYPE(type, swiglu_fp8_grad_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, n_rows_dev, (int)f, limit, codes_dev, ld_codes,
-                      scales_dev, ld_scales, wide, wide_codes(codes_dev, ld_codes)));
+    const cudaStream_t s = (cudaStream_t)stream;
+    const bool wide_c = wide_codes(codes_dev, ld_codes);
+    if (limit > 0.f)
+        BY_TYPE(type, swiglu_fp8_grad_kernel<V, true><<<c.grid, c.threads, 0, s>>>(
+                          (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, (int)rows, n_rows_dev, (int)f, limit, codes_dev, ld_codes,
+                          scales_dev, ld_scales, wide, wide_c));
+    else
+        BY_TYPE(type, swiglu_fp8_grad_kernel<V, false><<<c.grid, c.threads, 0, s>>>(
+                          (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, (int)rows, n_rows_dev, (int)f, limit, codes_dev, ld_codes,
+                          scales_dev, ld_scales, wide, wide_c));
     return launched(what);
 }

@@ -241,15 +241,30 @@ __device__ __forceinline__ int columns_at(int c, int cols, int most = 8) { retur
 // A stable counting sort of the n = T k assignments by expert in one launch:
 // one CTA, or a cluster of 8 for more than 4096 assignments.  Each warp owns a
 // run of assignments and counts them by expert in its own row of shared memory
-// (lanes with one expert found by match.any; the lowest of them adds), the
-// rows and then the CTAs' totals are summed up in order, and the same walk
-// gives each assignment its place.  No atomics: the order inside an expert is
-// the assignments' own.
+// (the lowest lane of those with one expert adds), the rows and then the CTAs'
+// totals are summed up in order, and the same walk gives each assignment its
+// place.  No atomics: the order inside an expert is the assignments' own.
+// The lanes with one expert are found by a vote for each bit of its number:
+// match.any takes the longer the more experts there are among 32 assignments,
+// and took most of the time (14.4 us at 32768 assignments to 256 experts).
 constexpr int kSortMaxExperts = 1024;
 constexpr int kSortCluster = 8;
 
+// lanes whose e is this lane's; bits: of the largest e and of -1
+__device__ __forceinline__ uint32_t lanes_with(int e, int bits) {
+    uint32_t same = 0xffffffffu;
+#pragma unroll 4
+    for (int b = 0; b < bits; b++) {
+        const bool one = e >> b & 1;
+        const uint32_t v = __ballot_sync(0xffffffffu, one);
+        same &= one ? v : ~v;
+    }
+    return same;
+}
+
+template <int C>   // CTAs
 __global__ void __launch_bounds__(1024)
-sort_tokens_kernel(const int32_t* __restrict__ idx, long long n, int first, int E, int32_t* __restrict__ perm,
+sort_tokens_kernel(const int32_t* __restrict__ idx, long long n, int first, int E, int bits, int32_t* __restrict__ perm,
                    int32_t* __restrict__ pos, int32_t* __restrict__ offsets) {
     extern __shared__ int32_t sort_sm[];
     const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -257,46 +272,63 @@ sort_tokens_kernel(const int32_t* __restrict__ idx, long long n, int first, int 
     int32_t* start = sort_sm + E;        // [E] place of this CTA's first assignment of each expert
     int32_t* count = sort_sm + 2 * E;    // [W][E] each warp's count, then its running place
     __shared__ int32_t warp_sum[32];
-    __shared__ int32_t all;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int rank = C > 1 ? (int)cluster.block_rank() : 0;
 
     for (int i = threadIdx.x; i < W * E; i += blockDim.x) count[i] = 0;
-    __syncthreads();
     const long long per = ((n + (long long)C * W - 1) / ((long long)C * W) + 31) & ~31ll;
     const long long a0 = ((long long)rank * W + warp) * per, a1 = a0 + per < n ? a0 + per : n;
     int32_t* mine = count + warp * E;
-    for (long long a = a0; a < a1; a += 32) {
-        const long long i = a + lane;
-        int e = i < a1 ? idx[i] - first : -1;
-        if (e < 0 || e >= E) e = -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-        __syncwarp();
+    __syncthreads();
+    auto expert = [&](long long i) {   // -1: none of these
+        const int e = i < a1 ? idx[i] - first : -1;
+        return e < 0 || e >= E ? -1 : e;
+    };
+    for (long long a = a0; a < a1; a += 128) {
+        int e[4];   // loads in flight together
+#pragma unroll
+        for (int u = 0; u < 4; u++) e[u] = expert(a + 32 * u + lane);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (a + 32 * u >= a1) break;
+            const uint32_t same = lanes_with(e[u], bits);
+            if (e[u] >= 0 && lane == __ffs(same) - 1) mine[e[u]] += __popc(same);
+            __syncwarp();
+        }
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int32_t sum = 0;
-        for (int w = 0; w < W; w++) {
-            const int32_t c = count[w * E + e];
-            count[w * E + e] = sum;
-            sum += c;
+        for (int w0 = 0; w0 < W; w0 += 8) {   // W is a multiple of 8
+            int32_t c[8];
+#pragma unroll
+            for (int w = 0; w < 8; w++) c[w] = count[(w0 + w) * E + e];
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                count[(w0 + w) * E + e] = sum;
+                sum += c[w];
+            }
         }
         total[e] = sum;
     }
-    cluster.sync();
+    if (C > 1) cluster.sync();
+    else __syncthreads();
     // places: experts in order, inside an expert the CTAs in order
     int32_t before = 0;   // assignments of the experts already passed
     for (int e0 = 0; e0 < E; e0 += blockDim.x) {
         const int e = e0 + threadIdx.x;
         int32_t sum = 0, lower = 0;
-        if (e < E)
-            for (int c = 0; c < C; c++) {
-                const int32_t t = cluster.map_shared_rank(total, c)[e];
-                if (c < rank) lower += t;
-                sum += t;
+        if (e < E) {
+            int32_t c[C];
+#pragma unroll
+            for (int r = 0; r < C; r++) c[r] = C > 1 ? cluster.map_shared_rank(total, r)[e] : total[e];
+#pragma unroll
+            for (int r = 0; r < C; r++) {
+                if (r < rank) lower += c[r];
+                sum += c[r];
             }
+        }
         int32_t scan = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -305,43 +337,44 @@ sort_tokens_kernel(const int32_t* __restrict__ idx, long long n, int first, int 
         }
         if (lane == 31) warp_sum[warp] = scan;
         __syncthreads();
-        if (warp == 0) {
-            int32_t v = lane < W ? warp_sum[lane] : 0;
+        int32_t v = lane < W ? warp_sum[lane] : 0, lane_sum = v;   // every warp sums the warps up for itself
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += u;
-            }
-            if (lane < W) warp_sum[lane] = v;
-            if (lane == 31) all = v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int32_t u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
         }
-        __syncthreads();
-        const int32_t at = before + scan - sum + (warp ? warp_sum[warp - 1] : 0);
+        const int32_t at = before + scan - sum + __shfl_sync(0xffffffffu, v - lane_sum, warp);
         if (e < E) {
             start[e] = at + lower;
             if (rank == 0) offsets[e] = at;
         }
-        before += all;
+        before += __shfl_sync(0xffffffffu, v, 31);
         __syncthreads();
     }
     if (rank == 0 && threadIdx.x == 0) offsets[E] = before;
-    cluster.sync();   // the totals have been read everywhere, the starts are written
-    for (long long a = a0; a < a1; a += 32) {
-        const long long i = a + lane;
-        int e = i < a1 ? idx[i] - first : -1;
-        if (e < 0 || e >= E) e = -1;
-        const uint32_t same = __match_any_sync(0xffffffffu, e);
-        const int32_t at = e >= 0 ? start[e] + mine[e] + __popc(same & ((1u << lane) - 1u)) : -1;
-        __syncwarp();
-        if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-        __syncwarp();
-        if (i < a1) {
-            pos[i] = at;
-            if (at >= 0) perm[at] = (int32_t)i;
+    if (C > 1) cluster.barrier_arrive();   // this CTA has read the others' totals
+    for (long long a = a0; a < a1; a += 128) {
+        int e[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) e[u] = expert(a + 32 * u + lane);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (a + 32 * u >= a1) break;
+            const long long i = a + 32 * u + lane;
+            const uint32_t same = lanes_with(e[u], bits);
+            const int32_t at = e[u] >= 0 ? start[e[u]] + mine[e[u]] + __popc(same & ((1u << lane) - 1u)) : -1;
+            __syncwarp();
+            if (e[u] >= 0 && lane == __ffs(same) - 1) mine[e[u]] += __popc(same);
+            __syncwarp();
+            if (i < a1) {
+                pos[i] = at;
+                if (at >= 0) perm[at] = (int32_t)i;
+            }
         }
     }
     for (long long i = before + (long long)rank * blockDim.x + threadIdx.x; i < n; i += (long long)C * blockDim.x)
         perm[i] = -1;
+    if (C > 1) cluster.barrier_wait();   // and they this one's
 }
 
 // ------------------------------------------------------------ rows out and back
@@ -425,158 +458,202 @@ gather_rows_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* _
     }
 }
 
-// out[t] = add[t] + sum_j w[t, j] rows[pos[t, j]], in slot order; w NULL: 1
+// out[t] = add[t] + sum_j w[t, j] rows[pos[t, j]], in slot order; w NULL: 1.
+// The CTAs walk the tokens; a token's first positions and weights come while
+// the one before it is summed up (a lane holds a slot's), so one wait for
+// memory a token is left.
 template <typename T>
 __global__ void __launch_bounds__(256, 4)
 combine_rows_kernel(const T* __restrict__ rows, long long ld_rows, uint32_t n_rows, const int32_t* __restrict__ pos,
-                    const float* __restrict__ w, int k, int d, const T* __restrict__ add, long long ld_add,
+                    const float* __restrict__ w, int tokens, int k, int d, const T* __restrict__ add, long long ld_add,
                     T* __restrict__ out, long long ld_out, bool wide) {
     constexpr int S = sizeof(T) == 4 ? 4 : 8;   // rows whose loads are in flight: 32 registers
-    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, d);
-    if (!n) return;
-    pos += (size_t)t * k;
-    if (w) w += (size_t)t * k;
-    Pairs8 acc;
-#pragma unroll
-    for (int i = 0; i < 4; i++) acc.p[i] = 0;
-    Raw8<T> first;
-    if (add) first = load_raw8(add + t * ld_add + c, n, wide);
-    for (int j0 = 0; j0 < k; j0 += S) {
-        Raw8<T> r[S];
-        float wj[S];
-        uint32_t held = 0;
-#pragma unroll
-        for (int j = 0; j < S; j++) {
-            if (j0 + j >= k) break;
-            const uint32_t p = pos[j0 + j];
-            if (p >= n_rows) continue;
-            held |= 1u << j;
-            r[j] = load_raw8(rows + p * ld_rows + c, n, wide);
-            wj[j] = w ? w[j0 + j] : 1.f;
+    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, d), lane = threadIdx.x & 31;
+    int t = blockIdx.x;
+    uint32_t p_next = ~0u;
+    float w_next = 1.f;
+    auto ahead = [&](int at) {   // slots lane < min(k, S) of token `at`
+        if (at < tokens && lane < S && lane < k) {
+            p_next = pos[(size_t)at * k + lane];
+            if (w) w_next = w[(size_t)at * k + lane];
         }
-        if (add && j0 == 0) acc = values8(first);
+    };
+    ahead(t);
+    for (; t < tokens; t += gridDim.x) {
+        Pairs8 acc;
 #pragma unroll
-        for (int j = 0; j < S; j++)
-            if (held >> j & 1) {
-                const Pair wp = pair(wj[j], wj[j]);
-                const Pairs8 v = values8(r[j]);
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc.p[i] = fma2(wp, v.p[i], acc.p[i]);
+        for (int i = 0; i < 4; i++) acc.p[i] = 0;
+        Raw8<T> first;
+        if (add) first = load_raw8(add + t * ld_add + c, n, wide);
+        for (int j0 = 0; j0 < k; j0 += S) {
+            uint32_t p_lane = p_next;
+            float w_lane = w_next;
+            if (j0) {
+                const int j = j0 + lane;
+                p_lane = lane < S && j < k ? (uint32_t)pos[(size_t)t * k + j] : ~0u;
+                w_lane = w && lane < S && j < k ? w[(size_t)t * k + j] : 1.f;
             }
-    }
-    Vec8 o;
+            Raw8<T> r[S];
+            uint32_t held = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 f = unpair(acc.p[i]);
-        o.v[2 * i] = f.x;
-        o.v[2 * i + 1] = f.y;
+            for (int j = 0; j < S; j++) {
+                const uint32_t p = __shfl_sync(0xffffffffu, p_lane, j);
+                if (j0 + j >= k || p >= n_rows) continue;
+                held |= 1u << j;
+                r[j] = load_raw8(rows + p * ld_rows + c, n, wide);
+            }
+            if (j0 == 0) {
+                ahead(t + gridDim.x);
+                if (add) acc = values8(first);
+            }
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                const float wj = __shfl_sync(0xffffffffu, w_lane, j);
+                if (held >> j & 1) {
+                    const Pair wp = pair(wj, wj);
+                    const Pairs8 v = values8(r[j]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc.p[i] = fma2(wp, v.p[i], acc.p[i]);
+                }
+            }
+        }
+        Vec8 o;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = unpair(acc.p[i]);
+            o.v[2 * i] = f.x;
+            o.v[2 * i + 1] = f.y;
+        }
+        store8(out + t * ld_out + c, o, n, wide);
     }
-    store8(out + t * ld_out + c, o, n, wide);
 }
 
 // The gradient of combine_rows: drows[pos[t, j]] = w[t, j] dout[t] (T or 8
-// bits) and dw[t, j] = <dout[t], rows[pos[t, j]]>.  One CTA per token: dw
-// needs the whole row.  Eight slots at a time, whose sums stay in registers.
+// bits) and dw[t, j] = <dout[t], rows[pos[t, j]]>.  One CTA per token, up to
+// eight slots at a time, one or more of the eight warps to a slot, so a slot's
+// sum stays in its warps and a thread has few registers (which keeps enough
+// loads in flight).  dout goes through shared memory, 8192 columns at a time.
 // Rounding does not change an order, so the largest magnitude of w dout is the
 // rounded product of |w| and dout's: it is looked for once for all slots, and
-// the eight slots' scales and reciprocals are computed by eight lanes of the
-// half warp, one each, and handed round.
-template <typename T, bool FP8>
-__global__ void __launch_bounds__(512, 2)
+// each (slot, block)'s scale and reciprocal are computed by one thread.
+constexpr int kGradCols = 8192;
+
+// FAST: every row of every array starts on its widest access, d is a multiple of 8
+template <typename T, bool FP8, bool FAST>
+__global__ void __launch_bounds__(256)
 combine_grad_kernel(const T* __restrict__ dout, long long ld_dout, const T* __restrict__ rows, long long ld_rows,
                     uint32_t n_rows, const int32_t* __restrict__ pos, const float* __restrict__ w, int k, int d,
                     T* __restrict__ drows, uint8_t* __restrict__ codes, long long ld_d, float* __restrict__ scales,
                     long long ld_s, float* __restrict__ dw, bool wide, bool wide_d) {
-    constexpr int S = 8, B = sizeof(T) == 4 ? 2 : 4;   // slots; rows whose loads are in flight
-    __shared__ float part[S][16];
-    __shared__ uint32_t at[S];   // the slots' rows
-    __shared__ float wn[S];      // minus their weights
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    constexpr int S = 8, NB = kGradCols / kFp8Block;
+    constexpr int U = sizeof(T) == 4 ? 2 : 4;   // row loads in flight
+    extern __shared__ float4 g_sm[];            // min(d, kGradCols) columns of dout, in whole blocks
+    __shared__ float amax[NB];
+    __shared__ float2 sc[S][NB];                // scale, minus its reciprocal
+    __shared__ float part[S];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int t = blockIdx.x;
     pos += (size_t)t * k;
     if (w) w += (size_t)t * k;
     dout += t * ld_dout;
     for (int j0 = 0; j0 < k; j0 += S) {
-        Pair dot[S];
+        const int slots = min(S, k - j0), each = S / slots;   // warps to a slot
+        const int slot = warp / each, mine = warp - slot * each;
+        const bool busy = slot < slots;
+        const uint32_t p = busy ? (uint32_t)pos[j0 + slot] : ~0u;
+        const bool held = p < n_rows;
+        const float wn = !busy ? 0.f : w ? -w[j0 + slot] : -1.f;   // minus the weight
+        Pair dot = 0;
+        for (int base = 0; base < d; base += kGradCols) {
+            const int cols = min(kGradCols, d - base), blocks = (cols + kFp8Block - 1) / kFp8Block;
+            for (int c = threadIdx.x * 8; c < blocks * kFp8Block; c += 256 * 8) {   // whole half warps
+                const Pairs8 g = values8(load_raw8(dout + base + c, columns_at(c, cols), wide));
 #pragma unroll
-        for (int j = 0; j < S; j++) dot[j] = 0;
-        if (threadIdx.x < S) {
-            const int j = j0 + threadIdx.x;
-            at[threadIdx.x] = j < k ? (uint32_t)pos[j] : ~0u;
-            wn[threadIdx.x] = j >= k ? 0.f : w ? -w[j] : -1.f;
-        }
-        __syncthreads();
-        const int mine = j0 + (lane & 7);
-        const float w_lane = !FP8 || mine >= k ? 0.f : w ? fabsf(w[mine]) : 1.f;
-        for (int c0 = 0; c0 < d; c0 += blockDim.x * 8) {
-            const int c = c0 + threadIdx.x * 8, n = columns_at(c, d);
-            const Raw8<T> g_raw = load_raw8(dout + c, n, wide);
-            float s_lane = 0.f, r_lane = 0.f;
-#pragma unroll
-            for (int jb = 0; jb < S; jb += B) {
-                Raw8<T> r[B];
-                if (dw)
-#pragma unroll
-                    for (int j = 0; j < B; j++)
-                        if (at[jb + j] < n_rows) r[j] = load_raw8(rows + at[jb + j] * ld_rows + c, n, wide);
-                const Pairs8 g = values8(g_raw);
-                if (FP8 && jb == 0) {
-                    s_lane = block_scale(__fmul_rn(w_lane, half_warp_max(amax8(g))));
-                    r_lane = -1.f / s_lane;
+                for (int i = 0; i < 2; i++) {
+                    const float2 x = unpair(g.p[2 * i]), y = unpair(g.p[2 * i + 1]);
+                    g_sm[c / 4 + i] = make_float4(x.x, x.y, y.x, y.y);
                 }
+                if constexpr (FP8) {
+                    float m = amax8(g);   // a half warp's columns are one block: its threads stay together
 #pragma unroll
-                for (int u = 0; u < B; u++) {
-                    const int j = jb + u;
-                    const uint32_t p = at[j];
-                    if (p >= n_rows) continue;   // the same for all threads of the CTA
-                    Pairs8 v;   // minus w dout
-                    const Pair wp = pair(wn[j], wn[j]);
+                    for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffu << (lane & 16), m, o));
+                    if ((lane & 15) == 0) amax[c / kFp8Block] = m;
+                }
+            }
+            __syncthreads();
+            if constexpr (FP8) {
+                for (int i = threadIdx.x; i < slots * blocks; i += 256) {
+                    const int j = i / blocks, b = i - j * blocks;
+                    const float s = block_scale(__fmul_rn(w ? fabsf(w[j0 + j]) : 1.f, amax[b]));
+                    sc[j][b] = make_float2(s, -1.f / s);
+                    const uint32_t q = pos[j0 + j];
+                    if (q < n_rows) scales[q * ld_s + base / kFp8Block + b] = s;
+                }
+                __syncthreads();
+            }
+            if (held) {
+                const Pair wp = pair(wn, wn);
+                const T* from = rows + p * ld_rows + base;
+                for (int c0 = (mine * 32 + lane) * 8; c0 < cols; c0 += each * 256 * U) {
+                    Raw8<T> r[U];
+                    if (dw)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) v.p[i] = mul2(wp, g.p[i]);
-                    if constexpr (FP8) {
-                        const float s = __shfl_sync(0xffffffffu, s_lane, j, 16), q = __shfl_sync(0xffffffffu, r_lane, j, 16);
-                        if (n) {
-                            store_codes8(codes + p * ld_d + c, codes8(v, Quant{pair(s, s), pair(q, q)}), n, wide_d);
-                            if ((threadIdx.x & 15) == 0) scales[p * ld_s + c / kFp8Block] = s;
+                        for (int u = 0; u < U; u++) {
+                            const int c = c0 + u * each * 256;
+                            if (!FAST) r[u] = load_raw8(from + c, columns_at(c, cols), wide);
+                            else if (c < cols) r[u] = load_raw8(from + c, 8, true);
                         }
-                    } else if (n) {
-                        Vec8 o;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float2 f = unpair(v.p[i]);
-                            o.v[2 * i] = -f.x;
-                            o.v[2 * i + 1] = -f.y;
+                    for (int u = 0; u < U; u++) {
+                        const int c = c0 + u * each * 256, n = FAST ? 8 : columns_at(c, cols);
+                        if (c >= cols) break;
+                        Pairs8 g;
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const float4 x = g_sm[c / 4 + i];
+                            g.p[2 * i] = pair(x.x, x.y);
+                            g.p[2 * i + 1] = pair(x.z, x.w);
                         }
-                        store8(drows + p * ld_d + c, o, n, wide_d);
-                    }
-                    if (dw) {
-                        const Pairs8 x = values8(r[u]);
+                        Pairs8 v;   // minus w dout
 #pragma unroll
-                        for (int i = 0; i < 4; i++) dot[j] = fma2(g.p[i], x.p[i], dot[j]);
+                        for (int i = 0; i < 4; i++) v.p[i] = mul2(wp, g.p[i]);
+                        if constexpr (FP8) {
+                            const float2 s = sc[slot][c / kFp8Block];
+                            store_codes8(codes + p * ld_d + base + c, codes8(v, Quant{pair(s.x, s.x), pair(s.y, s.y)}), n, FAST || wide_d);
+                        } else {
+                            Vec8 o;
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const float2 f = unpair(v.p[i]);
+                                o.v[2 * i] = -f.x;
+                                o.v[2 * i + 1] = -f.y;
+                            }
+                            store8(drows + p * ld_d + base + c, o, n, FAST || wide_d);
+                        }
+                        if (dw) {
+                            const Pairs8 x = values8(r[u]);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) dot = fma2(g.p[i], x.p[i], dot);
+                        }
                     }
                 }
             }
+            __syncthreads();   // before the next columns, or slots
         }
-        if (!dw) {
-            __syncthreads();   // before the next slots' rows
-            continue;
-        }
-#pragma unroll
-        for (int j = 0; j < S; j++) {
-            const float2 f = unpair(dot[j]);
+        if (dw) {
+            const float2 f = unpair(dot);
             float sum = f.x + f.y;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) part[j][warp] = sum;
+            if (lane == 0) part[warp] = sum;
+            __syncthreads();
+            if (threadIdx.x < slots) {
+                float v = 0.f;
+                for (int i = 0; i < each; i++) v += part[threadIdx.x * each + i];
+                dw[(size_t)t * k + j0 + threadIdx.x] = v;   // 0 for a slot without a row
+            }
+            __syncthreads();
         }
-        __syncthreads();
-        if (warp < S && j0 + warp < k) {
-            float v = lane < warps ? part[warp][lane] : 0.f;
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-            if (lane == 0) dw[(size_t)t * k + j0 + warp] = v;   // 0 for a slot without a row
-        }
-        __syncthreads();
     }
 }
 
@@ -637,83 +714,143 @@ quantize_fp8_weights_kernel(const T* __restrict__ w, int rows, int cols, uint8_t
 //   h = g sigma(g) u
 //   dg = dh u (sigma(g) + g sigma(g) (1 - sigma(g))), 0 where the gate was cut off
 //   du = dh g sigma(g), 0 where up was cut off
-struct Swiglu {
-    float g, u, sig;
-    bool g_in, u_in;
+// Two columns at a time.  sigma(g) = num / (1 + e) with e = exp(-|g|), which
+// never overflows, and num = 1 or e by g's sign.  e is 2^x for x = -|g| log2 e
+// with the rounding of that product made good (x + lo is exact to 2^-45 or so),
+// so only the two approximate instructions' own errors remain (2 ulp and 1 ulp).
+struct Swiglu2 {
+    Pair g, u, sig;   // after the cut-offs
 };
-__device__ __forceinline__ Swiglu swiglu_parts(float gate, float up, float limit) {
-    Swiglu r;
-    r.g_in = r.u_in = true;
-    r.g = gate;
-    r.u = up;
-    if (limit > 0.f) {
-        r.g_in = !(gate > limit);
-        r.u_in = !(fabsf(up) > limit);
-        if (!r.g_in) r.g = limit;                       // a NaN stays one
-        if (!r.u_in) r.u = copysignf(limit, up);
-    }
-    const float e = expf(-fabsf(r.g));   // never overflows
-    r.sig = __fdividef(r.g < 0.f ? e : 1.f, 1.f + e);   // the divisor is in [1, 2]: within 2 ulp
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = (float)(1.4426950408889634074 - (double)kLog2e);
+constexpr float kLn2 = 0.6931471805599453f;
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float reciprocal_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <bool LIMIT>
+__device__ __forceinline__ Swiglu2 swiglu2(float2 gate, float2 up, float limit) {
+    if (LIMIT) {   // a NaN stays one
+        gate = make_float2(min_nan(gate.x, limit), min_nan(gate.y, limit));
+        up = make_float2(max_nan(min_nan(up.x, limit), -limit), max_nan(min_nan(up.y, limit), -limit));
+    }
+    const Pair n = pair(-fabsf(gate.x), -fabsf(gate.y)), l2e = pair(kLog2e, kLog2e);
+    const Pair x = mul2(n, l2e);
+    const float2 xf = unpair(x);
+    const Pair lo = fma2(n, pair(kLog2eLow, kLog2eLow), fma2(n, l2e, pair(-xf.x, -xf.y)));
+    const Pair e0 = pair(exp2_approx(xf.x), exp2_approx(xf.y));
+    const float2 e = unpair(fma2(mul2(e0, lo), pair(kLn2, kLn2), e0));
+    const float2 r = make_float2(reciprocal_approx(1.f + e.x), reciprocal_approx(1.f + e.y));
+    Swiglu2 s;
+    s.g = pair(gate.x, gate.y);
+    s.u = pair(up.x, up.y);
+    s.sig = mul2(pair(gate.x < 0.f ? e.x : 1.f, gate.y < 0.f ? e.y : 1.f), pair(r.x, r.y));
+    return s;
+}
+__device__ __forceinline__ Pair negative(Pair p) { return p ^ 0x8000000080000000ull; }
 
-template <typename T>
+// The CTAs walk the rows; a row's loads are on their way while the one before
+// it is computed.
+template <typename T, bool LIMIT>
 __global__ void __launch_bounds__(256)
-swiglu_fp8_kernel(const T* __restrict__ gu, long long ld, const int32_t* __restrict__ n_dev, int f, float limit,
+swiglu_fp8_kernel(const T* __restrict__ gu, long long ld, int rows, const int32_t* __restrict__ n_dev, int f, float limit,
                   uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales, long long ld_s, bool wide,
                   bool wide_c) {
-    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
-    if (n_dev && t >= *n_dev) return;
-    gu += t * ld + c;
-    const Raw8<T> g = load_raw8(gu, n, wide), u = load_raw8(gu + f, n, wide);   // absent columns are 0, and so is h there
-    Pairs8 h;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float v[2];
-#pragma unroll
-        for (int q = 0; q < 2; q++) {
-            const Swiglu p = swiglu_parts(column(g, 2 * i + q), column(u, 2 * i + q), limit);
-            v[q] = p.g * p.sig * -p.u;
+    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
+    if (n_dev) rows = min(rows, *n_dev);
+    int t = blockIdx.x;
+    if (t >= rows) return;
+    gu += c;
+    Raw8<T> g = load_raw8(gu + t * ld, n, wide), u = load_raw8(gu + t * ld + f, n, wide);   // absent columns are 0, and h there
+    for (;;) {
+        const int next = t + gridDim.x;
+        Raw8<T> g1 = g, u1 = u;
+        if (next < rows) {
+            g1 = load_raw8(gu + next * ld, n, wide);
+            u1 = load_raw8(gu + next * ld + f, n, wide);
         }
-        h.p[i] = pair(v[0], v[1]);
+        Pairs8 h;   // negated
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const Swiglu2 p = swiglu2<LIMIT>(make_float2(column(g, 2 * i), column(g, 2 * i + 1)),
+                                             make_float2(column(u, 2 * i), column(u, 2 * i + 1)), limit);
+            h.p[i] = mul2(mul2(p.g, p.sig), negative(p.u));
+        }
+        const float s = block_scale(half_warp_max(amax8(h)));
+        if (n) {
+            store_codes8(codes + t * ld_c + c, codes8(h, quant(s)), n, wide_c);
+            if ((threadIdx.x & 15) == 0) scales[t * ld_s + c / kFp8Block] = s;
+        }
+        if (next >= rows) return;
+        t = next;
+        g = g1;
+        u = u1;
     }
-    const float s = block_scale(half_warp_max(amax8(h)));
-    if (!n) return;
-    store_codes8(codes + t * ld_c + c, codes8(h, quant(s)), n, wide_c);
-    if ((threadIdx.x & 15) == 0) scales[t * ld_s + c / kFp8Block] = s;
 }
 
 // f is a multiple of 128 here, so no block of the 2f columns holds both halves
-template <typename T>
+template <typename T, bool LIMIT>
 __global__ void __launch_bounds__(256)
-swiglu_fp8_grad_kernel(const T* __restrict__ gu, long long ld, const T* __restrict__ dh, long long ld_dh,
+swiglu_fp8_grad_kernel(const T* __restrict__ gu, long long ld, const T* __restrict__ dh, long long ld_dh, int rows,
                        const int32_t* __restrict__ n_dev, int f, float limit, uint8_t* __restrict__ codes, long long ld_c,
                        float* __restrict__ scales, long long ld_s, bool wide, bool wide_c) {
-    const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
-    if (n_dev && t >= *n_dev) return;
-    gu += t * ld + c;
-    const Raw8<T> g = load_raw8(gu, n, wide), u = load_raw8(gu + f, n, wide), d = load_raw8(dh + t * ld_dh + c, n, wide);
-    Pairs8 dg, du;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float a[2], b[2];
-#pragma unroll
-        for (int q = 0; q < 2; q++) {
-            const Swiglu p = swiglu_parts(column(g, 2 * i + q), column(u, 2 * i + q), limit);
-            const float nd = -column(d, 2 * i + q);
-            a[q] = p.g_in ? nd * p.u * (p.sig * fmaf(p.g, 1.f - p.sig, 1.f)) : 0.f;
-            b[q] = p.u_in ? nd * (p.g * p.sig) : 0.f;
+    const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
+    if (n_dev) rows = min(rows, *n_dev);
+    int t = blockIdx.x;
+    if (t >= rows) return;
+    gu += c;
+    dh += c;
+    Raw8<T> g = load_raw8(gu + t * ld, n, wide), u = load_raw8(gu + t * ld + f, n, wide), d = load_raw8(dh + t * ld_dh, n, wide);
+    for (;;) {
+        const int next = t + gridDim.x;
+        Raw8<T> g1 = g, u1 = u, d1 = d;
+        if (next < rows) {
+            g1 = load_raw8(gu + next * ld, n, wide);
+            u1 = load_raw8(gu + next * ld + f, n, wide);
+            d1 = load_raw8(dh + next * ld_dh, n, wide);
         }
-        dg.p[i] = pair(a[0], a[1]);
-        du.p[i] = pair(b[0], b[1]);
-    }
-    const float sg = block_scale(half_warp_max(amax8(dg))), su = block_scale(half_warp_max(amax8(du)));
-    if (!n) return;
-    store_codes8(codes + t * ld_c + c, codes8(dg, quant(sg)), n, wide_c);
-    store_codes8(codes + t * ld_c + f + c, codes8(du, quant(su)), n, wide_c);
-    if ((threadIdx.x & 15) == 0) {
-        scales[t * ld_s + c / kFp8Block] = sg;
-        scales[t * ld_s + (f + c) / kFp8Block] = su;
+        Pairs8 dg, du;   // negated
+        const Pair one = pair(1.f, 1.f), minus = pair(-1.f, -1.f);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 gate = make_float2(column(g, 2 * i), column(g, 2 * i + 1)), up = make_float2(column(u, 2 * i), column(u, 2 * i + 1));
+            const Swiglu2 p = swiglu2<LIMIT>(gate, up, limit);
+            const Pair nd = pair(-column(d, 2 * i), -column(d, 2 * i + 1));
+            // u sigma (1 + g (1 - sigma)) and g sigma, times minus dh
+            dg.p[i] = mul2(mul2(nd, p.u), mul2(p.sig, fma2(p.g, fma2(p.sig, minus, one), one)));
+            du.p[i] = mul2(nd, mul2(p.g, p.sig));
+            if (LIMIT) {   // nothing comes back through a cut-off
+                float2 a = unpair(dg.p[i]), b = unpair(du.p[i]);
+                a = make_float2(gate.x > limit ? 0.f : a.x, gate.y > limit ? 0.f : a.y);
+                b = make_float2(fabsf(up.x) > limit ? 0.f : b.x, fabsf(up.y) > limit ? 0.f : b.y);
+                dg.p[i] = pair(a.x, a.y);
+                du.p[i] = pair(b.x, b.y);
+            }
+        }
+        const float sg = block_scale(half_warp_max(amax8(dg))), su = block_scale(half_warp_max(amax8(du)));
+        if (n) {
+            store_codes8(codes + t * ld_c + c, codes8(dg, quant(sg)), n, wide_c);
+            store_codes8(codes + t * ld_c + f + c, codes8(du, quant(su)), n, wide_c);
+            if ((threadIdx.x & 15) == 0) {
+                scales[t * ld_s + c / kFp8Block] = sg;
+                scales[t * ld_s + (f + c) / kFp8Block] = su;
+            }
+        }
+        if (next >= rows) return;
+        t = next;
+        g = g1;
+        u = u1;
+        d = d1;
     }
 }
 
