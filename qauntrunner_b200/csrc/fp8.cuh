@@ -76,6 +76,19 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 }
 // 16 / 32 columns of this warp's 32 tensor-memory lanes; the wait is part of
 // the statement, so nothing that uses the registers can move before it
+__device__ __forceinline__ void tmem_ld16_now(uint32_t taddr, float* v) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
     uint32_t r[32];
     asm volatile(
@@ -90,32 +103,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
         : "memory");
 #pragma unroll
     for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-}
-
-// 32 columns of this warp's 32 tensor-memory lanes, in two steps: the load goes
-// on while other work is done, and the wait names the registers, so nothing
-// that uses them can move before it (it waits for all loads of the warp)
-__device__ __forceinline__ void tmem_ld32_begin(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
-          "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
-          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
-          "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld32_end(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
 }
 
 template <typename T> __device__ __forceinline__ T round_to(float v);
@@ -505,7 +492,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
                     }
                 } else if (n > 0) {
                     float v[16];
-                    tmem_ld16(from, v);
+                    tmem_ld16_now(from, v);
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         const float4 w = sc[c];
@@ -914,22 +901,19 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                 const float f = sc_ring[sr.i * kFp8PairScaleSlot + j * 256 + 128 * half + row];
                 const float2 f2 = make_float2(f, f);
                 const uint32_t from = taddr + 128 * a.i;
-                uint32_t v[2][32];
-                tmem_ld32_begin(from, v[0]);
+                // (16 columns at a time: with the next load issued before a load's sums, or 32 and 64 at a time, it was
+                // 430 to 527 us in place of 428 at 4096 x 28672 x 4096: the scheduler's other warp fills the gaps)
 #pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    tmem_ld32_end(v[h & 1]);
-                    if (h < 3) {
-                        tmem_ld32_begin(from + 32 * (h + 1), v[(h + 1) & 1]);
-                    } else {   // all of it is in registers
+                for (int h = 0; h < 8; h++) {
+                    float v[16];
+                    tmem_ld16_now(from + 16 * h, v);
+                    if (h == 7) {   // all of it is in registers
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) bar_arrive_cluster(acc_empty0 + 8 * a.i);
                     }
 #pragma unroll
-                    for (int c = 0; c < 16; c++)
-                        acc[16 * h + c] = ffma2(make_float2(__uint_as_float(v[h & 1][2 * c]), __uint_as_float(v[h & 1][2 * c + 1])), f2,
-                                                acc[16 * h + c]);
+                    for (int c = 0; c < 8; c++) acc[8 * h + c] = ffma2(make_float2(v[2 * c], v[2 * c + 1]), f2, acc[8 * h + c]);
                 }
                 if (j == 3 || kb + 1 == KB) {
                     if (lane == 0) bar_arrive(sc_empty0 + 8 * sr.i);
