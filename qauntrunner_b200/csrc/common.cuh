@@ -90,6 +90,12 @@ static inline cudaError_t set_wait_limit_here(uint64_t ns) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// both, for kernels that do nothing before: the next may be scheduled, the one before is over
+__device__ __forceinline__ void pdl_start() {
+    pdl_trigger();
+    pdl_wait();
+}
+
 // Device-side error flag bits, read back by qrm_sync().
 enum : uint32_t { ERR_TIMEOUT = 1u, ERR_BOUNDS = 2u, ERR_INTERNAL = 4u };
 

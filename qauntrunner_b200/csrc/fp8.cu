@@ -204,14 +204,14 @@ int product(const char* what, qrm_fp8* m, bool back, const void* x, int64_t ld_x
     if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
     if (pair) {
         const int wide_out = aligned(out, 32) && ld_out * b % 32 == 0, wide_xs = aligned(xs, 16) && ld_xs % 4 == 0;
-        fp8_pair_kernel<<<m->sms / 2 * 2, kFp8Warps * 32, pair_smem(m->groups), (cudaStream_t)stream>>>(
-            back ? m->pair_map_t : m->pair_map, x_map, p, wide_out, wide_xs);
-        return launched(what);
+        e = launch_ahead(fp8_pair_kernel, dim3(m->sms / 2 * 2), kFp8Warps * 32, pair_smem(m->groups), (cudaStream_t)stream,
+                         back ? m->pair_map_t : m->pair_map, x_map, p, wide_out, wide_xs);
+        return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
     }
     const int x_rows = (int)std::min<int64_t>(kFp8MaxRows, (T + 15) / 16 * 16);
-    fp8_stream_kernel<<<m->sms, kFp8Warps * 32, smem_for(m->groups, x_rows), (cudaStream_t)stream>>>(
-        m->map, x_map, p, stages_for(m->groups, x_rows), x_rows);
-    return launched(what);
+    e = launch_ahead(fp8_stream_kernel, dim3(m->sms), kFp8Warps * 32, smem_for(m->groups, x_rows), (cudaStream_t)stream, m->map,
+                     x_map, p, stages_for(m->groups, x_rows), x_rows);
+    return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
 }
 
 }  // namespace

@@ -209,7 +209,8 @@ struct Fp8Plan {
     int groups, mb, kb;
     long long total;             // blocks of all tiles
     int ctas;                    // that share them, at most `total`
-    __device__ long long cut(int c) const { return total * c / ctas; }
+    bool whole;                  // no tile is shared
+    __device__ long long cut(int c) const { return whole ? total / kb * c / ctas * kb : total * c / ctas; }
     // the CTA whose run holds block q
     __device__ int owner(long long q) const { return (int)(((q + 1) * ctas - 1) / total); }
     __device__ Fp8Piece piece(long long q, long long q_end) const {
@@ -235,6 +236,32 @@ struct Fp8Plan {
         return r;
     }
 };
+
+// How `tiles` tiles of kb blocks are shared out.  Parts of a tile have to be
+// announced and added up, which costs about 6 us (16 blocks), 3 of them for the
+// second part where a CTA has parts of two.  So
+// - with fewer tiles than CTAs, each tile gets the same whole number of CTAs,
+//   unless that gives the busiest CTA 8 blocks more than an even share (one
+//   row through 4096 x 7168: 11.4 us in place of 14.9);
+// - with more, CTAs take whole tiles, unless that is 16 blocks more;
+// - otherwise all blocks in equal runs, kFp8MinRun at least.
+__device__ inline void fp8_share_out(Fp8Plan& plan, int tiles, int kb, int ctas) {
+    plan.total = (long long)tiles * kb;
+    plan.whole = false;
+    const long long even = (plan.total + ctas - 1) / ctas;
+    if (tiles > 0 && tiles <= ctas) {
+        const int each = max(1, min(ctas / tiles, kb / kFp8MinRun));
+        if ((kb + each - 1) / each <= even + 8) {
+            plan.ctas = tiles * each;
+            return;
+        }
+    } else if (tiles > ctas && (long long)((tiles + ctas - 1) / ctas) * kb <= even + 16) {
+        plan.ctas = ctas;
+        plan.whole = true;
+        return;
+    }
+    plan.ctas = (int)min((long long)ctas, (plan.total + kFp8MinRun - 1) / kFp8MinRun);
+}
 
 // The groups' tables in shared memory, by one warp; the caller synchronises.
 // Offsets that do not ascend within [0, T] make a group empty and raise an
@@ -339,6 +366,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
         fence_barrier_init();
     }
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
+    pdl_start();   // nothing before this reads or writes global memory
     if (warp == 2) fp8_tables(p, first_tile, start, rows, kFp8MaxRows, p.mb, blockIdx.x == 0);
     tc_fence_before();
     __syncthreads();
@@ -347,9 +375,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     const Fp8Ctl ctl{abort_flag, p.err};
     const uint32_t full0 = smem_u32(full), done0 = smem_u32(done), acc_empty0 = smem_u32(acc_empty);
     const uint32_t sc_full0 = smem_u32(sc_full), sc_empty0 = smem_u32(sc_empty);
-    Fp8Plan plan{first_tile, start, rows, p.groups, p.mb, p.kb, (long long)first_tile[p.groups] * p.kb, 0};
-    // a CTA has kFp8MinRun blocks at least, unless there are fewer in all
-    plan.ctas = (int)min((long long)gridDim.x, (plan.total + kFp8MinRun - 1) / kFp8MinRun);
+    Fp8Plan plan{first_tile, start, rows, p.groups, p.mb, p.kb};
+    fp8_share_out(plan, first_tile[p.groups], p.kb, gridDim.x);
     const bool idle = (int)blockIdx.x >= plan.ctas;
     const long long q0 = idle ? 0 : plan.cut(blockIdx.x), q1 = idle ? 0 : plan.cut(blockIdx.x + 1);
 
@@ -733,6 +760,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
+    pdl_start();   // nothing before this reads or writes global memory
     if (warp == 2) fp8_tables(p, first_tile, start, rows, 256, (p.M + 255) / 256, blockIdx.x == 0);
     tc_fence_before();
     __syncthreads();

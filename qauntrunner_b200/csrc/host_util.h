@@ -55,9 +55,25 @@ inline bool pitch_ok(int64_t* ld, int64_t cols) {
 
 inline bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-inline int launched(const char* what) {
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+// A launch whose CTAs may start while the kernel before it in the stream still
+// runs (programmatic dependent launch): every kernel of these units begins
+// with pdl_start(), which lets the next one start likewise and then waits for
+// the one before, in every CTA, so that waiting for a kernel means waiting for
+// all that came before it.  Back to back, the launch and the set-up are hidden
+// behind the other kernel's end (one row through 4096 x 7168: REPLACE us).
+template <typename... P, typename... A>
+cudaError_t launch_ahead(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute at = {};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
 }  // namespace qrm

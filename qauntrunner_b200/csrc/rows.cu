@@ -75,6 +75,10 @@ int check_ints(const char* what, const char* name, const void* p) {
         else { using V = __nv_bfloat16; __VA_ARGS__; }      \
     } while (0)
 
+int done(const char* what, cudaError_t e) {
+    return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+}
+
 int64_t blocks_of(int64_t cols) { return (cols + kFp8Block - 1) / kFp8Block; }
 
 }  // namespace
@@ -98,6 +102,7 @@ extern "C" int qrm_sort_tokens(const int32_t* topk_idx_dev, int64_t T, int k, in
     }
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     const int64_t n = T * k;
     const bool many = n > 4096;
     const int warps = (int)std::min<int64_t>(32, std::max<int64_t>(8, (n + 255) / 256 * 8));
@@ -108,20 +113,22 @@ extern "C" int qrm_sort_tokens(const int32_t* topk_idx_dev, int64_t T, int k, in
     cfg.blockDim = dim3(32 * warps);
     cfg.dynamicSmemBytes = sizeof(int32_t) * (size_t)(2 + warps) * n_experts;
     cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute at = {};
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = cfg.gridDim.x;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cfg.gridDim.x;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // as in launch_ahead
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
     auto kernel = many ? sort_tokens_kernel<kSortCluster> : sort_tokens_kernel<1>;
-    cudaError_t e = cudaSuccess;
+    e = cudaSuccess;
     if (cfg.dynamicSmemBytes > 48 * 1024)
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)(sizeof(int32_t) * 34 * kSortMaxExperts));
     if (e == cudaSuccess)
         e = cudaLaunchKernelEx(&cfg, kernel, topk_idx_dev, (long long)n, first, n_experts, bits, perm_dev, pos_dev, offsets_dev);
-    return e == cudaSuccess ? launched(what) : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+    return done(what, e);
 }
 
 extern "C" int qrm_gather_rows(int type, const void* x_dev, int64_t ld_x, const int32_t* pos_dev, int64_t T, int k,
@@ -136,11 +143,11 @@ extern "C" int qrm_gather_rows(int type, const void* x_dev, int64_t ld_x, const 
     TRY(check_ints(what, "pos", pos_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     const Cut c = cut_columns(T, d, 8);
     const bool wide = wide_rows(x_dev, ld_x, b) && wide_rows(rows_dev, ld_rows, b);
-    BY_TYPE(type, gather_rows_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)x_dev, ld_x, pos_dev, k, (int)d, (uint32_t)n_rows, (V*)rows_dev, ld_rows, wide));
-    return launched(what);
+    BY_TYPE(type, e = launch_ahead(gather_rows_kernel<V>, c.grid, c.threads, 0, (cudaStream_t)stream, (const V*)x_dev, ld_x, pos_dev, k, (int)d, (uint32_t)n_rows, (V*)rows_dev, ld_rows, wide));
+    return done(what, e);
 }
 
 extern "C" int qrm_gather_rows_fp8(int type, const void* x_dev, int64_t ld_x, const int32_t* pos_dev, int64_t T, int k,
@@ -157,11 +164,11 @@ extern "C" int qrm_gather_rows_fp8(int type, const void* x_dev, int64_t ld_x, co
     TRY(check_ints(what, "pos", pos_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     const Cut c = cut_columns(T, d, 16);
-    BY_TYPE(type, gather_rows_fp8_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)x_dev, ld_x, pos_dev, k, (int)d, (uint32_t)n_rows, codes_dev, ld_codes, scales_dev,
+    BY_TYPE(type, e = launch_ahead(gather_rows_fp8_kernel<V>, c.grid, c.threads, 0, (cudaStream_t)stream, (const V*)x_dev, ld_x, pos_dev, k, (int)d, (uint32_t)n_rows, codes_dev, ld_codes, scales_dev,
                       ld_scales, wide_rows(x_dev, ld_x, b), wide_codes16(codes_dev, ld_codes)));
-    return launched(what);
+    return done(what, e);
 }
 
 extern "C" int qrm_combine_rows(int type, const void* rows_dev, int64_t n_rows, int64_t ld_rows, const int32_t* pos_dev,
@@ -179,14 +186,14 @@ extern "C" int qrm_combine_rows(int type, const void* rows_dev, int64_t n_rows, 
     if (w_dev) TRY(check_ints(what, "w", w_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     Cut c = cut_columns(T, d, 8);
     c.grid.x = walkers(T, c.grid.y, sms, 4 * 256 / c.threads);
     const bool wide = wide_rows(rows_dev, ld_rows, b) && wide_rows(out_dev, ld_out, b) &&
                       (!add_dev || wide_rows(add_dev, ld_add, b));
-    BY_TYPE(type, combine_rows_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, (int)T, k, (int)d, (const V*)add_dev, ld_add,
+    BY_TYPE(type, e = launch_ahead(combine_rows_kernel<V>, c.grid, c.threads, 0, (cudaStream_t)stream, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, (int)T, k, (int)d, (const V*)add_dev, ld_add,
                       (V*)out_dev, ld_out, wide));
-    return launched(what);
+    return done(what, e);
 }
 
 // drows in the activations' type, or (codes, scales) in 8 bits
@@ -213,6 +220,7 @@ static int combine_grad(const char* what, int type, const void* dout_dev, int64_
     if (dw_dev) TRY(check_ints(what, "dw", dw_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     // one CTA per token, dout's columns in shared memory
     const size_t smem = sizeof(float) * blocks_of(std::min<int64_t>(d, kGradCols)) * kFp8Block;   // 32 KB at most
     const bool wide = wide_rows(dout_dev, ld_dout, b) && (!dw_dev || wide_rows(rows_dev, ld_rows, b));
@@ -220,7 +228,7 @@ static int combine_grad(const char* what, int type, const void* dout_dev, int64_
     const bool fast = wide && wide_d && d % 8 == 0;
     const cudaStream_t s = (cudaStream_t)stream;
 #define QRM_GRAD(FP8, FAST)                                                                                             \
-    BY_TYPE(type, combine_grad_kernel<V, FP8, FAST><<<(unsigned)T, 256, smem, s>>>(                                     \
+    BY_TYPE(type, e = launch_ahead(combine_grad_kernel<V, FP8, FAST>, dim3((unsigned)T), 256, smem, s, \
                       (const V*)dout_dev, ld_dout, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, k, (int)d, \
                       (V*)drows_dev, codes_dev, ld_d, scales_dev, ld_scales, dw_dev, wide, wide_d))
     if (fp8 && fast) QRM_GRAD(true, true);
@@ -228,7 +236,7 @@ static int combine_grad(const char* what, int type, const void* dout_dev, int64_
     else if (fast) QRM_GRAD(false, true);
     else QRM_GRAD(false, false);
 #undef QRM_GRAD
-    return launched(what);
+    return done(what, e);
 }
 
 extern "C" int qrm_combine_rows_grad(int type, const void* dout_dev, int64_t ld_dout, const void* rows_dev,
@@ -260,11 +268,11 @@ extern "C" int qrm_quantize_fp8(int type, const void* x_dev, int64_t ld_x, int64
     if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     const Cut c = cut_columns(rows, cols, 16);
-    BY_TYPE(type, quantize_fp8_kernel<V><<<c.grid, c.threads, 0, (cudaStream_t)stream>>>(
-                      (const V*)x_dev, ld_x, n_rows_dev, (int)cols, codes_dev, ld_codes, scales_dev, ld_scales,
+    BY_TYPE(type, e = launch_ahead(quantize_fp8_kernel<V>, c.grid, c.threads, 0, (cudaStream_t)stream, (const V*)x_dev, ld_x, n_rows_dev, (int)cols, codes_dev, ld_codes, scales_dev, ld_scales,
                       wide_rows(x_dev, ld_x, b), wide_codes16(codes_dev, ld_codes)));
-    return launched(what);
+    return done(what, e);
 }
 
 extern "C" int qrm_quantize_fp8_weights(int type, const void* w_dev, int groups, int64_t rows, int64_t cols,
@@ -280,11 +288,12 @@ extern "C" int qrm_quantize_fp8_weights(int type, const void* w_dev, int groups,
     TRY(check_array(what, "scales", scales_dev, &lds, blocks_of(cols), 4));
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     const dim3 grid((unsigned)blocks_of(cols), (unsigned)blocks_of(rows), (unsigned)groups);
     const bool wide = wide_rows(w_dev, cols, b) && wide_codes(codes_dev, cols);
-    BY_TYPE(type, quantize_fp8_weights_kernel<V><<<grid, 256, 0, (cudaStream_t)stream>>>((const V*)w_dev, (int)rows, (int)cols,
+    BY_TYPE(type, e = launch_ahead(quantize_fp8_weights_kernel<V>, grid, 256, 0, (cudaStream_t)stream, (const V*)w_dev, (int)rows, (int)cols,
                                                                                          codes_dev, scales_dev, wide));
-    return launched(what);
+    return done(what, e);
 }
 
 static int check_limit(const char* what, float limit) {
@@ -305,18 +314,19 @@ extern "C" int qrm_swiglu_fp8(int type, const void* gu_dev, int64_t ld_gu, int64
     if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     Cut c = cut_columns(rows, f, 8);
     c.grid.x = walkers(rows, c.grid.y, sms, 6 * 256 / c.threads);
     const bool wide = wide_rows(gu_dev, ld_gu, b) && f * b % 16 == 0;
     const cudaStream_t s = (cudaStream_t)stream;
     const bool wide_c = wide_codes(codes_dev, ld_codes);
     if (limit > 0.f)
-        BY_TYPE(type, swiglu_fp8_kernel<V, true><<<c.grid, c.threads, 0, s>>>((const V*)gu_dev, ld_gu, (int)rows, n_rows_dev, (int)f,
+        BY_TYPE(type, e = launch_ahead(swiglu_fp8_kernel<V, true>, c.grid, c.threads, 0, s, (const V*)gu_dev, ld_gu, (int)rows, n_rows_dev, (int)f,
                           limit, codes_dev, ld_codes, scales_dev, ld_scales, wide, wide_c));
     else
-        BY_TYPE(type, swiglu_fp8_kernel<V, false><<<c.grid, c.threads, 0, s>>>((const V*)gu_dev, ld_gu, (int)rows, n_rows_dev, (int)f,
+        BY_TYPE(type, e = launch_ahead(swiglu_fp8_kernel<V, false>, c.grid, c.threads, 0, s, (const V*)gu_dev, ld_gu, (int)rows, n_rows_dev, (int)f,
                           limit, codes_dev, ld_codes, scales_dev, ld_scales, wide, wide_c));
-    return launched(what);
+    return done(what, e);
 }
 
 extern "C" int qrm_swiglu_fp8_grad(int type, const void* gu_dev, int64_t ld_gu, const void* dh_dev, int64_t ld_dh,
@@ -337,18 +347,17 @@ extern "C" int qrm_swiglu_fp8_grad(int type, const void* gu_dev, int64_t ld_gu, 
     if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
     int device, sms;
     TRY(current_device(&device, &sms));
+    cudaError_t e;
     Cut c = cut_columns(rows, f, 8);
     c.grid.x = walkers(rows, c.grid.y, sms, 4 * 256 / c.threads);
     const bool wide = wide_rows(gu_dev, ld_gu, b) && wide_rows(dh_dev, ld_dh, b);
     const cudaStream_t s = (cudaStream_t)stream;
     const bool wide_c = wide_codes(codes_dev, ld_codes);
     if (limit > 0.f)
-        BY_TYPE(type, swiglu_fp8_grad_kernel<V, true><<<c.grid, c.threads, 0, s>>>(
-                          (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, (int)rows, n_rows_dev, (int)f, limit, codes_dev, ld_codes,
+        BY_TYPE(type, e = launch_ahead(swiglu_fp8_grad_kernel<V, true>, c.grid, c.threads, 0, s, (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, (int)rows, n_rows_dev, (int)f, limit, codes_dev, ld_codes,
                           scales_dev, ld_scales, wide, wide_c));
     else
-        BY_TYPE(type, swiglu_fp8_grad_kernel<V, false><<<c.grid, c.threads, 0, s>>>(
-                          (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, (int)rows, n_rows_dev, (int)f, limit, codes_dev, ld_codes,
+        BY_TYPE(type, e = launch_ahead(swiglu_fp8_grad_kernel<V, false>, c.grid, c.threads, 0, s, (const V*)gu_dev, ld_gu, (const V*)dh_dev, ld_dh, (int)rows, n_rows_dev, (int)f, limit, codes_dev, ld_codes,
                           scales_dev, ld_scales, wide, wide_c));
-    return launched(what);
+    return done(what, e);
 }

@@ -26,6 +26,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "common.cuh"
+
 namespace qrm {
 
 constexpr int kFp8Block = 128;
@@ -266,6 +268,7 @@ template <int C>   // CTAs
 __global__ void __launch_bounds__(1024)
 sort_tokens_kernel(const int32_t* __restrict__ idx, long long n, int first, int E, int bits, int32_t* __restrict__ perm,
                    int32_t* __restrict__ pos, int32_t* __restrict__ offsets) {
+    pdl_start();
     extern __shared__ int32_t sort_sm[];
     const int W = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int32_t* total = sort_sm;            // [E] this CTA's count of each expert
@@ -386,6 +389,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 gather_rows_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ pos, int k, int d, uint32_t n_rows,
                    T* __restrict__ rows, long long ld_rows, bool wide) {
+    pdl_start();
     const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, d);
     if (!n) return;
     pos += (size_t)t * k;
@@ -444,6 +448,7 @@ __global__ void __launch_bounds__(256)
 gather_rows_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ pos, int k, int d,
                        uint32_t n_rows, uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales,
                        long long ld_s, bool wide_x, bool wide_c) {
+    pdl_start();
     const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 16, n = columns_at(c, d, 16);
     pos += (size_t)t * k;
     const Codes16 q = quantize16(x + t * ld_x + c, n, wide_x);
@@ -467,6 +472,7 @@ __global__ void __launch_bounds__(256, 4)
 combine_rows_kernel(const T* __restrict__ rows, long long ld_rows, uint32_t n_rows, const int32_t* __restrict__ pos,
                     const float* __restrict__ w, int tokens, int k, int d, const T* __restrict__ add, long long ld_add,
                     T* __restrict__ out, long long ld_out, bool wide) {
+    pdl_start();
     constexpr int S = sizeof(T) == 4 ? 4 : 8;   // rows whose loads are in flight: 32 registers
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, d), lane = threadIdx.x & 31;
     int t = blockIdx.x;
@@ -545,6 +551,7 @@ combine_grad_kernel(const T* __restrict__ dout, long long ld_dout, const T* __re
                     uint32_t n_rows, const int32_t* __restrict__ pos, const float* __restrict__ w, int k, int d,
                     T* __restrict__ drows, uint8_t* __restrict__ codes, long long ld_d, float* __restrict__ scales,
                     long long ld_s, float* __restrict__ dw, bool wide, bool wide_d) {
+    pdl_start();
     constexpr int S = 8, NB = kGradCols / kFp8Block;
     constexpr int U = sizeof(T) == 4 ? 2 : 4;   // row loads in flight
     extern __shared__ float4 g_sm[];            // min(d, kGradCols) columns of dout, in whole blocks
@@ -665,6 +672,7 @@ __global__ void __launch_bounds__(256)
 quantize_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ n_dev, int cols,
                     uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales, long long ld_s, bool wide_x,
                     bool wide_c) {
+    pdl_start();
     const int t = blockIdx.x, c = (blockIdx.y * blockDim.x + threadIdx.x) * 16, n = columns_at(c, cols, 16);
     if (n_dev && t >= *n_dev) return;
     const Codes16 q = quantize16(x + t * ld_x + c, n, wide_x);
@@ -679,6 +687,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 quantize_fp8_weights_kernel(const T* __restrict__ w, int rows, int cols, uint8_t* __restrict__ codes,
                             float* __restrict__ scales, bool wide) {
+    pdl_start();
     __shared__ float top[8];
     const int r0 = blockIdx.y * kFp8Block, c = blockIdx.x * kFp8Block + (threadIdx.x & 15) * 8;
     const long long base = (long long)blockIdx.z * rows * cols;
@@ -766,6 +775,7 @@ __global__ void __launch_bounds__(256)
 swiglu_fp8_kernel(const T* __restrict__ gu, long long ld, int rows, const int32_t* __restrict__ n_dev, int f, float limit,
                   uint8_t* __restrict__ codes, long long ld_c, float* __restrict__ scales, long long ld_s, bool wide,
                   bool wide_c) {
+    pdl_start();
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
     if (n_dev) rows = min(rows, *n_dev);
     int t = blockIdx.x;
@@ -804,6 +814,7 @@ __global__ void __launch_bounds__(256)
 swiglu_fp8_grad_kernel(const T* __restrict__ gu, long long ld, const T* __restrict__ dh, long long ld_dh, int rows,
                        const int32_t* __restrict__ n_dev, int f, float limit, uint8_t* __restrict__ codes, long long ld_c,
                        float* __restrict__ scales, long long ld_s, bool wide, bool wide_c) {
+    pdl_start();
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
     if (n_dev) rows = min(rows, *n_dev);
     int t = blockIdx.x;
