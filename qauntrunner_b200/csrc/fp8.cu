@@ -17,7 +17,7 @@ struct qrm_fp8 {
     int device = 0, sms = 0, groups = 0;
     int form = -1;                           // QRM_FP8_PAIR: 1 always / 0 never rows of x on the MMA's M side
     int64_t rows = 0, cols = 0, pitch = 0;   // of one matrix; pitch: bytes of a stored row
-    uint8_t* codes = nullptr;                // [groups][rows][pitch]
+    uint8_t* codes = nullptr;                // [groups][rows][pitch]; the other arrays are in the same allocation
     float* scales = nullptr;                 // [groups][row blocks][column blocks]
     float* part = nullptr;                   // partial tiles of the CTAs
     int32_t* arrivals = nullptr;
@@ -36,10 +36,6 @@ void release(qrm_fp8* m) {
     cudaSetDevice(m->device);
     cudaDeviceSynchronize();
     cudaFree(m->codes);
-    cudaFree(m->scales);
-    cudaFree(m->part);
-    cudaFree(m->arrivals);
-    cudaFree(m->err);
     delete m;
 }
 
@@ -104,21 +100,24 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     m->rows = rows;
     m->cols = cols;
     m->pitch = (cols + 15) / 16 * 16;
-    const size_t part = sizeof(float) * (size_t)sms * 2 * kFp8MaxRows * 128;
-    const size_t arrivals = sizeof(int32_t) * (size_t)sms * kFp8EpiWarps;
-    if (cudaMalloc(&m->codes, (size_t)groups * rows * m->pitch) != cudaSuccess ||
-        cudaMalloc(&m->scales, scale_bytes) != cudaSuccess || cudaMalloc(&m->part, part) != cudaSuccess ||
-        cudaMalloc(&m->arrivals, arrivals) != cudaSuccess || cudaMalloc(&m->err, sizeof(int32_t)) != cudaSuccess) {
+    // one allocation: codes, scales, partial tiles, arrivals, error flags
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    const size_t codes_at = up((size_t)groups * rows * m->pitch), scales_at = codes_at + up(scale_bytes);
+    const size_t part_at = scales_at + up(sizeof(float) * (size_t)sms * 2 * kFp8MaxRows * 128);
+    const size_t counts = sizeof(int32_t) * ((size_t)sms * kFp8EpiWarps + 1);
+    if (cudaMalloc(&m->codes, part_at + counts) != cudaSuccess) {
         cudaGetLastError();
-        return bail(failf(QRM_E_NOMEM, "%s: cannot allocate %lld bytes", what, (long long)(groups * rows * m->pitch)));
+        return bail(failf(QRM_E_NOMEM, "%s: cannot allocate %zu bytes", what, part_at + counts));
     }
+    m->scales = reinterpret_cast<float*>(m->codes + codes_at);
+    m->part = reinterpret_cast<float*>(m->codes + scales_at);
+    m->arrivals = reinterpret_cast<int32_t*>(m->codes + part_at);
+    m->err = m->arrivals + (size_t)sms * kFp8EpiWarps;
     // device sources: what any stream still writes there is awaited, as in qrm_upload_expert_device
     cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess)
-        e = cudaMemcpy2D(m->codes, m->pitch, codes, cols, cols, (size_t)groups * rows, kind);
+    if (e == cudaSuccess) e = cudaMemcpy2D(m->codes, m->pitch, codes, cols, cols, (size_t)groups * rows, kind);
     if (e == cudaSuccess) e = cudaMemcpy(m->scales, scales, scale_bytes, kind);
-    if (e == cudaSuccess) e = cudaMemset(m->arrivals, 0, arrivals);
-    if (e == cudaSuccess) e = cudaMemset(m->err, 0, sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaMemset(m->arrivals, 0, counts);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
@@ -134,21 +133,35 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     return QRM_OK;
 }
 
-// Which kernel a product takes, by what both would cost with the rows spread
-// evenly over the groups.  Measured (us; weights on the M side / rows of x on
-// the M side, K and N of the product):
-//   1 x 4096 x 7168:  1 row 15 / 32, 64 rows 23 / 33, 128 rows 28 / 35, 512 rows 48 / 39, 1024 rows 72 / 42
-//   1 x 28672 x 4096: 1 row 31 / 46, 128 rows 48 / 44, 256 rows 86 / 47, 4096 rows 877 / 530
-//   32 x 4096 x 7168: 16 rows each 179 / 253, 96 rows each 253 / 280, 128 rows each 315 / 306, 256 rows each 561 / 389
-//   8 x 5632 x 1024:  16 rows each 21 / 20, 64 rows each 27 / 23; 1 x 1024 x 2816: 1 row 12 / 15, 16 rows 13 / 15
-// The first shares all blocks out to all SMs; a block costs it 0.38 us (the
-// weights' bytes) and 2 ns a row.  The second does whole tiles, 0.55 us a
-// block of 256 rows x 256 outputs, in waves over the pairs of SMs.
+// Which kernel a product takes, by an estimate of what both would cost with the
+// rows spread evenly over the groups.  Measured (us; weights on the MMA's M
+// side / rows of x on it), outputs x contracted:
+//   1 x 4096 x 7168:  1 row 15 / 30, 64 rows 21 / 30, 256 rows 30 / 31, 512 rows 38 / 32
+//   1 x 28672 x 4096: 1 row 32 / 42, 64 rows 39 / 38, 128 rows 46 / 39, 256 rows 78 / 40, 4096 rows 877 / 425
+//   1 x 4096 x 28672: 1 row 30 / 95, 128 rows 46 / 96, 512 rows 128 / 99
+//   1 x 1024 x 2816:  1 row 12 / 16, 64 rows 18 / 16, 512 rows 19 / 18
+//   8 x 5632 x 1024:  1 row each 14 / 17, 64 rows each 24 / 23, 256 rows each 41 / 31
+//   32 x 4096 x 7168: 16 rows each 179 / 222, 64 rows each 204 / 233, 128 rows each 304 / 252, 256 rows each 572 / 324
+// The first shares all blocks out to all SMs: a block costs it 0.3 us and 2 ns
+// a row, a tile that several SMs share 50 ns a row more in the end.  The second
+// does whole tiles of 256 rows x 256 outputs in waves over the pairs of SMs, a
+// block in 0.42 us, or 0.55 when most pairs are at work.  The worst choice
+// among 90 measured sizes takes 1.2 times as long as the other kernel.
 bool pair_is_faster(int64_t T, int groups, int64_t M, int64_t mb, int64_t kb, int sms) {
     const double used = (double)std::min<int64_t>(T, groups), rows = T / used;   // groups with rows, rows of each
-    const double tiles = used * mb * std::ceil(rows / kFp8MaxRows), pairs = used * ((M + 255) / 256) * std::ceil(rows / 256);
-    const double in_tile = rows / std::ceil(rows / kFp8MaxRows);
-    const double one = 10 + (0.38 + 0.002 * in_tile) * std::ceil(tiles * kb / sms), two = 6 + 0.55 * std::ceil(pairs / (sms / 2)) * kb;
+    const double blocks = std::ceil(rows / kFp8MaxRows), in_tile = rows / blocks, tiles = used * mb * blocks;
+    const double even = tiles * kb / sms;
+    double busy, shared = 0;   // blocks of the busiest CTA
+    if (tiles > sms) {
+        busy = std::min(std::ceil(tiles / sms) * kb, even + 16);
+    } else {
+        const double each = std::max(1.0, std::floor(sms / tiles));
+        busy = std::min(kb / each, even + 8);
+        if (each > 1) shared = 8;
+    }
+    const double one = 5 + (0.30 + 0.0021 * in_tile) * (busy + shared) + (tiles <= sms ? 0.05 * in_tile : 0);
+    const double pairs = used * ((M + 255) / 256) * std::ceil(rows / 256), room = sms / 2;
+    const double two = 4 + (pairs > room / 2 ? 0.55 : 0.42) * std::ceil(pairs / room) * kb;
     return two < one;
 }
 

@@ -638,7 +638,7 @@ __device__ __forceinline__ uint32_t map_to_rank0(uint32_t addr) {
 }
 // (What it hands over was read from tensor memory and is ordered by the
 // tcgen05 fence before it; with cluster scope here a full memory barrier came
-// with every block: 1010 us in place of REPLACE at 4096 x 28672 x 4096.)
+// with every block: 1010 us in place of 560 at 4096 x 28672 x 4096, then.)
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -801,7 +801,8 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                     if (elect_one()) {
                         const uint32_t st = ring0 + r.i * kFp8PairStage, bar = full0 + 8 * r.i;
                         if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * kFp8PairStage);
-                        tma_pair_2d(st, &x_map, kb * 128, t.pos, bar);
+                        // (no rows for this CTA: from past the end, which is zeros and no traffic)
+                        tma_pair_2d(st, &x_map, kb * 128, t.rows > 0 ? t.pos : p.T, bar);
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
                             const uint32_t to = st + kFp8Tile + h * (kFp8Tile / 2);
@@ -916,6 +917,22 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
         Ring r, a, sr;
         for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
             const Fp8PairTile t = tile_at(i);
+            if (t.rows <= 32 * (warp & 3)) {   // none of this warp's rows: it only keeps the hand-overs going
+                for (int kb = 0; kb < KB && ok; kb++) {
+                    if (((kb & 3) == 0 && !bar_wait(sc_full0 + 8 * sr.i, sr.phase, ctl)) || !bar_wait(ready0 + 8 * r.i, r.phase, ctl)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) bar_arrive_cluster(acc_empty0 + 8 * a.i);
+                    if ((kb & 3) == 3 || kb + 1 == KB) {
+                        if (lane == 0) bar_arrive(sc_empty0 + 8 * sr.i);
+                        sr.next(kFp8PairScaleRing);
+                    }
+                    r.next(kFp8PairStages);
+                    a.next(kFp8PairAcc);
+                }
+                continue;
+            }
             float2 acc[64];
 #pragma unroll
             for (int c = 0; c < 64; c++) acc[c] = make_float2(0.f, 0.f);
