@@ -200,13 +200,12 @@ def _check(rc):
 
 
 def _ptr(a):
-    if a is None:
-        return None
-    if isinstance(a, int):
+    if a is None or isinstance(a, int):
         return a
-    if hasattr(a, "data_ptr"):
+    try:
         return a.data_ptr()
-    return a.ctypes.data_as(P).value
+    except AttributeError:
+        return a.ctypes.data_as(P).value
 
 
 def qw_layer_desc(path, layer_index, device=0, max_tokens=1):
@@ -508,57 +507,57 @@ def sort_tokens(topk_idx, T, k, n_experts, perm, pos, offsets, first=0, stream=N
 
 def gather_rows(type, x, pos, T, k, d, rows, n_rows, ld_x=0, ld_rows=0, stream=None):
     """rows[pos[t, j]] = x[t]."""
-    _check(lib().qrm_gather_rows(int(type), _ptr(x), ld_x, _ptr(pos), T, k, d, _ptr(rows), n_rows, ld_rows, stream))
+    _check(lib().qrm_gather_rows(type, _ptr(x), ld_x, _ptr(pos), T, k, d, _ptr(rows), n_rows, ld_rows, stream))
 
 
 def gather_rows_fp8(type, x, pos, T, k, d, codes, scales, n_rows, ld_x=0, ld_codes=0, ld_scales=0, stream=None):
     """gather_rows into 8-bit rows (codes, scales)."""
-    _check(lib().qrm_gather_rows_fp8(int(type), _ptr(x), ld_x, _ptr(pos), T, k, d, _ptr(codes), n_rows, ld_codes,
+    _check(lib().qrm_gather_rows_fp8(type, _ptr(x), ld_x, _ptr(pos), T, k, d, _ptr(codes), n_rows, ld_codes,
                                      _ptr(scales), ld_scales, stream))
 
 
 def combine_rows(type, rows, n_rows, pos, w, T, k, d, out, add=None, ld_rows=0, ld_add=0, ld_out=0, stream=None):
     """out[t] = add[t] + sum_j w[t, j] rows[pos[t, j]] (w None: 1)."""
-    _check(lib().qrm_combine_rows(int(type), _ptr(rows), n_rows, ld_rows, _ptr(pos), _ptr(w), T, k, d, _ptr(add), ld_add,
+    _check(lib().qrm_combine_rows(type, _ptr(rows), n_rows, ld_rows, _ptr(pos), _ptr(w), T, k, d, _ptr(add), ld_add,
                                   _ptr(out), ld_out, stream))
 
 
 def combine_rows_grad(type, dout, rows, n_rows, pos, w, T, k, d, drows, dw=None, ld_dout=0, ld_rows=0, ld_drows=0,
                       stream=None):
     """drows[pos[t, j]] = w[t, j] dout[t], dw[t, j] = <dout[t], rows[pos[t, j]]>."""
-    _check(lib().qrm_combine_rows_grad(int(type), _ptr(dout), ld_dout, _ptr(rows), n_rows, ld_rows, _ptr(pos), _ptr(w),
+    _check(lib().qrm_combine_rows_grad(type, _ptr(dout), ld_dout, _ptr(rows), n_rows, ld_rows, _ptr(pos), _ptr(w),
                                        T, k, d, _ptr(drows), ld_drows, _ptr(dw), stream))
 
 
 def combine_rows_grad_fp8(type, dout, rows, n_rows, pos, w, T, k, d, codes, scales, dw=None, ld_dout=0, ld_rows=0,
                           ld_codes=0, ld_scales=0, stream=None):
     """combine_rows_grad with the rows' gradient in 8 bits (codes, scales)."""
-    _check(lib().qrm_combine_rows_grad_fp8(int(type), _ptr(dout), ld_dout, _ptr(rows), n_rows, ld_rows, _ptr(pos),
+    _check(lib().qrm_combine_rows_grad_fp8(type, _ptr(dout), ld_dout, _ptr(rows), n_rows, ld_rows, _ptr(pos),
                                            _ptr(w), T, k, d, _ptr(codes), ld_codes, _ptr(scales), ld_scales, _ptr(dw),
                                            stream))
 
 
 def quantize_fp8(type, x, rows, cols, codes, scales, n_rows=None, ld_x=0, ld_codes=0, ld_scales=0, stream=None):
     """Rows into 8 bits; n_rows: how many of them, on the device."""
-    _check(lib().qrm_quantize_fp8(int(type), _ptr(x), ld_x, rows, cols, _ptr(n_rows), _ptr(codes), ld_codes,
+    _check(lib().qrm_quantize_fp8(type, _ptr(x), ld_x, rows, cols, _ptr(n_rows), _ptr(codes), ld_codes,
                                   _ptr(scales), ld_scales, stream))
 
 
 def quantize_fp8_weights(type, w, rows, cols, codes, scales, groups=1, stream=None):
     """Matrices into 8 bits, one scale for each 128 x 128 block."""
-    _check(lib().qrm_quantize_fp8_weights(int(type), _ptr(w), groups, rows, cols, _ptr(codes), _ptr(scales), stream))
+    _check(lib().qrm_quantize_fp8_weights(type, _ptr(w), groups, rows, cols, _ptr(codes), _ptr(scales), stream))
 
 
 def swiglu_fp8(type, gu, rows, f, codes, scales, limit=0.0, n_rows=None, ld_gu=0, ld_codes=0, ld_scales=0, stream=None):
     """silu(gate) up of gu [rows][2f] (gate's columns, then up's) into 8-bit rows."""
-    _check(lib().qrm_swiglu_fp8(int(type), _ptr(gu), ld_gu, rows, f, _ptr(n_rows), limit, _ptr(codes), ld_codes,
+    _check(lib().qrm_swiglu_fp8(type, _ptr(gu), ld_gu, rows, f, _ptr(n_rows), limit, _ptr(codes), ld_codes,
                                 _ptr(scales), ld_scales, stream))
 
 
 def swiglu_fp8_grad(type, gu, dh, rows, f, codes, scales, limit=0.0, n_rows=None, ld_gu=0, ld_dh=0, ld_codes=0,
                     ld_scales=0, stream=None):
     """The gradients of gate and up [rows][2f], given dh [rows][f], into 8-bit rows."""
-    _check(lib().qrm_swiglu_fp8_grad(int(type), _ptr(gu), ld_gu, _ptr(dh), ld_dh, rows, f, _ptr(n_rows), limit,
+    _check(lib().qrm_swiglu_fp8_grad(type, _ptr(gu), ld_gu, _ptr(dh), ld_dh, rows, f, _ptr(n_rows), limit,
                                      _ptr(codes), ld_codes, _ptr(scales), ld_scales, stream))
 
 
@@ -591,12 +590,12 @@ class Fp8Matrix:
 
     def product(self, type, x, x_scales, T, y, offsets=None, ld_x=0, ld_scales=0, ld_y=0, stream=None):
         """y[t] = W_g x[t] for the 8-bit rows x of each group g (offsets)."""
-        _check(lib().qrm_fp8_product(self._h, _ptr(x), ld_x, _ptr(x_scales), ld_scales, _ptr(offsets), T, int(type),
+        _check(lib().qrm_fp8_product(self._h, _ptr(x), ld_x, _ptr(x_scales), ld_scales, _ptr(offsets), T, type,
                                      _ptr(y), ld_y, stream))
 
     def product_t(self, type, y, y_scales, T, x, offsets=None, ld_y=0, ld_scales=0, ld_x=0, stream=None):
         """x[t] = W_g^T y[t]: the gradient of the product's input."""
-        _check(lib().qrm_fp8_product_t(self._h, _ptr(y), ld_y, _ptr(y_scales), ld_scales, _ptr(offsets), T, int(type),
+        _check(lib().qrm_fp8_product_t(self._h, _ptr(y), ld_y, _ptr(y_scales), ld_scales, _ptr(offsets), T, type,
                                        _ptr(x), ld_x, stream))
 
     def sync(self):

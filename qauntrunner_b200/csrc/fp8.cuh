@@ -917,22 +917,6 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
         Ring r, a, sr;
         for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
             const Fp8PairTile t = tile_at(i);
-            if (t.rows <= 32 * (warp & 3)) {   // none of this warp's rows: it only keeps the hand-overs going
-                for (int kb = 0; kb < KB && ok; kb++) {
-                    if (((kb & 3) == 0 && !bar_wait(sc_full0 + 8 * sr.i, sr.phase, ctl)) || !bar_wait(ready0 + 8 * r.i, r.phase, ctl)) {
-                        ok = false;
-                        break;
-                    }
-                    if (lane == 0) bar_arrive_cluster(acc_empty0 + 8 * a.i);
-                    if ((kb & 3) == 3 || kb + 1 == KB) {
-                        if (lane == 0) bar_arrive(sc_empty0 + 8 * sr.i);
-                        sr.next(kFp8PairScaleRing);
-                    }
-                    r.next(kFp8PairStages);
-                    a.next(kFp8PairAcc);
-                }
-                continue;
-            }
             float2 acc[64];
 #pragma unroll
             for (int c = 0; c < 64; c++) acc[c] = make_float2(0.f, 0.f);
