@@ -121,7 +121,11 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    cudaFuncAttributes pair{};
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&pair, fp8_pair_kernel);
     if (e != cudaSuccess) return bail(failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e)));
+    if (pair.numRegs * kFp8Warps * 32 < kFp8PairRegs)
+        return bail(failf(QRM_E_CUDA, "%s: built with %d registers a thread, too few for its split", what, pair.numRegs));
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)groups};
     const cuuint64_t strides[2] = {(cuuint64_t)m->pitch, (cuuint64_t)(m->pitch * rows)};
     const cuuint32_t box[3] = {128, 128, 1};

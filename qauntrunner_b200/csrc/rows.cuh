@@ -287,8 +287,8 @@ sort_tokens_kernel(const int32_t* __restrict__ idx, long long n, int first, int 
     int32_t* mine = count + warp * E;
     __syncthreads();
     auto expert = [&](long long i) {   // -1: none of these
-        const int e = i < a1 ? idx[i] - first : -1;
-        return e < 0 || e >= E ? -1 : e;
+        const uint32_t e = i < a1 ? (uint32_t)idx[i] - (uint32_t)first : ~0u;
+        return e < (uint32_t)E ? (int)e : -1;
     };
     for (long long a = a0; a < a1; a += 128) {
         int e[4];   // loads in flight together
