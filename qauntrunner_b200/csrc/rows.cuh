@@ -203,21 +203,19 @@ __device__ __forceinline__ float half_warp_max(float m) {
 // Eight stored columns, negated, as f32 (the sign bits are turned over where
 // two 16-bit values still share a word)
 template <typename T>
-__device__ __forceinline__ Pair negated_pair(const Raw8<T>& r, int i) {
-    if constexpr (sizeof(T) == 4) {
-        return pair(-__uint_as_float(r.w[2 * i]), -__uint_as_float(r.w[2 * i + 1]));
-    } else {
-        const uint32_t w = r.w[i] ^ 0x80008000u;
-        T h[2];
-        memcpy(h, &w, 4);
-        return pair(to_f32(h[0]), to_f32(h[1]));
-    }
-}
-template <typename T>
 __device__ __forceinline__ Pairs8 negated(const Raw8<T>& r) {
     Pairs8 v;
 #pragma unroll
-    for (int i = 0; i < 4; i++) v.p[i] = negated_pair(r, i);
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            v.p[i] = pair(-__uint_as_float(r.w[2 * i]), -__uint_as_float(r.w[2 * i + 1]));
+        } else {
+            const uint32_t w = r.w[i] ^ 0x80008000u;
+            T h[2];
+            memcpy(h, &w, 4);
+            v.p[i] = pair(to_f32(h[0]), to_f32(h[1]));
+        }
+    }
     return v;
 }
 template <typename T>
@@ -726,16 +724,14 @@ quantize_fp8_weights_kernel(const T* __restrict__ w, int rows, int cols, uint8_t
 //   dg = dh u (sigma(g) + g sigma(g) (1 - sigma(g))), 0 where the gate was cut off
 //   du = dh g sigma(g), 0 where up was cut off
 // Two columns at a time.  sigma(g) = num / (1 + e) with e = exp(-|g|), which
-// never overflows, and num = 1 or e by g's sign.  e is the square of 2^x for
-// x = -|g| log2(e) / 2, so that the flushing form of the instruction reaches
-// denormal e too, and the rounding of that product is made good: x - t is
-// exact to 2^-45 or so.  What remains is twice the instruction's 2 ulp, and the
-// reciprocal's 1.
+// never overflows, and num = 1 or e by g's sign.  e is 2^x for x = -|g| log2 e
+// with the rounding of that product made good (x + lo is exact to 2^-45 or so),
+// so only the two approximate instructions' own errors remain (2 ulp and 1 ulp).
 struct Swiglu2 {
     Pair g, u, sig;   // after the cut-offs
 };
-constexpr float kHalfLog2e = 0.7213475204444817f, kHalfLog2eLow = (float)(0.7213475204444817037 - (double)kHalfLog2e);
-constexpr float kTwoLn2 = 1.3862943611198906f;
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = (float)(1.4426950408889634074 - (double)kLog2e);
+constexpr float kLn2 = 0.6931471805599453f;
 __device__ __forceinline__ float min_nan(float a, float b) {
     float r;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -743,7 +739,7 @@ __device__ __forceinline__ float min_nan(float a, float b) {
 }
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
 __device__ __forceinline__ float reciprocal_approx(float x) {
@@ -757,14 +753,12 @@ __device__ __forceinline__ Swiglu2 swiglu2(float2 gate, float2 up, float limit) 
         gate = make_float2(min_nan(gate.x, limit), min_nan(gate.y, limit));
         up = make_float2(max_nan(min_nan(up.x, limit), -limit), max_nan(min_nan(up.y, limit), -limit));
     }
-    const Pair g = pair(fabsf(gate.x), fabsf(gate.y));
-    const Pair x = mul2(g, pair(-kHalfLog2e, -kHalfLog2e));
-    // t = |g| log2(e) / 2 + x, what x is off
-    const Pair t = fma2(g, pair(kHalfLog2eLow, kHalfLog2eLow), fma2(g, pair(kHalfLog2e, kHalfLog2e), x));
+    const Pair n = pair(-fabsf(gate.x), -fabsf(gate.y)), l2e = pair(kLog2e, kLog2e);
+    const Pair x = mul2(n, l2e);
     const float2 xf = unpair(x);
-    const Pair h = pair(exp2_approx(xf.x), exp2_approx(xf.y));
-    const Pair e0 = mul2(h, h);
-    const float2 e = unpair(fma2(mul2(e0, t), pair(-kTwoLn2, -kTwoLn2), e0));
+    const Pair lo = fma2(n, pair(kLog2eLow, kLog2eLow), fma2(n, l2e, pair(-xf.x, -xf.y)));
+    const Pair e0 = pair(exp2_approx(xf.x), exp2_approx(xf.y));
+    const float2 e = unpair(fma2(mul2(e0, lo), pair(kLn2, kLn2), e0));
     const float2 r = make_float2(reciprocal_approx(1.f + e.x), reciprocal_approx(1.f + e.y));
     Swiglu2 s;
     s.g = pair(gate.x, gate.y);
@@ -842,7 +836,7 @@ swiglu_fp8_grad_kernel(const T* __restrict__ gu, long long ld, const T* __restri
         for (int i = 0; i < 4; i++) {
             const float2 gate = make_float2(column(g, 2 * i), column(g, 2 * i + 1)), up = make_float2(column(u, 2 * i), column(u, 2 * i + 1));
             const Swiglu2 p = swiglu2<LIMIT>(gate, up, limit);
-            const Pair nd = negated_pair(d, i);
+            const Pair nd = pair(-column(d, 2 * i), -column(d, 2 * i + 1));
             // u sigma (1 + g (1 - sigma)) and g sigma, times minus dh
             dg.p[i] = mul2(mul2(nd, p.u), mul2(p.sig, fma2(p.g, fma2(p.sig, minus, one), one)));
             du.p[i] = mul2(nd, mul2(p.g, p.sig));
