@@ -170,12 +170,15 @@ struct Ring {
 // rows of x (its N, rounded up to 16 only), so a group of a few rows costs
 // about what its weights cost to read: this form is for memory-bound sizes.
 //
-// All tiles' blocks, one after the other, are cut into as many equal runs as
-// there are CTAs (one per SM), wherever that falls inside a tile: one token
-// through one matrix still reads it with every SM.  A CTA that did only part
-// of a tile's blocks leaves its f32 sums in the workspace, and the last one to
-// arrive adds the parts up in the CTAs' order, so that the result does not
-// depend on who was last.  Nobody waits.
+// All tiles' blocks, one after the other, are cut into runs for one CTA on each
+// SM, inside a tile where that pays (fp8_share_out): one token through one
+// matrix still reads it with every SM.  A CTA that did only part of a tile's
+// blocks leaves its f32 sums in the workspace, and the last one to arrive adds
+// the parts up in the CTAs' order, so that the result does not depend on who
+// was last.  Nobody waits.
+//
+// 512 rows over 32 matrices of 4096 x 7168 (940 MB): 175 us, 5.4 TB/s.  One row
+// through one such matrix: 12 us, latencies.
 //
 // Warps: 0 loads tiles (TMA), 1 issues the MMAs, 2 brings the scales (their
 // product sx sw for each row of x and block), 4-11 add up: lane quarter
@@ -618,7 +621,9 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
 // What bounds it is the way around an accumulator: MMAs, hand-over, the
 // epilogue's loads out of tensor memory, hand-over back.  So the tile's two
 // blocks of 128 outputs have MMAs, accumulators (two each) and epilogue warps
-// of their own, and take turns on the tensor cores.
+// of their own, and take turns on the tensor cores.  4096 rows, 28672 x 4096:
+// 425 us, 2.26 PFLOP/s, tensor pipe 62 % active; 497 us under sustained load
+// (power cap, 1.5 GHz).
 //
 // Warps: 0 loads tiles, 1 issues the MMAs (in the pair's first CTA), 2 brings
 // the scales, 4-11 add up: lane quarter (warp & 3), outputs 128 (warp >= 8).

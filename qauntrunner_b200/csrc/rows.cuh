@@ -246,9 +246,10 @@ __device__ __forceinline__ int columns_at(int c, int cols, int most = 8) { retur
 // (the lowest lane of those with one expert adds), the rows and then the CTAs'
 // totals are summed up in order, and the same walk gives each assignment its
 // place.  No atomics: the order inside an expert is the assignments' own.
-// The lanes with one expert are found by a vote for each bit of its number:
-// match.any takes the longer the more experts there are among 32 assignments,
-// and took most of the time (14.4 us at 32768 assignments to 256 experts).
+// The lanes with one expert are found by a vote for each bit of its number.
+// Latencies bound it (8 SMs, a few passes over shared memory, two cluster
+// barriers): 12 us at 32768 assignments to 256 experts, 14.6 with one load in
+// flight instead of four; 4 us at 8 assignments.
 constexpr int kSortMaxExperts = 1024;
 constexpr int kSortCluster = 8;
 
@@ -442,7 +443,8 @@ __device__ __forceinline__ void store_codes16(uint8_t* __restrict__ p, const Cod
 
 // the same into 8 bits: a token's row is quantised once for all its slots.  A
 // thread holds 16 columns: the slots' addresses and checks were most of what
-// it did with 8.
+// it did with 8.  Memory bounds it: 4096 tokens x 8 slots of 7168 bf16 columns
+// in 51 us, 5.8 TB/s (69 us with 8 columns and positions in 64 bits).
 template <typename T>
 __global__ void __launch_bounds__(256)
 gather_rows_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ pos, int k, int d,
@@ -466,7 +468,9 @@ gather_rows_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* _
 // out[t] = add[t] + sum_j w[t, j] rows[pos[t, j]], in slot order; w NULL: 1.
 // The CTAs walk the tokens; a token's first positions and weights come while
 // the one before it is summed up (a lane holds a slot's), so one wait for
-// memory a token is left.
+// memory a token is left.  2048 tokens x 6 slots of 4096 bf16 columns on the
+// residual stream: 24.9 us, 5.4 TB/s (55 us with one CTA a token and four
+// widened rows in registers).
 template <typename T>
 __global__ void __launch_bounds__(256, 4)
 combine_rows_kernel(const T* __restrict__ rows, long long ld_rows, uint32_t n_rows, const int32_t* __restrict__ pos,
@@ -542,6 +546,8 @@ combine_rows_kernel(const T* __restrict__ rows, long long ld_rows, uint32_t n_ro
 // Rounding does not change an order, so the largest magnitude of w dout is the
 // rounded product of |w| and dout's: it is looked for once for all slots, and
 // each (slot, block)'s scale and reciprocal are computed by one thread.
+// 4096 tokens x 8 slots of 7168 bf16 columns into 8 bits: 145 us, 5.3 TB/s
+// (594 us with all slots in each thread, a maximum and divisions for each).
 constexpr int kGradCols = 8192;
 
 // FAST: every row of every array starts on its widest access, d is a multiple of 8
@@ -769,7 +775,9 @@ __device__ __forceinline__ Swiglu2 swiglu2(float2 gate, float2 up, float limit) 
 __device__ __forceinline__ Pair negative(Pair p) { return p ^ 0x8000000080000000ull; }
 
 // The CTAs walk the rows; a row's loads are on their way while the one before
-// it is computed.
+// it is computed.  The gradient takes 66 us for 16384 rows of 2048 bf16 columns
+// with a limit, 4.1 TB/s: issue slots (74 % busy) bound it, some 50 operations
+// a value; two rows ahead, or more CTAs of fewer registers, change nothing.
 template <typename T, bool LIMIT>
 __global__ void __launch_bounds__(256)
 swiglu_fp8_kernel(const T* __restrict__ gu, long long ld, int rows, const int32_t* __restrict__ n_dev, int f, float limit,
