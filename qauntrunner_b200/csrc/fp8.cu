@@ -15,7 +15,7 @@ using namespace qrm;
 
 struct qrm_fp8 {
     int device = 0, sms = 0, groups = 0;
-    int form = -1;                           // QRM_FP8_PAIR: 1 always / 0 never rows of x on the MMA's M side
+    int form = -1;                           // QRM_FP8_PAIR: 1 wherever it can / 0 never rows of x on the MMA's M side
     int64_t rows = 0, cols = 0, pitch = 0;   // of one matrix; pitch: bytes of a stored row
     uint8_t* codes = nullptr;                // [groups][rows][pitch]; the other arrays are in the same allocation
     float* scales = nullptr;                 // [groups][row blocks][column blocks]
@@ -216,7 +216,9 @@ int product(const char* what, qrm_fp8* m, bool back, const void* x, int64_t ld_x
     p.s_k = back ? wkb : 1;
     p.back = back;
     p.type = type;
-    const bool pair = m->form >= 0 ? m->form : pair_is_faster(T, m->groups, M, mb, kb, m->sms);
+    // the kernel for large groups writes rows that start on 16 bytes
+    const bool pair = aligned(out, 16) && ld_out * b % 16 == 0 &&
+                      (m->form >= 0 ? m->form : pair_is_faster(T, m->groups, M, mb, kb, m->sms));
     const cuuint32_t box[2] = {128, pair ? 128u : 16u};
     if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
     if (pair) {

@@ -622,7 +622,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
 // epilogue's loads out of tensor memory, hand-over back.  So the tile's two
 // blocks of 128 outputs have MMAs, accumulators (two each) and epilogue warps
 // of their own, and take turns on the tensor cores.  4096 rows, 28672 x 4096:
-// 425 us, 2.26 PFLOP/s, tensor pipe 62 % active; 497 us under sustained load
+// 425 us, 2.26 PFLOP/s, tensor pipe 62 % active; 483 us under sustained load
 // (power cap, 1.5 GHz).
 //
 // Warps: 0 loads tiles, 1 issues the MMAs (in the pair's first CTA), 2 brings
@@ -692,19 +692,17 @@ struct Fp8PairTile {
     int pos, rows;   // first row of x of the tile, rows of the group from there on
 };
 
-__device__ __forceinline__ void store_32b(void* to, const uint32_t (&w)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
-                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-// 128 outputs of one row, 32 bytes at a time; `wide`: they start on 32 bytes.
-// (A warp writes 32 rows at once, so what counts is how few stores a row takes.)
+// 128 outputs of one row that starts on 16 bytes, or on 32 (`wide`): a warp
+// writes 32 rows at once, so what counts is how few stores a row takes (483 us
+// in place of 535 at 4096 x 28672 x 4096).  One value at a time took some 20 us
+// a tile: where the rows of out do not start on 16 bytes, the other kernel
+// runs, whose warps write neighbouring outputs.
 template <typename T>
 __device__ __forceinline__ void store_row(T* out, int left, const float2 (&acc)[64], bool wide) {
     constexpr int V = 32 / sizeof(T);   // values of one store
 #pragma unroll
     for (int c = 0; c < 128 / V; c++) {
-        if (wide && V * c + V <= left) {
+        if (V * c + V <= left) {
             uint32_t w[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
@@ -716,8 +714,16 @@ __device__ __forceinline__ void store_row(T* out, int left, const float2 (&acc)[
                     memcpy(&w[i], h, 4);
                 }
             }
-            store_32b(out + V * c, w);
-        } else {
+            if (wide) {
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + V * c), "r"(w[0]), "r"(w[1]),
+                             "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                             : "memory");
+            } else {
+                uint4* to = reinterpret_cast<uint4*>(out + V * c);
+                to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+        } else {   // the last few
 #pragma unroll
             for (int i = 0; i < V / 2; i++) {
                 const float2 v = acc[V / 2 * c + i];
