@@ -733,11 +733,14 @@ quantize_fp8_weights_kernel(const T* __restrict__ w, int rows, int cols, uint8_t
 // never overflows, and num = 1 or e by g's sign.  e is 2^x for x = -|g| log2 e
 // with the rounding of that product made good (x + lo is exact to 2^-45 or so),
 // so only the two approximate instructions' own errors remain (2 ulp and 1 ulp).
+// |g| is cut off at 128 there, where e is 0 in f32 already: from 2^128 / log2 e
+// on x would be infinite, and the good made of it not a number.
 struct Swiglu2 {
     Pair g, u, sig;   // after the cut-offs
 };
 constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = (float)(1.4426950408889634074 - (double)kLog2e);
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kGateMost = 128.f;
 __device__ __forceinline__ float min_nan(float a, float b) {
     float r;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -759,10 +762,10 @@ __device__ __forceinline__ Swiglu2 swiglu2(float2 gate, float2 up, float limit) 
         gate = make_float2(min_nan(gate.x, limit), min_nan(gate.y, limit));
         up = make_float2(max_nan(min_nan(up.x, limit), -limit), max_nan(min_nan(up.y, limit), -limit));
     }
-    const Pair n = pair(-fabsf(gate.x), -fabsf(gate.y)), l2e = pair(kLog2e, kLog2e);
-    const Pair x = mul2(n, l2e);
+    const Pair a = pair(min_nan(fabsf(gate.x), kGateMost), min_nan(fabsf(gate.y), kGateMost)), l2e = pair(-kLog2e, -kLog2e);
+    const Pair x = mul2(a, l2e);
     const float2 xf = unpair(x);
-    const Pair lo = fma2(n, pair(kLog2eLow, kLog2eLow), fma2(n, l2e, pair(-xf.x, -xf.y)));
+    const Pair lo = fma2(a, pair(-kLog2eLow, -kLog2eLow), fma2(a, l2e, pair(-xf.x, -xf.y)));
     const Pair e0 = pair(exp2_approx(xf.x), exp2_approx(xf.y));
     const float2 e = unpair(fma2(mul2(e0, lo), pair(kLn2, kLn2), e0));
     const float2 r = make_float2(reciprocal_approx(1.f + e.x), reciprocal_approx(1.f + e.y));

@@ -1,0 +1,89 @@
+"""The 8-bit expert operators at the ends of their types' ranges, on the GPU
+against the plain forms in 64 bits.
+
+Tolerances as in test_gpu_fp8.py: 32 u of the value (u = 2^-24; 16 u of each of
+two factors), then half the distance between neighbouring codes.  The gate's
+gradient is a sum, 1 + g (1 - sigma), whose parts cancel nowhere here: sigma is
+0 or 1 to the last bit at the gates that are large, and the others are ordinary.
+"""
+import pytest
+
+import qauntrunner_b200 as Q
+from tests import fp8_plain as F
+from tests.test_gpu_fp8 import BF16, F16, F32, U, gen, randn
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+# ------------------------------------------------------------ SwiGLU's gate
+
+def large_gates(type):
+    """Gates at and below the type's largest magnitude, and around 2^128 / log2(e)
+    = 2.3587e38, where g log2(e) passes the f32 range."""
+    top = float(torch.finfo(F.DTYPE[type]).max)
+    return [v for v in (top, 0.99 * top, 2.4e38, 2.36e38, 2.358e38, 2.3e38, 1e30, 60000.0, 129.0, 128.0, 105.0, 89.0)
+            if v <= top]
+
+
+def extremes(type, f, sign):
+    """gu, dh of four rows: ordinary values, and among the first block of 128
+    some large gates of one sign.  Where the gate passes, up and dh are small
+    enough for the f32 range, and half of the columns are masked by 0."""
+    g = gen(f + type)
+    gu, dh = randn(g, 4, 2 * f, type=type), randn(g, 4, f, type=type)
+    for i, v in enumerate(large_gates(type)):
+        for row in range(4):
+            c = 7 * i + row
+            gu[row, c] = sign * v
+            if sign > 0:
+                small = 0.0 if row % 2 else 1.0 / max(v, 1.0)
+                gu[row, f + c] = small if type != F16 else 2.0 ** -10
+                dh[row, c] = dh[row, c] * (2.0 ** -10 if v < 1e30 else 2.0 ** -40)
+    return gu, dh
+
+
+def close(codes, scales, want, size):
+    assert not bool(scales.isnan().any()) and not bool((codes & 0x7F == 0x7F).any())
+    err = (F.values(codes, scales) - want).abs()
+    return bool((err <= F.code_bound(want.abs() + 32 * U * size, scales) * (1 + 32 * U) + 32 * U * size).all())
+
+
+@pytest.mark.parametrize("type", [F32, F16, BF16])
+@pytest.mark.parametrize("limit", [0.0, 7.0])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_swiglu_of_large_gates(type, limit, sign):
+    f = 256
+    gu, _ = extremes(type, f, sign)
+    codes, scales = torch.zeros(4, f, dtype=torch.uint8).cuda(), torch.zeros(4, 2).cuda()
+    Q.swiglu_fp8(type, gu.cuda(), 4, f, codes, scales, limit=limit)
+    h = F.swiglu(gu[:, :f], gu[:, f:], limit)
+    assert close(codes.cpu(), scales.cpu(), h, h.abs())
+
+
+@pytest.mark.parametrize("type", [F32, F16, BF16])
+@pytest.mark.parametrize("limit", [0.0, 7.0])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_swiglu_grad_of_large_gates(type, limit, sign):
+    f = 256
+    gu, dh = extremes(type, f, sign)
+    codes, scales = torch.zeros(4, 2 * f, dtype=torch.uint8).cuda(), torch.zeros(4, 4).cuda()
+    Q.swiglu_fp8_grad(type, gu.cuda(), dh.cuda(), 4, f, codes, scales, limit=limit)
+    dg, du, parts = F.swiglu_grad(gu[:, :f], gu[:, f:], dh, limit)
+    ordinary = gu[:, :f].double().abs() < 80
+    size = torch.where(ordinary & (dg != 0), parts, dg.abs())
+    assert close(codes.cpu(), scales.cpu(), torch.cat([dg, du], 1), torch.cat([size, du.abs()], 1))
+
+
+def test_a_masked_gate_leaves_its_block_as_it_is():
+    """The type's lowest value as a gate, as a mask would put it: h is 0 there and
+    the other columns' codes are what they are without it."""
+    for type in (F32, BF16):
+        gu = randn(gen(3), 2, 512, type=type)
+        gu[1] = gu[0]
+        gu[1, 5:256:9] = torch.finfo(F.DTYPE[type]).min
+        gu[0, 5:256:9] = 0.0
+        codes, scales = torch.zeros(2, 256, dtype=torch.uint8).cuda(), torch.zeros(2, 2).cuda()
+        Q.swiglu_fp8(type, gu.cuda(), 2, 256, codes, scales)
+        v = F.values(codes.cpu(), scales.cpu())
+        assert torch.equal(v[0], v[1]) and bool((v[1, 5:256:9] == 0).all())
