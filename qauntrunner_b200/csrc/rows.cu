@@ -123,7 +123,8 @@ extern "C" int qrm_sort_tokens(const int32_t* topk_idx_dev, int64_t T, int k, in
     cfg.numAttrs = 2;
     auto kernel = many ? sort_tokens_kernel<kSortCluster> : sort_tokens_kernel<1>;
     e = cudaSuccess;
-    if (cfg.dynamicSmemBytes > 48 * 1024)
+    // a launch has 48 KB without asking, the kernel's own warp sums included
+    if (cfg.dynamicSmemBytes + kSortOwnSmem > 48 * 1024)
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (int)(sizeof(int32_t) * 34 * kSortMaxExperts));
     if (e == cudaSuccess)

@@ -252,6 +252,7 @@ __device__ __forceinline__ int columns_at(int c, int cols, int most = 8) { retur
 // flight instead of four; 4 us at 8 assignments.
 constexpr int kSortMaxExperts = 1024;
 constexpr int kSortCluster = 8;
+constexpr int kSortOwnSmem = 32 * sizeof(int32_t);   // bytes beside the dynamic ones: a sum of each warp
 
 // lanes whose e is this lane's; bits: of the largest e and of -1
 __device__ __forceinline__ uint32_t lanes_with(int e, int bits) {
@@ -275,7 +276,7 @@ sort_tokens_kernel(const int32_t* __restrict__ idx, long long n, int first, int 
     int32_t* total = sort_sm;            // [E] this CTA's count of each expert
     int32_t* start = sort_sm + E;        // [E] place of this CTA's first assignment of each expert
     int32_t* count = sort_sm + 2 * E;    // [W][E] each warp's count, then its running place
-    __shared__ int32_t warp_sum[32];
+    __shared__ int32_t warp_sum[kSortOwnSmem / sizeof(int32_t)];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = C > 1 ? (int)cluster.block_rank() : 0;
