@@ -120,7 +120,8 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     if (e == cudaSuccess) e = cudaMemset(m->arrivals, 0, counts);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_stream_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(fp8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(kFp8MaxGroups));
     cudaFuncAttributes pair{};
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&pair, fp8_pair_kernel);
     if (e != cudaSuccess) return bail(failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e)));

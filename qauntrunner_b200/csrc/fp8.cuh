@@ -16,6 +16,7 @@
 
 #include "common.cuh"
 #include "gemv_imma.cuh"
+#include "pair_drain.h"
 #include "umma_ptx.cuh"
 
 namespace qrm {
@@ -153,6 +154,10 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
     return p != 0;
+}
+// the last `stages` of a CTA's own copies have landed (out of line: it runs only when a wait gave up)
+__device__ __noinline__ void drain_own(uint64_t* full, uint32_t issued, uint32_t stages) {
+    for (uint32_t j = issued > stages ? issued - stages : 0; j < issued; j++) mbar_wait(&full[j % stages], (j / stages) & 1u);
 }
 // position in a ring: slot and the parity of its current phase
 struct Ring {
@@ -346,6 +351,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     uint64_t* done_bar = sc_empty + kFp8ScaleRing;
     volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + 768);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 776);
+    volatile uint32_t* issued = reinterpret_cast<volatile uint32_t*>(sm + 780);   // stages, once their warp is through
     float* sc_ring = reinterpret_cast<float*>(sm + kFp8ScaleOff);
     int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp8TableOff);
     int32_t* start = first_tile + p.groups + 1;
@@ -387,7 +393,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
         // ------------------------------------------------ tiles
         bool ok = true;
         Ring r;
-        uint32_t issued = 0;
+        uint32_t n_issued = 0;
         for (long long q = q0; q < q1 && ok;) {
             const Fp8Piece t = plan.piece(q, q1);
             const int boxes = (t.n + 15) >> 4;
@@ -403,13 +409,11 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
                 }
                 __syncwarp();
                 r.next(stages);
-                issued++;
+                n_issued++;
             }
             q += t.k1 - t.k0;
         }
-        if (!ok && lane == 0)   // copies already issued must land before the CTA exits
-            for (uint32_t j = issued > (uint32_t)stages ? issued - stages : 0; j < issued; j++)
-                mbar_wait(&full[j % stages], (j / stages) & 1u);
+        if (lane == 0) *issued = n_issued;
     } else if (warp == 1) {
         // ------------------------------------------------ MMAs (one thread issues)
         bool ok = true;
@@ -606,6 +610,8 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    // a role that gave up may have left copies that nothing waited for: they land before the CTA exits
+    if (threadIdx.x == 0 && *abort_flag) drain_own(full, *issued, stages);
     if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
@@ -687,6 +693,25 @@ __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// a word of the peer's shared memory, at the same place as ours; the cluster barrier after it makes it visible
+__device__ __forceinline__ void store_peer(uint32_t* p, uint32_t rank, uint32_t v) {
+    asm volatile(
+        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n st.shared::cluster.u32 [a], %2;\n}\n" ::"r"(smem_u32(p)),
+        "r"(rank), "r"(v)
+        : "memory");
+}
+// the first CTA's barriers, as drain_pair moves them on
+struct PairBars {
+    uint64_t* full;
+    __device__ void expect(uint32_t slot) { mbar_arrive_expect_tx(&full[slot], kFp8PairStage); }
+    __device__ void complete(uint32_t slot) {
+        asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[slot])),
+                     "r"((uint32_t)kFp8PairStage)
+                     : "memory");
+    }
+    __device__ void wait(uint32_t slot, uint32_t parity) { mbar_wait(&full[slot], parity); }
+};
+
 struct Fp8PairTile {
     int group, n;    // matrix, first output
     int pos, rows;   // first row of x of the tile, rows of the group from there on
@@ -748,7 +773,11 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     uint64_t* sc_full = acc_empty + 2 * kFp8PairAcc;
     uint64_t* sc_empty = sc_full + kFp8PairScaleRing;
     uint64_t* done_bar = sc_empty + kFp8PairScaleRing;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + 768);
+    uint64_t* left_bar = done_bar + 1;                // both, when the first CTA gave up: its commits are through
+    // (not in the dynamic part, whose addresses would take registers through the sums)
+    __shared__ volatile int given_up;
+    __shared__ volatile uint32_t from_peer, issued;   // issued: stages, once their warp is through
+    volatile int* abort_flag = &given_up;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 776);
     float* sc_ring = reinterpret_cast<float*>(sm + kFp8ScaleOff);
     int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp8PairTableOff);
@@ -770,6 +799,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             mbar_init(&sc_empty[i], kFp8EpiWarps);
         }
         mbar_init(done_bar, 1);
+        mbar_init(left_bar, 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -808,7 +838,7 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             // -------------------------------------------- tiles
             bool ok = true;
             Ring r;
-            uint32_t issued = 0;
+            uint32_t n_issued = 0;
             const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
                 const Fp8PairTile t = tile_at(i);
@@ -829,13 +859,10 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                     }
                     __syncwarp();
                     r.next(kFp8PairStages);
-                    issued++;
+                    n_issued++;
                 }
             }
-            // copies already issued must land before the CTAs exit (both CTAs' complete on the first's barriers)
-            if (!ok && rank == 0 && lane == 0)
-                for (uint32_t j = issued > (uint32_t)kFp8PairStages ? issued - kFp8PairStages : 0; j < issued; j++)
-                    mbar_wait(&full[j % kFp8PairStages], (j / kFp8PairStages) & 1u);
+            if (lane == 0) issued = n_issued;
         } else if (warp == 1 && rank == 0) {
             // -------------------------------------------- MMAs (one thread issues for both CTAs)
             bool ok = true;
@@ -982,8 +1009,25 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     // ---------------- teardown: every role of both CTAs is done (or gave up); free tensor memory
     tc_fence_before();
     __syncthreads();
+    // Copies that nothing waited for are left only where the MMAs did not run to their end, and then the first CTA's
+    // flag is set.  It learns how many stages the other has issued, which learns whether to stay.
+    if (threadIdx.x == 0) store_peer(const_cast<uint32_t*>(&from_peer), rank ^ 1, rank == 0 ? (uint32_t)given_up : issued);
+    __syncwarp();
     cluster_sync_all();
     tc_fence_after();
+    if (rank == 0 ? given_up != 0 : from_peer != 0) {
+        if (rank == 0 && threadIdx.x == 0) {
+            PairBars bars{full};
+            drain_pair(issued, from_peer, kFp8PairStages, bars);
+        }
+        if (warp == 1) {
+            if (rank == 0 && elect_one()) umma_commit_pair(smem_u32(left_bar));
+            __syncwarp();
+            if (lane == 0) mbar_wait(left_bar, 0u);
+        }
+        __syncwarp();
+        cluster_sync_all();
+    }
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
