@@ -341,7 +341,8 @@ int qrm_swiglu_fp8_grad(int type, const void* gu_dev, int64_t ld_gu, const void*
  * included).  type is the result's.  Products on one handle must not overlap:
  * they share its workspace (128 KiB for each SM).  qrm_fp8_sync waits for the
  * device and reports what the products met: QRM_E_INVALID for offsets that do
- * not ascend within [0, T] (such a group counts as empty), QRM_E_TIMEOUT for a
+ * not ascend within [0, T] (such a group counts as empty, and one that starts
+ * below an offset before it, so no row is in two groups), QRM_E_TIMEOUT for a
  * wait that gave up (QRM_WAIT_LIMIT_US in the environment at creation). */
 typedef struct qrm_fp8 qrm_fp8;
 int  qrm_fp8_create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes,

@@ -273,12 +273,14 @@ __device__ inline void fp8_share_out(Fp8Plan& plan, int tiles, int kb, int ctas)
 
 // The groups' tables in shared memory, by one warp; the caller synchronises.
 // Offsets that do not ascend within [0, T] make a group empty and raise an
-// error: no row outside x or out is ever touched.
+// error, and so does a start below any offset before it: no row outside x or
+// out is ever touched, and none belongs to two groups (whose CTAs would both
+// write it, and whose tiles together could be more than a count of them holds).
 // tile_rows rows of x a tile, `across` tiles along the outputs.
 __device__ inline void fp8_tables(const Fp8Params& p, int32_t* first_tile, int32_t* start, int32_t* rows, int tile_rows,
                                   int across, bool report) {
     const int lane = threadIdx.x & 31;
-    int before = 0;
+    int before = 0, top = 0;   // tiles, largest offset so far
     bool bad = false;
     for (int g0 = 0; g0 < p.groups; g0 += 32) {
         const int g = g0 + lane;
@@ -286,10 +288,17 @@ __device__ inline void fp8_tables(const Fp8Params& p, int32_t* first_tile, int32
         if (g < p.groups) {
             a = p.offsets ? p.offsets[g] : 0;
             b = p.offsets ? p.offsets[g + 1] : p.T;
-            if (a < 0 || b < a || b > p.T) {
-                bad = true;
-                a = b = 0;
-            }
+        }
+        int most = a;   // of the offsets up to this one
+        if (p.groups > 1) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) most = max(most, __shfl_up_sync(0xffffffffu, most, o));   // (lanes below o get their own)
+            most = max(most, top);
+            top = __shfl_sync(0xffffffffu, most, 31);
+        }
+        if (a < most || a < 0 || b < a || b > p.T) {
+            bad |= g < p.groups;
+            a = b = 0;
         }
         const int tiles = (b - a + tile_rows - 1) / tile_rows * across;
         int scan = tiles;
