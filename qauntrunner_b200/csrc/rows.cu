@@ -192,7 +192,7 @@ extern "C" int qrm_combine_rows(int type, const void* rows_dev, int64_t n_rows, 
     c.grid.x = walkers(T, c.grid.y, sms, 4 * 256 / c.threads);
     const bool wide = wide_rows(rows_dev, ld_rows, b) && wide_rows(out_dev, ld_out, b) &&
                       (!add_dev || wide_rows(add_dev, ld_add, b));
-    BY_TYPE(type, e = launch_ahead(combine_rows_kernel<V>, c.grid, c.threads, 0, (cudaStream_t)stream, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, (int)T, k, (int)d, (const V*)add_dev, ld_add,
+    BY_TYPE(type, e = launch_ahead(combine_rows_kernel<V>, c.grid, c.threads, 0, (cudaStream_t)stream, (const V*)rows_dev, ld_rows, (uint32_t)n_rows, pos_dev, w_dev, (uint32_t)T, k, (int)d, (const V*)add_dev, ld_add,
                       (V*)out_dev, ld_out, wide));
     return done(what, e);
 }

@@ -475,15 +475,15 @@ gather_rows_fp8_kernel(const T* __restrict__ x, long long ld_x, const int32_t* _
 template <typename T>
 __global__ void __launch_bounds__(256, 4)
 combine_rows_kernel(const T* __restrict__ rows, long long ld_rows, uint32_t n_rows, const int32_t* __restrict__ pos,
-                    const float* __restrict__ w, int tokens, int k, int d, const T* __restrict__ add, long long ld_add,
+                    const float* __restrict__ w, uint32_t tokens, int k, int d, const T* __restrict__ add, long long ld_add,
                     T* __restrict__ out, long long ld_out, bool wide) {
     pdl_start();
     constexpr int S = sizeof(T) == 4 ? 4 : 8;   // rows whose loads are in flight: 32 registers
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, d), lane = threadIdx.x & 31;
-    int t = blockIdx.x;
+    uint32_t t = blockIdx.x;   // (unsigned: a step past the last of 2^31 - 1 tokens stays a number past it)
     uint32_t p_next = ~0u;
     float w_next = 1.f;
-    auto ahead = [&](int at) {   // slots lane < min(k, S) of token `at`
+    auto ahead = [&](uint32_t at) {   // slots lane < min(k, S) of token `at`
         if (at < tokens && lane < S && lane < k) {
             p_next = pos[(size_t)at * k + lane];
             if (w) w_next = w[(size_t)at * k + lane];
@@ -789,15 +789,16 @@ swiglu_fp8_kernel(const T* __restrict__ gu, long long ld, int rows, const int32_
                   bool wide_c) {
     pdl_start();
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
-    if (n_dev) rows = min(rows, *n_dev);
-    int t = blockIdx.x;
-    if (t >= rows) return;
+    if (n_dev) rows = max(min(rows, *n_dev), 0);
+    const uint32_t end = rows;
+    uint32_t t = blockIdx.x;   // (unsigned, as in combine_rows_kernel)
+    if (t >= end) return;
     gu += c;
     Raw8<T> g = load_raw8(gu + t * ld, n, wide), u = load_raw8(gu + t * ld + f, n, wide);   // absent columns are 0, and h there
     for (;;) {
-        const int next = t + gridDim.x;
+        const uint32_t next = t + gridDim.x;
         Raw8<T> g1 = g, u1 = u;
-        if (next < rows) {
+        if (next < end) {
             g1 = load_raw8(gu + next * ld, n, wide);
             u1 = load_raw8(gu + next * ld + f, n, wide);
         }
@@ -813,7 +814,7 @@ swiglu_fp8_kernel(const T* __restrict__ gu, long long ld, int rows, const int32_
             store_codes8(codes + t * ld_c + c, codes8(h, quant(s)), n, wide_c);
             if ((threadIdx.x & 15) == 0) scales[t * ld_s + c / kFp8Block] = s;
         }
-        if (next >= rows) return;
+        if (next >= end) return;
         t = next;
         g = g1;
         u = u1;
@@ -828,16 +829,17 @@ swiglu_fp8_grad_kernel(const T* __restrict__ gu, long long ld, const T* __restri
                        float* __restrict__ scales, long long ld_s, bool wide, bool wide_c) {
     pdl_start();
     const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8, n = columns_at(c, f);
-    if (n_dev) rows = min(rows, *n_dev);
-    int t = blockIdx.x;
-    if (t >= rows) return;
+    if (n_dev) rows = max(min(rows, *n_dev), 0);
+    const uint32_t end = rows;
+    uint32_t t = blockIdx.x;   // (unsigned, as in combine_rows_kernel)
+    if (t >= end) return;
     gu += c;
     dh += c;
     Raw8<T> g = load_raw8(gu + t * ld, n, wide), u = load_raw8(gu + t * ld + f, n, wide), d = load_raw8(dh + t * ld_dh, n, wide);
     for (;;) {
-        const int next = t + gridDim.x;
+        const uint32_t next = t + gridDim.x;
         Raw8<T> g1 = g, u1 = u, d1 = d;
-        if (next < rows) {
+        if (next < end) {
             g1 = load_raw8(gu + next * ld, n, wide);
             u1 = load_raw8(gu + next * ld + f, n, wide);
             d1 = load_raw8(dh + next * ld_dh, n, wide);
@@ -869,7 +871,7 @@ swiglu_fp8_grad_kernel(const T* __restrict__ gu, long long ld, const T* __restri
                 scales[t * ld_s + (f + c) / kFp8Block] = su;
             }
         }
-        if (next >= rows) return;
+        if (next >= end) return;
         t = next;
         g = g1;
         u = u1;

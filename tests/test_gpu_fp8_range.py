@@ -87,3 +87,35 @@ def test_a_masked_gate_leaves_its_block_as_it_is():
         Q.swiglu_fp8(type, gu.cuda(), 2, 256, codes, scales)
         v = F.values(codes.cpu(), scales.cpu())
         assert torch.equal(v[0], v[1]) and bool((v[1, 5:256:9] == 0).all())
+
+
+# ------------------------------------------------------------ as many rows as a count holds
+
+MANY = 2 ** 31 - 1
+
+
+def test_combine_of_the_most_tokens():
+    """One column, one slot: the walk's last steps, where a signed row number would turn negative (13 GB)."""
+    pos = torch.full((MANY,), -1, dtype=torch.int32, device="cuda")
+    pos[0], pos[MANY - 5000], pos[-1] = 1, 2, 0
+    rows = torch.tensor([3.0, -2.0, 0.5], dtype=torch.float16, device="cuda")
+    out = torch.full((MANY,), 5.0, dtype=torch.float16, device="cuda")
+    Q.combine_rows(F16, rows, 3, pos, None, MANY, 1, 1, out)
+    torch.cuda.synchronize()
+    assert (float(out[0]), float(out[MANY - 5000]), float(out[-1])) == (-2.0, 0.5, 3.0)
+    assert int(out.count_nonzero()) == 3
+
+
+def test_swiglu_of_the_most_rows():
+    """One column: 20 GB."""
+    gu = torch.zeros(MANY, 2, dtype=torch.float16, device="cuda")
+    gu[0], gu[-1] = 1.0, -1.0
+    codes = torch.full((MANY,), 9, dtype=torch.uint8, device="cuda")
+    scales = torch.full((MANY,), 5.0, device="cuda")
+    Q.swiglu_fp8(F16, gu, MANY, 1, codes, scales)
+    torch.cuda.synchronize()
+    h = F.swiglu(gu[:, :1][[0, -1]].cpu(), gu[:, 1:][[0, -1]].cpu(), 0.0)[:, 0]
+    got = torch.tensor([float(scales[0]), float(scales[-1])], dtype=torch.float64) * 448
+    assert bool(((got - h.abs()).abs() <= 32 * U * h.abs()).all())
+    assert int((codes & 0x7F == 0x7E).count_nonzero()) == 2 and int(codes.count_nonzero()) == 2   # 448, and 0
+    assert float(scales[1:-1].max()) == F.MIN_SCALE
