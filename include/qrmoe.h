@@ -272,7 +272,9 @@ int  qrm_matrix_gemv_static(qrm_matrix* m, const float* x_dev, int T, float* y_d
  * sums, scales and weights w are f32.  ld_*: elements from row to row, 0 for
  * dense rows.  Everything is asynchronous on `stream` (NULL: the default
  * stream) and may be captured in a graph.  The calls without a handle run on
- * the calling thread's current device and keep nothing.  Arrays must be
+ * the calling thread's current device and keep nothing; those of qrm_fp8 run on
+ * the matrix's, with arrays that are there, and leave the thread's as it was
+ * (the calls of the other handles make theirs current).  Arrays must be
  * aligned to their own values; 16-byte rows (8-byte for codes) are faster.
  *
  * qrm_sort_tokens: the n = T k assignments a = t k + j, in order of their
@@ -331,7 +333,7 @@ int qrm_swiglu_fp8_grad(int type, const void* gu_dev, int64_t ld_gu, const void*
 /* groups matrices [rows x cols] in 8 bits, kept in HBM: codes
  * [groups][rows][cols] (code_bytes = their number) and scales
  * [groups][ceil(rows/128)][ceil(cols/128)] are copied, from the host or
- * (_device, after a device synchronise) from the device.  At most 1024 groups
+ * (_device) from any device, after a synchronise of it.  At most 1024 groups
  * (QRM_E_CAPACITY).
  * qrm_fp8_product: y[t] = W_g x[t] for the rows t in [offsets[g],
  * offsets[g+1]) of each group g (offsets NULL: one group, all T rows), x

@@ -565,9 +565,11 @@ class Fp8Matrix:
     """`groups` matrices [rows x cols] in 8-bit floating point with a scale for
     each 128 x 128 block, kept in HBM (qrm_fp8_*).  codes [groups][rows][cols]
     (one byte each) and scales [groups][ceil(rows/128)][ceil(cols/128)] are
-    NumPy arrays or tensors, on the host or the device, and are copied."""
+    NumPy arrays or tensors, on the host or a device, and are copied.  device:
+    where they are kept (None: where codes are, 0 if that is the host); the
+    products' arrays are there too."""
 
-    def __init__(self, rows, cols, codes, scales, groups=1, device=0):
+    def __init__(self, rows, cols, codes, scales, groups=1, device=None):
         on_device = [bool(getattr(a, "is_cuda", False)) for a in (codes, scales)]
         if on_device[0] != on_device[1]:
             raise ValueError("codes and scales must both be on the host or both on the device")
@@ -583,6 +585,8 @@ class Fp8Matrix:
             scales = np.ascontiguousarray(scales, dtype=np.float32)
             if codes.itemsize != 1:
                 raise ValueError("codes of one byte are needed")
+        if device is None:
+            device = codes.device.index if on_device[0] else 0
         create = lib().qrm_fp8_create_device if on_device[0] else lib().qrm_fp8_create
         h = P()
         _check(create(device, groups, rows, cols, _ptr(codes), codes.nbytes, _ptr(scales), scales.nbytes, C.byref(h)))

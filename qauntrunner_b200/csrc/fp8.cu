@@ -33,10 +33,24 @@ int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
 
 void release(qrm_fp8* m) {
     if (!m) return;
-    cudaSetDevice(m->device);
+    DeviceGuard here;
+    here.enter(m->device);
     cudaDeviceSynchronize();
     cudaFree(m->codes);
     delete m;
+}
+
+// waits for what any stream still writes at p, when that is on another device
+cudaError_t await_source(const void* p, int device) {
+    cudaPointerAttributes at{};
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();   // the copy will say what is wrong with it
+        return cudaSuccess;
+    }
+    if (at.type != cudaMemoryTypeDevice || at.device == device) return cudaSuccess;
+    DeviceGuard there;
+    const cudaError_t e = there.enter(at.device);
+    return e == cudaSuccess ? cudaDeviceSynchronize() : e;
 }
 
 // 8-bit tensor of up to three dimensions, innermost first, as a TMA map; what
@@ -82,7 +96,8 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) return failf(QRM_E_CUDA, "%s: no CUDA device", what);
     if (device < 0 || device >= count) return failf(QRM_E_INVALID, "%s: device %d out of range", what, device);
     int sms;
-    if (cudaSetDevice(device) != cudaSuccess) return failf(QRM_E_CUDA, "%s: device %d", what, device);
+    DeviceGuard here;
+    if (here.enter(device) != cudaSuccess) return failf(QRM_E_CUDA, "%s: device %d", what, device);
     if (int rc = current_device(&device, &sms)) return rc;
     if (const char* e = getenv("QRM_WAIT_LIMIT_US"))
         if (set_wait_limit_here((uint64_t)std::max(1LL, atoll(e)) * 1000ull) != cudaSuccess)
@@ -113,8 +128,13 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     m->part = reinterpret_cast<float*>(m->codes + scales_at);
     m->arrivals = reinterpret_cast<int32_t*>(m->codes + part_at);
     m->err = m->arrivals + (size_t)sms * kFp8EpiWarps;
-    // device sources: what any stream still writes there is awaited, as in qrm_upload_expert_device
+    // device sources: what any stream still writes there is awaited, as in qrm_upload_expert_device, and on their own
+    // device if that is another one
     cudaError_t e = cudaDeviceSynchronize();
+    if (kind == cudaMemcpyDeviceToDevice) {
+        if (e == cudaSuccess) e = await_source(codes, device);
+        if (e == cudaSuccess) e = await_source(scales, device);
+    }
     if (e == cudaSuccess) e = cudaMemcpy2D(m->codes, m->pitch, codes, cols, cols, (size_t)groups * rows, kind);
     if (e == cudaSuccess) e = cudaMemcpy(m->scales, scales, scale_bytes, kind);
     if (e == cudaSuccess) e = cudaMemset(m->arrivals, 0, counts);
@@ -191,7 +211,8 @@ int product(const char* what, qrm_fp8* m, bool back, const void* x, int64_t ld_x
         return failf(QRM_E_INVALID, "%s: rows of codes must start on 16 bytes (pitch %lld)", what, (long long)ld_x);
     if (!aligned(xs, 4) || !aligned(out, b) || (offsets && !aligned(offsets, 4)))
         return failf(QRM_E_INVALID, "%s: a pointer is not aligned to its values", what);
-    cudaError_t e = cudaSetDevice(m->device);
+    DeviceGuard here;
+    cudaError_t e = here.enter(m->device);
     if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
     CUtensorMap x_map;
     const cuuint64_t dims[2] = {(cuuint64_t)in, (cuuint64_t)T};
@@ -264,7 +285,8 @@ extern "C" int qrm_fp8_product_t(qrm_fp8* m, const void* y_codes_dev, int64_t ld
 
 extern "C" int qrm_fp8_sync(qrm_fp8* m) {
     if (!m) return failf(QRM_E_INVALID, "qrm_fp8_sync: NULL matrix");
-    cudaError_t e = cudaSetDevice(m->device);
+    DeviceGuard here;
+    cudaError_t e = here.enter(m->device);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     int32_t err = 0;
     if (e == cudaSuccess) e = cudaMemcpy(&err, m->err, sizeof err, cudaMemcpyDeviceToHost);

@@ -47,6 +47,28 @@ inline int current_device(int* device, int* sms) {
     return QRM_OK;
 }
 
+// Makes a device current and the caller's current again at the end: calls that
+// have no handle run on the caller's, so a handle's may not change it.
+class DeviceGuard {
+public:
+    DeviceGuard() = default;
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+    cudaError_t enter(int device) {
+        int now;
+        cudaError_t e = cudaGetDevice(&now);
+        if (e != cudaSuccess || now == device) return e;
+        if ((e = cudaSetDevice(device)) == cudaSuccess) caller_ = now;
+        return e;
+    }
+    ~DeviceGuard() {
+        if (caller_ >= 0) cudaSetDevice(caller_);
+    }
+
+private:
+    int caller_ = -1;   // the device to go back to, if another one is current
+};
+
 // a pitch in elements: 0 stands for dense rows
 inline bool pitch_ok(int64_t* ld, int64_t cols) {
     if (*ld == 0) *ld = cols;
