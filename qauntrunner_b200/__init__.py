@@ -202,10 +202,12 @@ def _check(rc):
 def _ptr(a):
     if a is None or isinstance(a, int):
         return a
+    if type(a) is np.ndarray:   # first: an exception caught costs more than the rest of a host array's way
+        return a.ctypes.data
     try:
         return a.data_ptr()
     except AttributeError:
-        return a.ctypes.data_as(P).value
+        return a.ctypes.data
 
 
 def qw_layer_desc(path, layer_index, device=0, max_tokens=1):
