@@ -340,8 +340,12 @@ int qrm_swiglu_fp8_grad(int type, const void* gu_dev, int64_t ld_gu, const void*
  * [T][cols] and y [T][rows]; rows outside every group are not written.
  * qrm_fp8_product_t: x[t] = W_g^T y[t], the gradient of the product's input,
  * from the same stored matrix.  Rows of codes start on 16 bytes (pitch
- * included).  type is the result's.  Products on one handle must not overlap:
- * they share its workspace (128 KiB for each SM).  qrm_fp8_sync waits for the
+ * included).  type is the result's.  A row's scale times a matrix's is rounded
+ * to f32 before it meets their sum: results below some 1e-29 may lose bits, and
+ * a product of scales from 2^128 on is infinite.  Products on one handle must not overlap:
+ * they share its workspace (128 KiB for each SM), and sums come out wrong where
+ * they do.  On several streams the caller orders them (events), or keeps a
+ * handle for each.  qrm_fp8_sync waits for the
  * device and reports what the products met: QRM_E_INVALID for offsets that do
  * not ascend within [0, T] (such a group counts as empty, and one that starts
  * below an offset before it, so no row is in two groups), QRM_E_TIMEOUT for a

@@ -569,7 +569,11 @@ class Fp8Matrix:
     (one byte each) and scales [groups][ceil(rows/128)][ceil(cols/128)] are
     NumPy arrays or tensors, on the host or a device, and are copied.  device:
     where they are kept (None: where codes are, 0 if that is the host); the
-    products' arrays are there too."""
+    products' arrays are there too.
+
+    Products on one object share its workspace and must not overlap in time:
+    from several streams or graphs, order them by events or keep an object for
+    each, else their sums come out wrong, without an error."""
 
     def __init__(self, rows, cols, codes, scales, groups=1, device=None):
         on_device = [bool(getattr(a, "is_cuda", False)) for a in (codes, scales)]

@@ -158,8 +158,11 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     return QRM_OK;
 }
 
-// Which kernel a product takes, by an estimate of what both would cost with the
-// rows spread evenly over the groups.  Measured (us; weights on the MMA's M
+// Which kernel a product takes, by an estimate of what both would cost with all
+// T rows held and spread evenly over the groups: where offsets leave many of
+// them out (another rank's slots), it takes the large-group kernel too early, as
+// 16 rows each counted as 128 at 32 x 4096 x 7168 would take 222 us in place of
+// 179; a caller that knows how many are held passes that as T.  Measured (us; weights on the MMA's M
 // side / rows of x on it), outputs x contracted:
 //   1 x 4096 x 7168:  1 row 15 / 30, 64 rows 21 / 30, 256 rows 30 / 31, 512 rows 38 / 32
 //   1 x 28672 x 4096: 1 row 32 / 42, 64 rows 39 / 38, 128 rows 46 / 39, 256 rows 78 / 40, 4096 rows 877 / 425
@@ -171,7 +174,8 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
 // a row, a tile that several SMs share 50 ns a row more in the end.  The second
 // does whole tiles of 256 rows x 256 outputs in waves over the pairs of SMs, a
 // block in 0.42 us, or 0.55 when most pairs are at work.  The worst choice
-// among 90 measured sizes takes 1.2 times as long as the other kernel.
+// among 90 measured sizes, all of even groups with every row held, takes 1.2
+// times as long as the other kernel.
 bool pair_is_faster(int64_t T, int groups, int64_t M, int64_t mb, int64_t kb, int sms) {
     const double used = (double)std::min<int64_t>(T, groups), rows = T / used;   // groups with rows, rows of each
     const double blocks = std::ceil(rows / kFp8MaxRows), in_tile = rows / blocks, tiles = used * mb * blocks;

@@ -6,7 +6,10 @@
 // with blocks of 128 along the contracted dimension.  The inner sums are
 // tcgen05.mma (kind::f8f6f4, e4m3 x e4m3) into f32 tensor memory, a fresh
 // accumulator per block; the outer sum is one f32 FMA per value and block in
-// the epilogue warps' registers.  The transposed product (the input gradient,
+// the epilogue warps' registers.  Its factor sx sw is formed first, in f32: it
+// loses bits below 2^-126, which only results below some 1e-29 show, and is
+// infinite from 2^128 on (two factors, one after the other, would cost the
+// large-group kernel's sums another operation a value).  The transposed product (the input gradient,
 // y = W^T x) reads the same stored matrix: its tiles enter the MMA with M as
 // their contiguous dimension instead of K, and the scales' two block indices
 // change places.
@@ -182,7 +185,7 @@ struct Ring {
 // the parts up in the CTAs' order, so that the result does not depend on who
 // was last.  Nobody waits.
 //
-// 512 rows over 32 matrices of 4096 x 7168 (940 MB): 175 us, 5.4 TB/s.  One row
+// 512 rows over 32 matrices of 4096 x 7168 (940 MB): 163 us, 5.8 TB/s.  One row
 // through one such matrix: 12 us, latencies.
 //
 // Warps: 0 loads tiles (TMA), 1 issues the MMAs, 2 brings the scales (their
@@ -637,7 +640,7 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
 // epilogue's loads out of tensor memory, hand-over back.  So the tile's two
 // blocks of 128 outputs have MMAs, accumulators (two each) and epilogue warps
 // of their own, and take turns on the tensor cores.  4096 rows, 28672 x 4096:
-// 425 us, 2.26 PFLOP/s, tensor pipe 62 % active; 483 us under sustained load
+// 427 us, 2.25 PFLOP/s, tensor pipe 62 % active; 497 us under sustained load
 // (power cap, 1.5 GHz).
 //
 // Warps: 0 loads tiles, 1 issues the MMAs (in the pair's first CTA), 2 brings
@@ -727,8 +730,10 @@ struct Fp8PairTile {
 };
 
 // 128 outputs of one row that starts on 16 bytes, or on 32 (`wide`): a warp
-// writes 32 rows at once, so what counts is how few stores a row takes (483 us
-// in place of 535 at 4096 x 28672 x 4096).  One value at a time took some 20 us
+// writes 32 rows at once, so what counts is how few stores a row takes (32 bytes
+// a store: 495 us in place of 531 at 4096 x 28672 x 4096 in bf16, 542 in place
+// of 621 in f32, 420 in place of 435 for 8192 rows over 32 x 4096 x 7168, each
+// under sustained load).  One value at a time took some 20 us
 // a tile: where the rows of out do not start on 16 bytes, the other kernel
 // runs, whose warps write neighbouring outputs.
 template <typename T>

@@ -248,8 +248,8 @@ __device__ __forceinline__ int columns_at(int c, int cols, int most = 8) { retur
 // place.  No atomics: the order inside an expert is the assignments' own.
 // The lanes with one expert are found by a vote for each bit of its number.
 // Latencies bound it (8 SMs, a few passes over shared memory, two cluster
-// barriers): 12 us at 32768 assignments to 256 experts, 14.6 with one load in
-// flight instead of four; 4 us at 8 assignments.
+// barriers): 10.5 to 12 us at 32768 assignments to 256 experts, 14.6 with one
+// load in flight instead of four; 4 us at 8 assignments.
 constexpr int kSortMaxExperts = 1024;
 constexpr int kSortCluster = 8;
 constexpr int kSortOwnSmem = 32 * sizeof(int32_t);   // bytes beside the dynamic ones: a sum of each warp
@@ -779,8 +779,8 @@ __device__ __forceinline__ Swiglu2 swiglu2(float2 gate, float2 up, float limit) 
 __device__ __forceinline__ Pair negative(Pair p) { return p ^ 0x8000000080000000ull; }
 
 // The CTAs walk the rows; a row's loads are on their way while the one before
-// it is computed.  The gradient takes 66 us for 16384 rows of 2048 bf16 columns
-// with a limit, 4.1 TB/s: issue slots (74 % busy) bound it, some 50 operations
+// it is computed.  The gradient takes 63 us for 16384 rows of 2048 bf16 columns
+// with a limit, 4.3 TB/s (67 us under sustained load), the forward 43 us: issue slots (74 % busy) bound it, some 50 operations
 // a value; two rows ahead, or more CTAs of fewer registers, change nothing.
 template <typename T, bool LIMIT>
 __global__ void __launch_bounds__(256)
