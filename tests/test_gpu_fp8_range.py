@@ -119,3 +119,50 @@ def test_swiglu_of_the_most_rows():
     assert bool(((got - h.abs()).abs() <= 32 * U * h.abs()).all())
     assert int((codes & 0x7F == 0x7E).count_nonzero()) == 2 and int(codes.count_nonzero()) == 2   # 448, and 0
     assert float(scales[1:-1].max()) == F.MIN_SCALE
+
+
+# ------------------------------------------------------------ blocks of tiny values
+
+def tiny_blocks(g, type):
+    """Blocks whose largest magnitude is 2^-149 to 2^-85.  In three rows of four that is 7 times an odd number up to 15,
+    so the scale (a 448th) is that odd number and some power of two, and the others are the scale times 5 bits, which is
+    a tie between codes; in the fourth row any values.  (Where a value does not fit the type it is no tie any more.)"""
+    e = torch.arange(-149, -84).repeat_interleave(64)[:, None].float()
+    n = e.shape[0]
+    odd = 2 * torch.randint(0, 8, (n, 1), generator=g).float() + 1
+    ties = odd * (2 * torch.randint(8, 16, (n, 128), generator=g).float() + 1)
+    ties = torch.where(torch.rand(n, 128, generator=g) < 0.5, ties, -ties) * torch.exp2(torch.randint(-19, -3, (n, 128), generator=g).float())
+    any_ = 7 * odd * (2 * torch.rand(n, 128, generator=g) - 1)
+    x = torch.where(torch.arange(n)[:, None] % 4 > 0, ties, any_)
+    x[:, 0:1] = 7 * odd
+    return torch.ldexp(x, e - 5).to(F.DTYPE[type])
+
+
+@pytest.mark.parametrize("type", [F32, BF16])
+def test_quotients_of_tiny_blocks(type):
+    """Codes and scales bit for bit, against IEEE division (bf16's few bits make more ties)."""
+    x = tiny_blocks(gen(3 + type), type)
+    n = x.shape[0]
+    codes, scales = torch.zeros(n, 128, dtype=torch.uint8).cuda(), torch.zeros(n, 1).cuda()
+    Q.quantize_fp8(type, x.cuda(), n, 128, codes, scales)
+    v = x.float()
+    s = (v.abs().amax(1, keepdim=True) / 448.0).clamp_min(F.MIN_SCALE)
+    want = (v / s).to(torch.float8_e4m3fn).view(torch.uint8)
+    assert torch.equal(scales.cpu(), s) and torch.equal(codes.cpu(), want)
+    # the other operators that write 8-bit rows of given values
+    rows, rs = torch.zeros_like(codes), torch.zeros_like(scales)
+    pos = torch.arange(n, dtype=torch.int32).cuda()
+    Q.gather_rows_fp8(type, x.cuda(), pos, n, 1, 128, rows, rs, n)
+    assert torch.equal(rows.cpu(), want) and torch.equal(rs.cpu(), s)
+    rows, rs, w = torch.zeros_like(codes), torch.zeros_like(scales), torch.full((n, 1), -1.0).cuda()
+    Q.combine_rows_grad_fp8(type, x.cuda(), None, n, pos, w, n, 1, 128, rows, rs)
+    assert torch.equal(rows.cpu(), want ^ 0x80) and torch.equal(rs.cpu(), s)
+
+
+def test_quotients_of_tiny_weights():
+    x = tiny_blocks(gen(9), F32)[:4096].reshape(32, 128, 128)   # a block of 128 x 128 for each exponent or two
+    codes, scales = torch.zeros(32, 128, 128, dtype=torch.uint8).cuda(), torch.zeros(32, 1, 1).cuda()
+    Q.quantize_fp8_weights(F32, x.cuda(), 128, 128, codes, scales, groups=32)
+    s = (x.abs().amax((1, 2), keepdim=True) / 448.0).clamp_min(F.MIN_SCALE)
+    assert torch.equal(scales.cpu(), s)
+    assert torch.equal(codes.cpu(), (x / s).to(torch.float8_e4m3fn).view(torch.uint8))
