@@ -362,6 +362,88 @@ int  qrm_fp8_product_t(qrm_fp8* m, const void* y_codes_dev, int64_t ld_y, const 
                        const int32_t* offsets_dev, int64_t T, int type, void* x_dev, int64_t ld_x, void* stream);
 int  qrm_fp8_sync(qrm_fp8* m);
 
+/* ---- root-mean-square norm of rows, with the residual's addition (the step in
+ * front of the experts; the reference's RmsNorm, TransformerOps.cs, on any
+ * activation type) ----
+ * s = x + add, rounded to type (add NULL: x), inv = 1 / sqrt(mean(s^2) + eps),
+ * y = s inv w; w is f32 [d] (NULL: 1).  The norm is that of the sum as it is
+ * stored; sum_dev (NULL: not wanted) receives it.  Squares are summed in f32: a
+ * row whose sum of squares passes 2^128 gives zeros.
+ * qrm_rms_norm writes y in type, _fp8 in 8-bit rows, _fp4 in 4-bit rows; the
+ * latter two also write it in type where y_dev is not NULL (the router's
+ * input).  sum may be x or add, y any of them, in the same place and pitch.
+ * qrm_rms_norm_grad: with n = x inv (x is the forward's sum) and g = dy w,
+ *   dx = inv (g - n mean(g n)) + add,  dw = sum over the rows of dy n,
+ * add (NULL: none) being the gradient that the residual stream brings; dx is
+ * then the gradient of both of the forward's summands.  dw is f32 [d] (NULL:
+ * not wanted); work_dev: qrm_rms_norm_grad_work(rows, d) floats, which
+ * calls that overlap in time (two captured graphs, say) may not share (NULL
+ * where that is 0 or dw is not wanted).  dx may be dy, x or add.  The same call
+ * gives the same bits. */
+int qrm_rms_norm(int type, const void* x_dev, int64_t ld_x, const void* add_dev, int64_t ld_add, int64_t rows, int64_t d,
+                 const float* w_dev, float eps, void* sum_dev, int64_t ld_sum, void* y_dev, int64_t ld_y, void* stream);
+int qrm_rms_norm_fp8(int type, const void* x_dev, int64_t ld_x, const void* add_dev, int64_t ld_add, int64_t rows,
+                     int64_t d, const float* w_dev, float eps, void* sum_dev, int64_t ld_sum, void* y_dev, int64_t ld_y,
+                     uint8_t* codes_dev, int64_t ld_codes, float* scales_dev, int64_t ld_scales, void* stream);
+int qrm_rms_norm_fp4(int type, const void* x_dev, int64_t ld_x, const void* add_dev, int64_t ld_add, int64_t rows,
+                     int64_t d, const float* w_dev, float eps, void* sum_dev, int64_t ld_sum, void* y_dev, int64_t ld_y,
+                     uint8_t* codes_dev, int64_t ld_codes, uint8_t* scales_dev, int64_t ld_scales, void* stream);
+int64_t qrm_rms_norm_grad_work(int64_t rows, int64_t d);
+int qrm_rms_norm_grad(int type, const void* dy_dev, int64_t ld_dy, const void* x_dev, int64_t ld_x, int64_t rows,
+                      int64_t d, const float* w_dev, float eps, const void* add_dev, int64_t ld_add, void* dx_dev,
+                      int64_t ld_dx, float* dw_dev, float* work_dev, void* stream);
+
+/* ---- experts in 4-bit microscaled floating point (no counterpart in the
+ * reference) ----
+ * 4-bit rows: e2m1 codes, two to a byte (the even column in the low four bits),
+ * and one e8m0 scale (byte b stands for 2^(b - 127), 255 for NaN) for each 32
+ * columns, scale = 2^max(floor(log2 max|v|) - 2, -127), code = e2m1(v / scale) to
+ * nearest even, saturating at 6.  A row of codes takes whole blocks, 16 bytes
+ * each (the last one filled up with codes 0); a block that holds a NaN or an
+ * infinity gets scale 255 and codes 0.  type, ld_*, streams and devices as
+ * above; ld_codes and ld_scales in bytes.
+ * qrm_quantize_fp4 writes rows (or a matrix's: its blocks lie along the rows)
+ * in 4 bits, qrm_gather_rows_fp4 does that on the way to the experts (as
+ * qrm_gather_rows). */
+int qrm_quantize_fp4(int type, const void* x_dev, int64_t ld_x, int64_t rows, int64_t cols, const int32_t* n_rows_dev,
+                     uint8_t* codes_dev, int64_t ld_codes, uint8_t* scales_dev, int64_t ld_scales, void* stream);
+int qrm_gather_rows_fp4(int type, const void* x_dev, int64_t ld_x, const int32_t* pos_dev, int64_t T, int k, int64_t d,
+                        uint8_t* codes_dev, int64_t n_rows, int64_t ld_codes, uint8_t* scales_dev, int64_t ld_scales,
+                        void* stream);
+
+/* groups matrices [rows x cols] in 4 bits, kept in HBM: codes
+ * [groups][rows][16 ceil(cols/32)] and scales [groups][rows][ceil(cols/32)],
+ * bytes both, are copied, from the host or (_device) from any device, after a
+ * synchronise of it.  At most 1024 groups (QRM_E_CAPACITY).
+ * qrm_fp4_product: y[t] = W_g x[t] for the rows t in [offsets[g], offsets[g+1])
+ * of each group g (offsets NULL: one group, all T rows), x [T][cols] in 4 bits
+ * and y [T][rows]; rows outside every group are not written.
+ * qrm_fp4_swiglu: the matrix holds gate's f rows, then up's (rows = 2 f);
+ * h[t] = silu(W_gate x[t]) (W_up x[t]) [T][f], in one kernel; limit > 0: gate is
+ * cut off above it and up to [-limit, limit] first.  _fp4 writes h in 4-bit
+ * rows, as the next product takes them.
+ * Rows of codes start on 16 bytes (pitch included); rows of scales that start on
+ * 8 are faster.  type is the result's; sums are f32.  A handle's calls need no
+ * workspace and may overlap in time.  qrm_fp4_sync waits for the device and
+ * reports what the products met: QRM_E_INVALID for offsets that do not ascend
+ * within [0, T] (such a group counts as empty, and one that starts below an
+ * offset before it), QRM_E_TIMEOUT for a wait that gave up (QRM_WAIT_LIMIT_US in
+ * the environment at creation). */
+typedef struct qrm_fp4 qrm_fp4;
+int  qrm_fp4_create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes,
+                    const void* scales, size_t scale_bytes, qrm_fp4** out);
+int  qrm_fp4_create_device(int device, int groups, int64_t rows, int64_t cols, const void* codes_dev, size_t code_bytes,
+                           const void* scales_dev, size_t scale_bytes, qrm_fp4** out);
+void qrm_fp4_destroy(qrm_fp4* m);
+int  qrm_fp4_product(qrm_fp4* m, const void* x_codes_dev, int64_t ld_x, const uint8_t* x_scales_dev, int64_t ld_xs,
+                     const int32_t* offsets_dev, int64_t T, int type, void* y_dev, int64_t ld_y, void* stream);
+int  qrm_fp4_swiglu(qrm_fp4* m, const void* x_codes_dev, int64_t ld_x, const uint8_t* x_scales_dev, int64_t ld_xs,
+                    const int32_t* offsets_dev, int64_t T, float limit, int type, void* h_dev, int64_t ld_h, void* stream);
+int  qrm_fp4_swiglu_fp4(qrm_fp4* m, const void* x_codes_dev, int64_t ld_x, const uint8_t* x_scales_dev, int64_t ld_xs,
+                        const int32_t* offsets_dev, int64_t T, float limit, uint8_t* codes_dev, int64_t ld_codes,
+                        uint8_t* scales_dev, int64_t ld_scales, void* stream);
+int  qrm_fp4_sync(qrm_fp4* m);
+
 /* ---- expert parallelism (no counterpart in the reference, whose MoE layer
  * runs in one process) ----
  * world ranks, one process and GPU each; rank r holds the routed experts

@@ -150,6 +150,27 @@ _SIGS = {
     "qrm_fp8_product": (C.c_int, [P, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int, P, C.c_int64, P]),
     "qrm_fp8_product_t": (C.c_int, [P, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int, P, C.c_int64, P]),
     "qrm_fp8_sync": (C.c_int, [P]),
+    "qrm_rms_norm": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int64, C.c_int64, P, C.c_float, P, C.c_int64, P,
+                               C.c_int64, P]),
+    "qrm_rms_norm_fp8": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int64, C.c_int64, P, C.c_float, P, C.c_int64, P,
+                                   C.c_int64, P, C.c_int64, P, C.c_int64, P]),
+    "qrm_rms_norm_fp4": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int64, C.c_int64, P, C.c_float, P, C.c_int64, P,
+                                   C.c_int64, P, C.c_int64, P, C.c_int64, P]),
+    "qrm_rms_norm_grad_work": (C.c_int64, [C.c_int64, C.c_int64]),
+    "qrm_rms_norm_grad": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int64, C.c_int64, P, C.c_float, P, C.c_int64, P,
+                                    C.c_int64, P, P, P]),
+    "qrm_quantize_fp4": (C.c_int, [C.c_int, P, C.c_int64, C.c_int64, C.c_int64, P, P, C.c_int64, P, C.c_int64, P]),
+    "qrm_gather_rows_fp4": (C.c_int, [C.c_int, P, C.c_int64, P, C.c_int64, C.c_int, C.c_int64, P, C.c_int64, C.c_int64,
+                                      P, C.c_int64, P]),
+    "qrm_fp4_create": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, P, C.c_size_t, P, C.c_size_t, C.POINTER(P)]),
+    "qrm_fp4_create_device": (C.c_int, [C.c_int, C.c_int, C.c_int64, C.c_int64, P, C.c_size_t, P, C.c_size_t,
+                                        C.POINTER(P)]),
+    "qrm_fp4_destroy": (None, [P]),
+    "qrm_fp4_product": (C.c_int, [P, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_int, P, C.c_int64, P]),
+    "qrm_fp4_swiglu": (C.c_int, [P, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_float, C.c_int, P, C.c_int64, P]),
+    "qrm_fp4_swiglu_fp4": (C.c_int, [P, P, C.c_int64, P, C.c_int64, P, C.c_int64, C.c_float, P, C.c_int64, P, C.c_int64,
+                                     P]),
+    "qrm_fp4_sync": (C.c_int, [P]),
     "qrm_nccl_unique_id": (C.c_int, [P]),
     "qrm_create_ep": (C.c_int, [C.POINTER(LayerDesc), C.c_int, C.c_int, P, C.POINTER(P)]),
     "qrm_expert_range": (C.c_int, [P, P, P]),
@@ -563,6 +584,35 @@ def swiglu_fp8_grad(type, gu, dh, rows, f, codes, scales, limit=0.0, n_rows=None
                                      _ptr(codes), ld_codes, _ptr(scales), ld_scales, stream))
 
 
+def _block_arrays(codes, scales, scale_type, device):
+    """A block-scaled matrix's arrays as the library takes them, where it is to
+    be kept, and whether they are on a device."""
+    name = np.dtype(scale_type).name
+    on_device = [bool(getattr(a, "is_cuda", False)) for a in (codes, scales)]
+    if on_device[0] != on_device[1]:
+        raise ValueError("codes and scales must both be on the host or both on the device")
+    if on_device[0]:
+        codes, scales = codes.contiguous(), scales.contiguous()
+        size = np.dtype(scale_type).itemsize
+        if codes.element_size() != 1 or (scales.element_size() != 1 if size == 1 else str(scales.dtype) != "torch." + name):
+            raise ValueError(f"codes of one byte and scales of {name} are needed")
+    else:
+        codes, scales = (_bytes(codes), _bytes(scales) if name == "uint8" else np.ascontiguousarray(scales, dtype=scale_type))
+        if codes.itemsize != 1 or scales.itemsize != np.dtype(scale_type).itemsize:
+            raise ValueError(f"codes of one byte and scales of {name} are needed")
+    if device is None:
+        device = codes.device.index if on_device[0] else 0
+    return codes, scales, device, on_device[0]
+
+
+def _bytes(a):
+    """A host array of one-byte values as it is."""
+    if hasattr(a, "data_ptr"):
+        import torch
+        a = a.view(torch.uint8)
+    return np.ascontiguousarray(a)
+
+
 class Fp8Matrix:
     """`groups` matrices [rows x cols] in 8-bit floating point with a scale for
     each 128 x 128 block, kept in HBM (qrm_fp8_*).  codes [groups][rows][cols]
@@ -576,24 +626,8 @@ class Fp8Matrix:
     each, else their sums come out wrong, without an error."""
 
     def __init__(self, rows, cols, codes, scales, groups=1, device=None):
-        on_device = [bool(getattr(a, "is_cuda", False)) for a in (codes, scales)]
-        if on_device[0] != on_device[1]:
-            raise ValueError("codes and scales must both be on the host or both on the device")
-        if on_device[0]:
-            codes, scales = codes.contiguous(), scales.contiguous()
-            if codes.element_size() != 1 or str(scales.dtype) != "torch.float32":
-                raise ValueError("codes of one byte and scales of float32 are needed")
-        else:
-            if hasattr(codes, "data_ptr"):
-                import torch
-                codes = codes.view(torch.uint8)
-            codes = np.ascontiguousarray(codes)
-            scales = np.ascontiguousarray(scales, dtype=np.float32)
-            if codes.itemsize != 1:
-                raise ValueError("codes of one byte are needed")
-        if device is None:
-            device = codes.device.index if on_device[0] else 0
-        create = lib().qrm_fp8_create_device if on_device[0] else lib().qrm_fp8_create
+        codes, scales, device, on_device = _block_arrays(codes, scales, np.float32, device)
+        create = lib().qrm_fp8_create_device if on_device else lib().qrm_fp8_create
         h = P()
         _check(create(device, groups, rows, cols, _ptr(codes), codes.nbytes, _ptr(scales), scales.nbytes, C.byref(h)))
         self._h, self.rows, self.cols, self.groups = h, rows, cols, groups
@@ -615,6 +649,104 @@ class Fp8Matrix:
     def close(self):
         if getattr(self, "_h", None):
             lib().qrm_fp8_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# ---- root-mean-square norm (include/qrmoe.h); arrays, types and pitches as above
+
+
+def rms_norm(type, x, rows, d, w, eps, y, add=None, sum=None, ld_x=0, ld_add=0, ld_sum=0, ld_y=0, stream=None):
+    """s = x + add (into sum, if given), y = s w / sqrt(mean(s^2) + eps)."""
+    _check(lib().qrm_rms_norm(type, _ptr(x), ld_x, _ptr(add), ld_add, rows, d, _ptr(w), eps, _ptr(sum), ld_sum, _ptr(y),
+                              ld_y, stream))
+
+
+def rms_norm_fp8(type, x, rows, d, w, eps, codes, scales, add=None, sum=None, y=None, ld_x=0, ld_add=0, ld_sum=0, ld_y=0,
+                 ld_codes=0, ld_scales=0, stream=None):
+    """rms_norm into 8-bit rows (and y, if given)."""
+    _check(lib().qrm_rms_norm_fp8(type, _ptr(x), ld_x, _ptr(add), ld_add, rows, d, _ptr(w), eps, _ptr(sum), ld_sum, _ptr(y),
+                                  ld_y, _ptr(codes), ld_codes, _ptr(scales), ld_scales, stream))
+
+
+def rms_norm_fp4(type, x, rows, d, w, eps, codes, scales, add=None, sum=None, y=None, ld_x=0, ld_add=0, ld_sum=0, ld_y=0,
+                 ld_codes=0, ld_scales=0, stream=None):
+    """rms_norm into 4-bit rows (and y, if given)."""
+    _check(lib().qrm_rms_norm_fp4(type, _ptr(x), ld_x, _ptr(add), ld_add, rows, d, _ptr(w), eps, _ptr(sum), ld_sum, _ptr(y),
+                                  ld_y, _ptr(codes), ld_codes, _ptr(scales), ld_scales, stream))
+
+
+def rms_norm_grad_work(rows, d):
+    """Floats of workspace that rms_norm_grad with dw needs."""
+    return lib().qrm_rms_norm_grad_work(rows, d)
+
+
+def rms_norm_grad(type, dy, x, rows, d, w, eps, dx, dw=None, work=None, add=None, ld_dy=0, ld_x=0, ld_add=0, ld_dx=0,
+                  stream=None):
+    """The gradients of rms_norm's summands (dx, the same for both, on top of
+    add) and of w (dw); x is the forward's sum."""
+    _check(lib().qrm_rms_norm_grad(type, _ptr(dy), ld_dy, _ptr(x), ld_x, rows, d, _ptr(w), eps, _ptr(add), ld_add, _ptr(dx),
+                                   ld_dx, _ptr(dw), _ptr(work), stream))
+
+
+# ---- experts in 4-bit microscaled floating point (include/qrmoe.h: 4-bit
+# rows).  Codes and scales are bytes, their pitches too.
+
+
+def quantize_fp4(type, x, rows, cols, codes, scales, n_rows=None, ld_x=0, ld_codes=0, ld_scales=0, stream=None):
+    """Rows, or a matrix's, into 4 bits; n_rows: how many of them, on the device."""
+    _check(lib().qrm_quantize_fp4(type, _ptr(x), ld_x, rows, cols, _ptr(n_rows), _ptr(codes), ld_codes, _ptr(scales),
+                                  ld_scales, stream))
+
+
+def gather_rows_fp4(type, x, pos, T, k, d, codes, scales, n_rows, ld_x=0, ld_codes=0, ld_scales=0, stream=None):
+    """gather_rows into 4-bit rows (codes, scales)."""
+    _check(lib().qrm_gather_rows_fp4(type, _ptr(x), ld_x, _ptr(pos), T, k, d, _ptr(codes), n_rows, ld_codes, _ptr(scales),
+                                     ld_scales, stream))
+
+
+class Fp4Matrix:
+    """`groups` matrices [rows x cols] in 4-bit microscaled floating point, kept
+    in HBM (qrm_fp4_*).  codes [groups][rows][16 ceil(cols/32)] and scales
+    [groups][rows][ceil(cols/32)], bytes both, are NumPy arrays or tensors, on
+    the host or a device, and are copied.  device: where they are kept (None:
+    where codes are, 0 if that is the host); the calls' arrays are there too."""
+
+    def __init__(self, rows, cols, codes, scales, groups=1, device=None):
+        codes, scales, device, on_device = _block_arrays(codes, scales, np.uint8, device)
+        create = lib().qrm_fp4_create_device if on_device else lib().qrm_fp4_create
+        h = P()
+        _check(create(device, groups, rows, cols, _ptr(codes), codes.nbytes, _ptr(scales), scales.nbytes, C.byref(h)))
+        self._h, self.rows, self.cols, self.groups = h, rows, cols, groups
+
+    def product(self, type, x, x_scales, T, y, offsets=None, ld_x=0, ld_scales=0, ld_y=0, stream=None):
+        """y[t] = W_g x[t] for the 4-bit rows x of each group g (offsets)."""
+        _check(lib().qrm_fp4_product(self._h, _ptr(x), ld_x, _ptr(x_scales), ld_scales, _ptr(offsets), T, type,
+                                     _ptr(y), ld_y, stream))
+
+    def swiglu(self, type, x, x_scales, T, h, offsets=None, limit=0.0, ld_x=0, ld_scales=0, ld_h=0, stream=None):
+        """h[t] = silu(W_gate x[t]) (W_up x[t]); gate's rows come first in the matrix, then up's."""
+        _check(lib().qrm_fp4_swiglu(self._h, _ptr(x), ld_x, _ptr(x_scales), ld_scales, _ptr(offsets), T, limit, type,
+                                    _ptr(h), ld_h, stream))
+
+    def swiglu_fp4(self, x, x_scales, T, codes, scales, offsets=None, limit=0.0, ld_x=0, ld_xs=0, ld_codes=0, ld_scales=0,
+                   stream=None):
+        """swiglu into 4-bit rows (codes, scales)."""
+        _check(lib().qrm_fp4_swiglu_fp4(self._h, _ptr(x), ld_x, _ptr(x_scales), ld_xs, _ptr(offsets), T, limit, _ptr(codes),
+                                        ld_codes, _ptr(scales), ld_scales, stream))
+
+    def sync(self):
+        """Waits for the device and raises what the products met."""
+        _check(lib().qrm_fp4_sync(self._h))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            lib().qrm_fp4_destroy(self._h)
             self._h = None
 
     def __del__(self):

@@ -1,0 +1,310 @@
+// fp4.cu -- matrices in 4-bit microscaled floating point, resident in HBM, and
+// their products (kernels: fp4.cuh).
+#include <stdlib.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <new>
+
+#include "fp4.cuh"
+#include "matrix_host.h"
+
+using namespace qrm;
+
+struct qrm_fp4 {
+    int device = 0, sms = 0, groups = 0;
+    int form = -1;                       // QRM_FP4_PAIR: 1 wherever it can / 0 never rows of x on the MMA's M side
+    int64_t rows = 0, cols = 0;
+    int tiles = 0, steps = 0;            // of 128 rows; of 256 columns
+    int halves = 0, second = 0;          // gated: tiles with gate's and up's rows in tiles of their own; up's first
+    uint8_t* codes = nullptr;            // [groups][rows][whole blocks of 16 bytes]; the other arrays are in the same allocation
+    uint8_t* units = nullptr;            // scales, [groups][tiles][steps][2][512]
+    uint8_t* gated_units = nullptr;      // [groups][halves][steps][2][512]
+    int32_t* err = nullptr;
+    CUtensorMap map, units_map, gated_map;   // codes in boxes of 256 columns x 128 rows; units in boxes of one stage's
+};
+
+namespace {
+
+int64_t blocks_of(int64_t n) { return (n + kFp4Block - 1) / kFp4Block; }
+
+void release(qrm_fp4* m) {
+    if (!m) return;
+    DeviceGuard here;
+    here.enter(m->device);
+    cudaDeviceSynchronize();
+    cudaFree(m->codes);
+    delete m;
+}
+
+size_t pair_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4PairStages * kFp4PairStage; }
+
+template <int MODE>
+cudaError_t prepare_kernels() {
+    cudaError_t e = cudaFuncSetAttribute(fp4_split_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(fp4_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(kFp4MaxGroups));
+    return e;
+}
+// registers a thread that the pair kernels were built with: their split may not pass what a launch has
+template <int MODE>
+int pair_regs() {
+    cudaFuncAttributes at{};
+    return cudaFuncGetAttributes(&at, fp4_pair_kernel<MODE>) == cudaSuccess ? at.numRegs : 0;
+}
+
+int create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes, const void* scales,
+           size_t scale_bytes, cudaMemcpyKind kind, qrm_fp4** out) {
+    const char* what = "qrm_fp4_create";
+    if (!out) return failf(QRM_E_INVALID, "%s: out is NULL", what);
+    *out = nullptr;
+    if (!codes || !scales) return failf(QRM_E_INVALID, "%s: NULL argument", what);
+    if (groups <= 0 || rows <= 0 || cols <= 0 || rows > (1 << 22) || cols > (1 << 24))
+        return failf(QRM_E_INVALID, "%s: %d matrices of %lld x %lld", what, groups, (long long)rows, (long long)cols);
+    if (groups > kFp4MaxGroups) return failf(QRM_E_CAPACITY, "%s: %d matrices, at most %d", what, groups, kFp4MaxGroups);
+    const int64_t blocks = blocks_of(cols), all = groups * rows;
+    if (code_bytes != (size_t)(all * blocks * 16))
+        return failf(QRM_E_SIZE, "%s: %zu bytes of codes, %d x %lld rows of %lld blocks of 16 is %lld", what, code_bytes, groups,
+                     (long long)rows, (long long)blocks, (long long)(all * blocks * 16));
+    if (scale_bytes != (size_t)(all * blocks))
+        return failf(QRM_E_SIZE, "%s: %zu bytes of scales, one for each of %lld blocks", what, scale_bytes, (long long)(all * blocks));
+    int count = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) return failf(QRM_E_CUDA, "%s: no CUDA device", what);
+    if (device < 0 || device >= count) return failf(QRM_E_INVALID, "%s: device %d out of range", what, device);
+    int sms;
+    DeviceGuard here;
+    if (here.enter(device) != cudaSuccess) return failf(QRM_E_CUDA, "%s: device %d", what, device);
+    if (int rc = current_device(&device, &sms)) return rc;
+    if (const char* e = getenv("QRM_WAIT_LIMIT_US"))
+        if (set_wait_limit_here((uint64_t)std::max(1LL, atoll(e)) * 1000ull) != cudaSuccess)
+            return failf(QRM_E_CUDA, "%s: wait limit", what);
+    qrm_fp4* m = new (std::nothrow) qrm_fp4();
+    if (!m) return failf(QRM_E_NOMEM, "%s: host memory", what);
+    auto bail = [&](int rc) {
+        release(m);
+        return rc;
+    };
+    if (const char* e = getenv("QRM_FP4_PAIR")) m->form = atoi(e) != 0;
+    m->device = device;
+    m->sms = sms;
+    m->groups = groups;
+    m->rows = rows;
+    m->cols = cols;
+    m->tiles = (int)((rows + 127) / 128);
+    m->steps = (int)((cols + kFp4Step - 1) / kFp4Step);
+    const int64_t f = rows / 2;
+    const bool gated = rows % 2 == 0, apart = gated && f % 128;   // up's rows begin inside a tile
+    m->second = gated ? (int)((f + 127) / 128) : 0;
+    m->halves = 2 * m->second;
+    // one allocation: codes, units, units for the gated product where they differ, the error flags
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    const size_t stage = (size_t)m->steps * kFp4Scales, pitch = (size_t)blocks * 16;
+    const size_t units_at = up(code_bytes), gated_at = units_at + (size_t)groups * m->tiles * stage;
+    const size_t err_at = gated_at + (apart ? (size_t)groups * m->halves * stage : 0);
+    uint8_t* staged = nullptr;   // the scales as they came, until they are in units
+    if (cudaMalloc(&m->codes, err_at + 256) != cudaSuccess || cudaMalloc(&staged, scale_bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return bail(failf(QRM_E_NOMEM, "%s: cannot allocate %zu bytes", what, err_at + 256 + scale_bytes));
+    }
+    m->units = m->codes + units_at;
+    m->gated_units = apart ? m->codes + gated_at : m->units;
+    m->err = reinterpret_cast<int32_t*>(m->codes + err_at);
+    // device sources: what any stream still writes there is awaited, on their own device if that is another one
+    cudaError_t e = cudaDeviceSynchronize();
+    if (kind == cudaMemcpyDeviceToDevice) {
+        if (e == cudaSuccess) e = await_source(codes, device);
+        if (e == cudaSuccess) e = await_source(scales, device);
+    }
+    if (e == cudaSuccess) e = cudaMemcpy(m->codes, codes, code_bytes, kind);
+    if (e == cudaSuccess) e = cudaMemcpy(staged, scales, scale_bytes, kind);
+    if (e == cudaSuccess) e = cudaMemset(m->err, 0, sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e == cudaSuccess && cols % kFp4Block)
+        e = launch_ahead(fp4_clear_tail_kernel, dim3((unsigned)((all + 255) / 256)), 256, 0, nullptr, m->codes, all, (int)cols, (int)pitch);
+    if (e == cudaSuccess)
+        e = launch_ahead(fp4_scale_units_kernel, dim3(2 * m->steps, m->tiles, groups), 128, 0, nullptr, staged, (int)rows, (int)blocks,
+                         (int)rows, m->tiles, m->tiles, m->steps, reinterpret_cast<uint32_t*>(m->units));
+    if (e == cudaSuccess && apart)
+        e = launch_ahead(fp4_scale_units_kernel, dim3(2 * m->steps, m->halves, groups), 128, 0, nullptr, staged, (int)rows, (int)blocks,
+                         (int)f, m->halves, m->second, m->steps, reinterpret_cast<uint32_t*>(m->gated_units));
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    cudaFree(staged);
+    if (e == cudaSuccess) e = prepare_kernels<kFp4Plain>();
+    if (e == cudaSuccess) e = prepare_kernels<kFp4Gated>();
+    if (e == cudaSuccess) e = prepare_kernels<kFp4GatedRows>();
+    if (e != cudaSuccess) return bail(failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e)));
+    if (std::min({pair_regs<kFp4Plain>(), pair_regs<kFp4Gated>(), pair_regs<kFp4GatedRows>()}) * kFp4PairThreads < kFp4PairRegs)
+        return bail(failf(QRM_E_CUDA, "%s: built with too few registers a thread for their split", what));
+    const cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)rows, (cuuint64_t)groups};
+    const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
+    const cuuint32_t box[3] = {128, 128, 1}, unit_box[2] = {256, kFp4Scales / 256};
+    const cuuint64_t unit_strides[1] = {256};
+    const cuuint64_t unit_dims[2] = {256, (cuuint64_t)groups * m->tiles * stage / 256};
+    const cuuint64_t gated_dims[2] = {256, (cuuint64_t)groups * (apart ? m->halves : m->tiles) * stage / 256};
+    if (!encode(&m->map, m->codes, 3, dims, strides, box) ||
+        !encode(&m->units_map, m->units, 2, unit_dims, unit_strides, unit_box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        !encode(&m->gated_map, m->gated_units, 2, gated_dims, unit_strides, unit_box, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return bail(failf(QRM_E_CUDA, "%s: tensor map", what));
+    *out = m;
+    return QRM_OK;
+}
+
+// Which kernel a product takes: rows of x on the MMA's M side from 64 rows a group on.
+bool pair_is_faster(int64_t T, int groups, int64_t tiles_across, int steps, int sms) {
+    const double used = (double)std::min<int64_t>(T, groups), rows = T / used;
+    return rows >= 64;
+}
+
+template <int MODE>
+cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, Fp4Params& p, bool pair, int wide_out, int64_t T, cudaStream_t s) {
+    if (pair)
+        return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, m->map,
+                            MODE == kFp4Plain ? m->units_map : m->gated_map, x_map, p, wide_out);
+    const int64_t across = MODE == kFp4Plain ? (p.M + 255) / 256 : (p.M + 127) / 128;
+    const int64_t used = std::min<int64_t>(T, m->groups), per = (T / used + kFp4Rows - 1) / kFp4Rows;
+    const int64_t tiles = used * per * across;
+    int ranks = 1;
+    while (ranks < 8 && tiles * ranks * 2 <= 2 * m->sms && p.steps >= 4 * ranks) ranks *= 2;
+    const int x_rows = (int)std::min<int64_t>(kFp4Rows, (T + 15) / 16 * 16);
+    const int64_t ctas = (int64_t)p.row_tiles * across * ranks;
+    const int room = ctas <= m->sms ? kSmemMost : kSmemMost / 2 - 512;   // two CTAs on an SM, 1 KB of it kept for each
+    const int stages = std::max(2, std::min(kFp4MaxStages, (room - 1024 - kFp4Header) / fp4_stage_bytes(x_rows)));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kFp4Threads);
+    cfg.dynamicSmemBytes = 1024 + kFp4Header + (size_t)stages * fp4_stage_bytes(x_rows);
+    cfg.stream = s;
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = ranks;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // as in launch_ahead
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, fp4_split_kernel<MODE>, m->map, x_map, p, stages, x_rows);
+}
+
+int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x, const uint8_t* xs, int64_t ld_xs,
+            const int32_t* offsets, int64_t T, float limit, int type, void* out, int64_t ld_out, uint8_t* out_scales,
+            int64_t ld_os, void* stream) {
+    if (!m) return failf(QRM_E_INVALID, "%s: NULL matrix", what);
+    if (mode != kFp4Plain && m->rows % 2) return failf(QRM_E_INVALID, "%s: %lld rows are no two halves", what, (long long)m->rows);
+    const int64_t M = mode == kFp4Plain ? m->rows : m->rows / 2, blocks = blocks_of(m->cols);
+    const int b = mode == kFp4GatedRows ? 1 : type_bytes(type);
+    if (!b) return failf(QRM_E_FORMAT, "%s: type %d is not F32, F16 or BF16", what, type);
+    if (!(limit >= 0.f)) return failf(QRM_E_INVALID, "%s: limit %g", what, (double)limit);
+    if (T < 0 || T > INT_MAX) return failf(QRM_E_INVALID, "%s: %lld rows", what, (long long)T);
+    const int64_t across = (M + 127) / 128, row_tiles = T / kFp4Rows + std::min<int64_t>(T, m->groups);
+    if (row_tiles * across > INT_MAX / 8)
+        return failf(QRM_E_CAPACITY, "%s: %lld rows in %d groups are too many tiles", what, (long long)T, m->groups);
+    if (T == 0) return QRM_OK;
+    if (!x || !xs || !out) return failf(QRM_E_INVALID, "%s: NULL argument", what);
+    if (!offsets && m->groups > 1) return failf(QRM_E_INVALID, "%s: %d matrices need offsets", what, m->groups);
+    const int64_t out_cols = mode == kFp4GatedRows ? 16 * blocks_of(M) : M;
+    if (!pitch_ok(&ld_x, 16 * blocks) || !pitch_ok(&ld_xs, blocks) || !pitch_ok(&ld_out, out_cols))
+        return failf(QRM_E_INVALID, "%s: a pitch is below its row (x %lld, scales %lld, out %lld)", what, (long long)ld_x,
+                     (long long)ld_xs, (long long)ld_out);
+    if (!aligned(x, 16) || ld_x % 16)
+        return failf(QRM_E_INVALID, "%s: rows of codes must start on 16 bytes (pitch %lld)", what, (long long)ld_x);
+    if (!aligned(out, b) || (offsets && !aligned(offsets, 4)))
+        return failf(QRM_E_INVALID, "%s: a pointer is not aligned to its values", what);
+    if (mode == kFp4GatedRows) {
+        if (!out_scales) return failf(QRM_E_INVALID, "%s: NULL argument", what);
+        if (!pitch_ok(&ld_os, blocks_of(M)))
+            return failf(QRM_E_INVALID, "%s: a pitch is below its row (scales %lld)", what, (long long)ld_os);
+        if (!aligned(out, 16) || ld_out % 16)
+            return failf(QRM_E_INVALID, "%s: rows of codes must start on 16 bytes (pitch %lld)", what, (long long)ld_out);
+    }
+    DeviceGuard here;
+    cudaError_t e = here.enter(m->device);
+    if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    // the kernel for large groups writes rows that start on 16 bytes
+    const bool pair = aligned(out, 16) && ld_out * b % 16 == 0 &&
+                      (m->form >= 0 ? m->form : pair_is_faster(T, m->groups, across, m->steps, m->sms));
+    const int wide_out = aligned(out, 32) && ld_out * b % 32 == 0;
+    CUtensorMap x_map;
+    const cuuint64_t dims[2] = {(cuuint64_t)(16 * blocks), (cuuint64_t)T};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld_x};
+    const cuuint32_t box[2] = {128, pair ? 128u : 16u};
+    if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
+    Fp4Params p{};
+    p.w_scales = mode == kFp4Plain ? m->units : m->gated_units;
+    p.x_scales = xs;
+    p.offsets = offsets;
+    p.out = out;
+    p.out_scales = out_scales;
+    p.err = m->err;
+    p.ld_xs = ld_xs;
+    p.ld_out = ld_out;
+    p.ld_os = ld_os;
+    p.limit = limit;
+    p.T = (int)T;
+    p.groups = m->groups;
+    p.M = (int)M;
+    p.tiles = mode == kFp4Plain ? m->tiles : m->halves;
+    p.second = m->second;
+    p.steps = m->steps;
+    p.blocks = (int)blocks;
+    p.type = type;
+    p.row_tiles = (int)(offsets ? row_tiles : (T + kFp4Rows - 1) / kFp4Rows);
+    p.wide_xs = aligned(xs, 8) && ld_xs % 8 == 0;
+    const cudaStream_t s = (cudaStream_t)stream;
+    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, p, pair, wide_out, T, s)
+        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_map, p, pair, wide_out, T, s)
+                            : launch<kFp4GatedRows>(m, x_map, p, pair, wide_out, T, s);
+    return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" int qrm_fp4_create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes,
+                              const void* scales, size_t scale_bytes, qrm_fp4** out) {
+    return create(device, groups, rows, cols, codes, code_bytes, scales, scale_bytes, cudaMemcpyHostToDevice, out);
+}
+
+extern "C" int qrm_fp4_create_device(int device, int groups, int64_t rows, int64_t cols, const void* codes_dev,
+                                     size_t code_bytes, const void* scales_dev, size_t scale_bytes, qrm_fp4** out) {
+    return create(device, groups, rows, cols, codes_dev, code_bytes, scales_dev, scale_bytes, cudaMemcpyDeviceToDevice, out);
+}
+
+extern "C" void qrm_fp4_destroy(qrm_fp4* m) { release(m); }
+
+extern "C" int qrm_fp4_product(qrm_fp4* m, const void* x_codes_dev, int64_t ld_x, const uint8_t* x_scales_dev,
+                               int64_t ld_xs, const int32_t* offsets_dev, int64_t T, int type, void* y_dev, int64_t ld_y,
+                               void* stream) {
+    return product("qrm_fp4_product", kFp4Plain, m, x_codes_dev, ld_x, x_scales_dev, ld_xs, offsets_dev, T, 0.f, type, y_dev,
+                   ld_y, nullptr, 0, stream);
+}
+
+extern "C" int qrm_fp4_swiglu(qrm_fp4* m, const void* x_codes_dev, int64_t ld_x, const uint8_t* x_scales_dev,
+                              int64_t ld_xs, const int32_t* offsets_dev, int64_t T, float limit, int type, void* h_dev,
+                              int64_t ld_h, void* stream) {
+    return product("qrm_fp4_swiglu", kFp4Gated, m, x_codes_dev, ld_x, x_scales_dev, ld_xs, offsets_dev, T, limit, type, h_dev,
+                   ld_h, nullptr, 0, stream);
+}
+
+extern "C" int qrm_fp4_swiglu_fp4(qrm_fp4* m, const void* x_codes_dev, int64_t ld_x, const uint8_t* x_scales_dev,
+                                  int64_t ld_xs, const int32_t* offsets_dev, int64_t T, float limit, uint8_t* codes_dev,
+                                  int64_t ld_codes, uint8_t* scales_dev, int64_t ld_scales, void* stream) {
+    return product("qrm_fp4_swiglu_fp4", kFp4GatedRows, m, x_codes_dev, ld_x, x_scales_dev, ld_xs, offsets_dev, T, limit,
+                   QRM_F32, codes_dev, ld_codes, scales_dev, ld_scales, stream);
+}
+
+extern "C" int qrm_fp4_sync(qrm_fp4* m) {
+    if (!m) return failf(QRM_E_INVALID, "qrm_fp4_sync: NULL matrix");
+    DeviceGuard here;
+    cudaError_t e = here.enter(m->device);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    int32_t err = 0;
+    if (e == cudaSuccess) e = cudaMemcpy(&err, m->err, sizeof err, cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && err) {
+        e = cudaMemset(m->err, 0, sizeof err);
+        if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    }
+    if (e != cudaSuccess) return failf(QRM_E_CUDA, "qrm_fp4_sync: %s", cudaGetErrorString(e));
+    if (err & ERR_TIMEOUT) return failf(QRM_E_TIMEOUT, "qrm_fp4_sync: a device wait timed out");
+    if (err) return failf(QRM_E_INVALID, "qrm_fp4_sync: offsets do not ascend within the rows (flags 0x%x)", err);
+    return QRM_OK;
+}

@@ -1,0 +1,738 @@
+// fp4.cuh -- product of 4-bit microscaled rows with 4-bit microscaled matrices,
+// dense or grouped (rows of group g times matrix g), and the gated product of
+// gate and up with SwiGLU behind it.
+//
+//   y[t][m] = sum_b 2^(sx[t][b] + sw[m][b] - 254) sum_{c in block b} qx[t][c] qw[m][c]
+//   h[t][j] = silu(y[t][j]) y[t][f + j]                       (gated; a matrix of 2 f rows)
+//
+// with blocks of 32 along the contracted dimension, e2m1 codes and e8m0 scales.
+// All of it is tcgen05.mma kind::mxf4, which takes the scales from tensor memory
+// and multiplies by them on its way: 64 contracted values, two blocks, an
+// instruction.  Products of two codes and their sums by powers of two are exact
+// as far as f32 goes, and nothing is left for the epilogue but the output.
+//
+// Scales enter tensor memory in units of 512 bytes for 128 rows x 128 contracted
+// values: row r's four bytes at 16 (r % 32) + 4 (r / 32), which tcgen05.cp
+// spreads over four columns.  A matrix's are laid out that way when it is made;
+// those of x stay as they are and are brought into that order on their way to
+// shared memory, because a group may start at any row.
+#pragma once
+#include "pair_drain.h"
+#include "rows4.cuh"
+#include "umma_sync.cuh"
+
+namespace qrm {
+
+constexpr int kFp4MaxGroups = 1024;
+constexpr int kFp4Step = 256;                // contracted values of a stage: 128 bytes of a row
+constexpr int kFp4Tile = 128 * 128;          // bytes of 128 rows of codes in a stage
+constexpr int kFp4Scales = 1024;             // bytes of their scales
+
+enum Fp4Mode { kFp4Plain = 0, kFp4Gated = 1, kFp4GatedRows = 2 };   // y; h; h in 4-bit rows
+
+struct Fp4Params {
+    const uint8_t* w_scales;   // units [groups][tiles][steps][2][512]
+    const uint8_t* x_scales;   // [T][ld_xs]
+    const int32_t* offsets;    // [groups+1] rows of each group, or NULL (one group)
+    void* out;                 // [T][ld_out], or codes (ld_out in bytes)
+    uint8_t* out_scales;       // [T][ld_os]
+    int32_t* err;
+    long long ld_xs, ld_out, ld_os;
+    float limit;
+    int T, groups;
+    int M;                     // outputs (gated: f)
+    int tiles;                 // of 128 rows in w_scales, of one matrix
+    int second;                // gated: the tile where up's begin
+    int steps;                 // stages of the contracted dimension
+    int blocks;                // of 32 in it
+    int type;                  // of out
+    int row_tiles;             // room for tiles of rows in the grid (weights on the M side)
+    bool wide_xs;              // rows of scales start on 8 bytes
+};
+
+// Instruction descriptor of kind::mxf4: f32 accumulators, e2m1 A and B, e8m0
+// scales, of which bytes `part` and `part` + 1 of each word are used (0 or 2).
+__device__ __forceinline__ constexpr uint32_t umma_idesc_mxf4(int m, int n, int part) {
+    return ((uint32_t)part << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) |
+           ((uint32_t)part << 29);
+}
+// Descriptor of a unit of scales in shared memory for tcgen05.cp: 32 rows of 16
+// bytes one after the other, no swizzle (8-row groups 128 bytes apart).
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+template <int CTAS>
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
+                                          uint32_t b_scales, uint32_t accumulate) {
+    if constexpr (CTAS == 1)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d_tmem),
+            "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(a_scales), "r"(b_scales), "r"(accumulate)
+            : "memory");
+}
+// a unit of scales to four columns of tensor memory (of both CTAs: each its own)
+template <int CTAS>
+__device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
+    if constexpr (CTAS == 1)
+        asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else
+        asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// what this thread wrote to shared memory is there for copies and MMAs
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// the eight scales of a row from block b on (0 for those past the last)
+__device__ __forceinline__ uint2 eight_scales(const uint8_t* __restrict__ row, int b, int blocks, bool wide) {
+    if (wide && b + 8 <= blocks) return __ldg(reinterpret_cast<const uint2*>(row + b));
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        if (b + i < blocks) w[i >> 2] |= (uint32_t)__ldg(row + b + i) << (8 * (i & 3));
+    return make_uint2(w[0], w[1]);
+}
+
+__device__ __forceinline__ float2 gated2(float2 gate, float2 up, float limit) {
+    const Swiglu2 s = limit > 0.f ? swiglu2<true>(gate, up, limit) : swiglu2<false>(gate, up, 0.f);
+    return unpair(mul2(mul2(s.g, s.sig), s.u));
+}
+
+// ------------------------------------------------------------ weights on the MMA's M side
+// For groups of few rows, which reading the weights bounds.  A tile is 256
+// outputs (two blocks of 128; gated: 128 of gate and the same of up) x up to 64
+// rows of x, the MMA's N, rounded up to 16 only.  A cluster of CTAs shares a
+// tile's contracted dimension, so that one token through one matrix is read by
+// most SMs; each leaves its f32 sums in its shared memory, and then each adds up
+// its share of the outputs over all of them, in their order.  No partial sums in
+// global memory, so calls need no workspace and may overlap; two CTAs fit on an
+// SM, and one's start and end go on behind the other's loads.
+//
+// Warps: 0 loads codes and the weights' scales, 1 issues the MMAs, 2 finds the
+// tile and brings the scales of x; all eight write the output.
+constexpr int kFp4Threads = 256;
+constexpr int kFp4Rows = 64;                 // most rows of x in a tile
+constexpr int kFp4MaxStages = 6;
+constexpr int kFp4TmemCols = 256;            // two accumulators of 64 columns, scales behind them
+constexpr int kFp4TmemScales = 128;
+constexpr int kFp4ScaleCols = 24;            // of one stage: weights 2 x 2 x 4, x 2 x 4
+constexpr int kFp4Header = 1024;
+__host__ __device__ inline int fp4_stage_bytes(int x_rows) { return x_rows * 128 + 2 * kFp4Tile + 3 * kFp4Scales; }
+
+struct Fp4Tile {
+    int group, pos, n;   // matrix, first row of x, rows (none: no such tile)
+};
+
+// The tile of rows number `at`, by one warp, in all its lanes.  Groups count as
+// in group_tables; `report`: look at all of them and raise an error for offsets
+// that make no sense.
+__device__ inline Fp4Tile fp4_find(const Fp4Params& p, int at, bool report) {
+    if (!p.offsets) return {0, at * kFp4Rows, min(max(p.T - at * kFp4Rows, 0), kFp4Rows)};
+    const int lane = threadIdx.x & 31;
+    Fp4Tile r{0, 0, 0};
+    int before = 0, top = 0;
+    bool bad = false, found = false;
+    for (int g0 = 0; g0 < p.groups && (report || !found); g0 += 32) {
+        const int g = g0 + lane;
+        int a = 0, b = 0;
+        if (g < p.groups) {
+            a = p.offsets[g];
+            b = p.offsets[g + 1];
+        }
+        int most = a;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) most = max(most, __shfl_up_sync(0xffffffffu, most, o));
+        most = max(most, top);
+        top = __shfl_sync(0xffffffffu, most, 31);
+        if (a < most || a < 0 || b < a || b > p.T) {
+            bad |= g < p.groups;
+            a = b = 0;
+        }
+        const int tiles = (b - a + kFp4Rows - 1) / kFp4Rows;
+        int scan = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += v;
+        }
+        const int in = at - (before + scan - tiles);
+        const uint32_t here = __ballot_sync(0xffffffffu, in >= 0 && in < tiles);
+        if (here && !found) {
+            const int from = __ffs(here) - 1;
+            r.group = g0 + from;
+            r.pos = __shfl_sync(0xffffffffu, a + in * kFp4Rows, from);
+            r.n = __shfl_sync(0xffffffffu, min(b - a - in * kFp4Rows, kFp4Rows), from);
+            found = true;
+        }
+        before += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (report && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.err, (int)ERR_BOUNDS);
+    return r;
+}
+
+// f32 of a CTA of the cluster, at the address that `mine` has here
+__device__ __forceinline__ float load_peer(uint32_t mine, uint32_t rank) {
+    uint32_t a;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(mine), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// One output of row t for each lane (m = the lane's; absent ones are not
+// written), in the type asked for
+__device__ __forceinline__ void store_lane(const Fp4Params& p, long long t, int m, float v) {
+    if (m >= p.M) return;
+    if (p.type == 0) reinterpret_cast<float*>(p.out)[t * p.ld_out + m] = v;
+    else if (p.type == 1) reinterpret_cast<__half*>(p.out)[t * p.ld_out + m] = __float2half_rn(v);
+    else reinterpret_cast<__nv_bfloat16*>(p.out)[t * p.ld_out + m] = __float2bfloat16_rn(v);
+}
+// a warp's 32 outputs from m0 on, a block, as 4-bit codes
+__device__ __forceinline__ void store_lane4(const Fp4Params& p, long long t, int m0, float v) {
+    if (m0 >= p.M) return;
+    const int lane = threadIdx.x & 31;
+    v = m0 + lane < p.M ? v : 0.f;
+    const uint32_t scale = fp4_scale(__reduce_max_sync(0xffffffffu, magnitude(v)));
+    uint32_t c;
+    asm("{\n .reg .b8 a;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n mov.b32 %0, {a, a, a, a};\n}"
+        : "=r"(c)
+        : "f"(v * fp4_inverse(scale)), "f"(0.f));
+    c = scale == 255 ? 0 : (c & 15) << (4 * (lane & 7));
+    c |= __shfl_xor_sync(0xffffffffu, c, 1);
+    c |= __shfl_xor_sync(0xffffffffu, c, 2);
+    c |= __shfl_xor_sync(0xffffffffu, c, 4);
+    uint8_t* out = reinterpret_cast<uint8_t*>(p.out) + t * p.ld_out + m0 / 2;   // rows of codes start on 16 bytes
+    if ((lane & 7) == 0) reinterpret_cast<uint32_t*>(out)[lane >> 3] = c;
+    if (lane == 0) p.out_scales[t * p.ld_os + m0 / kFp4Block] = (uint8_t)scale;
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kFp4Threads, 2)
+fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                 const __grid_constant__ Fp4Params p, int stages, int x_rows /* room for rows of x in a stage */) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // [stages] copies are there
+    uint64_t* x_full = full + kFp4MaxStages;            // [stages] scales of x are there
+    uint64_t* done = x_full + kFp4MaxStages;            // [stages] their MMAs are done
+    uint64_t* done_bar = done + kFp4MaxStages;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + 512);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 516);
+    volatile uint32_t* issued = reinterpret_cast<volatile uint32_t*>(sm + 520);   // stages, once their warp is through
+    Fp4Tile* found = reinterpret_cast<Fp4Tile*>(sm + 528);
+    const uint32_t stage_bytes = fp4_stage_bytes(x_rows);
+    // a stage: codes of x (the MMA of 16 rows of x reads no more), codes of both blocks, their scales, scales of x
+    const uint32_t w_off = x_rows * 128, ws_off = w_off + 2 * kFp4Tile, xs_off = ws_off + 2 * kFp4Scales;
+    uint8_t* ring = sm + kFp4Header;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t rank, ranks;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    const int tile = blockIdx.x / ranks, row_tile = tile % p.row_tiles, block = tile / p.row_tiles;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < stages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&x_full[i], 1);
+            mbar_init(&done[i], 1);
+        }
+        mbar_init(done_bar, 1);
+        *abort_flag = 0;
+        *issued = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), kFp4TmemCols);
+    pdl_start();   // nothing before this reads or writes global memory
+    if (warp == 2) {
+        const Fp4Tile t = fp4_find(p, row_tile, blockIdx.x == 0);
+        if (lane == 0) *found = t;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const Fp4Tile t = *found;
+    if (t.n == 0) {   // (for all of the cluster)
+        if (warp == 1) tmem_dealloc(tmem, kFp4TmemCols);
+        return;
+    }
+    const WaitCtl ctl{abort_flag, p.err};
+    const int k0 = (int)((long long)p.steps * rank / ranks), k1 = (int)((long long)p.steps * (rank + 1) / ranks);
+    const int m0 = block * (MODE == kFp4Plain ? 256 : 128);
+    const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), done0 = smem_u32(done);
+    const int boxes = (t.n + 15) >> 4;
+
+    if (warp == 0) {
+        // ------------------------------------------------ codes and the weights' scales
+        Ring r;
+        uint32_t n_issued = 0;
+        const long long units = (long long)t.group * p.tiles;
+        const int u0 = m0 >> 7, u1 = MODE == kFp4Plain ? min(u0 + 1, p.tiles - 1) : u0 + p.second;   // an absent second block is not stored
+        const uint8_t* s0 = p.w_scales + (units + u0) * p.steps * kFp4Scales;
+        const uint8_t* s1 = p.w_scales + (units + u1) * p.steps * kFp4Scales;
+        const int m1 = MODE == kFp4Plain ? m0 + 128 : p.M + m0;
+        for (int k = k0; k < k1; k++) {
+            if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) break;
+            uint8_t* st = ring + r.i * stage_bytes;
+            if (elect_one()) {
+                mbar_arrive_expect_tx(&full[r.i], (uint32_t)(boxes * 2048 + 2 * kFp4Tile + 2 * kFp4Scales));
+                tma_load_3d(st + w_off, &w_map, k * 128, m0, t.group, &full[r.i]);
+                tma_load_3d(st + w_off + kFp4Tile, &w_map, k * 128, m1, t.group, &full[r.i]);
+                bulk_g2s(st + ws_off, s0 + (size_t)k * kFp4Scales, kFp4Scales, &full[r.i]);
+                bulk_g2s(st + ws_off + kFp4Scales, s1 + (size_t)k * kFp4Scales, kFp4Scales, &full[r.i]);
+                for (int b = 0; b < boxes; b++) tma_load_2d(st + b * 2048, &x_map, k * 128, t.pos + 16 * b, &full[r.i]);
+            }
+            __syncwarp();
+            r.next(stages);
+            n_issued++;
+        }
+        if (lane == 0) *issued = n_issued;
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMAs (one thread issues)
+        Ring r;
+        const uint32_t ring0 = smem_u32(ring);
+        const uint64_t x_desc = sw128_desc(ring0), w_desc = sw128_desc(ring0 + w_off);
+        const uint64_t ws_desc = scale_desc(ring0 + ws_off), xs_desc = scale_desc(ring0 + xs_off);
+        const uint32_t idesc = umma_idesc_mxf4(128, (t.n + 15) & ~15, 0), odd = umma_idesc_mxf4(0, 0, 2) & ~umma_idesc_mxf4(0, 0, 0);
+        for (int k = k0; k < k1; k++) {
+            if (!bar_wait(full0 + 8 * r.i, r.phase, ctl) || !bar_wait(x_full0 + 8 * r.i, r.phase, ctl)) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t at = r.i * stage_bytes >> 4;
+                const uint32_t ws = tmem + kFp4TmemScales + kFp4ScaleCols * ((k - k0) & 1), xs = ws + 16;
+#pragma unroll
+                for (int u = 0; u < 4; u++) scales_to_tmem<1>(ws + 4 * u, ws_desc + at + u * (512 >> 4));   // block u / 2, half u % 2
+#pragma unroll
+                for (int u = 0; u < 2; u++) scales_to_tmem<1>(xs + 4 * u, xs_desc + at + u * (512 >> 4));
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
+                        umma_mxf4<1>(tmem + 64 * b, w_desc + at + b * (kFp4Tile >> 4) + 2 * j, x_desc + at + 2 * j,
+                                     j & 1 ? idesc | odd : idesc, ws + 8 * b + 4 * (j >> 1), xs + 4 * (j >> 1), k > k0 || j > 0);
+                umma_commit(&done[r.i]);
+            }
+            __syncwarp();
+            r.next(stages);
+        }
+        // every MMA of this CTA has completed before its sums are read (or tensor memory is released)
+        if (elect_one()) umma_commit(done_bar);
+        __syncwarp();
+    } else if (warp == 2) {
+        // ------------------------------------------------ scales of x: rows lane and lane + 32
+        Ring r;
+        const uint8_t* row = p.x_scales + (long long)(t.pos + lane) * p.ld_xs;
+        const bool in0 = lane < t.n, in1 = lane + 32 < t.n;
+        for (int k = k0; k < k1; k++) {
+            const uint2 none = make_uint2(0, 0);
+            const uint2 a = in0 ? eight_scales(row, 8 * k, p.blocks, p.wide_xs) : none;
+            const uint2 b = in1 ? eight_scales(row + 32 * p.ld_xs, 8 * k, p.blocks, p.wide_xs) : none;
+            if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) break;
+            uint4* to = reinterpret_cast<uint4*>(ring + r.i * stage_bytes + xs_off) + lane;
+            to[0] = make_uint4(a.x, b.x, 0, 0);
+            to[32] = make_uint4(a.y, b.y, 0, 0);
+            fence_async();
+            __syncwarp();
+            if (lane == 0) bar_arrive(x_full0 + 8 * r.i);
+            r.next(stages);
+        }
+    }
+    __syncwarp();
+    // ---------------- every warp: the sums into shared memory, [row of x][output], where the ring was
+    mbar_wait(done_bar, 0u);   // (of MMAs that were issued: it comes)
+    tc_fence_after();
+    __syncthreads();           // no role still waits on the ring
+    float* sums = reinterpret_cast<float*>(ring);
+    if (threadIdx.x == 0 && *abort_flag) drain_own(full, *issued, stages);
+    __syncthreads();
+    {
+        const int quarter = warp & 3, b = warp >> 2;
+        for (int c = 0; c < t.n; c += 16) {
+            float v[16];
+            tmem_ld16_now(tmem + ((uint32_t)(32 * quarter) << 16) + 64 * b + c, v);
+#pragma unroll
+            for (int i = 0; i < 16; i++) sums[(c + i) * 256 + 128 * b + 32 * quarter + lane] = v[i];
+        }
+    }
+    tc_fence_before();
+    cluster_sync_all();
+    if (warp == 1) tmem_dealloc(tmem, kFp4TmemCols);
+    // ---------------- this CTA's share of (row, 32 outputs), over all of the cluster
+    constexpr int per_row = MODE == kFp4Plain ? 8 : 4;
+    const uint32_t mine = smem_u32(sums);
+    for (int i = rank + ranks * warp; i < t.n * per_row && !*abort_flag; i += ranks * (kFp4Threads / 32)) {
+        const int row = i / per_row, o = 32 * (i % per_row);
+        const uint32_t at = mine + 4 * (row * 256 + o + lane);
+        float y = 0.f, up = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; q++) {
+            if (q >= (int)ranks) break;
+            y += load_peer(at, q);
+            if (MODE != kFp4Plain) up += load_peer(at + 512, q);
+        }
+        const long long to = t.pos + row;
+        if (MODE == kFp4Plain) {
+            store_lane(p, to, m0 + o + lane, y);
+        } else {
+            const float h = gated2(make_float2(y, y), make_float2(up, up), p.limit).x;
+            if (MODE == kFp4Gated) store_lane(p, to, m0 + o + lane, h);
+            else store_lane4(p, to, m0 + o, h);
+        }
+    }
+    cluster_sync_all();   // the others may still read this CTA's sums
+}
+
+// ------------------------------------------------------------ rows of x on the MMA's M side
+// For groups of many rows, which the tensor cores bound.  A pair of SMs
+// (cta_group::2) shares a tile of 256 rows of x times 256 outputs (gated: 128 of
+// gate, which the first CTA loads, and 128 of up): each CTA loads 128 rows of x
+// and 128 of the weights, 32 KB of codes for 256 contracted values, 64 bytes a
+// cycle at the full MMA rate.
+//
+// Tensor memory holds two accumulators of 256 columns but for the scales' 48
+// columns: the second begins 48 before the first ends, and a tile's MMAs wait
+// for the epilogue of the one before to have read its accumulator (a few hundred
+// cycles, in which the ring of stages fills up).
+//
+// Warps: 0 loads codes and the weights' scales, 1 issues the MMAs (in the
+// pair's first CTA), 2 and 3 bring the scales of x, a stage each in turn, 4-11
+// write the output: lane quarter (warp & 3), half of the columns (warp >= 8).
+constexpr int kFp4PairThreads = 384;
+constexpr int kFp4PairStages = 6;
+constexpr int kFp4PairTx = 2 * kFp4Tile + 2 * kFp4Scales;            // bytes of a CTA's copies of a stage
+constexpr int kFp4PairStage = kFp4PairTx + kFp4Scales;               // and the scales of x
+constexpr int kFp4PairSecond = 208, kFp4PairTmemScales = 464;
+constexpr int kFp4PairTableOff = 1024;
+constexpr int kFp4PairRegsFew = 72, kFp4PairRegsMany = 216;
+constexpr int kFp4PairRegs = 128 * kFp4PairRegsFew + 256 * kFp4PairRegsMany;
+static_assert(kFp4PairRegs <= kFp4PairThreads * 168, "register split");
+__host__ __device__ inline int fp4_pair_stage_off(int groups) { return (kFp4PairTableOff + 12 * (groups + 1) + 1023) / 1024 * 1024; }
+
+// the first CTA's barriers, as drain_pair moves them on
+struct Fp4PairBars {
+    uint64_t* full;
+    __device__ void expect(uint32_t slot) { mbar_arrive_expect_tx(&full[slot], kFp4PairTx); }
+    __device__ void complete(uint32_t slot) {
+        asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[slot])),
+                     "r"((uint32_t)kFp4PairTx)
+                     : "memory");
+    }
+    __device__ void wait(uint32_t slot, uint32_t parity) { mbar_wait(&full[slot], parity); }
+};
+// an arrival on the first CTA's barrier that also hands over what this thread's CTA wrote to its shared memory
+__device__ __forceinline__ void bar_arrive_release_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// 2 N outputs of a row in 4-bit blocks, m of them (from a block's start on)
+template <int N>
+__device__ __forceinline__ void store_row4(uint8_t* codes, uint8_t* scales, int left, const float2 (&h)[N]) {
+#pragma unroll
+    for (int b = 0; b < N / 16; b++) {
+        if (32 * b >= left) return;
+        float v[4][8];
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+            const float2 f = h[16 * b + i / 2];
+            const float x = 32 * b + i < left ? (i & 1 ? f.y : f.x) : 0.f;
+            v[i >> 3][i & 7] = x;
+            m = max(m, magnitude(x));
+        }
+        const uint32_t scale = fp4_scale(m);
+        reinterpret_cast<uint4*>(codes)[b] = make_uint4(e2m1x8(v[0], scale), e2m1x8(v[1], scale), e2m1x8(v[2], scale), e2m1x8(v[3], scale));
+        scales[b] = (uint8_t)scale;
+    }
+}
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp4PairThreads, 1)
+fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap s_map,
+                const __grid_constant__ CUtensorMap x_map, const __grid_constant__ Fp4Params p, int wide_out) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // first CTA: both CTAs' copies are there
+    uint64_t* x_full = full + kFp4PairStages;           // first CTA: both CTAs' scales of x are there
+    uint64_t* done = x_full + kFp4PairStages;           // both: the stage's MMAs are done
+    uint64_t* tile_done = done + kFp4PairStages;        // [2] both: a tile's are
+    uint64_t* tile_read = tile_done + 2;                // first CTA: both epilogues have read an accumulator
+    uint64_t* done_bar = tile_read + 1;
+    uint64_t* left_bar = done_bar + 1;                  // both, when the first CTA gave up: its commits are through
+    __shared__ volatile int given_up;
+    __shared__ volatile uint32_t from_peer, issued;     // issued: stages, once their warp is through
+    volatile int* abort_flag = &given_up;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 776);
+    int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp4PairTableOff);
+    int32_t* start = first_tile + p.groups + 1;
+    int32_t* rows = start + p.groups + 1;
+    uint8_t* ring = sm + fp4_pair_stage_off(p.groups);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & 1;   // in the pair: the cluster is two CTAs along x
+    constexpr int kOut = MODE == kFp4Plain ? 256 : 128;   // outputs of a tile
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kFp4PairStages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&x_full[i], 2);
+            mbar_init(&done[i], 1);
+        }
+        mbar_init(&tile_done[0], 1);
+        mbar_init(&tile_done[1], 1);
+        mbar_init(tile_read, 16);
+        mbar_init(done_bar, 1);
+        mbar_init(left_bar, 1);
+        *abort_flag = 0;
+        issued = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    pdl_start();   // nothing before this reads or writes global memory
+    if (warp == 2) group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows, 256, (p.M + kOut - 1) / kOut, blockIdx.x == 0);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();   // the peer's barriers are ready
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const WaitCtl ctl{abort_flag, p.err};
+    const uint32_t done0 = smem_u32(done);
+    const int tiles = first_tile[p.groups], pairs = gridDim.x >> 1, steps = p.steps;
+
+    struct Tile {
+        int group, m;      // matrix, first output
+        int pos, rows;     // first row of x of this CTA, rows of the group from there on
+    };
+    // the tiles of one block of outputs follow each other, so its weights come from HBM once
+    auto tile_at = [&](int i) {
+        int lo = 0, hi = p.groups;   // the last group with first_tile <= i has rows
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first_tile[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        const int blocks = (rows[lo] + 255) >> 8, in = i - first_tile[lo];
+        const int n = in / blocks, at = (in - n * blocks) * 256 + 128 * (int)rank;
+        return Tile{lo, n * kOut, start[lo] + at, rows[lo] - at};
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp4PairRegsFew));
+        if (warp == 0) {
+            // -------------------------------------------- codes and the weights' scales
+            bool ok = true;
+            Ring r;
+            uint32_t n_issued = 0;
+            const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
+                const Tile t = tile_at(i);
+                // this CTA's half of the weights; both have all 256 outputs' scales
+                const int m = MODE == kFp4Plain ? t.m + 128 * (int)rank : t.m + p.M * (int)rank;
+                const int u = t.group * p.tiles + (t.m >> 7);
+                const int s0 = u * steps * 4, s1 = (u + (MODE == kFp4Plain ? 1 : p.second)) * steps * 4;
+                for (int k = 0; k < steps; k++) {
+                    if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                    if (elect_one()) {
+                        const uint32_t st = ring0 + r.i * kFp4PairStage, bar = full0 + 8 * r.i;
+                        if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * kFp4PairTx);
+                        // (no rows for this CTA: from past the end, which is zeros and no traffic)
+                        tma_pair_2d(st, &x_map, k * 128, t.rows > 0 ? t.pos : p.T, bar);
+                        tma_pair_3d(st + kFp4Tile, &w_map, k * 128, m, t.group, bar);
+                        tma_pair_2d(st + 2 * kFp4Tile, &s_map, 0, s0 + 4 * k, bar);
+                        tma_pair_2d(st + 2 * kFp4Tile + kFp4Scales, &s_map, 0, s1 + 4 * k, bar);
+                    }
+                    __syncwarp();
+                    r.next(kFp4PairStages);
+                    n_issued++;
+                }
+            }
+            if (lane == 0) issued = n_issued;
+        } else if (warp == 1 && rank == 0) {
+            // -------------------------------------------- MMAs (one thread issues for both CTAs)
+            bool ok = true;
+            Ring r;
+            uint32_t n = 0, buffer = 0;   // tiles; of scales
+            const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), ring0 = smem_u32(ring);
+            const uint64_t x_desc = sw128_desc(ring0), w_desc = sw128_desc(ring0 + kFp4Tile);
+            const uint64_t ws_desc = scale_desc(ring0 + 2 * kFp4Tile), xs_desc = scale_desc(ring0 + kFp4PairTx);
+            constexpr uint32_t idesc[2] = {umma_idesc_mxf4(256, 256, 0), umma_idesc_mxf4(256, 256, 2)};
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs, n++) {
+                // the accumulator of the tile before has been read
+                if (n > 0 && !bar_wait(smem_u32(tile_read), (n - 1) & 1u, ctl)) break;
+                const uint32_t d = tmem + (n & 1 ? kFp4PairSecond : 0);
+                for (int k = 0; k < steps; k++) {
+                    if (!bar_wait(full0 + 8 * r.i, r.phase, ctl) || !bar_wait(x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t at = r.i * (kFp4PairStage >> 4);
+                        const uint32_t xs = tmem + kFp4PairTmemScales + kFp4ScaleCols * buffer, ws = xs + 8;
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {   // half of the stage's contracted values
+                            scales_to_tmem<2>(xs + 4 * u, xs_desc + at + u * (512 >> 4));
+                            scales_to_tmem<2>(ws + 8 * u, ws_desc + at + u * (512 >> 4));
+                            scales_to_tmem<2>(ws + 8 * u + 4, ws_desc + at + (kFp4Scales + u * 512 >> 4));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            umma_mxf4<2>(d, x_desc + at + 2 * j, w_desc + at + 2 * j, idesc[j & 1], xs + 4 * (j >> 1), ws + 8 * (j >> 1), k > 0 || j > 0);
+                        umma_commit_pair(done0 + 8 * r.i);
+                        if (k + 1 == steps) umma_commit_pair(smem_u32(tile_done) + 8 * (n & 1));
+                    }
+                    __syncwarp();
+                    r.next(kFp4PairStages);
+                    buffer ^= 1;
+                }
+            }
+            // every MMA has completed before tensor memory is released
+            if (elect_one()) {
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done_bar)) : "memory");
+                mbar_wait(done_bar, 0u);
+            }
+            __syncwarp();
+        } else if (warp >= 2) {
+            // -------------------------------------------- scales of x, every second stage
+            bool ok = true;
+            Ring r;
+            const uint32_t x_full0 = map_to_rank0(smem_u32(x_full));
+            uint32_t turn = 0;   // of the stages, all tiles' one after the other
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
+                const Tile t = tile_at(i);
+                const uint8_t* row = p.x_scales + (long long)(t.pos + lane) * p.ld_xs;
+                uint2 v[4];
+                auto load = [&](int k) {
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        v[c] = lane + 32 * c < t.rows && k < steps ? eight_scales(row + 32 * c * p.ld_xs, 8 * k, p.blocks, p.wide_xs) : make_uint2(0, 0);
+                };
+                int k = (warp ^ turn) & 1;   // the first of the tile that is this warp's
+                load(k);
+                for (int j = 0; j < steps; j++, turn ^= 1) {
+                    if (((warp ^ turn) & 1) == 0) {
+                        const uint4 lo = make_uint4(v[0].x, v[1].x, v[2].x, v[3].x), hi = make_uint4(v[0].y, v[1].y, v[2].y, v[3].y);
+                        k += 2;
+                        load(k);
+                        if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                        uint4* to = reinterpret_cast<uint4*>(ring + r.i * kFp4PairStage + kFp4PairTx) + lane;
+                        to[0] = lo;
+                        to[32] = hi;
+                        fence_async();
+                        __syncwarp();
+                        if (lane == 0) bar_arrive_release_cluster(x_full0 + 8 * r.i);
+                    }
+                    r.next(kFp4PairStages);
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------ output
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp4PairRegsMany));
+        const int half = (warp - 4) >> 2, row = 32 * (warp & 3) + lane;
+        const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t read0 = map_to_rank0(smem_u32(tile_read));
+        uint32_t n = 0;
+        for (int i = blockIdx.x >> 1; i < tiles; i += pairs, n++) {
+            const Tile t = tile_at(i);
+            if (!bar_wait(smem_u32(tile_done) + 8 * (n & 1), (n >> 1) & 1u, ctl)) break;
+            tc_fence_after();
+            const uint32_t from = taddr + (n & 1 ? kFp4PairSecond : 0);
+            float2 acc[64];   // 128 columns; gated: 64 of gate, the same of up
+            if (t.rows > 32 * (warp & 3)) {
+#pragma unroll
+                for (int h = 0; h < 4; h++)
+                    tmem_ld32(from + (MODE == kFp4Plain ? 128 * half + 32 * h : 64 * half + 32 * (h & 1) + 128 * (h >> 1)),
+                              reinterpret_cast<float*>(acc + 16 * h));
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive_cluster(read0);
+            if (row < t.rows) {
+                if (MODE == kFp4Plain) {
+                    const long long o = (long long)(t.pos + row) * p.ld_out + t.m + 128 * half;
+                    const int left = p.M - t.m - 128 * half;
+                    if (p.type == 0) store_row(reinterpret_cast<float*>(p.out) + o, left, acc, wide_out);
+                    else if (p.type == 1) store_row(reinterpret_cast<__half*>(p.out) + o, left, acc, wide_out);
+                    else store_row(reinterpret_cast<__nv_bfloat16*>(p.out) + o, left, acc, wide_out);
+                } else {
+                    float2 h[32];
+#pragma unroll
+                    for (int c = 0; c < 32; c++) h[c] = gated2(acc[c], acc[32 + c], p.limit);
+                    const int m = t.m + 64 * half, left = p.M - m;
+                    const long long at = t.pos + row;
+                    if (MODE == kFp4GatedRows) {
+                        store_row4(reinterpret_cast<uint8_t*>(p.out) + at * p.ld_out + m / 2, p.out_scales + at * p.ld_os + m / kFp4Block, left, h);
+                    } else if (p.type == 0) {
+                        store_row(reinterpret_cast<float*>(p.out) + at * p.ld_out + m, left, h, wide_out);
+                    } else if (p.type == 1) {
+                        store_row(reinterpret_cast<__half*>(p.out) + at * p.ld_out + m, left, h, wide_out);
+                    } else {
+                        store_row(reinterpret_cast<__nv_bfloat16*>(p.out) + at * p.ld_out + m, left, h, wide_out);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+    }
+    // ---------------- teardown: every role of both CTAs is done (or gave up); free tensor memory
+    tc_fence_before();
+    __syncthreads();
+    // (as in fp8_pair_kernel: the first CTA learns how many stages the other has issued, which learns whether to stay)
+    if (threadIdx.x == 0) store_peer(const_cast<uint32_t*>(&from_peer), rank ^ 1, rank == 0 ? (uint32_t)given_up : issued);
+    __syncwarp();
+    cluster_sync_all();
+    tc_fence_after();
+    if (rank == 0 ? given_up != 0 : from_peer != 0) {
+        if (rank == 0 && threadIdx.x == 0) {
+            Fp4PairBars bars{full};
+            drain_pair(issued, from_peer, kFp4PairStages, bars);
+        }
+        if (warp == 1) {
+            if (rank == 0 && elect_one()) umma_commit_pair(smem_u32(left_bar));
+            __syncwarp();
+            if (lane == 0) mbar_wait(left_bar, 0u);
+        }
+        __syncwarp();
+        cluster_sync_all();
+    }
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ------------------------------------------------------------ a matrix's scales into units
+// scales [groups][rows][blocks] of 32 columns -> [groups][tiles][steps][2][512];
+// tile i holds rows 128 i ... of the first `split` rows, and those from split on
+// begin with tile `second` (split = rows: there are none).  What does not exist
+// is 0.
+__global__ void fp4_scale_units_kernel(const uint8_t* __restrict__ scales, int rows, int blocks, int split, int tiles, int second,
+                                       int steps, uint32_t* __restrict__ units) {
+    pdl_start();
+    // a word: four scales of one row; blockIdx.z: matrix, y: tile, x: unit of 128 words along the contracted dimension
+    const int lane = threadIdx.x, q = lane & 3, l = lane >> 2;
+    const int tile = blockIdx.y, in = 128 * (tile < second ? tile : tile - second) + 32 * q + l;
+    const int row = tile < second ? (in < split ? in : -1) : (split + in < rows ? split + in : -1);
+    const size_t g = blockIdx.z;
+    uint32_t w = 0;
+    if (row >= 0) {
+        const uint8_t* from = scales + (g * rows + row) * blocks;
+        for (int i = 0; i < 4; i++) {
+            const int b = 4 * blockIdx.x + i;
+            if (b < blocks) w |= (uint32_t)from[b] << (8 * i);
+        }
+    }
+    units[((g * tiles + tile) * 2 * steps + blockIdx.x) * 128 + lane] = w;
+}
+// codes past the last column of a row are 0: cols of them, in whole blocks of 32
+__global__ void fp4_clear_tail_kernel(uint8_t* codes, long long rows, int cols, int pitch) {
+    pdl_start();
+    const long long r = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+    if (r >= rows) return;
+    uint8_t* p = codes + r * pitch;
+    if (cols & 1) p[cols / 2] &= 15;
+    for (int i = (cols + 1) / 2; i < pitch; i++) p[i] = 0;
+}
+
+}  // namespace qrm

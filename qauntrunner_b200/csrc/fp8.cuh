@@ -17,10 +17,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "common.cuh"
 #include "gemv_imma.cuh"
 #include "pair_drain.h"
-#include "umma_ptx.cuh"
+#include "umma_sync.cuh"
 
 namespace qrm {
 
@@ -71,108 +70,6 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
-        "[%5];" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
-        : "memory");
-}
-// 16 / 32 columns of this warp's 32 tensor-memory lanes; the wait is part of
-// the statement, so nothing that uses the registers can move before it
-__device__ __forceinline__ void tmem_ld16_now(uint32_t taddr, float* v) {
-    uint32_t r[16];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];\n"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-}
-
-template <typename T> __device__ __forceinline__ T round_to(float v);
-template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-// ------------------------------------------------------------ waits
-// A ready barrier costs one try_wait and a vote; the bounded loop is out of
-// line.  (The single-lane waits with an integer division for the ring's slot
-// that this kernel began with cost some 300 cycles each, ready or not, and
-// were what bounded it: 710 TFLOP/s at 4096 x 28672 x 4096.)
-struct Fp8Ctl {
-    volatile int* abort_flag;
-    int32_t* err;
-};
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
-    const uint64_t t0 = global_ns(), lim = wait_limit_ns();
-    bool ok = false;
-    for (;;) {
-        for (int i = 0; i < 8 && !ok; i++) ok = bar_try(bar, parity);
-        if (ok || *abort_flag || global_ns() - t0 > lim) break;
-    }
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok && (threadIdx.x & 31) == 0) {
-        *abort_flag = 1;
-        atomicOr(err, (int)ERR_TIMEOUT);
-    }
-    return ok;
-}
-// all lanes; false for all of them when the wait gave up
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const Fp8Ctl& c) {
-    if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
-    return bar_wait_slow(bar, parity, c.abort_flag, c.err);
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
-    return p != 0;
-}
-// the last `stages` of a CTA's own copies have landed (out of line: it runs only when a wait gave up)
-__device__ __noinline__ void drain_own(uint64_t* full, uint32_t issued, uint32_t stages) {
-    for (uint32_t j = issued > stages ? issued - stages : 0; j < issued; j++) mbar_wait(&full[j % stages], (j / stages) & 1u);
-}
-// position in a ring: slot and the parity of its current phase
-struct Ring {
-    uint32_t i = 0, phase = 0;
-    __device__ __forceinline__ void next(uint32_t n) {
-        if (++i == n) {
-            i = 0;
-            phase ^= 1;
-        }
-    }
-};
-
 // ------------------------------------------------------------ weights on the MMA's M side
 // A tile is 128 outputs (one block row of the matrix, the MMA's M) x up to 128
 // rows of x (its N, rounded up to 16 only), so a group of a few rows costs
@@ -274,53 +171,6 @@ __device__ inline void fp8_share_out(Fp8Plan& plan, int tiles, int kb, int ctas)
     plan.ctas = (int)min((long long)ctas, (plan.total + kFp8MinRun - 1) / kFp8MinRun);
 }
 
-// The groups' tables in shared memory, by one warp; the caller synchronises.
-// Offsets that do not ascend within [0, T] make a group empty and raise an
-// error, and so does a start below any offset before it: no row outside x or
-// out is ever touched, and none belongs to two groups (whose CTAs would both
-// write it, and whose tiles together could be more than a count of them holds).
-// tile_rows rows of x a tile, `across` tiles along the outputs.
-__device__ inline void fp8_tables(const Fp8Params& p, int32_t* first_tile, int32_t* start, int32_t* rows, int tile_rows,
-                                  int across, bool report) {
-    const int lane = threadIdx.x & 31;
-    int before = 0, top = 0;   // tiles, largest offset so far
-    bool bad = false;
-    for (int g0 = 0; g0 < p.groups; g0 += 32) {
-        const int g = g0 + lane;
-        int a = 0, b = 0;
-        if (g < p.groups) {
-            a = p.offsets ? p.offsets[g] : 0;
-            b = p.offsets ? p.offsets[g + 1] : p.T;
-        }
-        int most = a;   // of the offsets up to this one
-        if (p.groups > 1) {
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) most = max(most, __shfl_up_sync(0xffffffffu, most, o));   // (lanes below o get their own)
-            most = max(most, top);
-            top = __shfl_sync(0xffffffffu, most, 31);
-        }
-        if (a < most || a < 0 || b < a || b > p.T) {
-            bad |= g < p.groups;
-            a = b = 0;
-        }
-        const int tiles = (b - a + tile_rows - 1) / tile_rows * across;
-        int scan = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, scan, o);
-            if (lane >= o) scan += v;
-        }
-        if (g < p.groups) {
-            first_tile[g] = before + scan - tiles;
-            start[g] = a;
-            rows[g] = b - a;
-        }
-        before += __shfl_sync(0xffffffffu, scan, 31);
-    }
-    if (lane == 0) first_tile[p.groups] = before;
-    if (__any_sync(0xffffffffu, bad) && report && lane == 0) atomicOr(p.err, (int)ERR_BOUNDS);
-}
-
 // f(0) ... f(n - 1), n <= 64, by constant indices (the columns are registers),
 // 16 at a time: what is not needed is jumped over.  This code runs once or
 // twice in a launch, cold, and straight through all 64 it took 2.5 us for one.
@@ -388,12 +238,12 @@ fp8_stream_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_consta
     }
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
     pdl_start();   // nothing before this reads or writes global memory
-    if (warp == 2) fp8_tables(p, first_tile, start, rows, kFp8MaxRows, p.mb, blockIdx.x == 0);
+    if (warp == 2) group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows, kFp8MaxRows, p.mb, blockIdx.x == 0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const Fp8Ctl ctl{abort_flag, p.err};
+    const WaitCtl ctl{abort_flag, p.err};
     const uint32_t full0 = smem_u32(full), done0 = smem_u32(done), acc_empty0 = smem_u32(acc_empty);
     const uint32_t sc_full0 = smem_u32(sc_full), sc_empty0 = smem_u32(sc_empty);
     Fp8Plan plan{first_tile, start, rows, p.groups, p.mb, p.kb};
@@ -660,56 +510,12 @@ constexpr int kFp8PairTableOff = kFp8ScaleOff + kFp8PairScaleRing * kFp8PairScal
 __host__ __device__ inline int fp8_pair_stage_off(int groups) {
     return (kFp8PairTableOff + 12 * (groups + 1) + 1023) / 1024 * 1024;
 }
-__device__ __forceinline__ uint32_t map_to_rank0(uint32_t addr) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
-    return r;
-}
-// (What it hands over was read from tensor memory and is ordered by the
-// tcgen05 fence before it; with cluster scope here a full memory barrier came
-// with every block: 1010 us in place of 560 at 4096 x 28672 x 4096, then.)
-__device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// loads of a pair's CTA that complete on a barrier of its first CTA
-__device__ __forceinline__ void tma_pair_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-        "%3}], [%4];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void tma_pair_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-        "%3, %4}], [%5];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
-}
 __device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                              uint32_t accumulate) {
     asm volatile(
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
         " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d_tmem),
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-// arrives on the barrier at `bar`'s offset in both CTAs once the MMAs are done
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-        "h"((uint16_t)3)
-        : "memory");
-}
-__device__ __forceinline__ void cluster_sync_all() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// a word of the peer's shared memory, at the same place as ours; the cluster barrier after it makes it visible
-__device__ __forceinline__ void store_peer(uint32_t* p, uint32_t rank, uint32_t v) {
-    asm volatile(
-        "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n st.shared::cluster.u32 [a], %2;\n}\n" ::"r"(smem_u32(p)),
-        "r"(rank), "r"(v)
         : "memory");
 }
 // the first CTA's barriers, as drain_pair moves them on
@@ -728,51 +534,6 @@ struct Fp8PairTile {
     int group, n;    // matrix, first output
     int pos, rows;   // first row of x of the tile, rows of the group from there on
 };
-
-// 128 outputs of one row that starts on 16 bytes, or on 32 (`wide`): a warp
-// writes 32 rows at once, so what counts is how few stores a row takes (32 bytes
-// a store: 495 us in place of 531 at 4096 x 28672 x 4096 in bf16, 542 in place
-// of 621 in f32, 420 in place of 435 for 8192 rows over 32 x 4096 x 7168, each
-// under sustained load).  One value at a time took some 20 us
-// a tile: where the rows of out do not start on 16 bytes, the other kernel
-// runs, whose warps write neighbouring outputs.
-template <typename T>
-__device__ __forceinline__ void store_row(T* out, int left, const float2 (&acc)[64], bool wide) {
-    constexpr int V = 32 / sizeof(T);   // values of one store
-#pragma unroll
-    for (int c = 0; c < 128 / V; c++) {
-        if (V * c + V <= left) {
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if constexpr (sizeof(T) == 4) {
-                    const float2 v = acc[4 * c + i / 2];
-                    w[i] = __float_as_uint(i & 1 ? v.y : v.x);
-                } else {
-                    const T h[2] = {round_to<T>(acc[8 * c + i].x), round_to<T>(acc[8 * c + i].y)};
-                    memcpy(&w[i], h, 4);
-                }
-            }
-            if (wide) {
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + V * c), "r"(w[0]), "r"(w[1]),
-                             "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                             : "memory");
-            } else {
-                uint4* to = reinterpret_cast<uint4*>(out + V * c);
-                to[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                to[1] = make_uint4(w[4], w[5], w[6], w[7]);
-            }
-        } else {   // the last few
-#pragma unroll
-            for (int i = 0; i < V / 2; i++) {
-                const float2 v = acc[V / 2 * c + i];
-                if (V * c + 2 * i < left) out[V * c + 2 * i] = round_to<T>(v.x);
-                if (V * c + 2 * i + 1 < left) out[V * c + 2 * i + 1] = round_to<T>(v.y);
-            }
-        }
-        asm volatile("" ::: "memory");   // one store's registers at a time
-    }
-}
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp8Warps * 32, 1)
 fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map, Fp8Params p,
@@ -822,13 +583,13 @@ fp8_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     pdl_start();   // nothing before this reads or writes global memory
-    if (warp == 2) fp8_tables(p, first_tile, start, rows, 256, (p.M + 255) / 256, blockIdx.x == 0);
+    if (warp == 2) group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows, 256, (p.M + 255) / 256, blockIdx.x == 0);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();   // the peer's barriers are ready
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const Fp8Ctl ctl{abort_flag, p.err};
+    const WaitCtl ctl{abort_flag, p.err};
     const uint32_t done0 = smem_u32(done), sc_full0 = smem_u32(sc_full), sc_empty0 = smem_u32(sc_empty);
     const int tiles = first_tile[p.groups], pairs = gridDim.x >> 1, KB = p.kb;
 

@@ -1,0 +1,141 @@
+// norm.cu -- entry points of the root-mean-square norm and its gradient
+// (kernels: norm.cuh).  Stateless, as those of rows.cu.
+#include <algorithm>
+#include <cmath>
+
+#include "norm.cuh"
+#include "rows_host.h"
+
+using namespace qrm;
+
+namespace {
+
+int64_t chunks_of(int64_t d) { return (d + 7) / 8; }
+int whole_warps(int64_t threads) { return (int)((threads + 31) / 32 * 32); }
+
+int check_eps(const char* what, float eps) {
+    return eps >= 0.f && std::isfinite(eps) ? QRM_OK : failf(QRM_E_INVALID, "%s: eps %g", what, (double)eps);
+}
+
+template <typename T, int OUT>
+cudaError_t launch(const NormArgs<T>& a, int64_t rows, cudaStream_t s) {
+    const int64_t chunks = chunks_of(a.d);
+    const dim3 grid((unsigned)rows);
+    if (chunks <= 256) return launch_ahead(rms_norm_kernel<T, OUT, 1>, grid, whole_warps(chunks), 0, s, a);
+    if (chunks <= 2 * kNormThreads) return launch_ahead(rms_norm_kernel<T, OUT, 2>, grid, whole_warps((chunks + 1) / 2), 0, s, a);
+    if (chunks <= 4 * kNormThreads) return launch_ahead(rms_norm_kernel<T, OUT, 4>, grid, whole_warps((chunks + 3) / 4), 0, s, a);
+    return launch_ahead(rms_norm_kernel<T, OUT, 0>, grid, kNormThreads, 0, s, a);
+}
+
+int norm(const char* what, int out, int type, const void* x, int64_t ld_x, const void* add, int64_t ld_add, int64_t rows,
+         int64_t d, const float* w, float eps, void* sum, int64_t ld_sum, void* y, int64_t ld_y, uint8_t* codes,
+         int64_t ld_codes, void* scales, int64_t ld_scales, void* stream) {
+    TRY(check_rows(what, type, rows, d));
+    TRY(check_eps(what, eps));
+    if (rows == 0) return QRM_OK;
+    const int b = type_bytes(type);
+    TRY(check_array(what, "x", x, &ld_x, d, b));
+    if (add) TRY(check_array(what, "add", add, &ld_add, d, b));
+    if (sum) TRY(check_array(what, "sum", sum, &ld_sum, d, b));
+    if (y || out == kNormTyped) TRY(check_array(what, "y", y, &ld_y, d, b));
+    if (out == kNorm8) {
+        TRY(check_array(what, "codes", codes, &ld_codes, d, 1));
+        TRY(check_array(what, "scales", scales, &ld_scales, blocks_of(d), 4));
+    } else if (out == kNorm4) {
+        TRY(check_array(what, "codes", codes, &ld_codes, 16 * blocks4_of(d), 1));
+        TRY(check_array(what, "scales", scales, &ld_scales, blocks4_of(d), 1));
+    }
+    if (w) TRY(check_ints(what, "w", w));
+    int device, sms;
+    TRY(current_device(&device, &sms));
+    const bool wide = wide_rows(x, ld_x, b) && (!add || wide_rows(add, ld_add, b)) && (!sum || wide_rows(sum, ld_sum, b)) &&
+                      (!y || wide_rows(y, ld_y, b));
+    const bool wide_c = out == kNorm8 ? wide_codes(codes, ld_codes) : aligned(codes, 4) && ld_codes % 4 == 0;
+    cudaError_t e;
+    const cudaStream_t s = (cudaStream_t)stream;
+    BY_TYPE(type, {
+        const NormArgs<V> a{(const V*)x, (const V*)add, w, (V*)sum, (V*)y, codes, scales, ld_x, ld_add, ld_sum, ld_y,
+                            ld_codes, ld_scales, (int)d, eps, wide, aligned(w, 16), wide_c};
+        e = out == kNormTyped ? launch<V, kNormTyped>(a, rows, s) : out == kNorm8 ? launch<V, kNorm8>(a, rows, s)
+                                                                                  : launch<V, kNorm4>(a, rows, s);
+    });
+    return done(what, e);
+}
+
+// The gradient's CTAs: those that fit on the 148 SMs at once, and so many parts
+// of dw.  (A number of its own, so that the room for them needs no device.)
+int grad_threads(int64_t d) { return whole_warps(std::min<int64_t>(chunks_of(d), kNormGradThreads)); }
+int64_t grad_ctas(int64_t rows, int64_t d) {
+    return std::min<int64_t>(rows, 148 * std::max(1, std::min(4, 1024 / grad_threads(d))));
+}
+
+}  // namespace
+
+extern "C" int qrm_rms_norm(int type, const void* x_dev, int64_t ld_x, const void* add_dev, int64_t ld_add, int64_t rows,
+                            int64_t d, const float* w_dev, float eps, void* sum_dev, int64_t ld_sum, void* y_dev,
+                            int64_t ld_y, void* stream) {
+    return norm("qrm_rms_norm", kNormTyped, type, x_dev, ld_x, add_dev, ld_add, rows, d, w_dev, eps, sum_dev, ld_sum, y_dev,
+                ld_y, nullptr, 0, nullptr, 0, stream);
+}
+
+extern "C" int qrm_rms_norm_fp8(int type, const void* x_dev, int64_t ld_x, const void* add_dev, int64_t ld_add, int64_t rows,
+                                int64_t d, const float* w_dev, float eps, void* sum_dev, int64_t ld_sum, void* y_dev,
+                                int64_t ld_y, uint8_t* codes_dev, int64_t ld_codes, float* scales_dev, int64_t ld_scales,
+                                void* stream) {
+    return norm("qrm_rms_norm_fp8", kNorm8, type, x_dev, ld_x, add_dev, ld_add, rows, d, w_dev, eps, sum_dev, ld_sum, y_dev,
+                ld_y, codes_dev, ld_codes, scales_dev, ld_scales, stream);
+}
+
+extern "C" int qrm_rms_norm_fp4(int type, const void* x_dev, int64_t ld_x, const void* add_dev, int64_t ld_add, int64_t rows,
+                                int64_t d, const float* w_dev, float eps, void* sum_dev, int64_t ld_sum, void* y_dev,
+                                int64_t ld_y, uint8_t* codes_dev, int64_t ld_codes, uint8_t* scales_dev, int64_t ld_scales,
+                                void* stream) {
+    return norm("qrm_rms_norm_fp4", kNorm4, type, x_dev, ld_x, add_dev, ld_add, rows, d, w_dev, eps, sum_dev, ld_sum, y_dev,
+                ld_y, codes_dev, ld_codes, scales_dev, ld_scales, stream);
+}
+
+extern "C" int64_t qrm_rms_norm_grad_work(int64_t rows, int64_t d) {
+    if (rows <= 1 || rows > INT_MAX || d <= 0 || d > kMaxCols) return 0;
+    return grad_ctas(rows, d) * d;
+}
+
+extern "C" int qrm_rms_norm_grad(int type, const void* dy_dev, int64_t ld_dy, const void* x_dev, int64_t ld_x, int64_t rows,
+                                 int64_t d, const float* w_dev, float eps, const void* add_dev, int64_t ld_add, void* dx_dev,
+                                 int64_t ld_dx, float* dw_dev, float* work_dev, void* stream) {
+    const char* what = "qrm_rms_norm_grad";
+    TRY(check_rows(what, type, rows, d));
+    TRY(check_eps(what, eps));
+    const int b = type_bytes(type);
+    if (dw_dev) TRY(check_ints(what, "dw", dw_dev));
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (rows == 0) {   // a sum of nothing
+        if (!dw_dev) return QRM_OK;
+        int device, sms;
+        TRY(current_device(&device, &sms));
+        return done(what, launch_ahead(rms_norm_dw_kernel, dim3((unsigned)((d + 31) / 32)), 32 * kNormRuns, 0, s, dw_dev, 0, (int)d, dw_dev));
+    }
+    TRY(check_array(what, "dy", dy_dev, &ld_dy, d, b));
+    TRY(check_array(what, "x", x_dev, &ld_x, d, b));
+    if (add_dev) TRY(check_array(what, "add", add_dev, &ld_add, d, b));
+    TRY(check_array(what, "dx", dx_dev, &ld_dx, d, b));
+    if (w_dev) TRY(check_ints(what, "w", w_dev));
+    const int64_t ctas = grad_ctas(rows, d);
+    if (dw_dev && ctas > 1) TRY(check_ints(what, "work", work_dev));
+    int device, sms;
+    TRY(current_device(&device, &sms));
+    const bool wide = wide_rows(dy_dev, ld_dy, b) && wide_rows(x_dev, ld_x, b) && wide_rows(dx_dev, ld_dx, b) &&
+                      (!add_dev || wide_rows(add_dev, ld_add, b));
+    float* part = !dw_dev ? nullptr : ctas > 1 ? work_dev : dw_dev;
+    cudaError_t e;
+    BY_TYPE(type, {
+        const NormGradArgs<V> a{(const V*)dy_dev, (const V*)x_dev, (const V*)add_dev, w_dev, (V*)dx_dev, part, ld_dy, ld_x,
+                                ld_add, ld_dx, (int)rows, (int)d, eps, wide, aligned(w_dev, 16),
+                                aligned(part, 16) && d % 4 == 0};
+        e = chunks_of(d) <= kNormGradThreads
+                ? launch_ahead(rms_norm_grad_kernel<V, 1>, dim3((unsigned)ctas), grad_threads(d), 0, s, a)
+                : launch_ahead(rms_norm_grad_kernel<V, 0>, dim3((unsigned)ctas), grad_threads(d), 0, s, a);
+    });
+    if (e == cudaSuccess && dw_dev && ctas > 1)
+        e = launch_ahead(rms_norm_dw_kernel, dim3((unsigned)((d + 31) / 32)), 32 * kNormRuns, 0, s, work_dev, (int)ctas, (int)d, dw_dev);
+    return done(what, e);
+}

@@ -4,7 +4,8 @@
 #include <climits>
 
 #include "host_util.h"
-#include "rows.cuh"
+#include "rows4.cuh"
+#include "rows_host.h"
 
 namespace qrm {
 namespace {
@@ -27,59 +28,6 @@ Cut cut_columns(int64_t rows, int64_t cols, int each) {
     const int64_t threads = ((lanes + pieces - 1) / pieces + 31) / 32 * 32;
     return {(int)threads, dim3((unsigned)rows, (unsigned)pieces)};
 }
-
-bool wide_rows(const void* p, int64_t ld, int bytes) { return aligned(p, 16) && ld * bytes % 16 == 0; }
-bool wide_codes(const void* p, int64_t ld) { return aligned(p, 8) && ld % 8 == 0; }
-bool wide_codes16(const void* p, int64_t ld) { return aligned(p, 16) && ld % 16 == 0; }
-
-constexpr int64_t kMaxCols = 1 << 24;   // columns of a row (a grid's y holds its pieces)
-
-int check_rows(const char* what, int type, int64_t rows, int64_t cols) {
-    if (!type_bytes(type)) return failf(QRM_E_FORMAT, "%s: type %d is not F32, F16 or BF16", what, type);
-    if (rows < 0 || rows > (int64_t)INT_MAX) return failf(QRM_E_INVALID, "%s: %lld rows", what, (long long)rows);
-    if (cols <= 0 || cols > kMaxCols) return failf(QRM_E_INVALID, "%s: %lld columns", what, (long long)cols);
-    return QRM_OK;
-}
-int check_tokens(const char* what, int64_t T, int k, int64_t n_rows) {
-    if (T < 0 || k <= 0 || T > INT_MAX / (int64_t)k)
-        return failf(QRM_E_INVALID, "%s: %lld tokens x %d slots", what, (long long)T, k);
-    if (n_rows < 0 || n_rows > (int64_t)INT_MAX) return failf(QRM_E_INVALID, "%s: %lld rows", what, (long long)n_rows);
-    return QRM_OK;
-}
-// an array of values of `bytes` bytes each, in rows `ld` apart (0: dense)
-int check_array(const char* what, const char* name, const void* p, int64_t* ld, int64_t cols, int bytes) {
-    if (!p) return failf(QRM_E_INVALID, "%s: %s is NULL", what, name);
-    if (!aligned(p, bytes)) return failf(QRM_E_INVALID, "%s: %s is not aligned to its %d-byte values", what, name, bytes);
-    if (!pitch_ok(ld, cols))
-        return failf(QRM_E_INVALID, "%s: pitch %lld of %s is below its %lld columns", what, (long long)*ld, name,
-                     (long long)cols);
-    return QRM_OK;
-}
-int check_ints(const char* what, const char* name, const void* p) {
-    if (!p) return failf(QRM_E_INVALID, "%s: %s is NULL", what, name);
-    if (!aligned(p, 4)) return failf(QRM_E_INVALID, "%s: %s is not aligned to 4 bytes", what, name);
-    return QRM_OK;
-}
-
-#define TRY(expr)            \
-    do {                     \
-        int r_ = (expr);     \
-        if (r_) return r_;   \
-    } while (0)
-
-// the statement with V = float, __half or __nv_bfloat16, by the activation type
-#define BY_TYPE(type, ...)                                  \
-    do {                                                    \
-        if ((type) == QRM_F32) { using V = float; __VA_ARGS__; } \
-        else if ((type) == QRM_F16) { using V = __half; __VA_ARGS__; } \
-        else { using V = __nv_bfloat16; __VA_ARGS__; }      \
-    } while (0)
-
-int done(const char* what, cudaError_t e) {
-    return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
-}
-
-int64_t blocks_of(int64_t cols) { return (cols + kFp8Block - 1) / kFp8Block; }
 
 }  // namespace
 }  // namespace qrm
@@ -294,6 +242,51 @@ extern "C" int qrm_quantize_fp8_weights(int type, const void* w_dev, int groups,
     const bool wide = wide_rows(w_dev, cols, b) && wide_codes(codes_dev, cols);
     BY_TYPE(type, e = launch_ahead(quantize_fp8_weights_kernel<V>, grid, 256, 0, (cudaStream_t)stream, (const V*)w_dev, (int)rows, (int)cols,
                                                                                          codes_dev, scales_dev, wide));
+    return done(what, e);
+}
+
+// 4-bit rows: whole blocks of 16 bytes, and a byte for each block's scale
+static int check_rows4(const char* what, uint8_t* codes, int64_t* ld_codes, uint8_t* scales, int64_t* ld_scales, int64_t cols) {
+    TRY(check_array(what, "codes", codes, ld_codes, 16 * blocks4_of(cols), 1));
+    return check_array(what, "scales", scales, ld_scales, blocks4_of(cols), 1);
+}
+
+extern "C" int qrm_gather_rows_fp4(int type, const void* x_dev, int64_t ld_x, const int32_t* pos_dev, int64_t T, int k,
+                                   int64_t d, uint8_t* codes_dev, int64_t n_rows, int64_t ld_codes, uint8_t* scales_dev,
+                                   int64_t ld_scales, void* stream) {
+    const char* what = "qrm_gather_rows_fp4";
+    TRY(check_rows(what, type, T, d));
+    TRY(check_tokens(what, T, k, n_rows));
+    if (T == 0 || n_rows == 0) return QRM_OK;
+    const int b = type_bytes(type);
+    TRY(check_array(what, "x", x_dev, &ld_x, d, b));
+    TRY(check_rows4(what, codes_dev, &ld_codes, scales_dev, &ld_scales, d));
+    TRY(check_ints(what, "pos", pos_dev));
+    int device, sms;
+    TRY(current_device(&device, &sms));
+    cudaError_t e;
+    const Cut c = cut_columns(T, d, 16);
+    BY_TYPE(type, e = launch_ahead(gather_rows_fp4_kernel<V>, c.grid, c.threads, 0, (cudaStream_t)stream, (const V*)x_dev, ld_x, pos_dev, k, (int)d, (uint32_t)n_rows, codes_dev, ld_codes, scales_dev,
+                      ld_scales, wide_rows(x_dev, ld_x, b), wide_codes(codes_dev, ld_codes)));
+    return done(what, e);
+}
+
+extern "C" int qrm_quantize_fp4(int type, const void* x_dev, int64_t ld_x, int64_t rows, int64_t cols,
+                                const int32_t* n_rows_dev, uint8_t* codes_dev, int64_t ld_codes, uint8_t* scales_dev,
+                                int64_t ld_scales, void* stream) {
+    const char* what = "qrm_quantize_fp4";
+    TRY(check_rows(what, type, rows, cols));
+    if (rows == 0) return QRM_OK;
+    const int b = type_bytes(type);
+    TRY(check_array(what, "x", x_dev, &ld_x, cols, b));
+    TRY(check_rows4(what, codes_dev, &ld_codes, scales_dev, &ld_scales, cols));
+    if (n_rows_dev) TRY(check_ints(what, "n_rows", n_rows_dev));
+    int device, sms;
+    TRY(current_device(&device, &sms));
+    cudaError_t e;
+    const Cut c = cut_columns(rows, cols, 16);
+    BY_TYPE(type, e = launch_ahead(quantize_fp4_kernel<V>, c.grid, c.threads, 0, (cudaStream_t)stream, (const V*)x_dev, ld_x, n_rows_dev, (int)cols, codes_dev, ld_codes, scales_dev, ld_scales,
+                      wide_rows(x_dev, ld_x, b), wide_codes(codes_dev, ld_codes)));
     return done(what, e);
 }
 

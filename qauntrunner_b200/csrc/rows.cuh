@@ -189,7 +189,7 @@ __device__ __forceinline__ uint2 codes8(const Pairs8& v, const Quant& z) {
 // The check costs 0.3 us of 64 in gather_rows_fp8, 0.4 of 145 in the combine's
 // gradient and 0.4 of 67 in SwiGLU's, at the sizes stated there.
 constexpr float kFp8Tiny = 8.077935669463161e-28f;   // 2^-90
-__device__ __noinline__ uint2 codes8_divided(const Pairs8 v, float scale) {
+static __device__ __noinline__ uint2 codes8_divided(const Pairs8 v, float scale) {
     uint32_t w[4];
 #pragma unroll 1
     for (int i = 0; i < 4; i++) {
@@ -576,7 +576,7 @@ constexpr int kGradCols = 8192;
 // The codes of one slot's blocks with a tiny scale once more, by division, over
 // what the same threads have written (a choice for each eight columns where they
 // are written cost 8 us).
-__device__ __noinline__ void divide_tiny(const float4* g, const float2* sc, float minus_w, int cols, int c, int step,
+static __device__ __noinline__ void divide_tiny(const float4* g, const float2* sc, float minus_w, int cols, int c, int step,
                                          uint8_t* codes, bool wide) {
     const Pair wp = pair(minus_w, minus_w);
 #pragma unroll 1
