@@ -38,7 +38,7 @@ void release(qrm_fp4* m) {
     delete m;
 }
 
-size_t pair_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4PairStages * kFp4PairStage; }
+size_t pair_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4PairStages * kFp4PairStage + 8 * kFp4PairOut; }
 
 template <int MODE>
 cudaError_t prepare_kernels() {
@@ -220,10 +220,8 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     DeviceGuard here;
     cudaError_t e = here.enter(m->device);
     if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    // the kernel for large groups writes rows that start on 16 bytes
-    const bool pair = aligned(out, 16) && ld_out * b % 16 == 0 &&
-                      (m->form >= 0 ? m->form : pair_is_faster(T, m->groups, across, m->steps, m->sms));
-    const int wide_out = aligned(out, 32) && ld_out * b % 32 == 0;
+    const bool pair = m->form >= 0 ? m->form : pair_is_faster(T, m->groups, across, m->steps, m->sms);
+    const int wide_out = aligned(out, 16) && ld_out * b % 16 == 0;
     CUtensorMap x_map;
     const cuuint64_t dims[2] = {(cuuint64_t)(16 * blocks), (cuuint64_t)T};
     const cuuint64_t strides[1] = {(cuuint64_t)ld_x};
@@ -249,7 +247,7 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     p.blocks = (int)blocks;
     p.type = type;
     p.row_tiles = (int)(offsets ? row_tiles : (T + kFp4Rows - 1) / kFp4Rows);
-    p.wide_xs = aligned(xs, 8) && ld_xs % 8 == 0;
+    p.wide_xs = aligned(xs, 16) && ld_xs % 16 == 0 ? 2 : aligned(xs, 8) && ld_xs % 8 == 0 ? 1 : 0;
     const cudaStream_t s = (cudaStream_t)stream;
     e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, p, pair, wide_out, T, s)
         : mode == kFp4Gated ? launch<kFp4Gated>(m, x_map, p, pair, wide_out, T, s)

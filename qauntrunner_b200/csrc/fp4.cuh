@@ -47,7 +47,7 @@ struct Fp4Params {
     int blocks;                // of 32 in it
     int type;                  // of out
     int row_tiles;             // room for tiles of rows in the grid (weights on the M side)
-    bool wide_xs;              // rows of scales start on 8 bytes
+    int wide_xs;               // rows of scales start on 16 bytes: 2, on 8: 1
 };
 
 // Instruction descriptor of kind::mxf4: f32 accumulators, e2m1 A and B, e8m0
@@ -96,6 +96,13 @@ __device__ __forceinline__ uint2 eight_scales(const uint8_t* __restrict__ row, i
     for (int i = 0; i < 8; i++)
         if (b + i < blocks) w[i >> 2] |= (uint32_t)__ldg(row + b + i) << (8 * (i & 3));
     return make_uint2(w[0], w[1]);
+}
+
+// sixteen of them; wide: 2 when rows start on 16 bytes, 1 on 8
+__device__ __forceinline__ uint4 sixteen_scales(const uint8_t* __restrict__ row, int b, int blocks, int wide) {
+    if (wide == 2 && b + 16 <= blocks) return __ldg(reinterpret_cast<const uint4*>(row + b));
+    const uint2 lo = eight_scales(row, b, blocks, wide), hi = eight_scales(row, b + 8, blocks, wide);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
 
 __device__ __forceinline__ float2 gated2(float2 gate, float2 up, float limit) {
@@ -400,13 +407,14 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // cycles, in which the ring of stages fills up).
 //
 // Warps: 0 loads codes and the weights' scales, 1 issues the MMAs (in the
-// pair's first CTA), 2 and 3 bring the scales of x, a stage each in turn, 4-11
+// pair's first CTA), 2 and 3 bring the scales of x, 4-11
 // write the output: lane quarter (warp & 3), half of the columns (warp >= 8).
 constexpr int kFp4PairThreads = 384;
-constexpr int kFp4PairStages = 6;
+constexpr int kFp4PairStages = 5;
 constexpr int kFp4PairTx = 2 * kFp4Tile + 2 * kFp4Scales;            // bytes of a CTA's copies of a stage
 constexpr int kFp4PairStage = kFp4PairTx + kFp4Scales;               // and the scales of x
 constexpr int kFp4PairSecond = 208, kFp4PairTmemScales = 464;
+constexpr int kFp4PairOut = 32 * 144;          // a warp's room for rows on their way out: 32 of 128 bytes, 16 apart
 constexpr int kFp4PairTableOff = 1024;
 constexpr int kFp4PairRegsFew = 72, kFp4PairRegsMany = 216;
 constexpr int kFp4PairRegs = 128 * kFp4PairRegsFew + 256 * kFp4PairRegsMany;
@@ -424,11 +432,49 @@ struct Fp4PairBars {
     }
     __device__ void wait(uint32_t slot, uint32_t parity) { mbar_wait(&full[slot], parity); }
 };
-// an arrival on the first CTA's barrier that also hands over what this thread's CTA wrote to its shared memory
-__device__ __forceinline__ void bar_arrive_release_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// A warp's 32 rows of 2 N outputs each (a lane holds a row) to out, by way of
+// shared memory, so that a store's lanes write neighbouring outputs, of four
+// rows at once.  left: how many of a row's exist; rows: how many rows do.
+template <typename T, int N>
+__device__ __forceinline__ void store_rows(T* out, long long ld, int left, int rows, const float2 (&v)[N], uint8_t* room, bool wide) {
+    constexpr int C = 128 / sizeof(T);   // outputs of a row in one go
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int c = 0; c < 2 * N; c += C) {
+        if (c >= left) break;
+        __syncwarp();
+        uint4* to = reinterpret_cast<uint4*>(room + 144 * lane);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {   // 16 bytes each
+            uint32_t w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if constexpr (sizeof(T) == 4) {
+                    const float2 f = v[c / 2 + 2 * i + k / 2];
+                    w[k] = __float_as_uint(k & 1 ? f.y : f.x);
+                } else {
+                    const float2 f = v[c / 2 + 4 * i + k];
+                    const T h[2] = {round_to<T>(f.x), round_to<T>(f.y)};
+                    memcpy(&w[k], h, 4);
+                }
+            }
+            to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        __syncwarp();
+        if (wide && c + C <= left) {
+            const int r0 = lane >> 3, at = 16 * (lane & 7);
+            uint8_t* o = reinterpret_cast<uint8_t*>(out + r0 * ld + c) + at;
+#pragma unroll
+            for (int r = 0; r < 32; r += 4)
+                if (r + r0 < rows) *reinterpret_cast<uint4*>(o + r * ld * (long long)sizeof(T)) = *reinterpret_cast<const uint4*>(room + 144 * (r + r0) + at);
+        } else {   // one output a lane
+            for (int r = 0; r < min(rows, 32); r++)
+#pragma unroll
+                for (int k = 0; k < C; k += 32)
+                    if (c + k + lane < left) out[r * ld + c + k + lane] = reinterpret_cast<const T*>(room + 144 * r)[k + lane];
+        }
+    }
 }
-
 // 2 N outputs of a row in 4-bit blocks, m of them (from a block's start on)
 template <int N>
 __device__ __forceinline__ void store_row4(uint8_t* codes, uint8_t* scales, int left, const float2 (&h)[N]) {
@@ -478,7 +524,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     if (threadIdx.x == 0) {
         for (int i = 0; i < kFp4PairStages; i++) {
             mbar_init(&full[i], 1);
-            mbar_init(&x_full[i], 2);
+            mbar_init(&x_full[i], 4);
             mbar_init(&done[i], 1);
         }
         mbar_init(&tile_done[0], 1);
@@ -596,43 +642,53 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             }
             __syncwarp();
         } else if (warp >= 2) {
-            // -------------------------------------------- scales of x, every second stage
+            // -------------------------------------------- scales of x: rows 64 (warp - 2) + lane and + 32 of the CTA's
+            // Four stages' at a time, and the next four's are on their way while these are handed out: a load's way is
+            // longer than a stage.
             bool ok = true;
             Ring r;
+            const int first = 64 * (warp - 2) + lane;
             const uint32_t x_full0 = map_to_rank0(smem_u32(x_full));
-            uint32_t turn = 0;   // of the stages, all tiles' one after the other
-            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
-                const Tile t = tile_at(i);
-                const uint8_t* row = p.x_scales + (long long)(t.pos + lane) * p.ld_xs;
-                uint2 v[4];
-                auto load = [&](int k) {
+            uint4 next[2][2];   // [row][half]
+            auto load = [&](const Tile& t, int k) {
+                const uint8_t* row = p.x_scales + (long long)(t.pos + first) * p.ld_xs;
 #pragma unroll
-                    for (int c = 0; c < 4; c++)
-                        v[c] = lane + 32 * c < t.rows && k < steps ? eight_scales(row + 32 * c * p.ld_xs, 8 * k, p.blocks, p.wide_xs) : make_uint2(0, 0);
-                };
-                int k = (warp ^ turn) & 1;   // the first of the tile that is this warp's
-                load(k);
-                for (int j = 0; j < steps; j++, turn ^= 1) {
-                    if (((warp ^ turn) & 1) == 0) {
-                        const uint4 lo = make_uint4(v[0].x, v[1].x, v[2].x, v[3].x), hi = make_uint4(v[0].y, v[1].y, v[2].y, v[3].y);
-                        k += 2;
-                        load(k);
+                for (int c = 0; c < 2; c++) {
+                    const bool in = first + 32 * c < t.rows;
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        next[c][h] = in ? sixteen_scales(row + 32 * c * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            int i = blockIdx.x >> 1;
+            if (i < tiles) load(tile_at(i), 0);
+            for (; i < tiles && ok; i += pairs) {
+                const Tile t = tile_at(i);
+                for (int k4 = 0; k4 < steps && ok; k4 += 4) {
+                    const uint4 a0 = next[0][0], a1 = next[0][1], b0 = next[1][0], b1 = next[1][1];
+                    if (k4 + 4 < steps) load(t, k4 + 4);
+                    else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (k4 + j >= steps) break;
+                        const uint4 a = j < 2 ? a0 : a1, b = j < 2 ? b0 : b1;
                         if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
-                        uint4* to = reinterpret_cast<uint4*>(ring + r.i * kFp4PairStage + kFp4PairTx) + lane;
-                        to[0] = lo;
-                        to[32] = hi;
+                        uint2* to = reinterpret_cast<uint2*>(ring + r.i * kFp4PairStage + kFp4PairTx) + 2 * lane + (warp - 2);
+                        to[0] = j & 1 ? make_uint2(a.z, b.z) : make_uint2(a.x, b.x);
+                        to[64] = j & 1 ? make_uint2(a.w, b.w) : make_uint2(a.y, b.y);
                         fence_async();
                         __syncwarp();
-                        if (lane == 0) bar_arrive_release_cluster(x_full0 + 8 * r.i);
+                        if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
+                        r.next(kFp4PairStages);
                     }
-                    r.next(kFp4PairStages);
                 }
             }
         }
     } else {
         // ------------------------------------------------ output
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp4PairRegsMany));
-        const int half = (warp - 4) >> 2, row = 32 * (warp & 3) + lane;
+        const int half = (warp - 4) >> 2;
+        uint8_t* room = ring + kFp4PairStages * kFp4PairStage + (warp - 4) * kFp4PairOut;
         const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t read0 = map_to_rank0(smem_u32(tile_read));
         uint32_t n = 0;
@@ -651,27 +707,30 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             tc_fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive_cluster(read0);
-            if (row < t.rows) {
+            const int r0 = 32 * (warp & 3);   // the warp's first row
+            if (t.rows > r0) {
+                const long long at = t.pos + r0;
                 if (MODE == kFp4Plain) {
-                    const long long o = (long long)(t.pos + row) * p.ld_out + t.m + 128 * half;
-                    const int left = p.M - t.m - 128 * half;
-                    if (p.type == 0) store_row(reinterpret_cast<float*>(p.out) + o, left, acc, wide_out);
-                    else if (p.type == 1) store_row(reinterpret_cast<__half*>(p.out) + o, left, acc, wide_out);
-                    else store_row(reinterpret_cast<__nv_bfloat16*>(p.out) + o, left, acc, wide_out);
+                    const int m = t.m + 128 * half;
+                    const long long o = at * p.ld_out + m;
+                    if (p.type == 0) store_rows(reinterpret_cast<float*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
+                    else if (p.type == 1) store_rows(reinterpret_cast<__half*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
+                    else store_rows(reinterpret_cast<__nv_bfloat16*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
                 } else {
                     float2 h[32];
 #pragma unroll
                     for (int c = 0; c < 32; c++) h[c] = gated2(acc[c], acc[32 + c], p.limit);
-                    const int m = t.m + 64 * half, left = p.M - m;
-                    const long long at = t.pos + row;
+                    const int m = t.m + 64 * half;
+                    const long long o = at * p.ld_out + m;
                     if (MODE == kFp4GatedRows) {
-                        store_row4(reinterpret_cast<uint8_t*>(p.out) + at * p.ld_out + m / 2, p.out_scales + at * p.ld_os + m / kFp4Block, left, h);
+                        if (lane < t.rows - r0)
+                            store_row4(reinterpret_cast<uint8_t*>(p.out) + (at + lane) * p.ld_out + m / 2, p.out_scales + (at + lane) * p.ld_os + m / kFp4Block, p.M - m, h);
                     } else if (p.type == 0) {
-                        store_row(reinterpret_cast<float*>(p.out) + at * p.ld_out + m, left, h, wide_out);
+                        store_rows(reinterpret_cast<float*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
                     } else if (p.type == 1) {
-                        store_row(reinterpret_cast<__half*>(p.out) + at * p.ld_out + m, left, h, wide_out);
+                        store_rows(reinterpret_cast<__half*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
                     } else {
-                        store_row(reinterpret_cast<__nv_bfloat16*>(p.out) + at * p.ld_out + m, left, h, wide_out);
+                        store_rows(reinterpret_cast<__nv_bfloat16*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
                     }
                 }
             }
