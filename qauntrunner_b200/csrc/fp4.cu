@@ -14,15 +14,16 @@ using namespace qrm;
 
 struct qrm_fp4 {
     int device = 0, sms = 0, groups = 0;
-    int form = -1;                       // QRM_FP4_PAIR: 1 wherever it can / 0 never rows of x on the MMA's M side
+    int form = -1;                       // QRM_FP4_FORM: the kernel of every product (Fp4Form)
     int64_t rows = 0, cols = 0;
-    int tiles = 0, steps = 0;            // of 128 rows; of 256 columns
-    int halves = 0, second = 0;          // gated: tiles with gate's and up's rows in tiles of their own; up's first
+    int units = 0, gated_units = 0;      // of 128 rows; of 64 features, if there are two halves
+    int steps = 0;                       // of 256 columns
     uint8_t* codes = nullptr;            // [groups][rows][whole blocks of 16 bytes]; the other arrays are in the same allocation
-    uint8_t* units = nullptr;            // scales, [groups][tiles][steps][2][512]
-    uint8_t* gated_units = nullptr;      // [groups][halves][steps][2][512]
+    uint8_t* scales = nullptr;           // [groups][units][steps][2][512]
+    uint8_t* gated_scales = nullptr;     // [groups][gated_units][steps][2][512]
     int32_t* err = nullptr;
-    CUtensorMap map, units_map, gated_map;   // codes in boxes of 256 columns x 128 rows; units in boxes of one stage's
+    // codes in boxes of 256 columns x 128 and 16 rows; scales in boxes of a unit's for one stage
+    CUtensorMap map, map16, scales_map, gated_scales_map;
 };
 
 namespace {
@@ -38,6 +39,7 @@ void release(qrm_fp4* m) {
     delete m;
 }
 
+size_t fit_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4FitStages * kFp4FitStage + 2 * kFp4FitRoom; }
 size_t pair_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4PairStages * kFp4PairStage + 8 * kFp4PairOut; }
 
 template <int MODE>
@@ -45,13 +47,16 @@ cudaError_t prepare_kernels() {
     cudaError_t e = cudaFuncSetAttribute(fp4_split_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(fp4_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(kFp4MaxGroups));
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(fp4_fit_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fit_smem(kFp4MaxGroups));
     return e;
 }
 // registers a thread that the pair kernels were built with: their split may not pass what a launch has
 template <int MODE>
-int pair_regs() {
-    cudaFuncAttributes at{};
-    return cudaFuncGetAttributes(&at, fp4_pair_kernel<MODE>) == cudaSuccess ? at.numRegs : 0;
+bool enough_regs() {
+    cudaFuncAttributes pair{}, fit{};
+    return cudaFuncGetAttributes(&pair, fp4_pair_kernel<MODE>) == cudaSuccess && pair.numRegs * kFp4PairThreads >= kFp4PairRegs &&
+           cudaFuncGetAttributes(&fit, fp4_fit_kernel<MODE>) == cudaSuccess && fit.numRegs * kFp4PairThreads >= kFp4FitRegs;
 }
 
 int create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes, const void* scales,
@@ -85,30 +90,28 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
         release(m);
         return rc;
     };
-    if (const char* e = getenv("QRM_FP4_PAIR")) m->form = atoi(e) != 0;
+    if (const char* e = getenv("QRM_FP4_FORM")) m->form = std::max(0, std::min(2, atoi(e)));
     m->device = device;
     m->sms = sms;
     m->groups = groups;
     m->rows = rows;
     m->cols = cols;
-    m->tiles = (int)((rows + 127) / 128);
+    m->units = (int)((rows + 127) / 128);
     m->steps = (int)((cols + kFp4Step - 1) / kFp4Step);
-    const int64_t f = rows / 2;
-    const bool gated = rows % 2 == 0, apart = gated && f % 128;   // up's rows begin inside a tile
-    m->second = gated ? (int)((f + 127) / 128) : 0;
-    m->halves = 2 * m->second;
-    // one allocation: codes, units, units for the gated product where they differ, the error flags
+    const int f = rows % 2 ? 0 : (int)(rows / 2);
+    m->gated_units = (f + 63) / 64;
+    // one allocation: codes, scales in both orders, the error flags
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t stage = (size_t)m->steps * kFp4Scales, pitch = (size_t)blocks * 16;
-    const size_t units_at = up(code_bytes), gated_at = units_at + (size_t)groups * m->tiles * stage;
-    const size_t err_at = gated_at + (apart ? (size_t)groups * m->halves * stage : 0);
+    const size_t scales_at = up(code_bytes), gated_at = scales_at + (size_t)groups * m->units * stage;
+    const size_t err_at = gated_at + (size_t)groups * m->gated_units * stage;
     uint8_t* staged = nullptr;   // the scales as they came, until they are in units
     if (cudaMalloc(&m->codes, err_at + 256) != cudaSuccess || cudaMalloc(&staged, scale_bytes) != cudaSuccess) {
         cudaGetLastError();
         return bail(failf(QRM_E_NOMEM, "%s: cannot allocate %zu bytes", what, err_at + 256 + scale_bytes));
     }
-    m->units = m->codes + units_at;
-    m->gated_units = apart ? m->codes + gated_at : m->units;
+    m->scales = m->codes + scales_at;
+    m->gated_scales = m->codes + gated_at;
     m->err = reinterpret_cast<int32_t*>(m->codes + err_at);
     // device sources: what any stream still writes there is awaited, on their own device if that is another one
     cudaError_t e = cudaDeviceSynchronize();
@@ -123,44 +126,51 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     if (e == cudaSuccess && cols % kFp4Block)
         e = launch_ahead(fp4_clear_tail_kernel, dim3((unsigned)((all + 255) / 256)), 256, 0, nullptr, m->codes, all, (int)cols, (int)pitch);
     if (e == cudaSuccess)
-        e = launch_ahead(fp4_scale_units_kernel, dim3(2 * m->steps, m->tiles, groups), 128, 0, nullptr, staged, (int)rows, (int)blocks,
-                         (int)rows, m->tiles, m->tiles, m->steps, reinterpret_cast<uint32_t*>(m->units));
-    if (e == cudaSuccess && apart)
-        e = launch_ahead(fp4_scale_units_kernel, dim3(2 * m->steps, m->halves, groups), 128, 0, nullptr, staged, (int)rows, (int)blocks,
-                         (int)f, m->halves, m->second, m->steps, reinterpret_cast<uint32_t*>(m->gated_units));
+        e = launch_ahead(fp4_scale_units_kernel, dim3(2 * m->steps, m->units, groups), 128, 0, nullptr, staged, (int)rows, (int)blocks,
+                         0, m->units, m->steps, reinterpret_cast<uint32_t*>(m->scales));
+    if (e == cudaSuccess && f)
+        e = launch_ahead(fp4_scale_units_kernel, dim3(2 * m->steps, m->gated_units, groups), 128, 0, nullptr, staged, (int)rows,
+                         (int)blocks, f, m->gated_units, m->steps, reinterpret_cast<uint32_t*>(m->gated_scales));
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     cudaFree(staged);
     if (e == cudaSuccess) e = prepare_kernels<kFp4Plain>();
     if (e == cudaSuccess) e = prepare_kernels<kFp4Gated>();
     if (e == cudaSuccess) e = prepare_kernels<kFp4GatedRows>();
     if (e != cudaSuccess) return bail(failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e)));
-    if (std::min({pair_regs<kFp4Plain>(), pair_regs<kFp4Gated>(), pair_regs<kFp4GatedRows>()}) * kFp4PairThreads < kFp4PairRegs)
+    if (!enough_regs<kFp4Plain>() || !enough_regs<kFp4Gated>() || !enough_regs<kFp4GatedRows>())
         return bail(failf(QRM_E_CUDA, "%s: built with too few registers a thread for their split", what));
     const cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)rows, (cuuint64_t)groups};
     const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
-    const cuuint32_t box[3] = {128, 128, 1}, unit_box[2] = {256, kFp4Scales / 256};
+    const cuuint32_t box[3] = {128, 128, 1}, box16[3] = {128, 16, 1}, unit_box[2] = {256, kFp4Scales / 256};
     const cuuint64_t unit_strides[1] = {256};
-    const cuuint64_t unit_dims[2] = {256, (cuuint64_t)groups * m->tiles * stage / 256};
-    const cuuint64_t gated_dims[2] = {256, (cuuint64_t)groups * (apart ? m->halves : m->tiles) * stage / 256};
-    if (!encode(&m->map, m->codes, 3, dims, strides, box) ||
-        !encode(&m->units_map, m->units, 2, unit_dims, unit_strides, unit_box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
-        !encode(&m->gated_map, m->gated_units, 2, gated_dims, unit_strides, unit_box, CU_TENSOR_MAP_SWIZZLE_NONE))
+    const cuuint64_t unit_dims[2] = {256, (cuuint64_t)groups * m->units * stage / 256};
+    const cuuint64_t gated_dims[2] = {256, (cuuint64_t)groups * m->gated_units * stage / 256};
+    if (!encode(&m->map, m->codes, 3, dims, strides, box) || !encode(&m->map16, m->codes, 3, dims, strides, box16) ||
+        !encode(&m->scales_map, m->scales, 2, unit_dims, unit_strides, unit_box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        !encode(&m->gated_scales_map, f ? m->gated_scales : m->scales, 2, f ? gated_dims : unit_dims, unit_strides, unit_box,
+                CU_TENSOR_MAP_SWIZZLE_NONE))
         return bail(failf(QRM_E_CUDA, "%s: tensor map", what));
     *out = m;
     return QRM_OK;
 }
 
-// Which kernel a product takes: rows of x on the MMA's M side from 64 rows a group on.
-bool pair_is_faster(int64_t T, int groups, int64_t tiles_across, int steps, int sms) {
+enum Fp4Form { kSplit = 0, kPair = 1, kFit = 2 };
+
+// Which kernel a product takes.
+Fp4Form form_of(int64_t T, int groups) {
     const double used = (double)std::min<int64_t>(T, groups), rows = T / used;
-    return rows >= 64;
+    return rows < 64 ? kSplit : rows < 1024 ? kFit : kPair;
 }
 
 template <int MODE>
-cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, Fp4Params& p, bool pair, int wide_out, int64_t T, cudaStream_t s) {
-    if (pair)
-        return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, m->map,
-                            MODE == kFp4Plain ? m->units_map : m->gated_map, x_map, p, wide_out);
+cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, Fp4Params& p, Fp4Form form, int wide_out, int64_t T, cudaStream_t s) {
+    const CUtensorMap& w_map = MODE == kFp4Plain ? m->map : m->map16;
+    if (form == kFit)
+        return launch_ahead(fp4_fit_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, fit_smem(m->groups), s, w_map,
+                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_map, p, wide_out);
+    if (form == kPair)
+        return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, w_map,
+                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_map, p, wide_out);
     const int64_t across = MODE == kFp4Plain ? (p.M + 255) / 256 : (p.M + 127) / 128;
     const int64_t used = std::min<int64_t>(T, m->groups), per = (T / used + kFp4Rows - 1) / kFp4Rows;
     const int64_t tiles = used * per * across;
@@ -183,7 +193,7 @@ cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, Fp4Params& p, boo
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, fp4_split_kernel<MODE>, m->map, x_map, p, stages, x_rows);
+    return cudaLaunchKernelEx(&cfg, fp4_split_kernel<MODE>, w_map, x_map, p, stages, x_rows);
 }
 
 int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x, const uint8_t* xs, int64_t ld_xs,
@@ -220,15 +230,15 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     DeviceGuard here;
     cudaError_t e = here.enter(m->device);
     if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    const bool pair = m->form >= 0 ? m->form : pair_is_faster(T, m->groups, across, m->steps, m->sms);
+    const Fp4Form form = m->form >= 0 ? (Fp4Form)m->form : form_of(T, m->groups);
     const int wide_out = aligned(out, 16) && ld_out * b % 16 == 0;
     CUtensorMap x_map;
     const cuuint64_t dims[2] = {(cuuint64_t)(16 * blocks), (cuuint64_t)T};
     const cuuint64_t strides[1] = {(cuuint64_t)ld_x};
-    const cuuint32_t box[2] = {128, pair ? 128u : 16u};
+    const cuuint32_t box[2] = {128, form == kPair ? 128u : 16u};
     if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
     Fp4Params p{};
-    p.w_scales = mode == kFp4Plain ? m->units : m->gated_units;
+    p.w_scales = mode == kFp4Plain ? m->scales : m->gated_scales;
     p.x_scales = xs;
     p.offsets = offsets;
     p.out = out;
@@ -241,17 +251,16 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     p.T = (int)T;
     p.groups = m->groups;
     p.M = (int)M;
-    p.tiles = mode == kFp4Plain ? m->tiles : m->halves;
-    p.second = m->second;
+    p.units = mode == kFp4Plain ? m->units : m->gated_units;
     p.steps = m->steps;
     p.blocks = (int)blocks;
     p.type = type;
     p.row_tiles = (int)(offsets ? row_tiles : (T + kFp4Rows - 1) / kFp4Rows);
     p.wide_xs = aligned(xs, 16) && ld_xs % 16 == 0 ? 2 : aligned(xs, 8) && ld_xs % 8 == 0 ? 1 : 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, p, pair, wide_out, T, s)
-        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_map, p, pair, wide_out, T, s)
-                            : launch<kFp4GatedRows>(m, x_map, p, pair, wide_out, T, s);
+    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, p, form, wide_out, T, s)
+        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_map, p, form, wide_out, T, s)
+                            : launch<kFp4GatedRows>(m, x_map, p, form, wide_out, T, s);
     return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
 }
 

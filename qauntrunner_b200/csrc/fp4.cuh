@@ -15,7 +15,10 @@
 // values: row r's four bytes at 16 (r % 32) + 4 (r / 32), which tcgen05.cp
 // spreads over four columns.  A matrix's are laid out that way when it is made;
 // those of x stay as they are and are brought into that order on their way to
-// shared memory, because a group may start at any row.
+// shared memory, because a group may start at any row.  For the gated product
+// the matrix's rows enter the MMA in turns of 16: 16 of gate, the same 16 of up,
+// so that both halves of a feature are in the same 32 lanes of tensor memory (or
+// the same 32 columns), and its scales are kept in that order as well.
 #pragma once
 #include "pair_drain.h"
 #include "rows4.cuh"
@@ -31,7 +34,7 @@ constexpr int kFp4Scales = 1024;             // bytes of their scales
 enum Fp4Mode { kFp4Plain = 0, kFp4Gated = 1, kFp4GatedRows = 2 };   // y; h; h in 4-bit rows
 
 struct Fp4Params {
-    const uint8_t* w_scales;   // units [groups][tiles][steps][2][512]
+    const uint8_t* w_scales;   // [groups][units][steps][2][512]
     const uint8_t* x_scales;   // [T][ld_xs]
     const int32_t* offsets;    // [groups+1] rows of each group, or NULL (one group)
     void* out;                 // [T][ld_out], or codes (ld_out in bytes)
@@ -41,8 +44,7 @@ struct Fp4Params {
     float limit;
     int T, groups;
     int M;                     // outputs (gated: f)
-    int tiles;                 // of 128 rows in w_scales, of one matrix
-    int second;                // gated: the tile where up's begin
+    int units;                 // of 128 rows in w_scales, of one matrix (gated: 64 features)
     int steps;                 // stages of the contracted dimension
     int blocks;                // of 32 in it
     int type;                  // of out
@@ -84,6 +86,21 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
         asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
     else
         asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// 128 rows of a matrix's codes into a stage at `to`, by one thread: from row m
+// on, or (gated, f features) features m ... m + 63 of gate and up in turns of 16.
+// load(to, row): a box of the map's rows from there on.
+template <bool GATED, typename Load>
+__device__ __forceinline__ void load_weights(uint32_t to, int m, int f, Load load) {
+    if constexpr (!GATED) {
+        load(to, m);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            load(to + 4096 * q, m + 16 * q);
+            load(to + 4096 * q + 2048, f + m + 16 * q);
+        }
+    }
 }
 // what this thread wrote to shared memory is there for copies and MMAs
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -270,7 +287,8 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     }
     const WaitCtl ctl{abort_flag, p.err};
     const int k0 = (int)((long long)p.steps * rank / ranks), k1 = (int)((long long)p.steps * (rank + 1) / ranks);
-    const int m0 = block * (MODE == kFp4Plain ? 256 : 128);
+    constexpr int kBlock = MODE == kFp4Plain ? 128 : 64;   // outputs of a block
+    const int m0 = block * 2 * kBlock;
     const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), done0 = smem_u32(done);
     const int boxes = (t.n + 15) >> 4;
 
@@ -278,18 +296,18 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         // ------------------------------------------------ codes and the weights' scales
         Ring r;
         uint32_t n_issued = 0;
-        const long long units = (long long)t.group * p.tiles;
-        const int u0 = m0 >> 7, u1 = MODE == kFp4Plain ? min(u0 + 1, p.tiles - 1) : u0 + p.second;   // an absent second block is not stored
-        const uint8_t* s0 = p.w_scales + (units + u0) * p.steps * kFp4Scales;
-        const uint8_t* s1 = p.w_scales + (units + u1) * p.steps * kFp4Scales;
-        const int m1 = MODE == kFp4Plain ? m0 + 128 : p.M + m0;
+        const int u0 = m0 / kBlock, u1 = min(u0 + 1, p.units - 1);   // an absent second block is not stored
+        const uint8_t* s0 = p.w_scales + ((long long)t.group * p.units + u0) * p.steps * kFp4Scales;
+        const uint8_t* s1 = p.w_scales + ((long long)t.group * p.units + u1) * p.steps * kFp4Scales;
         for (int k = k0; k < k1; k++) {
             if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) break;
             uint8_t* st = ring + r.i * stage_bytes;
             if (elect_one()) {
                 mbar_arrive_expect_tx(&full[r.i], (uint32_t)(boxes * 2048 + 2 * kFp4Tile + 2 * kFp4Scales));
-                tma_load_3d(st + w_off, &w_map, k * 128, m0, t.group, &full[r.i]);
-                tma_load_3d(st + w_off + kFp4Tile, &w_map, k * 128, m1, t.group, &full[r.i]);
+                for (int b = 0; b < 2; b++)
+                    load_weights<MODE != kFp4Plain>(w_off + b * kFp4Tile, m0 + b * kBlock, p.M, [&](uint32_t to, int row) {
+                        tma_load_3d(st + to, &w_map, k * 128, row, t.group, &full[r.i]);
+                    });
                 bulk_g2s(st + ws_off, s0 + (size_t)k * kFp4Scales, kFp4Scales, &full[r.i]);
                 bulk_g2s(st + ws_off + kFp4Scales, s1 + (size_t)k * kFp4Scales, kFp4Scales, &full[r.i]);
                 for (int b = 0; b < boxes; b++) tma_load_2d(st + b * 2048, &x_map, k * 128, t.pos + 16 * b, &full[r.i]);
@@ -373,14 +391,15 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     constexpr int per_row = MODE == kFp4Plain ? 8 : 4;
     const uint32_t mine = smem_u32(sums);
     for (int i = rank + ranks * warp; i < t.n * per_row && !*abort_flag; i += ranks * (kFp4Threads / 32)) {
-        const int row = i / per_row, o = 32 * (i % per_row);
-        const uint32_t at = mine + 4 * (row * 256 + o + lane);
+        const int row = i / per_row, o = 32 * (i % per_row), j = o + lane;
+        // (gated: 16 of gate, 16 of up, and so on)
+        const uint32_t at = mine + 4 * (row * 256 + (MODE == kFp4Plain ? j : 2 * j - (j & 15)));
         float y = 0.f, up = 0.f;
 #pragma unroll
         for (int q = 0; q < 8; q++) {
             if (q >= (int)ranks) break;
             y += load_peer(at, q);
-            if (MODE != kFp4Plain) up += load_peer(at + 512, q);
+            if (MODE != kFp4Plain) up += load_peer(at + 64, q);
         }
         const long long to = t.pos + row;
         if (MODE == kFp4Plain) {
@@ -396,9 +415,8 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 
 // ------------------------------------------------------------ rows of x on the MMA's M side
 // For groups of many rows, which the tensor cores bound.  A pair of SMs
-// (cta_group::2) shares a tile of 256 rows of x times 256 outputs (gated: 128 of
-// gate, which the first CTA loads, and 128 of up): each CTA loads 128 rows of x
-// and 128 of the weights, 32 KB of codes for 256 contracted values, 64 bytes a
+// (cta_group::2) shares a tile of 256 rows of x times 256 outputs (gated: 128
+// features): each CTA loads 128 rows of x and 128 of the weights, 32 KB of codes for 256 contracted values, 64 bytes a
 // cycle at the full MMA rate.
 //
 // Tensor memory holds two accumulators of 256 columns but for the scales' 48
@@ -578,10 +596,9 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
                 const Tile t = tile_at(i);
-                // this CTA's half of the weights; both have all 256 outputs' scales
-                const int m = MODE == kFp4Plain ? t.m + 128 * (int)rank : t.m + p.M * (int)rank;
-                const int u = t.group * p.tiles + (t.m >> 7);
-                const int s0 = u * steps * 4, s1 = (u + (MODE == kFp4Plain ? 1 : p.second)) * steps * 4;
+                // this CTA's half of the weights; both have all scales
+                const int m = t.m + kOut / 2 * (int)rank;
+                const int s0 = (t.group * p.units + t.m / (kOut / 2)) * steps * 4, s1 = s0 + steps * 4;
                 for (int k = 0; k < steps; k++) {
                     if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
                     if (elect_one()) {
@@ -589,7 +606,9 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                         if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * kFp4PairTx);
                         // (no rows for this CTA: from past the end, which is zeros and no traffic)
                         tma_pair_2d(st, &x_map, k * 128, t.rows > 0 ? t.pos : p.T, bar);
-                        tma_pair_3d(st + kFp4Tile, &w_map, k * 128, m, t.group, bar);
+                        load_weights<MODE != kFp4Plain>(st + kFp4Tile, m, p.M, [&](uint32_t to, int row) {
+                            tma_pair_3d(to, &w_map, k * 128, row, t.group, bar);
+                        });
                         tma_pair_2d(st + 2 * kFp4Tile, &s_map, 0, s0 + 4 * k, bar);
                         tma_pair_2d(st + 2 * kFp4Tile + kFp4Scales, &s_map, 0, s1 + 4 * k, bar);
                     }
@@ -697,12 +716,11 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             if (!bar_wait(smem_u32(tile_done) + 8 * (n & 1), (n >> 1) & 1u, ctl)) break;
             tc_fence_after();
             const uint32_t from = taddr + (n & 1 ? kFp4PairSecond : 0);
-            float2 acc[64];   // 128 columns; gated: 64 of gate, the same of up
+            float2 acc[64];   // 128 columns
             if (t.rows > 32 * (warp & 3)) {
 #pragma unroll
                 for (int h = 0; h < 4; h++)
-                    tmem_ld32(from + (MODE == kFp4Plain ? 128 * half + 32 * h : 64 * half + 32 * (h & 1) + 128 * (h >> 1)),
-                              reinterpret_cast<float*>(acc + 16 * h));
+                    tmem_ld32(from + 128 * half + 32 * h, reinterpret_cast<float*>(acc + 16 * h));
             }
             tc_fence_before();
             __syncwarp();
@@ -719,7 +737,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                 } else {
                     float2 h[32];
 #pragma unroll
-                    for (int c = 0; c < 32; c++) h[c] = gated2(acc[c], acc[32 + c], p.limit);
+                    for (int c = 0; c < 32; c++) h[c] = gated2(acc[2 * c - (c & 7)], acc[2 * c - (c & 7) + 8], p.limit);
                     const int m = t.m + 64 * half;
                     const long long o = at * p.ld_out + m;
                     if (MODE == kFp4GatedRows) {
@@ -761,28 +779,425 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
+// ------------------------------------------------------------ pairs with weights on the MMA's M side
+// The same pair of SMs with the operands' places changed: 256 outputs (gated: 128
+// features) on the M side, up to 256 rows of x on the N side, rounded up to 32
+// only and shared evenly among a group's tiles.  Groups whose rows are no
+// multiple of 256 cost what their rows cost.
+//
+// A lane of tensor memory is an output, so rows go out by way of shared memory:
+// 32 rows of x at a time, [row][output] in f32, written by the lanes' columns and
+// read along the rows.  For the gated product the lanes of gate and of up
+// exchange half of their columns first, so that each has both sums of 16 rows.
+//
+// Warps: 0 loads codes and the weights' scales, 1 issues the MMAs (in the
+// pair's first CTA), 2 and 3 bring the scales of x (128 rows each, in both CTAs),
+// 4-7 and 8-11 write the output, every second 32 rows each.
+constexpr int kFp4FitStages = 5;
+constexpr int kFp4FitScalesW = 2 * kFp4Tile;                         // in a stage: codes of the weights, of x, scales
+constexpr int kFp4FitScalesX = kFp4FitScalesW + kFp4Scales;
+constexpr int kFp4FitStage = kFp4FitScalesX + 2 * kFp4Scales;
+constexpr int kFp4FitRoom = 32 * 132 * 4;      // four warps' room for 32 rows on their way out
+constexpr int kFp4FitRegsFew = 104, kFp4FitRegsMany = 200;
+constexpr int kFp4FitRegs = 128 * kFp4FitRegsFew + 256 * kFp4FitRegsMany;
+static_assert(kFp4FitRegs <= kFp4PairThreads * 168, "register split");
+
+// the first CTA's barriers, as drain_pair moves them on; the tiles' stages have different numbers of bytes
+struct Fp4FitBars {
+    uint64_t* full;
+    volatile uint32_t* bytes;   // a CTA's share of the stage that it issued last in each slot
+    __device__ uint32_t peer_bytes(uint32_t slot) const {
+        uint32_t a, v;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(a) : "r"(smem_u32(const_cast<uint32_t*>(&bytes[slot]))));
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+        return v;
+    }
+    __device__ void expect(uint32_t slot) { mbar_arrive_expect_tx(&full[slot], peer_bytes(slot)); }
+    __device__ void complete(uint32_t slot) {
+        asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[slot])), "r"(bytes[slot])
+                     : "memory");
+    }
+    __device__ void wait(uint32_t slot, uint32_t parity) { mbar_wait(&full[slot], parity); }
+};
+
+// whether it holds for all of `threads`, which meet here
+__device__ __forceinline__ bool all_of(int barrier, int threads, bool holds) {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(r)
+                 : "r"((uint32_t)holds), "r"(barrier), "r"(threads)
+                 : "memory");
+    return r != 0;
+}
+// eight outputs of a row, v, to out, of which `left` exist; wide: rows start on 16 bytes
+template <typename T>
+__device__ __forceinline__ void store_eight(T* out, int left, const float (&v)[8], bool wide) {
+    if (wide && left >= 8) {
+        uint4* to = reinterpret_cast<uint4*>(out);
+        if constexpr (sizeof(T) == 4) {
+            to[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+            to[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const T h[2] = {round_to<T>(v[2 * i]), round_to<T>(v[2 * i + 1])};
+                memcpy(&w[i], h, 4);
+            }
+            *to = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < left) out[i] = round_to<T>(v[i]);
+    }
+}
+// 32 rows of W outputs each (room: [row][pitch] f32) from output m of row t on, by 128 threads, of which `rows` and
+// `left` exist
+template <int W, typename T>
+__device__ __forceinline__ void room_out(const Fp4Params& p, const float* room, int pitch, long long t, int rows, int m, int left, int id,
+                                         bool wide) {
+    T* out = reinterpret_cast<T*>(p.out) + t * p.ld_out + m;
+    if (wide) {
+#pragma unroll
+        for (int j = 0; j < 32 * W / 8 / 128; j++) {
+            const int row = (id + 128 * j) / (W / 8), o = (id + 128 * j) % (W / 8) * 8;
+            const float4* from = reinterpret_cast<const float4*>(room + row * pitch + o);
+            const float4 a = from[0], b = from[1];
+            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            if (row < rows) store_eight(out + row * p.ld_out + o, left - o, v, true);
+        }
+    } else {   // neighbouring lanes write neighbouring outputs
+        for (int j = id; j < W * min(rows, 32); j += 128)
+            if (j % W < left) out[j / W * p.ld_out + j % W] = round_to<T>(room[j / W * pitch + j % W]);
+    }
+}
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp4PairThreads, 1)
+fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap s_map,
+               const __grid_constant__ CUtensorMap x_map, const __grid_constant__ Fp4Params p, int wide_out) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // first CTA: both CTAs' copies are there
+    uint64_t* x_full = full + kFp4FitStages;            // first CTA: both CTAs' scales of x are there
+    uint64_t* done = x_full + kFp4FitStages;            // both: the stage's MMAs are done
+    uint64_t* tile_done = done + kFp4FitStages;         // [2] both: a tile's are
+    uint64_t* tile_read = tile_done + 2;                // [2] first CTA: both epilogues have read an accumulator
+    uint64_t* done_bar = tile_read + 2;
+    uint64_t* left_bar = done_bar + 1;                  // both, when the first CTA gave up: its commits are through
+    __shared__ volatile int given_up;
+    __shared__ volatile uint32_t from_peer, issued;     // issued: stages, once their warp is through
+    __shared__ volatile uint32_t bytes[kFp4FitStages];
+    volatile int* abort_flag = &given_up;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 776);
+    int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp4PairTableOff);
+    int32_t* start = first_tile + p.groups + 1;
+    int32_t* rows = start + p.groups + 1;
+    uint8_t* ring = sm + fp4_pair_stage_off(p.groups);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x & 1;   // in the pair: the cluster is two CTAs along x
+    constexpr int kHalf = MODE == kFp4Plain ? 128 : 64;   // outputs of a CTA in a tile
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kFp4FitStages; i++) {
+            mbar_init(&full[i], 1);
+            mbar_init(&x_full[i], 4);
+            mbar_init(&done[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&tile_done[i], 1);
+            mbar_init(&tile_read[i], 16);
+        }
+        mbar_init(done_bar, 1);
+        mbar_init(left_bar, 1);
+        *abort_flag = 0;
+        issued = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    pdl_start();   // nothing before this reads or writes global memory
+    if (warp == 2) group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows, 256, (p.M + 2 * kHalf - 1) / (2 * kHalf), blockIdx.x == 0);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();   // the peer's barriers are ready
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const WaitCtl ctl{abort_flag, p.err};
+    const uint32_t done0 = smem_u32(done);
+    const int tiles = first_tile[p.groups], pairs = gridDim.x >> 1, steps = p.steps;
+
+    struct Tile {
+        int group, m;      // matrix, first output of the pair
+        int pos, n;        // first row of x, rows
+        int cols;          // n in whole 32s: columns of the accumulator
+    };
+    // the tiles of one block of outputs follow each other, so its weights come from HBM once
+    auto tile_at = [&](int i) {
+        int lo = 0, hi = p.groups;   // the last group with first_tile <= i has rows
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first_tile[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        const int blocks = (rows[lo] + 255) >> 8, in = i - first_tile[lo], m = in / blocks;
+        const int per = ((rows[lo] + blocks - 1) / blocks + 31) & ~31, at = (in - m * blocks) * per, n = min(per, rows[lo] - at);
+        return Tile{lo, m * 2 * kHalf, start[lo] + at, n, (n + 31) & ~31};
+    };
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp4FitRegsFew));
+        if (warp == 0) {
+            // -------------------------------------------- codes and the weights' scales
+            bool ok = true;
+            Ring r;
+            uint32_t n_issued = 0;
+            const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
+                const Tile t = tile_at(i);
+                const int m = t.m + kHalf * (int)rank, boxes = t.cols >> 5, pos = t.pos + (t.cols >> 1) * (int)rank;
+                const int s0 = (t.group * p.units + m / kHalf) * steps * 4;
+                const uint32_t share = kFp4Tile + boxes * 2048 + kFp4Scales;
+                for (int k = 0; k < steps; k++) {
+                    if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                    if (elect_one()) {
+                        const uint32_t st = ring0 + r.i * kFp4FitStage, bar = full0 + 8 * r.i;
+                        bytes[r.i] = share;
+                        if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * share);
+                        load_weights<MODE != kFp4Plain>(st, m, p.M, [&](uint32_t to, int row) {
+                            tma_pair_3d(to, &w_map, k * 128, row, t.group, bar);
+                        });
+                        tma_pair_2d(st + kFp4FitScalesW, &s_map, 0, s0 + 4 * k, bar);
+                        for (int b = 0; b < boxes; b++) tma_pair_2d(st + kFp4Tile + b * 2048, &x_map, k * 128, pos + 16 * b, bar);
+                    }
+                    __syncwarp();
+                    r.next(kFp4FitStages);
+                    n_issued++;
+                }
+            }
+            if (lane == 0) issued = n_issued;
+        } else if (warp == 1 && rank == 0) {
+            // -------------------------------------------- MMAs (one thread issues for both CTAs)
+            bool ok = true;
+            Ring r;
+            uint32_t n = 0, buffer = 0;   // tiles; of scales
+            int before = 0;               // columns of the tile before
+            const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), ring0 = smem_u32(ring), read0 = smem_u32(tile_read);
+            const uint64_t w_desc = sw128_desc(ring0), x_desc = sw128_desc(ring0 + kFp4Tile);
+            const uint64_t ws_desc = scale_desc(ring0 + kFp4FitScalesW), xs_desc = scale_desc(ring0 + kFp4FitScalesX);
+            const uint32_t odd = umma_idesc_mxf4(0, 0, 2) & ~umma_idesc_mxf4(0, 0, 0);
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs, n++) {
+                const Tile t = tile_at(i);
+                const uint32_t a = n & 1, d = tmem + (a ? kFp4PairSecond : 0), idesc = umma_idesc_mxf4(256, t.cols, 0);
+                // this accumulator has been read, and the other one where the two overlap
+                if (n > 1 && !bar_wait(read0 + 8 * a, ((n >> 1) - 1) & 1u, ctl)) break;
+                if (n > 0 && (a ? before : t.cols) > kFp4PairSecond && !bar_wait(read0 + 8 * (a ^ 1), ((n - 1) >> 1) & 1u, ctl)) break;
+                before = t.cols;
+                for (int k = 0; k < steps; k++) {
+                    if (!bar_wait(full0 + 8 * r.i, r.phase, ctl) || !bar_wait(x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint32_t at = r.i * (kFp4FitStage >> 4);
+                        const uint32_t ws = tmem + kFp4PairTmemScales + kFp4ScaleCols * buffer, xs = ws + 8;
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {   // half of the stage's contracted values
+                            scales_to_tmem<2>(ws + 4 * u, ws_desc + at + u * (512 >> 4));
+                            scales_to_tmem<2>(xs + 8 * u, xs_desc + at + u * (512 >> 4));
+                            if (t.cols > 128) scales_to_tmem<2>(xs + 8 * u + 4, xs_desc + at + (kFp4Scales + u * 512 >> 4));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            umma_mxf4<2>(d, w_desc + at + 2 * j, x_desc + at + 2 * j, j & 1 ? idesc | odd : idesc, ws + 4 * (j >> 1),
+                                         xs + 8 * (j >> 1), k > 0 || j > 0);
+                        umma_commit_pair(done0 + 8 * r.i);
+                        if (k + 1 == steps) umma_commit_pair(smem_u32(tile_done) + 8 * a);
+                    }
+                    __syncwarp();
+                    r.next(kFp4FitStages);
+                    buffer ^= 1;
+                }
+            }
+            // every MMA has completed before tensor memory is released
+            if (elect_one()) {
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done_bar)) : "memory");
+                mbar_wait(done_bar, 0u);
+            }
+            __syncwarp();
+        } else if (warp >= 2) {
+            // -------------------------------------------- scales of x: rows 128 (warp - 2) + lane, + 32, + 64, + 96 of the tile
+            // (as in fp4_pair_kernel: four stages' at a time, the next four's on their way)
+            bool ok = true;
+            Ring r;
+            const int first = 128 * (warp - 2) + lane;
+            const uint32_t x_full0 = map_to_rank0(smem_u32(x_full));
+            uint4 next[4][2];   // [row][half]
+            auto load = [&](const Tile& t, int k) {
+                const uint8_t* row = p.x_scales + (long long)(t.pos + first) * p.ld_xs;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const bool in = first + 32 * c < t.n;
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        next[c][h] = in ? sixteen_scales(row + 32 * c * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
+                }
+            };
+            int i = blockIdx.x >> 1;
+            if (i < tiles) load(tile_at(i), 0);
+            for (; i < tiles && ok; i += pairs) {
+                const Tile t = tile_at(i);
+                for (int k4 = 0; k4 < steps && ok; k4 += 4) {
+                    uint4 now[4][2];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) { now[c][0] = next[c][0]; now[c][1] = next[c][1]; }
+                    if (k4 + 4 < steps) load(t, k4 + 4);
+                    else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (k4 + j >= steps) break;
+                        if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                        if (t.cols > 128 * (warp - 2)) {
+                            uint4* to = reinterpret_cast<uint4*>(ring + r.i * kFp4FitStage + kFp4FitScalesX + kFp4Scales * (warp - 2)) + lane;
+                            const uint4 a = now[0][j >> 1], b = now[1][j >> 1], c = now[2][j >> 1], d = now[3][j >> 1];
+                            to[0] = j & 1 ? make_uint4(a.z, b.z, c.z, d.z) : make_uint4(a.x, b.x, c.x, d.x);
+                            to[32] = j & 1 ? make_uint4(a.w, b.w, c.w, d.w) : make_uint4(a.y, b.y, c.y, d.y);
+                            fence_async();
+                        }
+                        __syncwarp();
+                        if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
+                        r.next(kFp4FitStages);
+                    }
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------ output
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp4FitRegsMany));
+        const int half = (warp - 4) >> 2, quarter = warp & 3, id = 32 * quarter + lane;   // (warps 4-7, 8-11: quarters 0-3)
+        const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16), read0 = map_to_rank0(smem_u32(tile_read));
+        float* room = reinterpret_cast<float*>(ring + kFp4FitStages * kFp4FitStage + half * kFp4FitRoom);
+        constexpr int kPitch = MODE == kFp4Plain ? 132 : 80;   // floats of a row there (the lanes' banks differ)
+        uint32_t n = 0;
+        for (int i = blockIdx.x >> 1; i < tiles; i += pairs, n++) {
+            const Tile t = tile_at(i);
+            // (one of the four warps that gives up takes the others along: they meet at barriers from here on)
+            if (!all_of(1 + half, 128, bar_wait(smem_u32(tile_done) + 8 * (n & 1), (n >> 1) & 1u, ctl))) break;
+            tc_fence_after();
+            const uint32_t from = taddr + (n & 1 ? kFp4PairSecond : 0);
+            float acc[4][32];   // 32 rows of x of this lane's output, every second 32
+#pragma unroll
+            for (int h = 0; h < 4; h++)
+                if (64 * h + 32 * half < t.cols) tmem_ld32(from + 64 * h + 32 * half, acc[h]);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive_cluster(read0 + 8 * (n & 1));
+            const int m = t.m + kHalf * (int)rank, left = p.M - m;
+#pragma unroll
+            for (int h = 0; h < 4; h++) {
+                const int at = 64 * h + 32 * half, have = t.n - at;   // (the same for all four warps)
+                if (have <= 0) break;
+                float (&v)[32] = acc[h];
+                named_barrier(1 + half, 128);   // what was in the room is out
+                if (MODE == kFp4Plain) {
+#pragma unroll
+                    for (int c = 0; c < 32; c++) room[c * kPitch + id] = v[c];
+                } else {
+                    const bool up = lane & 16;
+                    float* to = room + (up ? kPitch : 0) + 16 * quarter + (lane & 15);
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {   // gate's lanes take rows c and c + 2, up's c + 1 and c + 3
+                        const float g0 = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 16);
+                        const float g1 = __shfl_xor_sync(0xffffffffu, up ? v[c + 2] : v[c + 3], 16);
+                        const float2 mine = up ? make_float2(v[c + 1], v[c + 3]) : make_float2(v[c], v[c + 2]);
+                        const float2 other = make_float2(g0, g1);
+                        const float2 y = gated2(up ? other : mine, up ? mine : other, p.limit);
+                        to[c * kPitch] = y.x;
+                        to[(c + 2) * kPitch] = y.y;
+                    }
+                }
+                named_barrier(1 + half, 128);   // 32 rows are there
+                const long long row = t.pos + at;
+                if (MODE == kFp4GatedRows) {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {   // eight features a lane, four lanes a block
+                        const int r = (id + 128 * j) >> 3, o = (id & 7) * 8;
+                        const float4* f = reinterpret_cast<const float4*>(room + r * kPitch + o);
+                        const float4 a = f[0], b = f[1];
+                        float e[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            if (o + k >= left) e[k] = 0.f;
+                            top = max(top, magnitude(e[k]));
+                        }
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                        const uint32_t scale = fp4_scale(top), q = e2m1x8(e, scale);
+                        if (r < have && o / kFp4Block * kFp4Block < left) {
+                            *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (row + r) * p.ld_out + (m + o) / 2) = q;
+                            if ((id & 3) == 0) p.out_scales[(row + r) * p.ld_os + (m + o) / kFp4Block] = (uint8_t)scale;
+                        }
+                    }
+                } else if (p.type == 0) {
+                    room_out<kHalf, float>(p, room, kPitch, row, have, m, left, id, wide_out);
+                } else if (p.type == 1) {
+                    room_out<kHalf, __half>(p, room, kPitch, row, have, m, left, id, wide_out);
+                } else {
+                    room_out<kHalf, __nv_bfloat16>(p, room, kPitch, row, have, m, left, id, wide_out);
+                }
+            }
+        }
+    }
+    // ---------------- teardown: every role of both CTAs is done (or gave up); free tensor memory
+    tc_fence_before();
+    __syncthreads();
+    // (as in fp8_pair_kernel: the first CTA learns how many stages the other has issued, which learns whether to stay)
+    if (threadIdx.x == 0) store_peer(const_cast<uint32_t*>(&from_peer), rank ^ 1, rank == 0 ? (uint32_t)given_up : issued);
+    __syncwarp();
+    cluster_sync_all();
+    tc_fence_after();
+    if (rank == 0 ? given_up != 0 : from_peer != 0) {
+        if (rank == 0 && threadIdx.x == 0) {
+            Fp4FitBars bars{full, bytes};
+            drain_pair(issued, from_peer, kFp4FitStages, bars);
+        }
+        if (warp == 1) {
+            if (rank == 0 && elect_one()) umma_commit_pair(smem_u32(left_bar));
+            __syncwarp();
+            if (lane == 0) mbar_wait(left_bar, 0u);
+        }
+        __syncwarp();
+        cluster_sync_all();
+    }
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
 // ------------------------------------------------------------ a matrix's scales into units
-// scales [groups][rows][blocks] of 32 columns -> [groups][tiles][steps][2][512];
-// tile i holds rows 128 i ... of the first `split` rows, and those from split on
-// begin with tile `second` (split = rows: there are none).  What does not exist
-// is 0.
-__global__ void fp4_scale_units_kernel(const uint8_t* __restrict__ scales, int rows, int blocks, int split, int tiles, int second,
-                                       int steps, uint32_t* __restrict__ units) {
+// scales [groups][rows][blocks] of 32 columns -> [groups][units][steps][2][512];
+// unit i holds rows 128 i ... (f = 0), or of a gated matrix's f features 64 i ...
+// those of gate and up in turns of 16.  What does not exist is 0.
+__global__ void fp4_scale_units_kernel(const uint8_t* __restrict__ scales, int rows, int blocks, int f, int units, int steps,
+                                       uint32_t* __restrict__ out) {
     pdl_start();
-    // a word: four scales of one row; blockIdx.z: matrix, y: tile, x: unit of 128 words along the contracted dimension
-    const int lane = threadIdx.x, q = lane & 3, l = lane >> 2;
-    const int tile = blockIdx.y, in = 128 * (tile < second ? tile : tile - second) + 32 * q + l;
-    const int row = tile < second ? (in < split ? in : -1) : (split + in < rows ? split + in : -1);
+    // a word: four scales of one row; blockIdx.z: matrix, y: unit, x: its 128 words along the contracted dimension
+    const int word = threadIdx.x, r = 32 * (word & 3) + (word >> 2);
+    int row = 128 * blockIdx.y + r;
+    if (f) {
+        const int feature = 64 * blockIdx.y + 16 * (r >> 5) + (r & 15);
+        row = feature < f ? feature + (r & 16 ? f : 0) : rows;
+    }
     const size_t g = blockIdx.z;
     uint32_t w = 0;
-    if (row >= 0) {
+    if (row < rows) {
         const uint8_t* from = scales + (g * rows + row) * blocks;
         for (int i = 0; i < 4; i++) {
             const int b = 4 * blockIdx.x + i;
             if (b < blocks) w |= (uint32_t)from[b] << (8 * i);
         }
     }
-    units[((g * tiles + tile) * 2 * steps + blockIdx.x) * 128 + lane] = w;
+    out[((g * units + blockIdx.y) * 2 * steps + blockIdx.x) * 128 + word] = w;
 }
 // codes past the last column of a row are 0: cols of them, in whole blocks of 32
 __global__ void fp4_clear_tail_kernel(uint8_t* codes, long long rows, int cols, int pitch) {
