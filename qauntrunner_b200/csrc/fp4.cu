@@ -22,8 +22,8 @@ struct qrm_fp4 {
     uint8_t* scales = nullptr;           // [groups][units][steps][2][512]
     uint8_t* gated_scales = nullptr;     // [groups][gated_units][steps][2][512]
     int32_t* err = nullptr;
-    // codes in boxes of 256 columns x 128 and 16 rows; scales in boxes of a unit's for one stage
-    CUtensorMap map, map16, scales_map, gated_scales_map;
+    // codes in boxes of 256 columns x 128 rows (gated: 64 features, in turns of 16); scales in boxes of a unit's for one stage
+    CUtensorMap map, gated_map, scales_map, gated_scales_map;
 };
 
 namespace {
@@ -103,7 +103,8 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     // one allocation: codes, scales in both orders, the error flags
     auto up = [](size_t n) { return (n + 255) / 256 * 256; };
     const size_t stage = (size_t)m->steps * kFp4Scales, pitch = (size_t)blocks * 16;
-    const size_t scales_at = up(code_bytes), gated_at = scales_at + (size_t)groups * m->units * stage;
+    // (the gated map's last sixteen features may reach 15 rows past the last matrix)
+    const size_t scales_at = up(code_bytes + 16 * pitch), gated_at = scales_at + (size_t)groups * m->units * stage;
     const size_t err_at = gated_at + (size_t)groups * m->gated_units * stage;
     uint8_t* staged = nullptr;   // the scales as they came, until they are in units
     if (cudaMalloc(&m->codes, err_at + 256) != cudaSuccess || cudaMalloc(&staged, scale_bytes) != cudaSuccess) {
@@ -141,14 +142,15 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
         return bail(failf(QRM_E_CUDA, "%s: built with too few registers a thread for their split", what));
     const cuuint64_t dims[3] = {(cuuint64_t)pitch, (cuuint64_t)rows, (cuuint64_t)groups};
     const cuuint64_t strides[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
-    const cuuint32_t box[3] = {128, 128, 1}, box16[3] = {128, 16, 1}, unit_box[2] = {256, kFp4Scales / 256};
+    const cuuint32_t box[3] = {128, 128, 1}, gated_box[5] = {128, 16, 2, 4, 1}, unit_box[2] = {256, kFp4Scales / 256};
+    const cuuint64_t by_gate[5] = {(cuuint64_t)pitch, 16, 2, (cuuint64_t)(f + 15) / 16, (cuuint64_t)groups};
+    const cuuint64_t by_gate_strides[4] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * f), (cuuint64_t)(pitch * 16), (cuuint64_t)(pitch * rows)};
     const cuuint64_t unit_strides[1] = {256};
     const cuuint64_t unit_dims[2] = {256, (cuuint64_t)groups * m->units * stage / 256};
     const cuuint64_t gated_dims[2] = {256, (cuuint64_t)groups * m->gated_units * stage / 256};
-    if (!encode(&m->map, m->codes, 3, dims, strides, box) || !encode(&m->map16, m->codes, 3, dims, strides, box16) ||
+    if (!encode(&m->map, m->codes, 3, dims, strides, box) || (f && !encode(&m->gated_map, m->codes, 5, by_gate, by_gate_strides, gated_box)) ||
         !encode(&m->scales_map, m->scales, 2, unit_dims, unit_strides, unit_box, CU_TENSOR_MAP_SWIZZLE_NONE) ||
-        !encode(&m->gated_scales_map, f ? m->gated_scales : m->scales, 2, f ? gated_dims : unit_dims, unit_strides, unit_box,
-                CU_TENSOR_MAP_SWIZZLE_NONE))
+        (f && !encode(&m->gated_scales_map, m->gated_scales, 2, gated_dims, unit_strides, unit_box, CU_TENSOR_MAP_SWIZZLE_NONE)))
         return bail(failf(QRM_E_CUDA, "%s: tensor map", what));
     *out = m;
     return QRM_OK;
@@ -163,14 +165,14 @@ Fp4Form form_of(int64_t T, int groups) {
 }
 
 template <int MODE>
-cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, Fp4Params& p, Fp4Form form, int wide_out, int64_t T, cudaStream_t s) {
-    const CUtensorMap& w_map = MODE == kFp4Plain ? m->map : m->map16;
+cudaError_t launch(const qrm_fp4* m, const Fp4RowMaps& x_maps, Fp4Params& p, Fp4Form form, int wide_out, int64_t T, cudaStream_t s) {
+    const CUtensorMap& w_map = MODE == kFp4Plain ? m->map : m->gated_map;
     if (form == kFit)
         return launch_ahead(fp4_fit_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, fit_smem(m->groups), s, w_map,
-                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_map, p, wide_out);
+                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps, p, wide_out);
     if (form == kPair)
         return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, w_map,
-                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_map, p, wide_out);
+                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps.rows[3], p, wide_out);
     const int64_t across = MODE == kFp4Plain ? (p.M + 255) / 256 : (p.M + 127) / 128;
     const int64_t used = std::min<int64_t>(T, m->groups), per = (T / used + kFp4Rows - 1) / kFp4Rows;
     const int64_t tiles = used * per * across;
@@ -193,7 +195,7 @@ cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, Fp4Params& p, Fp4
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, fp4_split_kernel<MODE>, w_map, x_map, p, stages, x_rows);
+    return cudaLaunchKernelEx(&cfg, fp4_split_kernel<MODE>, w_map, x_maps.rows[0], p, stages, x_rows);
 }
 
 int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x, const uint8_t* xs, int64_t ld_xs,
@@ -232,11 +234,14 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
     const Fp4Form form = m->form >= 0 ? (Fp4Form)m->form : form_of(T, m->groups);
     const int wide_out = aligned(out, 16) && ld_out * b % 16 == 0;
-    CUtensorMap x_map;
+    Fp4RowMaps x_maps;
     const cuuint64_t dims[2] = {(cuuint64_t)(16 * blocks), (cuuint64_t)T};
     const cuuint64_t strides[1] = {(cuuint64_t)ld_x};
-    const cuuint32_t box[2] = {128, form == kPair ? 128u : 16u};
-    if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
+    for (int i = 0; i < 4; i++) {   // the boxes that the kernel loads
+        const cuuint32_t box[2] = {128, 16u << i};
+        if ((form == kFit || i == (form == kPair ? 3 : 0)) && !encode(&x_maps.rows[i], x, 2, dims, strides, box))
+            return failf(QRM_E_CUDA, "%s: tensor map", what);
+    }
     Fp4Params p{};
     p.w_scales = mode == kFp4Plain ? m->scales : m->gated_scales;
     p.x_scales = xs;
@@ -258,9 +263,9 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     p.row_tiles = (int)(offsets ? row_tiles : (T + kFp4Rows - 1) / kFp4Rows);
     p.wide_xs = aligned(xs, 16) && ld_xs % 16 == 0 ? 2 : aligned(xs, 8) && ld_xs % 8 == 0 ? 1 : 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, p, form, wide_out, T, s)
-        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_map, p, form, wide_out, T, s)
-                            : launch<kFp4GatedRows>(m, x_map, p, form, wide_out, T, s);
+    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_maps, p, form, wide_out, T, s)
+        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_maps, p, form, wide_out, T, s)
+                            : launch<kFp4GatedRows>(m, x_maps, p, form, wide_out, T, s);
     return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
 }
 

@@ -87,20 +87,28 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t taddr, uint64_t desc) {
     else
         asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-// 128 rows of a matrix's codes into a stage at `to`, by one thread: from row m
-// on, or (gated, f features) features m ... m + 63 of gate and up in turns of 16.
-// load(to, row): a box of the map's rows from there on.
-template <bool GATED, typename Load>
-__device__ __forceinline__ void load_weights(uint32_t to, int m, int f, Load load) {
-    if constexpr (!GATED) {
-        load(to, m);
-    } else {
-#pragma unroll
-        for (int q = 0; q < 4; q++) {
-            load(to + 4096 * q, m + 16 * q);
-            load(to + 4096 * q + 2048, f + m + 16 * q);
-        }
-    }
+// 128 rows of a matrix's codes into shared memory: from row m on, or (gated)
+// features m ... m + 63 of gate and up in turns of 16, which the matrix's map has
+// as dimensions of their own: 16 rows, gate or up, sixteens of features.
+template <bool GATED>
+__device__ __forceinline__ void load_weights(void* dst, const CUtensorMap* map, int x, int m, int group, uint64_t* bar) {
+    if constexpr (!GATED) tma_load_3d(dst, map, x, m, group, bar);
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %5, %5, %3, %4}], "
+            "[%6];" ::"r"(smem_u32(dst)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(m >> 4), "r"(group), "r"(0), "r"(smem_u32(bar))
+            : "memory");
+}
+template <bool GATED>
+__device__ __forceinline__ void load_weights_pair(uint32_t dst, const CUtensorMap* map, int x, int m, int group, uint32_t bar) {
+    if constexpr (!GATED) tma_pair_3d(dst, map, x, m, group, bar);
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %5, %5, "
+            "%3, %4}], [%6];" ::"r"(dst),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(m >> 4), "r"(group), "r"(0), "r"(bar)
+            : "memory");
 }
 // what this thread wrote to shared memory is there for copies and MMAs
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -305,9 +313,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
             if (elect_one()) {
                 mbar_arrive_expect_tx(&full[r.i], (uint32_t)(boxes * 2048 + 2 * kFp4Tile + 2 * kFp4Scales));
                 for (int b = 0; b < 2; b++)
-                    load_weights<MODE != kFp4Plain>(w_off + b * kFp4Tile, m0 + b * kBlock, p.M, [&](uint32_t to, int row) {
-                        tma_load_3d(st + to, &w_map, k * 128, row, t.group, &full[r.i]);
-                    });
+                    load_weights<MODE != kFp4Plain>(st + w_off + b * kFp4Tile, &w_map, k * 128, m0 + b * kBlock, t.group, &full[r.i]);
                 bulk_g2s(st + ws_off, s0 + (size_t)k * kFp4Scales, kFp4Scales, &full[r.i]);
                 bulk_g2s(st + ws_off + kFp4Scales, s1 + (size_t)k * kFp4Scales, kFp4Scales, &full[r.i]);
                 for (int b = 0; b < boxes; b++) tma_load_2d(st + b * 2048, &x_map, k * 128, t.pos + 16 * b, &full[r.i]);
@@ -606,9 +612,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                         if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * kFp4PairTx);
                         // (no rows for this CTA: from past the end, which is zeros and no traffic)
                         tma_pair_2d(st, &x_map, k * 128, t.rows > 0 ? t.pos : p.T, bar);
-                        load_weights<MODE != kFp4Plain>(st + kFp4Tile, m, p.M, [&](uint32_t to, int row) {
-                            tma_pair_3d(to, &w_map, k * 128, row, t.group, bar);
-                        });
+                        load_weights_pair<MODE != kFp4Plain>(st + kFp4Tile, &w_map, k * 128, m, t.group, bar);
                         tma_pair_2d(st + 2 * kFp4Tile, &s_map, 0, s0 + 4 * k, bar);
                         tma_pair_2d(st + 2 * kFp4Tile + kFp4Scales, &s_map, 0, s1 + 4 * k, bar);
                     }
@@ -802,6 +806,9 @@ constexpr int kFp4FitRegsFew = 104, kFp4FitRegsMany = 200;
 constexpr int kFp4FitRegs = 128 * kFp4FitRegsFew + 256 * kFp4FitRegsMany;
 static_assert(kFp4FitRegs <= kFp4PairThreads * 168, "register split");
 
+struct Fp4RowMaps {
+    CUtensorMap rows[4];   // x in boxes of 256 columns x 16, 32, 64 and 128 rows
+};
 // the first CTA's barriers, as drain_pair moves them on; the tiles' stages have different numbers of bytes
 struct Fp4FitBars {
     uint64_t* full;
@@ -876,7 +883,7 @@ __device__ __forceinline__ void room_out(const Fp4Params& p, const float* room, 
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp4PairThreads, 1)
 fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap s_map,
-               const __grid_constant__ CUtensorMap x_map, const __grid_constant__ Fp4Params p, int wide_out) {
+               const __grid_constant__ Fp4RowMaps x_maps, const __grid_constant__ Fp4Params p, int wide_out) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // first CTA: both CTAs' copies are there
@@ -958,20 +965,23 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
                 const Tile t = tile_at(i);
-                const int m = t.m + kHalf * (int)rank, boxes = t.cols >> 5, pos = t.pos + (t.cols >> 1) * (int)rank;
+                const int m = t.m + kHalf * (int)rank, mine = t.cols >> 1, pos = t.pos + mine * (int)rank;
                 const int s0 = (t.group * p.units + m / kHalf) * steps * 4;
-                const uint32_t share = kFp4Tile + boxes * 2048 + kFp4Scales;
+                const uint32_t share = kFp4Tile + mine * 128 + kFp4Scales;
                 for (int k = 0; k < steps; k++) {
                     if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
                     if (elect_one()) {
                         const uint32_t st = ring0 + r.i * kFp4FitStage, bar = full0 + 8 * r.i;
                         bytes[r.i] = share;
                         if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * share);
-                        load_weights<MODE != kFp4Plain>(st, m, p.M, [&](uint32_t to, int row) {
-                            tma_pair_3d(to, &w_map, k * 128, row, t.group, bar);
-                        });
+                        load_weights_pair<MODE != kFp4Plain>(st, &w_map, k * 128, m, t.group, bar);
                         tma_pair_2d(st + kFp4FitScalesW, &s_map, 0, s0 + 4 * k, bar);
-                        for (int b = 0; b < boxes; b++) tma_pair_2d(st + kFp4Tile + b * 2048, &x_map, k * 128, pos + 16 * b, bar);
+                        // (a box for each power of two in the number of rows: 16 rows a box cost more to issue than to load)
+                        for (int b = 0, at = 0; b < 4; b++)
+                            if (mine >> b & 16) {
+                                tma_pair_2d(st + kFp4Tile + 128 * at, &x_maps.rows[b], k * 128, pos + at, bar);
+                                at += 16 << b;
+                            }
                     }
                     __syncwarp();
                     r.next(kFp4FitStages);
