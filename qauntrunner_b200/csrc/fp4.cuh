@@ -666,13 +666,13 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             __syncwarp();
         } else if (warp >= 2) {
             // -------------------------------------------- scales of x: rows 64 (warp - 2) + lane and + 32 of the CTA's
-            // Four stages' at a time, and the next four's are on their way while these are handed out: a load's way is
-            // longer than a stage.
+            // Four stages' at a time.  The next four's are asked for behind the last of these: a fence waits for loads that
+            // are on their way, and with these ahead of it cost up to a quarter of the time.
             bool ok = true;
             Ring r;
             const int first = 64 * (warp - 2) + lane;
             const uint32_t x_full0 = map_to_rank0(smem_u32(x_full));
-            uint4 next[2][2];   // [row][half]
+            uint4 four[2][2];   // [row][half]
             auto load = [&](const Tile& t, int k) {
                 const uint8_t* row = p.x_scales + (long long)(t.pos + first) * p.ld_xs;
 #pragma unroll
@@ -680,7 +680,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                     const bool in = first + 32 * c < t.rows;
 #pragma unroll
                     for (int h = 0; h < 2; h++)
-                        next[c][h] = in ? sixteen_scales(row + 32 * c * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
+                        four[c][h] = in ? sixteen_scales(row + 32 * c * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
                 }
             };
             int i = blockIdx.x >> 1;
@@ -688,13 +688,10 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             for (; i < tiles && ok; i += pairs) {
                 const Tile t = tile_at(i);
                 for (int k4 = 0; k4 < steps && ok; k4 += 4) {
-                    const uint4 a0 = next[0][0], a1 = next[0][1], b0 = next[1][0], b1 = next[1][1];
-                    if (k4 + 4 < steps) load(t, k4 + 4);
-                    else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         if (k4 + j >= steps) break;
-                        const uint4 a = j < 2 ? a0 : a1, b = j < 2 ? b0 : b1;
+                        const uint4 a = four[0][j >> 1], b = four[1][j >> 1];
                         if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
                         uint2* to = reinterpret_cast<uint2*>(ring + r.i * kFp4PairStage + kFp4PairTx) + 2 * lane + (warp - 2);
                         to[0] = j & 1 ? make_uint2(a.z, b.z) : make_uint2(a.x, b.x);
@@ -704,6 +701,8 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                         if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
                         r.next(kFp4PairStages);
                     }
+                    if (k4 + 4 < steps) load(t, k4 + 4);
+                    else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
                 }
             }
         }
@@ -1038,12 +1037,12 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             __syncwarp();
         } else if (warp >= 2) {
             // -------------------------------------------- scales of x: rows 128 (warp - 2) + lane, + 32, + 64, + 96 of the tile
-            // (as in fp4_pair_kernel: four stages' at a time, the next four's on their way)
+            // (as in fp4_pair_kernel: four stages' at a time, the next four's asked for behind the last of these)
             bool ok = true;
             Ring r;
             const int first = 128 * (warp - 2) + lane;
             const uint32_t x_full0 = map_to_rank0(smem_u32(x_full));
-            uint4 next[4][2];   // [row][half]
+            uint4 four[4][2];   // [row][half]
             auto load = [&](const Tile& t, int k) {
                 const uint8_t* row = p.x_scales + (long long)(t.pos + first) * p.ld_xs;
 #pragma unroll
@@ -1051,7 +1050,7 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     const bool in = first + 32 * c < t.n;
 #pragma unroll
                     for (int h = 0; h < 2; h++)
-                        next[c][h] = in ? sixteen_scales(row + 32 * c * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
+                        four[c][h] = in ? sixteen_scales(row + 32 * c * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
                 }
             };
             int i = blockIdx.x >> 1;
@@ -1059,18 +1058,13 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             for (; i < tiles && ok; i += pairs) {
                 const Tile t = tile_at(i);
                 for (int k4 = 0; k4 < steps && ok; k4 += 4) {
-                    uint4 now[4][2];
-#pragma unroll
-                    for (int c = 0; c < 4; c++) { now[c][0] = next[c][0]; now[c][1] = next[c][1]; }
-                    if (k4 + 4 < steps) load(t, k4 + 4);
-                    else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         if (k4 + j >= steps) break;
                         if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
                         if (t.cols > 128 * (warp - 2)) {
                             uint4* to = reinterpret_cast<uint4*>(ring + r.i * kFp4FitStage + kFp4FitScalesX + kFp4Scales * (warp - 2)) + lane;
-                            const uint4 a = now[0][j >> 1], b = now[1][j >> 1], c = now[2][j >> 1], d = now[3][j >> 1];
+                            const uint4 a = four[0][j >> 1], b = four[1][j >> 1], c = four[2][j >> 1], d = four[3][j >> 1];
                             to[0] = j & 1 ? make_uint4(a.z, b.z, c.z, d.z) : make_uint4(a.x, b.x, c.x, d.x);
                             to[32] = j & 1 ? make_uint4(a.w, b.w, c.w, d.w) : make_uint4(a.y, b.y, c.y, d.y);
                             fence_async();
@@ -1079,6 +1073,8 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                         if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
                         r.next(kFp4FitStages);
                     }
+                    if (k4 + 4 < steps) load(t, k4 + 4);
+                    else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
                 }
             }
         }
