@@ -17,14 +17,33 @@ int check_eps(const char* what, float eps) {
     return eps >= 0.f && std::isfinite(eps) ? QRM_OK : failf(QRM_E_INVALID, "%s: eps %g", what, (double)eps);
 }
 
+// Slots of a ring of rows, `bytes` each, that fit beside the other CTAs of the
+// SM; 0 where fewer than two do.
+constexpr int kRingRoom = 200 * 1024;   // of an SM's 227 KB
+int ring_slots(int64_t bytes, int ctas_an_sm, int64_t rows_a_cta) {
+    const int64_t fit = std::min<int64_t>(kRingRoom / ctas_an_sm / bytes, kNormSlots);
+    return fit < 2 ? 0 : (int)std::min(fit, rows_a_cta);
+}
+template <typename A>
+cudaError_t launch_ring(void (*kernel)(A), int64_t ctas, int threads, int slots, int64_t bytes, cudaStream_t s, const A& a) {
+    const size_t smem = (size_t)slots * bytes;
+    if (smem > 46 * 1024) {   // a launch has 48 KB without asking, the kernel's own included
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingRoom);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_ahead(kernel, dim3((unsigned)ctas), threads, smem, s, a);
+}
+
 template <typename T, int OUT>
-cudaError_t launch(const NormArgs<T>& a, int64_t rows, cudaStream_t s) {
+cudaError_t launch(NormArgs<T>& a, int sms, cudaStream_t s) {
     const int64_t chunks = chunks_of(a.d);
-    const dim3 grid((unsigned)rows);
-    if (chunks <= 256) return launch_ahead(rms_norm_kernel<T, OUT, 1>, grid, whole_warps(chunks), 0, s, a);
-    if (chunks <= 2 * kNormThreads) return launch_ahead(rms_norm_kernel<T, OUT, 2>, grid, whole_warps((chunks + 1) / 2), 0, s, a);
-    if (chunks <= 4 * kNormThreads) return launch_ahead(rms_norm_kernel<T, OUT, 4>, grid, whole_warps((chunks + 3) / 4), 0, s, a);
-    return launch_ahead(rms_norm_kernel<T, OUT, 0>, grid, kNormThreads, 0, s, a);
+    if (chunks > 4 * kNormThreads) return launch_ahead(rms_norm_kernel<T, OUT, 0>, dim3((unsigned)a.rows), kNormThreads, 0, s, a);
+    const int v = chunks <= 256 ? 1 : chunks <= 2 * kNormThreads ? 2 : 4, threads = whole_warps((chunks + v - 1) / v);
+    const int an_sm = std::max(1, std::min(8, 1024 / threads));
+    const int64_t ctas = std::min<int64_t>(a.rows, (int64_t)sms * an_sm), bytes = (int64_t)a.d * sizeof(T) * 2;
+    a.slots = a.wide && a.d * sizeof(T) % 16 == 0 ? ring_slots(bytes, an_sm, (a.rows + ctas - 1) / ctas) : 0;
+    return launch_ring(v == 1 ? rms_norm_kernel<T, OUT, 1> : v == 2 ? rms_norm_kernel<T, OUT, 2> : rms_norm_kernel<T, OUT, 4>, ctas, threads,
+                       a.slots, bytes, s, a);
 }
 
 int norm(const char* what, int out, int type, const void* x, int64_t ld_x, const void* add, int64_t ld_add, int64_t rows,
@@ -50,24 +69,24 @@ int norm(const char* what, int out, int type, const void* x, int64_t ld_x, const
     TRY(current_device(&device, &sms));
     const bool wide = wide_rows(x, ld_x, b) && (!add || wide_rows(add, ld_add, b)) && (!sum || wide_rows(sum, ld_sum, b)) &&
                       (!y || wide_rows(y, ld_y, b));
-    const bool wide_c = out == kNorm8 ? wide_codes(codes, ld_codes) : aligned(codes, 4) && ld_codes % 4 == 0;
+    const bool wide_c = wide_codes16(codes, ld_codes);
     cudaError_t e;
     const cudaStream_t s = (cudaStream_t)stream;
     BY_TYPE(type, {
-        const NormArgs<V> a{(const V*)x, (const V*)add, w, (V*)sum, (V*)y, codes, scales, ld_x, ld_add, ld_sum, ld_y,
-                            ld_codes, ld_scales, (int)d, eps, wide, aligned(w, 16), wide_c};
-        e = out == kNormTyped ? launch<V, kNormTyped>(a, rows, s) : out == kNorm8 ? launch<V, kNorm8>(a, rows, s)
-                                                                                  : launch<V, kNorm4>(a, rows, s);
+        NormArgs<V> a{(const V*)x, (const V*)add, w, (V*)sum, (V*)y, codes, scales, ld_x, ld_add, ld_sum, ld_y,
+                      ld_codes, ld_scales, (int)rows, (int)d, 0, eps, 1.f / (float)d, wide, aligned(w, 16), wide_c};
+        e = out == kNormTyped ? launch<V, kNormTyped>(a, sms, s) : out == kNorm8 ? launch<V, kNorm8>(a, sms, s)
+                                                                                 : launch<V, kNorm4>(a, sms, s);
     });
     return done(what, e);
 }
 
 // The gradient's CTAs: those that fit on the 148 SMs at once, and so many parts
 // of dw.  (A number of its own, so that the room for them needs no device.)
-int grad_threads(int64_t d) { return whole_warps(std::min<int64_t>(chunks_of(d), kNormGradThreads)); }
-int64_t grad_ctas(int64_t rows, int64_t d) {
-    return std::min<int64_t>(rows, 148 * std::max(1, std::min(4, 1024 / grad_threads(d))));
-}
+int grad_chunks(int64_t d) { return chunks_of(d) <= 128 ? 1 : chunks_of(d) <= 2 * kNormThreads ? 2 : 0; }   // of 8 columns a thread
+int grad_threads(int64_t d) { return grad_chunks(d) ? whole_warps((chunks_of(d) + grad_chunks(d) - 1) / grad_chunks(d)) : kNormThreads; }
+int grad_ctas_an_sm(int64_t d) { return std::max(1, std::min(4, 576 / grad_threads(d))); }
+int64_t grad_ctas(int64_t rows, int64_t d) { return std::min<int64_t>(rows, 148 * grad_ctas_an_sm(d)); }
 
 }  // namespace
 
@@ -128,12 +147,15 @@ extern "C" int qrm_rms_norm_grad(int type, const void* dy_dev, int64_t ld_dy, co
     float* part = !dw_dev ? nullptr : ctas > 1 ? work_dev : dw_dev;
     cudaError_t e;
     BY_TYPE(type, {
+        const int64_t bytes = d * b * 3;
+        const bool ring = wide && d * b % 16 == 0 && grad_chunks(d);
         const NormGradArgs<V> a{(const V*)dy_dev, (const V*)x_dev, (const V*)add_dev, w_dev, (V*)dx_dev, part, ld_dy, ld_x,
-                                ld_add, ld_dx, (int)rows, (int)d, eps, wide, aligned(w_dev, 16),
-                                aligned(part, 16) && d % 4 == 0};
-        e = chunks_of(d) <= kNormGradThreads
-                ? launch_ahead(rms_norm_grad_kernel<V, 1>, dim3((unsigned)ctas), grad_threads(d), 0, s, a)
-                : launch_ahead(rms_norm_grad_kernel<V, 0>, dim3((unsigned)ctas), grad_threads(d), 0, s, a);
+                                ld_add, ld_dx, (int)rows, (int)d, ring ? ring_slots(bytes, grad_ctas_an_sm(d), (rows + ctas - 1) / ctas) : 0,
+                                eps, 1.f / (float)d, wide, aligned(w_dev, 16), aligned(part, 16) && d % 4 == 0};
+        e = launch_ring(grad_chunks(d) == 1   ? rms_norm_grad_kernel<V, 1>
+                        : grad_chunks(d) == 2 ? rms_norm_grad_kernel<V, 2>
+                                              : rms_norm_grad_kernel<V, 0>,
+                        ctas, grad_threads(d), a.slots, bytes, s, a);
     });
     if (e == cudaSuccess && dw_dev && ctas > 1)
         e = launch_ahead(rms_norm_dw_kernel, dim3((unsigned)((d + 31) / 32)), 32 * kNormRuns, 0, s, work_dev, (int)ctas, (int)d, dw_dev);

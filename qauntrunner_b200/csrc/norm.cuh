@@ -9,19 +9,26 @@
 // else of the forward: a row's two sums (s^2 and g s) come in the one pass that
 // reads it.  Everything between load and store is in 32 bits, rounded once.
 //
-// Memory bounds both from some hundred rows on.  A CTA holds a row in
-// registers, 8 neighbouring columns to a load, so that each row is read once.
-// Rows that do not fit (more than 16384 columns, 8192 in the gradient) are read
-// twice by the same kernels' last form (V = 0).
+// Memory bounds both from some hundred rows on.  The CTAs walk the rows; one
+// holds a row in registers, 8 neighbouring columns to a load, so that each row is
+// read once.  Rows that start on 16 bytes come by bulk copies into a ring of
+// `slots` rows in shared memory, several ahead of the one that is worked on: a
+// slot is free again once all threads have its row in registers, which the row's
+// one barrier says.  Other rows are loaded where they are needed.  Rows that do
+// not fit (more than 16384 columns, 8192 in the gradient) are read twice by the
+// same kernels' last form (V = 0).
 #pragma once
+#include <type_traits>
+
+#include "gemv_tma.cuh"
 #include "rows4.cuh"
 
 namespace qrm {
 
 enum NormOut { kNormTyped = 0, kNorm8 = 1, kNorm4 = 2 };
 
-constexpr int kNormThreads = 512;        // most of a CTA of the forward
-constexpr int kNormGradThreads = 1024;   // of the gradient, one chunk of 8 columns each
+constexpr int kNormSlots = 8;            // most of a ring
+constexpr int kNormThreads = 512;   // most of a CTA
 
 // N sums over the CTA's threads, in every one of them; the order is fixed
 template <int N>
@@ -43,30 +50,131 @@ __device__ __forceinline__ void cta_sum(float (&v)[N], float (*scratch)[32]) {
     }
 }
 
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair both(float x) { return pair(x, x); }
+// the sum over two packed sums of squares or products
+__device__ __forceinline__ float joined(Pair p) {
+    const float2 f = unpair(p);
+    return f.x + f.y;
+}
+// eight values as they are stored
+template <typename T>
+__device__ __forceinline__ Raw8<T> rounded8(const Pairs8& v) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 f = unpair(v.p[i]);
+        if constexpr (sizeof(T) == 4) {
+            r.w[2 * i] = __float_as_uint(f.x);
+            r.w[2 * i + 1] = __float_as_uint(f.y);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = __floats2half2_rn(f.x, f.y);
+            memcpy(&r.w[i], &h, 4);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+            memcpy(&r.w[i], &h, 4);
+        }
+    }
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_raw8(T* p, const Raw8<T>& r, int n, bool wide) {
+    if (wide && n == 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++)
+            reinterpret_cast<uint4*>(p)[i] = make_uint4(r.w[4 * i], r.w[4 * i + 1], r.w[4 * i + 2], r.w[4 * i + 3]);
+    } else {
+        T h[8];
+        memcpy(h, r.w, sizeof h);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (i < n) p[i] = h[i];
+    }
+}
+
 // eight columns that this kernel may have written (no read-only path)
 template <typename T>
-__device__ __forceinline__ Vec8 load8_again(const T* p, int n) {
-    Vec8 r;
+__device__ __forceinline__ Raw8<T> load8_again(const T* p, int n) {
+    Raw8<T> r;
+    T h[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) r.v[i] = i < n ? to_f32(*const_cast<const volatile T*>(p + i)) : 0.f;
+    for (int i = 0; i < 8; i++) {
+        if constexpr (sizeof(T) == 4) {
+            h[i] = i < n ? *const_cast<const volatile T*>(p + i) : from_f32<T>(0.f);
+        } else {
+            const unsigned short b = i < n ? *reinterpret_cast<const volatile unsigned short*>(p + i) : 0;
+            memcpy(&h[i], &b, 2);
+        }
+    }
+    memcpy(r.w, h, sizeof h);
     return r;
 }
-template <>
-__device__ __forceinline__ Vec8 load8_again(const __half* p, int n) {
-    Vec8 r;
+
+// A ring of rows in shared memory: slot i % slots holds the CTA's i-th row of
+// each of N arrays (NULL: none), `bytes` of it.
+template <int N>
+struct RowRing {
+    const char* from[N];
+    long long pitch[N];   // bytes
+    char* at;
+    uint64_t* full;
+    int slots, bytes;
+    uint32_t i = 0, parity = 0, here = smem_u32(at);   // of the row that is worked on; its address
+    __device__ void init() {
+        if (threadIdx.x == 0) {
+            for (int k = 0; k < slots; k++) mbar_init(&full[k], 1);
+            fence_barrier_init();
+        }
+        __syncthreads();
+    }
+    // row t into slot k, by one thread
+    __device__ void load(uint32_t k, uint32_t t) {
+        uint32_t total = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        r.v[i] = i < n ? __half2float(__ushort_as_half(*reinterpret_cast<const volatile unsigned short*>(p + i))) : 0.f;
-    return r;
-}
-template <>
-__device__ __forceinline__ Vec8 load8_again(const __nv_bfloat16* p, int n) {
-    Vec8 r;
+        for (int j = 0; j < N; j++)
+            if (from[j]) total += bytes;
+        mbar_arrive_expect_tx(&full[k], total);
+        char* to = at + (size_t)k * N * bytes;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        r.v[i] = i < n ? __bfloat162float(__ushort_as_bfloat16(*reinterpret_cast<const volatile unsigned short*>(p + i))) : 0.f;
-    return r;
-}
+        for (int j = 0; j < N; j++, to += bytes)
+            if (from[j]) bulk_g2s(to, from[j] + t * pitch[j], bytes, &full[k]);
+    }
+    __device__ void start(uint32_t rows) {
+        if (threadIdx.x == 0)
+            for (uint32_t k = 0, t = blockIdx.x; k < (uint32_t)slots && t < rows; k++, t += gridDim.x) load(k, t);
+    }
+    // the row that is worked on is there (its copies were issued, so they come; the wait is bounded all the same)
+    __device__ void wait() { mbar_wait(&full[i], parity); }
+    // its slot takes the row `slots` turns on; all threads have read it
+    __device__ void next(uint32_t t, uint32_t rows) {
+        const unsigned long long ahead = t + (unsigned long long)slots * gridDim.x;
+        if (threadIdx.x == 0 && ahead < rows) load(i, (uint32_t)ahead);
+        here += N * bytes;
+        if (++i == (uint32_t)slots) {
+            i = 0;
+            parity ^= 1;
+            here = smem_u32(at);
+        }
+    }
+    // the n columns at c of array j (the others are 0); a row's 16 bytes are whole, so n is 0, 8 or, in f32, 4
+    template <typename T>
+    __device__ Raw8<T> row(int j, int c, int n) const {
+        Raw8<T> r;
+        const uint32_t p = here + j * bytes + c * (int)sizeof(T);
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(T) / 2; k++) {
+            uint4 a = make_uint4(0, 0, 0, 0);
+            if (n * (int)sizeof(T) > 16 * k)
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w) : "r"(p + 16 * k) : "memory");
+            r.w[4 * k] = a.x; r.w[4 * k + 1] = a.y; r.w[4 * k + 2] = a.z; r.w[4 * k + 3] = a.w;
+        }
+        return r;
+    }
+};
 
 template <typename T>
 struct NormArgs {
@@ -76,131 +184,191 @@ struct NormArgs {
     uint8_t* codes;
     void* scales;            // f32, or e8m0 bytes
     long long ld_x, ld_add, ld_sum, ld_y, ld_c, ld_s;
-    int d;
-    float eps;
+    int rows, d;
+    int slots;                   // of the ring, 0: rows are loaded where they are needed
+    float eps, per_d;            // per_d: 1 / d
     bool wide, wide_w, wide_c;   // rows (weights, codes) start on 16 (16, 8 or 4) bytes
 };
 
-// s of eight columns, as it is stored
+// s of eight columns as it is stored: x, or x + add rounded
 template <typename T>
-__device__ __forceinline__ Vec8 norm_sum(const NormArgs<T>& a, const Raw8<T>& x, const Raw8<T>& add) {
-    Vec8 v;
+__device__ __forceinline__ Raw8<T> norm_sum(const NormArgs<T>& a, const Raw8<T>& x, const Raw8<T>& add) {
+    if (!a.add) return x;
+    Pairs8 v = values8(x), u = values8(add);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        v.v[i] = column(x, i);
-        if (a.add) v.v[i] = to_f32(from_f32<T>(v.v[i] + column(add, i)));
-    }
-    return v;
+    for (int i = 0; i < 4; i++) v.p[i] = add2(v.p[i], u.p[i]);
+    return rounded8<T>(v);
 }
-// y of eight columns at c, of which n exist, to where it goes.  All 32 lanes take part.
-template <typename T, int OUT>
-__device__ __forceinline__ void norm_out(const NormArgs<T>& a, long long t, const Vec8& s, const Vec8& w, float inv, int c, int n) {
-    Vec8 y;
+__device__ __forceinline__ Pair squares(const Pairs8& s, Pair total) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) y.v[i] = s.v[i] * inv * w.v[i];
-    if (OUT == kNormTyped || a.y) {
-        if (n) store8(a.y + t * a.ld_y + c, y, n, a.wide);
-    }
-    if (OUT == kNorm8) {
-        Pairs8 neg;
-#pragma unroll
-        for (int i = 0; i < 4; i++) neg.p[i] = pair(2 * i < n ? -y.v[2 * i] : 0.f, 2 * i + 1 < n ? -y.v[2 * i + 1] : 0.f);
-        const float scale = block_scale(half_warp_max(amax8(neg)));
-        if (n) {
-            store_codes8(a.codes + t * a.ld_c + c, scale < kFp8Tiny ? codes8_divided(neg, scale) : codes8(neg, quant(scale)), n, a.wide_c);
-            if ((threadIdx.x & 15) == 0) static_cast<float*>(a.scales)[t * a.ld_s + c / kFp8Block] = scale;
-        }
-    } else if (OUT == kNorm4) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            y.v[i] = i < n ? y.v[i] : 0.f;
-            m = max(m, magnitude(y.v[i]));
-        }
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const uint32_t scale = fp4_scale(m), q = e2m1x8(y.v, scale);
-        if (c / kFp4Block * kFp4Block < a.d) {   // codes past the last column, 0, up to the block's end
-            uint8_t* to = a.codes + t * a.ld_c + c / 2;
-            if (a.wide_c) {
-                *reinterpret_cast<uint32_t*>(to) = q;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) to[i] = (uint8_t)(q >> (8 * i));
-            }
-            if ((threadIdx.x & 3) == 0) static_cast<uint8_t*>(a.scales)[t * a.ld_s + c / kFp4Block] = (uint8_t)scale;
-        }
-    }
+    for (int i = 0; i < 4; i++) total = fma2(s.p[i], s.p[i], total);
+    return total;
 }
-__device__ __forceinline__ Vec8 norm_weight(const float* w, int c, int n, bool wide) {
+__device__ __forceinline__ Pairs8 norm_weight(const float* w, int c, int n, bool wide) {
+    Pairs8 r;
+    if (w) return values8(load_raw8(w + c, n, wide));
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.p[i] = both(1.f);
+    return r;
+}
+__device__ __forceinline__ Vec8 weight8(const float* w, int c, int n, bool wide) {
     if (w) return load8(w + c, n, wide);
     Vec8 one;
 #pragma unroll
     for (int i = 0; i < 8; i++) one.v[i] = 1.f;
     return one;
 }
+// y of a thread's 8 V neighbouring columns from c on (of those that do not exist
+// s is 0, and so is y) to where it goes.  All 32 lanes take part.
+template <typename T, int OUT, int V>
+__device__ __forceinline__ void norm_out(const NormArgs<T>& a, long long t, const Pairs8 (&s)[V], const Pairs8 (&w)[V], float inv, int c) {
+    Pairs8 y[V];   // negated where they are to become 8-bit codes
+    const Pair f = both(OUT == kNorm8 ? -inv : inv);
+#pragma unroll
+    for (int v = 0; v < V; v++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[v].p[i] = mul2(mul2(s[v].p[i], f), w[v].p[i]);
+    if (OUT == kNormTyped || a.y) {
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            const int n = columns_at(c + 8 * v, a.d);
+            Pairs8 z = y[v];
+            if (OUT == kNorm8) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) z.p[i] = negative(z.p[i]);
+            }
+            if (n) store_raw8(a.y + t * a.ld_y + c + 8 * v, rounded8<T>(z), n, a.wide);
+        }
+    }
+    if (OUT == kNormTyped) return;
+    float top = 0.f;   // a NaN stays one
+#pragma unroll
+    for (int v = 0; v < V; v++) top = max_nan(top, amax8(y[v]));
+    constexpr int kLanes = (OUT == kNorm8 ? 16 : 4) / V;   // of a block
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool lead = (threadIdx.x & (kLanes - 1)) == 0;
+    if (OUT == kNorm8) {
+        if (c >= a.d) return;
+        const float scale = block_scale(top);
+        const Quant q = quant(scale);
+        uint2 codes[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) codes[v] = scale < kFp8Tiny ? codes8_divided(y[v], scale) : codes8(y[v], q);
+        uint8_t* to = a.codes + t * a.ld_c + c;
+        if (V > 1 && a.wide_c && c + 8 * V <= a.d) {
+#pragma unroll
+            for (int v = 0; v < V / 2; v++)
+                reinterpret_cast<uint4*>(to)[v] = make_uint4(codes[2 * v].x, codes[2 * v].y, codes[2 * v + 1].x, codes[2 * v + 1].y);
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const int n = columns_at(c + 8 * v, a.d);
+                if (n) store_codes8(to + 8 * v, codes[v], n, a.wide_c);
+            }
+        }
+        if (lead) static_cast<float*>(a.scales)[t * a.ld_s + c / kFp8Block] = scale;
+    } else {
+        if (c / kFp4Block * kFp4Block >= a.d) return;   // (codes past the last column, 0, go up to the block's end)
+        const uint32_t scale = fp4_scale(__float_as_uint(top));
+        uint32_t codes[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 g = unpair(y[v].p[i]);
+                e[2 * i] = g.x;
+                e[2 * i + 1] = g.y;
+            }
+            codes[v] = e2m1x8(e, scale);
+        }
+        uint8_t* to = a.codes + t * a.ld_c + c / 2;
+        if (a.wide_c) {
+            if constexpr (V == 4) *reinterpret_cast<uint4*>(to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+            else if constexpr (V == 2) *reinterpret_cast<uint2*>(to) = make_uint2(codes[0], codes[1]);
+            else *reinterpret_cast<uint32_t*>(to) = codes[0];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4 * V; i++) to[i] = (uint8_t)(codes[i >> 2] >> (8 * (i & 3)));
+        }
+        if (lead) static_cast<uint8_t*>(a.scales)[t * a.ld_s + c / kFp4Block] = (uint8_t)scale;
+    }
+}
+// 1 / sqrt(mean + eps), within 2 ulp
+__device__ __forceinline__ float norm_factor(float total, float per_d, float eps) { return rsqrtf(fmaf(total, per_d, eps)); }
 
-// A row of V chunks of 8 columns a thread (0: of any length, read twice).  sum
-// may be x or add, y any of them: a thread has read a column before it writes it.
+// A row of 8 V neighbouring columns a thread (0: of any length, read twice).  sum
+// may be x or add, y any of them: a thread has read a column before it writes it,
+// and a row is copied ahead of others only.
 template <typename T, int OUT, int V>
 __global__ void __launch_bounds__(kNormThreads)
 rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
-    pdl_start();
-    __shared__ float scratch[1][32];
-    const long long t = blockIdx.x;
-    const T* x = a.x + t * a.ld_x;
-    const T* add = a.add ? a.add + t * a.ld_add : nullptr;
-    float total[1] = {0.f};
-    const int step = 8 * blockDim.x, c0 = 8 * threadIdx.x;
+    extern __shared__ __align__(16) char ring_mem[];
+    __shared__ uint64_t full[kNormSlots];
+    __shared__ float scratch[2][1][32];   // two rows' turns
     if constexpr (V > 0) {
-        Raw8<T> raw[V], more[V];
-        Vec8 s[V], w[V];
+        const int c = 8 * V * threadIdx.x;
+        RowRing<2> ring{{reinterpret_cast<const char*>(a.x), reinterpret_cast<const char*>(a.add)},
+                        {a.ld_x * (long long)sizeof(T), a.ld_add * (long long)sizeof(T)}, ring_mem, full, a.slots, a.d * (int)sizeof(T)};
+        if (a.slots) ring.init();
+        pdl_start();
+        if (a.slots) ring.start(a.rows);
+        int turn = 0;
+        Pairs8 w[V];
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const int c = c0 + i * step, n = columns_at(c, a.d);
-            raw[i] = load_raw8(x + c, n, a.wide);
-            more[i] = add ? load_raw8(add + c, n, a.wide) : raw[i];
+        for (int i = 0; i < V; i++) w[i] = norm_weight(a.w, c + 8 * i, columns_at(c + 8 * i, a.d), a.wide_w);
+        for (uint32_t t = blockIdx.x; t < (uint32_t)a.rows; t += gridDim.x, turn ^= 1) {   // (unsigned, as in combine_rows_kernel)
+            Raw8<T> raw[V], more[V];
+            Pairs8 s[V];
+            if (a.slots) ring.wait();
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int at = c + 8 * i, n = columns_at(at, a.d);
+                raw[i] = a.slots ? ring.template row<T>(0, at, n) : load_raw8(a.x + t * a.ld_x + at, n, a.wide);
+                if (a.add) more[i] = a.slots ? ring.template row<T>(1, at, n) : load_raw8(a.add + t * a.ld_add + at, n, a.wide);
+            }
+            Pair part = 0;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int at = c + 8 * i, n = columns_at(at, a.d);
+                if (a.add) raw[i] = norm_sum(a, raw[i], more[i]);
+                if (a.sum && n) store_raw8(a.sum + t * a.ld_sum + at, raw[i], n, a.wide);
+                s[i] = values8(raw[i]);
+                part = squares(s[i], part);
+            }
+            float total[1] = {joined(part)};
+            cta_sum(total, scratch[turn]);   // (one barrier a row: the turns keep a row's sum from the next one's)
+            if (a.slots) ring.next(t, a.rows);
+            norm_out<T, OUT, V>(a, t, s, w, norm_factor(total[0], a.per_d, a.eps), c);
         }
-#pragma unroll
-        for (int i = 0; i < V; i++) w[i] = norm_weight(a.w, c0 + i * step, columns_at(c0 + i * step, a.d), a.wide_w);
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            const int c = c0 + i * step, n = columns_at(c, a.d);
-            s[i] = norm_sum(a, raw[i], more[i]);
-            if (a.sum && n) store8(a.sum + t * a.ld_sum + c, s[i], n, a.wide);
-#pragma unroll
-            for (int j = 0; j < 8; j++) total[0] = fmaf(s[i].v[j], s[i].v[j], total[0]);
-        }
-        cta_sum(total, scratch);
-        const float inv = 1.f / sqrtf(total[0] / (float)a.d + a.eps);
-#pragma unroll
-        for (int i = 0; i < V; i++) norm_out<T, OUT>(a, t, s[i], w[i], inv, c0 + i * step, columns_at(c0 + i * step, a.d));
     } else {
+        pdl_start();
+        const int step = 8 * blockDim.x, c0 = 8 * threadIdx.x;
+        const long long t = blockIdx.x;
+        const T* x = a.x + t * a.ld_x;
+        const T* add = a.add ? a.add + t * a.ld_add : nullptr;
+        Pair part = 0;
         for (int c = c0; c < a.d; c += step) {
             const int n = columns_at(c, a.d);
             const Raw8<T> raw = load_raw8(x + c, n, a.wide);
-            const Vec8 s = norm_sum(a, raw, add ? load_raw8(add + c, n, a.wide) : raw);
-            if (a.sum) store8(a.sum + t * a.ld_sum + c, s, n, a.wide);
-#pragma unroll
-            for (int j = 0; j < 8; j++) total[0] = fmaf(s.v[j], s.v[j], total[0]);
+            const Raw8<T> s = norm_sum(a, raw, add ? load_raw8(add + c, n, a.wide) : raw);
+            if (a.sum) store_raw8(a.sum + t * a.ld_sum + c, s, n, a.wide);
+            part = squares(values8(s), part);
         }
-        cta_sum(total, scratch);
-        const float inv = 1.f / sqrtf(total[0] / (float)a.d + a.eps);
+        float total[1] = {joined(part)};
+        cta_sum(total, scratch[0]);
+        const float inv = norm_factor(total[0], a.per_d, a.eps);
         for (int base = 0; base < a.d; base += step) {   // whole warps: a block's lanes meet in norm_out
             const int c = base + c0, n = columns_at(c, a.d);
-            Vec8 s;
-            if (a.sum) {
-                s = load8_again(a.sum + t * a.ld_sum + c, n);
-            } else {
-                const Vec8 u = load8_again(x + c, n);
-                s = u;
-                if (add) {
-                    const Vec8 v = load8_again(add + c, n);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) s.v[j] = to_f32(from_f32<T>(u.v[j] + v.v[j]));
-                }
+            Raw8<T> raw;
+            if (a.sum) raw = load8_again(a.sum + t * a.ld_sum + c, n);
+            else {
+                raw = load8_again(x + c, n);
+                if (add) raw = norm_sum(a, raw, load8_again(add + c, n));
             }
-            norm_out<T, OUT>(a, t, s, norm_weight(a.w, c, n, a.wide_w), inv, c, n);
+            const Pairs8 s[1] = {values8(raw)}, w[1] = {norm_weight(a.w, c, n, a.wide_w)};
+            norm_out<T, OUT, 1>(a, t, s, w, inv, c);
         }
     }
 }
@@ -213,60 +381,83 @@ struct NormGradArgs {
     float* part;             // [gridDim.x][d] sums over a CTA's rows, or NULL
     long long ld_dy, ld_x, ld_add, ld_dx;
     int rows, d;
-    float eps;
+    int slots;               // as in NormArgs
+    float eps, per_d;
     bool wide, wide_w, wide_part;
 };
 
-// The CTAs walk the rows, so that a thread keeps its columns' weights and their
-// sums over the rows in registers; a row's loads are on their way while the one
-// before it is worked on.
+// A thread keeps its 8 V columns' weights and their sums over the rows in
+// registers.
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormGradThreads)
+__global__ void __launch_bounds__(kNormThreads)
 rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
-    pdl_start();
+    extern __shared__ __align__(16) char ring_mem[];
+    __shared__ uint64_t full[kNormSlots];
     __shared__ float scratch[2][2][32];   // two rows' turns
     int turn = 0;
-    if constexpr (V == 1) {
-        const int c = 8 * threadIdx.x, n = columns_at(c, a.d);
-        const Vec8 w = norm_weight(a.w, c, n, a.wide_w);
-        Vec8 dw;
+    if constexpr (V > 0) {
+        RowRing<3> ring{{reinterpret_cast<const char*>(a.x), reinterpret_cast<const char*>(a.dy), reinterpret_cast<const char*>(a.add)},
+                        {a.ld_x * (long long)sizeof(T), a.ld_dy * (long long)sizeof(T), a.ld_add * (long long)sizeof(T)},
+                        ring_mem, full, a.slots, a.d * (int)sizeof(T)};
+        if (a.slots) ring.init();
+        pdl_start();
+        if (a.slots) ring.start(a.rows);
+        const int c = 8 * V * threadIdx.x;
+        Pairs8 w[V], dw[V];
 #pragma unroll
-        for (int j = 0; j < 8; j++) dw.v[j] = 0.f;
-        uint32_t t = blockIdx.x;   // (unsigned: a step past the last of 2^31 - 1 rows stays a number past it)
-        Raw8<T> x = load_raw8(a.x + t * a.ld_x + c, n, a.wide), dy = load_raw8(a.dy + t * a.ld_dy + c, n, a.wide);
-        for (; t < (uint32_t)a.rows; turn ^= 1) {
-            const uint32_t next = t + gridDim.x;
-            Raw8<T> x1 = x, dy1 = dy, add = x;
-            if (a.add) add = load_raw8(a.add + t * a.ld_add + c, n, a.wide);
-            if (next < (uint32_t)a.rows) {
-                x1 = load_raw8(a.x + next * a.ld_x + c, n, a.wide);
-                dy1 = load_raw8(a.dy + next * a.ld_dy + c, n, a.wide);
-            }
-            float sums[2] = {0.f, 0.f};
+        for (int i = 0; i < V; i++) {
+            w[i] = norm_weight(a.w, c + 8 * i, columns_at(c + 8 * i, a.d), a.wide_w);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float s = column(x, j), g = column(dy, j) * w.v[j];
-                sums[0] = fmaf(s, s, sums[0]);
-                sums[1] = fmaf(g, s, sums[1]);
-            }
-            cta_sum(sums, scratch[turn]);   // (one barrier a row: the turns keep a row's sums from the next one's)
-            const float inv = 1.f / sqrtf(sums[0] / (float)a.d + a.eps);
-            const float along = sums[1] / (float)a.d * inv;   // mean(g n)
-            Vec8 dx;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float nrm = column(x, j) * inv, g = column(dy, j);
-                dw.v[j] = fmaf(g, nrm, dw.v[j]);
-                dx.v[j] = inv * fmaf(-nrm, along, g * w.v[j]);
-                if (a.add) dx.v[j] += column(add, j);
-            }
-            if (n) store8(a.dx + t * a.ld_dx + c, dx, n, a.wide);
-            x = x1;
-            dy = dy1;
-            t = next;
+            for (int j = 0; j < 4; j++) dw[i].p[j] = 0;
         }
-        if (a.part && n) store8(a.part + (size_t)blockIdx.x * a.d + c, dw, n, a.wide_part);
+        for (uint32_t t = blockIdx.x; t < (uint32_t)a.rows; t += gridDim.x, turn ^= 1) {   // (unsigned, as in combine_rows_kernel)
+            Raw8<T> add[V];
+            Pairs8 x[V], dy[V];
+            if (a.slots) ring.wait();
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int at = c + 8 * i, n = columns_at(at, a.d);
+                x[i] = values8(a.slots ? ring.template row<T>(0, at, n) : load_raw8(a.x + t * a.ld_x + at, n, a.wide));
+                dy[i] = values8(a.slots ? ring.template row<T>(1, at, n) : load_raw8(a.dy + t * a.ld_dy + at, n, a.wide));
+                if (a.add) add[i] = a.slots ? ring.template row<T>(2, at, n) : load_raw8(a.add + t * a.ld_add + at, n, a.wide);
+            }
+            Pair square = 0, product = 0;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                square = squares(x[i], square);
+#pragma unroll
+                for (int j = 0; j < 4; j++) product = fma2(mul2(dy[i].p[j], w[i].p[j]), x[i].p[j], product);
+            }
+            float sums[2] = {joined(square), joined(product)};
+            cta_sum(sums, scratch[turn]);
+            if (a.slots) ring.next(t, a.rows);
+            const float inv = norm_factor(sums[0], a.per_d, a.eps);
+            const Pair f = both(inv), minus = both(-(sums[1] * a.per_d * inv));   // - mean(g n)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int at = c + 8 * i, n = columns_at(at, a.d);
+                Pairs8 dx;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const Pair nrm = mul2(x[i].p[j], f);
+                    dw[i].p[j] = fma2(dy[i].p[j], nrm, dw[i].p[j]);
+                    dx.p[j] = mul2(f, fma2(nrm, minus, mul2(dy[i].p[j], w[i].p[j])));
+                }
+                if (a.add) {
+                    const Pairs8 more = values8(add[i]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) dx.p[j] = add2(dx.p[j], more.p[j]);
+                }
+                if (n) store_raw8(a.dx + t * a.ld_dx + at, rounded8<T>(dx), n, a.wide);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const int at = c + 8 * i, n = columns_at(at, a.d);
+            if (a.part && n) store_raw8(a.part + (size_t)blockIdx.x * a.d + at, rounded8<float>(dw[i]), n, a.wide_part);
+        }
     } else {
+        pdl_start();
         float* part = a.part ? a.part + (size_t)blockIdx.x * a.d : nullptr;
         const int step = 8 * blockDim.x;
         bool first = true;
@@ -275,7 +466,7 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
             for (int c = 8 * threadIdx.x; c < a.d; c += step) {
                 const int n = columns_at(c, a.d);
                 const Vec8 x = load8(a.x + t * a.ld_x + c, n, a.wide), dy = load8(a.dy + t * a.ld_dy + c, n, a.wide);
-                const Vec8 w = norm_weight(a.w, c, n, a.wide_w);
+                const Vec8 w = weight8(a.w, c, n, a.wide_w);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     sums[0] = fmaf(x.v[j], x.v[j], sums[0]);
@@ -283,12 +474,12 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
                 }
             }
             cta_sum(sums, scratch[turn]);
-            const float inv = 1.f / sqrtf(sums[0] / (float)a.d + a.eps);
-            const float along = sums[1] / (float)a.d * inv;
+            const float inv = norm_factor(sums[0], a.per_d, a.eps);
+            const float along = sums[1] * a.per_d * inv;
             for (int c = 8 * threadIdx.x; c < a.d; c += step) {
                 const int n = columns_at(c, a.d);
                 const Vec8 x = load8(a.x + t * a.ld_x + c, n, a.wide), dy = load8(a.dy + t * a.ld_dy + c, n, a.wide);
-                const Vec8 w = norm_weight(a.w, c, n, a.wide_w);
+                const Vec8 w = weight8(a.w, c, n, a.wide_w);
                 Vec8 dx, add;
                 if (a.add) add = load8(a.add + t * a.ld_add + c, n, a.wide);
 #pragma unroll

@@ -40,7 +40,7 @@ def near(got, want, bound, type):
     assert bool((off <= slack).all()), float((off / slack).max())
 
 
-SHAPES = [(1, 1), (1, 7), (2, 8), (3, 33), (5, 130), (4, 1024), (3, 2049), (2, 2816), (3, 7168), (2, 8193), (2, 16385),
+SHAPES = [(1, 1), (1, 7), (2, 8), (3, 33), (5, 130), (4, 1024), (3, 2049), (2, 2816), (400, 300), (3, 2820), (3, 7168), (2, 8193), (2, 16385),
           (300, 64)]
 
 
@@ -137,7 +137,7 @@ def test_norm_of_zeros_large_and_not_finite():
     assert bool((codes[0] == 0).all())
 
 
-@pytest.mark.parametrize("rows,d", [(1, 1), (1, 7168), (2, 9), (3, 2816), (7, 33), (700, 64), (149, 7168), (600, 1030), (5, 8200), (301, 8300)])
+@pytest.mark.parametrize("rows,d", [(1, 1), (1, 7168), (2, 9), (3, 2816), (700, 300), (5, 2820), (7, 33), (700, 64), (149, 7168), (600, 1030), (5, 8200), (301, 8300)])
 @pytest.mark.parametrize("type", TYPES)
 @pytest.mark.parametrize("add", [False, True])
 def test_gradient(rows, d, type, add):
