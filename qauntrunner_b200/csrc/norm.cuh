@@ -506,9 +506,12 @@ rms_norm_dw_kernel(const float* __restrict__ part, int parts, int d, float* __re
     const int lane = threadIdx.x & 31, r = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     const int first = parts * r / kNormRuns, last = parts * (r + 1) / kNormRuns;
     float t = 0.f;
-    if (c < d) {
-#pragma unroll 8
-        for (int p = first; p < last; p++) t += part[(size_t)p * d + c];
+    for (int p = first; c < d && p < last; p += 10) {   // (ten loads on their way: the 148 parts of long rows are ten a run)
+        float v[10];
+#pragma unroll
+        for (int i = 0; i < 10; i++) v[i] = p + i < last ? __ldg(part + (size_t)(p + i) * d + c) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 10; i++) t += v[i];
     }
     run[r][lane] = t;
     __syncthreads();
