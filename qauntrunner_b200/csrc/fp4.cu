@@ -180,8 +180,8 @@ cudaError_t launch(const qrm_fp4* m, const Fp4RowMaps& x_maps, Fp4Params& p, Fp4
     while (ranks < 8 && tiles * ranks * 2 <= 2 * m->sms && p.steps >= 4 * ranks) ranks *= 2;
     const int x_rows = (int)std::min<int64_t>(kFp4Rows, (T + 15) / 16 * 16);
     const int64_t ctas = (int64_t)p.row_tiles * across * ranks;
-    const int room = ctas <= m->sms ? kSmemMost : kSmemMost / 2 - 512;   // two CTAs on an SM, 1 KB of it kept for each
-    const int stages = std::max(2, std::min(kFp4MaxStages, (room - 1024 - kFp4Header) / fp4_stage_bytes(x_rows)));
+    // two CTAs on an SM, 1 KB of it kept for each: of one launch, or the next one's first
+    const int stages = std::min(kFp4MaxStages, (kSmemMost / 2 - 512 - 1024 - kFp4Header) / fp4_stage_bytes(x_rows));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kFp4Threads);

@@ -249,7 +249,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
                  const __grid_constant__ Fp4Params p, int stages, int x_rows /* room for rows of x in a stage */) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // [stages] copies are there
+    uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // [stages] copies are there: the weights', those of x
     uint64_t* x_full = full + kFp4MaxStages;            // [stages] scales of x are there
     uint64_t* done = x_full + kFp4MaxStages;            // [stages] their MMAs are done
     uint64_t* done_bar = done + kFp4MaxStages;
@@ -258,7 +258,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     volatile uint32_t* issued = reinterpret_cast<volatile uint32_t*>(sm + 520);   // stages, once their warp is through
     Fp4Tile* found = reinterpret_cast<Fp4Tile*>(sm + 528);
     const uint32_t stage_bytes = fp4_stage_bytes(x_rows);
-    // a stage: codes of x (the MMA of 16 rows of x reads no more), codes of both blocks, their scales, scales of x
+    // a stage: codes of x, codes of both blocks, their scales, scales of x
     const uint32_t w_off = x_rows * 128, ws_off = w_off + 2 * kFp4Tile, xs_off = ws_off + 2 * kFp4Scales;
     uint8_t* ring = sm + kFp4Header;
 
@@ -267,9 +267,25 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     const int tile = blockIdx.x / ranks, row_tile = tile % p.row_tiles, block = tile / p.row_tiles;
+    constexpr int kBlock = MODE == kFp4Plain ? 128 : 64;   // outputs of a block
+    const int m0 = block * 2 * kBlock;
+    const int k0 = (int)((long long)p.steps * rank / ranks), k1 = (int)((long long)p.steps * (rank + 1) / ranks);
+    // one matrix: its first stages are asked for before the kernel before has ended, which does not write it
+    const int early = p.groups == 1 ? min(stages, k1 - k0) : 0;
+    // a stage's copies of the weights, by one thread
+    auto load_stage = [&](uint32_t slot, int k, int group) {
+        uint8_t* st = ring + slot * stage_bytes;
+        mbar_arrive_expect_tx(&full[slot], (uint32_t)(2 * kFp4Tile + 2 * kFp4Scales));
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            load_weights<MODE != kFp4Plain>(st + w_off + b * kFp4Tile, &w_map, k * 128, m0 + b * kBlock, group, &full[slot]);
+            const long long unit = (long long)group * p.units + min(m0 / kBlock + b, p.units - 1);   // an absent second block is not stored
+            bulk_g2s(st + ws_off + b * kFp4Scales, p.w_scales + (unit * p.steps + k) * kFp4Scales, kFp4Scales, &full[slot]);
+        }
+    };
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; i++) {
-            mbar_init(&full[i], 1);
+            mbar_init(&full[i], 2);
             mbar_init(&x_full[i], 1);
             mbar_init(&done[i], 1);
         }
@@ -277,9 +293,12 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         *abort_flag = 0;
         *issued = 0;
         fence_barrier_init();
+        pdl_trigger();
+        for (int i = 0; i < early; i++) load_stage(i, k0 + i, 0);
     }
+    __syncwarp();
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), kFp4TmemCols);
-    pdl_start();   // nothing before this reads or writes global memory
+    pdl_start();   // nothing before this reads or writes global memory, but for the weights
     if (warp == 2) {
         const Fp4Tile t = fp4_find(p, row_tile, blockIdx.x == 0);
         if (lane == 0) *found = t;
@@ -290,13 +309,15 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     const uint32_t tmem = *tmem_slot;
     const Fp4Tile t = *found;
     if (t.n == 0) {   // (for all of the cluster)
+        if (threadIdx.x == 0)
+            for (int i = 0; i < early; i++) {   // copies land before the CTA exits
+                mbar_arrive(&full[i]);
+                mbar_wait(&full[i], 0u);
+            }
         if (warp == 1) tmem_dealloc(tmem, kFp4TmemCols);
         return;
     }
     const WaitCtl ctl{abort_flag, p.err};
-    const int k0 = (int)((long long)p.steps * rank / ranks), k1 = (int)((long long)p.steps * (rank + 1) / ranks);
-    constexpr int kBlock = MODE == kFp4Plain ? 128 : 64;   // outputs of a block
-    const int m0 = block * 2 * kBlock;
     const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), done0 = smem_u32(done);
     const int boxes = (t.n + 15) >> 4;
 
@@ -304,19 +325,14 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         // ------------------------------------------------ codes and the weights' scales
         Ring r;
         uint32_t n_issued = 0;
-        const int u0 = m0 / kBlock, u1 = min(u0 + 1, p.units - 1);   // an absent second block is not stored
-        const uint8_t* s0 = p.w_scales + ((long long)t.group * p.units + u0) * p.steps * kFp4Scales;
-        const uint8_t* s1 = p.w_scales + ((long long)t.group * p.units + u1) * p.steps * kFp4Scales;
         for (int k = k0; k < k1; k++) {
-            if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) break;
-            uint8_t* st = ring + r.i * stage_bytes;
+            // (the early stages go through whatever happens: their weights are on their way)
+            if (k >= k0 + early && !bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) break;
             if (elect_one()) {
-                mbar_arrive_expect_tx(&full[r.i], (uint32_t)(boxes * 2048 + 2 * kFp4Tile + 2 * kFp4Scales));
-                for (int b = 0; b < 2; b++)
-                    load_weights<MODE != kFp4Plain>(st + w_off + b * kFp4Tile, &w_map, k * 128, m0 + b * kBlock, t.group, &full[r.i]);
-                bulk_g2s(st + ws_off, s0 + (size_t)k * kFp4Scales, kFp4Scales, &full[r.i]);
-                bulk_g2s(st + ws_off + kFp4Scales, s1 + (size_t)k * kFp4Scales, kFp4Scales, &full[r.i]);
-                for (int b = 0; b < boxes; b++) tma_load_2d(st + b * 2048, &x_map, k * 128, t.pos + 16 * b, &full[r.i]);
+                if (k >= k0 + early) load_stage(r.i, k, t.group);
+                mbar_arrive_expect_tx(&full[r.i], (uint32_t)(boxes * 2048));
+                for (int b = 0; b < boxes; b++)
+                    tma_load_2d(ring + r.i * stage_bytes + b * 2048, &x_map, k * 128, t.pos + 16 * b, &full[r.i]);
             }
             __syncwarp();
             r.next(stages);
@@ -355,22 +371,30 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         if (elect_one()) umma_commit(done_bar);
         __syncwarp();
     } else if (warp == 2) {
-        // ------------------------------------------------ scales of x: rows lane and lane + 32
+        // ------------------------------------------------ scales of x: rows lane and lane + 32, four stages' at a time
         Ring r;
         const uint8_t* row = p.x_scales + (long long)(t.pos + lane) * p.ld_xs;
-        const bool in0 = lane < t.n, in1 = lane + 32 < t.n;
-        for (int k = k0; k < k1; k++) {
-            const uint2 none = make_uint2(0, 0);
-            const uint2 a = in0 ? eight_scales(row, 8 * k, p.blocks, p.wide_xs) : none;
-            const uint2 b = in1 ? eight_scales(row + 32 * p.ld_xs, 8 * k, p.blocks, p.wide_xs) : none;
-            if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) break;
-            uint4* to = reinterpret_cast<uint4*>(ring + r.i * stage_bytes + xs_off) + lane;
-            to[0] = make_uint4(a.x, b.x, 0, 0);
-            to[32] = make_uint4(a.y, b.y, 0, 0);
-            fence_async();
-            __syncwarp();
-            if (lane == 0) bar_arrive(x_full0 + 8 * r.i);
-            r.next(stages);
+        bool ok = true;
+        for (int k4 = k0; k4 < k1 && ok; k4 += 4) {
+            uint2 four[2][4];   // (by eights: a CTA's first stage may begin inside sixteen)
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    four[c][j] = lane + 32 * c < t.n && k4 + j < k1 ? eight_scales(row + 32 * c * p.ld_xs, 8 * (k4 + j), p.blocks, p.wide_xs)
+                                                                    : make_uint2(0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (k4 + j >= k1) break;
+                if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                uint4* to = reinterpret_cast<uint4*>(ring + r.i * stage_bytes + xs_off) + lane;
+                to[0] = make_uint4(four[0][j].x, four[1][j].x, 0, 0);
+                to[32] = make_uint4(four[0][j].y, four[1][j].y, 0, 0);
+                fence_async();
+                __syncwarp();
+                if (lane == 0) bar_arrive(x_full0 + 8 * r.i);
+                r.next(stages);
+            }
         }
     }
     __syncwarp();
