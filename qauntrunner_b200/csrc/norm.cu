@@ -18,11 +18,12 @@ int check_eps(const char* what, float eps) {
 }
 
 // Slots of a ring of rows, `bytes` each, that fit beside the other CTAs of the
-// SM; 0 where fewer than two do.
+// SM; 0 where fewer than two do, or where a CTA has one row only (loads of its
+// own are there sooner: 4.3 us in place of 5.1 for one row of 7168 f32 columns).
 constexpr int kRingRoom = 200 * 1024;   // of an SM's 227 KB
 int ring_slots(int64_t bytes, int ctas_an_sm, int64_t rows_a_cta) {
     const int64_t fit = std::min<int64_t>(kRingRoom / ctas_an_sm / bytes, kNormSlots);
-    return fit < 2 ? 0 : (int)std::min(fit, rows_a_cta);
+    return fit < 2 || rows_a_cta < 2 ? 0 : (int)std::min(fit, rows_a_cta);
 }
 template <typename A>
 cudaError_t launch_ring(void (*kernel)(A), int64_t ctas, int threads, int slots, int64_t bytes, cudaStream_t s, const A& a) {
