@@ -11,12 +11,14 @@
 //
 // Memory bounds both from some hundred rows on.  The CTAs walk the rows; one
 // holds a row in registers, 8 neighbouring columns to a load, so that each row is
-// read once.  Rows that start on 16 bytes come by bulk copies into a ring of
-// `slots` rows in shared memory, several ahead of the one that is worked on: a
-// slot is free again once all threads have its row in registers, which the row's
-// one barrier says.  Other rows are loaded where they are needed.  Rows that do
-// not fit (more than 16384 columns, 8192 in the gradient) are read twice by the
-// same kernels' last form (V = 0).
+// read once.  Rows come by bulk copies into a ring of `slots` rows in shared
+// memory, several ahead of the one that is worked on: a slot is free again once
+// all threads have its row in registers, which the row's barrier says.  A copy
+// starts and ends on 16 bytes, so a row that does not is copied with the bytes
+// around it and shifted into place on its way to registers; such a row goes out
+// by way of shared memory, in words.  Where a CTA has one row, loads of its own
+// are sooner there.  Rows that do not fit (more than 16384 columns, 8192 in the
+// gradient) are read twice by the same kernels' last form (V = 0).
 #pragma once
 #include <type_traits>
 
@@ -115,15 +117,16 @@ __device__ __forceinline__ Raw8<T> load8_again(const T* p, int n) {
 }
 
 // A ring of rows in shared memory: slot i % slots holds the CTA's i-th row of
-// each of N arrays (NULL: none), `bytes` of it.
+// each of N arrays (NULL: none), `bytes` of it, with up to 15 bytes in front of it
+// and behind it.  (Those bytes share 16 aligned ones with the row's own.)
 template <int N>
 struct RowRing {
     const char* from[N];
     long long pitch[N];   // bytes
-    char* at;
+    uint32_t at;          // address in shared memory
     uint64_t* full;
-    int slots, bytes;
-    uint32_t i = 0, parity = 0, here = smem_u32(at);   // of the row that is worked on; its address
+    int slots, bytes, room;   // room: bytes of a row there
+    uint32_t i = 0, parity = 0, here = at;   // of the row that is worked on
     __device__ void init() {
         if (threadIdx.x == 0) {
             for (int k = 0; k < slots; k++) mbar_init(&full[k], 1);
@@ -131,17 +134,23 @@ struct RowRing {
         }
         __syncthreads();
     }
+    __device__ uint32_t offset(int j, uint32_t t) const {   // of row t from 16 bytes
+        return ((uint32_t)reinterpret_cast<uintptr_t>(from[j]) + t * (uint32_t)pitch[j]) & 15;
+    }
     // row t into slot k, by one thread
     __device__ void load(uint32_t k, uint32_t t) {
         uint32_t total = 0;
 #pragma unroll
         for (int j = 0; j < N; j++)
-            if (from[j]) total += bytes;
+            if (from[j]) total += (offset(j, t) + bytes + 15) & ~15u;
         mbar_arrive_expect_tx(&full[k], total);
-        char* to = at + (size_t)k * N * bytes;
 #pragma unroll
-        for (int j = 0; j < N; j++, to += bytes)
-            if (from[j]) bulk_g2s(to, from[j] + t * pitch[j], bytes, &full[k]);
+        for (int j = 0; j < N; j++)
+            if (from[j])
+                asm volatile(
+                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(at + (k * N + j) * room),
+                    "l"(from[j] + (long long)t * pitch[j] - offset(j, t)), "r"((offset(j, t) + bytes + 15) & ~15u), "r"(smem_u32(&full[k]))
+                    : "memory");
     }
     __device__ void start(uint32_t rows) {
         if (threadIdx.x == 0)
@@ -153,28 +162,83 @@ struct RowRing {
     __device__ void next(uint32_t t, uint32_t rows) {
         const unsigned long long ahead = t + (unsigned long long)slots * gridDim.x;
         if (threadIdx.x == 0 && ahead < rows) load(i, (uint32_t)ahead);
-        here += N * bytes;
+        here += N * room;
         if (++i == (uint32_t)slots) {
             i = 0;
             parity ^= 1;
-            here = smem_u32(at);
+            here = at;
         }
     }
-    // the n columns at c of array j (the others are 0); a row's 16 bytes are whole, so n is 0, 8 or, in f32, 4
-    template <typename T>
-    __device__ Raw8<T> row(int j, int c, int n) const {
-        Raw8<T> r;
-        const uint32_t p = here + j * bytes + c * (int)sizeof(T);
+    // the n columns at c (the others are 0) of array j's row t; WHOLE: rows start and end on 16 bytes
+    template <typename T, bool WHOLE>
+    __device__ Raw8<T> row(int j, uint32_t t, int c, int n) const {
+        constexpr int W = 2 * (int)sizeof(T);   // words of eight columns
+        const uint32_t off = WHOLE ? 0 : offset(j, t), p = here + j * room + c * (int)sizeof(T);
+        uint32_t w[W + 4];
 #pragma unroll
-        for (int k = 0; k < (int)sizeof(T) / 2; k++) {
-            uint4 a = make_uint4(0, 0, 0, 0);
-            if (n * (int)sizeof(T) > 16 * k)
-                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w) : "r"(p + 16 * k) : "memory");
-            r.w[4 * k] = a.x; r.w[4 * k + 1] = a.y; r.w[4 * k + 2] = a.z; r.w[4 * k + 3] = a.w;
+        for (int k = 0; k < (WHOLE ? W : W + 4); k += 4) {
+            w[k] = w[k + 1] = w[k + 2] = w[k + 3] = 0;
+            if (n && n * (int)sizeof(T) + (int)off > 4 * k)
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[k]), "=r"(w[k + 1]), "=r"(w[k + 2]), "=r"(w[k + 3])
+                             : "r"(p + 4 * k)
+                             : "memory");
+        }
+        if (!WHOLE && off) {   // (the same for all threads)
+            if (off & 8) {
+#pragma unroll
+                for (int k = 0; k < W + 2; k++) w[k] = w[k + 2];
+            }
+            if (off & 4) {
+#pragma unroll
+                for (int k = 0; k < W + 1; k++) w[k] = w[k + 1];
+            }
+            if (off & 2) {
+#pragma unroll
+                for (int k = 0; k < W; k++) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+            }
+        }
+        Raw8<T> r;
+#pragma unroll
+        for (int k = 0; k < W; k++) r.w[k] = w[k];
+        if (!WHOLE && n < 8) {
+#pragma unroll
+            for (int k = 0; k < W; k++) {
+                if (sizeof(T) == 4) r.w[k] = k < n ? r.w[k] : 0;
+                else r.w[k] = 2 * k + 1 < n ? r.w[k] : 2 * k < n ? r.w[k] & 0xffffu : 0;
+            }
         }
         return r;
     }
 };
+
+// A row's way out when it does not start on 16 bytes: its columns into shared
+// memory, then, behind a barrier, `bytes` of them to p by all threads, in words
+// but for the ends.
+template <int W>   // words
+__device__ __forceinline__ void to_room(uint32_t at, const uint32_t (&w)[W]) {
+    if constexpr (W == 2) {
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(w[0]), "r"(w[1]) : "memory");
+    } else {
+#pragma unroll
+        for (int k = 0; k < W; k += 4)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + 4 * k), "r"(w[k]), "r"(w[k + 1]), "r"(w[k + 2]), "r"(w[k + 3])
+                         : "memory");
+    }
+}
+__device__ __forceinline__ uint32_t room_word(uint32_t at) {   // four bytes at any address
+    uint32_t lo, hi;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(lo) : "r"(at & ~3u) : "memory");
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(hi) : "r"((at & ~3u) + 4) : "memory");
+    return __funnelshift_r(lo, hi, 8 * (at & 3));
+}
+__device__ __forceinline__ void room_to(void* to, uint32_t room, int bytes) {
+    char* p = static_cast<char*>(to);
+    const int head = min((int)(-reinterpret_cast<intptr_t>(p) & 3), bytes), words = (bytes - head) >> 2, tail = head + 4 * words;
+    for (int k = threadIdx.x; k < words; k += blockDim.x) *reinterpret_cast<uint32_t*>(p + head + 4 * k) = room_word(room + head + 4 * k);
+    if ((int)threadIdx.x < head) p[threadIdx.x] = (char)room_word(room + threadIdx.x);
+    if ((int)threadIdx.x < bytes - tail) p[tail + threadIdx.x] = (char)room_word(room + tail + threadIdx.x);
+}
 
 template <typename T>
 struct NormArgs {
@@ -185,9 +249,10 @@ struct NormArgs {
     void* scales;            // f32, or e8m0 bytes
     long long ld_x, ld_add, ld_sum, ld_y, ld_c, ld_s;
     int rows, d;
-    int slots;                   // of the ring, 0: rows are loaded where they are needed
+    int slots, room;             // of the ring (0: rows are loaded where they are needed), bytes of a row in it
+    int sum_room, y_room, c_room;   // where in shared memory a row of it is put on its way out, 0: it is written as it is
     float eps, per_d;            // per_d: 1 / d
-    bool wide, wide_w, wide_c;   // rows (weights, codes) start on 16 (16, 8 or 4) bytes
+    bool wide, wide_sum, wide_y, wide_w, wide_c;   // rows start on 16 bytes (wide: those that are read)
 };
 
 // s of eight columns as it is stored: x, or x + add rounded
@@ -220,8 +285,9 @@ __device__ __forceinline__ Vec8 weight8(const float* w, int c, int n, bool wide)
 }
 // y of a thread's 8 V neighbouring columns from c on (of those that do not exist
 // s is 0, and so is y) to where it goes.  All 32 lanes take part.
-template <typename T, int OUT, int V>
-__device__ __forceinline__ void norm_out(const NormArgs<T>& a, long long t, const Pairs8 (&s)[V], const Pairs8 (&w)[V], float inv, int c) {
+template <typename T, int OUT, int V, bool WHOLE>
+__device__ __forceinline__ void norm_out(const NormArgs<T>& a, uint32_t smem, long long t, const Pairs8 (&s)[V], const Pairs8 (&w)[V],
+                                         float inv, int c) {
     Pairs8 y[V];   // negated where they are to become 8-bit codes
     const Pair f = both(OUT == kNorm8 ? -inv : inv);
 #pragma unroll
@@ -237,7 +303,8 @@ __device__ __forceinline__ void norm_out(const NormArgs<T>& a, long long t, cons
 #pragma unroll
                 for (int i = 0; i < 4; i++) z.p[i] = negative(z.p[i]);
             }
-            if (n) store_raw8(a.y + t * a.ld_y + c + 8 * v, rounded8<T>(z), n, a.wide);
+            if (!WHOLE && a.y_room) to_room(smem + a.y_room + (c + 8 * v) * (int)sizeof(T), rounded8<T>(z).w);
+            else if (n) store_raw8(a.y + t * a.ld_y + c + 8 * v, rounded8<T>(z), n, a.wide_y);
         }
     }
     if (OUT == kNormTyped) return;
@@ -256,7 +323,13 @@ __device__ __forceinline__ void norm_out(const NormArgs<T>& a, long long t, cons
 #pragma unroll
         for (int v = 0; v < V; v++) codes[v] = scale < kFp8Tiny ? codes8_divided(y[v], scale) : codes8(y[v], q);
         uint8_t* to = a.codes + t * a.ld_c + c;
-        if (V > 1 && a.wide_c && c + 8 * V <= a.d) {
+        if (!WHOLE && a.c_room) {
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                const uint32_t e[2] = {codes[v].x, codes[v].y};
+                to_room(smem + a.c_room + c + 8 * v, e);
+            }
+        } else if (V > 1 && a.wide_c && c + 8 * V <= a.d) {
 #pragma unroll
             for (int v = 0; v < V / 2; v++)
                 reinterpret_cast<uint4*>(to)[v] = make_uint4(codes[2 * v].x, codes[2 * v].y, codes[2 * v + 1].x, codes[2 * v + 1].y);
@@ -300,17 +373,19 @@ __device__ __forceinline__ float norm_factor(float total, float per_d, float eps
 
 // A row of 8 V neighbouring columns a thread (0: of any length, read twice).  sum
 // may be x or add, y any of them: a thread has read a column before it writes it,
-// and a row is copied ahead of others only.
-template <typename T, int OUT, int V>
+// and a row is copied ahead of others only.  WHOLE: all rows start and end on 16
+// bytes (the code for others costs these a tenth of their time).
+template <typename T, int OUT, int V, bool WHOLE>
 __global__ void __launch_bounds__(kNormThreads)
 rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
     extern __shared__ __align__(16) char ring_mem[];
     __shared__ uint64_t full[kNormSlots];
     __shared__ float scratch[2][1][32];   // two rows' turns
+    const uint32_t smem = smem_u32(ring_mem);
     if constexpr (V > 0) {
         const int c = 8 * V * threadIdx.x;
         RowRing<2> ring{{reinterpret_cast<const char*>(a.x), reinterpret_cast<const char*>(a.add)},
-                        {a.ld_x * (long long)sizeof(T), a.ld_add * (long long)sizeof(T)}, ring_mem, full, a.slots, a.d * (int)sizeof(T)};
+                        {a.ld_x * (long long)sizeof(T), a.ld_add * (long long)sizeof(T)}, smem, full, a.slots, a.d * (int)sizeof(T), a.room};
         if (a.slots) ring.init();
         pdl_start();
         if (a.slots) ring.start(a.rows);
@@ -325,22 +400,31 @@ rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const int at = c + 8 * i, n = columns_at(at, a.d);
-                raw[i] = a.slots ? ring.template row<T>(0, at, n) : load_raw8(a.x + t * a.ld_x + at, n, a.wide);
-                if (a.add) more[i] = a.slots ? ring.template row<T>(1, at, n) : load_raw8(a.add + t * a.ld_add + at, n, a.wide);
+                raw[i] = a.slots ? ring.template row<T, WHOLE>(0, t, at, n) : load_raw8(a.x + t * a.ld_x + at, n, a.wide);
+                if (a.add) more[i] = a.slots ? ring.template row<T, WHOLE>(1, t, at, n) : load_raw8(a.add + t * a.ld_add + at, n, a.wide);
             }
             Pair part = 0;
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const int at = c + 8 * i, n = columns_at(at, a.d);
                 if (a.add) raw[i] = norm_sum(a, raw[i], more[i]);
-                if (a.sum && n) store_raw8(a.sum + t * a.ld_sum + at, raw[i], n, a.wide);
+                if (!WHOLE && a.sum_room) to_room(smem + a.sum_room + at * (int)sizeof(T), raw[i].w);
+                else if (a.sum && n) store_raw8(a.sum + t * a.ld_sum + at, raw[i], n, a.wide_sum);
                 s[i] = values8(raw[i]);
                 part = squares(s[i], part);
             }
             float total[1] = {joined(part)};
             cta_sum(total, scratch[turn]);   // (one barrier a row: the turns keep a row's sum from the next one's)
             if (a.slots) ring.next(t, a.rows);
-            norm_out<T, OUT, V>(a, t, s, w, norm_factor(total[0], a.per_d, a.eps), c);
+            if (!WHOLE && a.sum_room) room_to(a.sum + t * a.ld_sum, smem + a.sum_room, a.d * (int)sizeof(T));
+            norm_out<T, OUT, V, WHOLE>(a, smem, t, s, w, norm_factor(total[0], a.per_d, a.eps), c);
+            if (!WHOLE && (a.sum_room | a.y_room | a.c_room)) {
+                // What is in shared memory goes out.  It is written again behind the next row's barrier, but for the sum,
+                // which is out by this one.
+                __syncthreads();
+                if (a.y_room) room_to(a.y + t * a.ld_y, smem + a.y_room, a.d * (int)sizeof(T));
+                if (a.c_room) room_to(a.codes + t * a.ld_c, smem + a.c_room, a.d);
+            }
         }
     } else {
         pdl_start();
@@ -353,7 +437,7 @@ rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
             const int n = columns_at(c, a.d);
             const Raw8<T> raw = load_raw8(x + c, n, a.wide);
             const Raw8<T> s = norm_sum(a, raw, add ? load_raw8(add + c, n, a.wide) : raw);
-            if (a.sum) store_raw8(a.sum + t * a.ld_sum + c, s, n, a.wide);
+            if (a.sum) store_raw8(a.sum + t * a.ld_sum + c, s, n, a.wide_sum);
             part = squares(values8(s), part);
         }
         float total[1] = {joined(part)};
@@ -368,7 +452,7 @@ rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
                 if (add) raw = norm_sum(a, raw, load8_again(add + c, n));
             }
             const Pairs8 s[1] = {values8(raw)}, w[1] = {norm_weight(a.w, c, n, a.wide_w)};
-            norm_out<T, OUT, 1>(a, t, s, w, inv, c);
+            norm_out<T, OUT, 1, WHOLE>(a, 0, t, s, w, inv, c);
         }
     }
 }
@@ -381,14 +465,14 @@ struct NormGradArgs {
     float* part;             // [gridDim.x][d] sums over a CTA's rows, or NULL
     long long ld_dy, ld_x, ld_add, ld_dx;
     int rows, d;
-    int slots;               // as in NormArgs
+    int slots, room, dx_room;   // as in NormArgs
     float eps, per_d;
-    bool wide, wide_w, wide_part;
+    bool wide, wide_dx, wide_w, wide_part;
 };
 
 // A thread keeps its 8 V columns' weights and their sums over the rows in
 // registers.
-template <typename T, int V>
+template <typename T, int V, bool WHOLE>
 __global__ void __launch_bounds__(kNormThreads)
 rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
     extern __shared__ __align__(16) char ring_mem[];
@@ -396,9 +480,10 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
     __shared__ float scratch[2][2][32];   // two rows' turns
     int turn = 0;
     if constexpr (V > 0) {
+        const uint32_t smem = smem_u32(ring_mem);
         RowRing<3> ring{{reinterpret_cast<const char*>(a.x), reinterpret_cast<const char*>(a.dy), reinterpret_cast<const char*>(a.add)},
                         {a.ld_x * (long long)sizeof(T), a.ld_dy * (long long)sizeof(T), a.ld_add * (long long)sizeof(T)},
-                        ring_mem, full, a.slots, a.d * (int)sizeof(T)};
+                        smem, full, a.slots, a.d * (int)sizeof(T), a.room};
         if (a.slots) ring.init();
         pdl_start();
         if (a.slots) ring.start(a.rows);
@@ -417,9 +502,9 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const int at = c + 8 * i, n = columns_at(at, a.d);
-                x[i] = values8(a.slots ? ring.template row<T>(0, at, n) : load_raw8(a.x + t * a.ld_x + at, n, a.wide));
-                dy[i] = values8(a.slots ? ring.template row<T>(1, at, n) : load_raw8(a.dy + t * a.ld_dy + at, n, a.wide));
-                if (a.add) add[i] = a.slots ? ring.template row<T>(2, at, n) : load_raw8(a.add + t * a.ld_add + at, n, a.wide);
+                x[i] = values8(a.slots ? ring.template row<T, WHOLE>(0, t, at, n) : load_raw8(a.x + t * a.ld_x + at, n, a.wide));
+                dy[i] = values8(a.slots ? ring.template row<T, WHOLE>(1, t, at, n) : load_raw8(a.dy + t * a.ld_dy + at, n, a.wide));
+                if (a.add) add[i] = a.slots ? ring.template row<T, WHOLE>(2, t, at, n) : load_raw8(a.add + t * a.ld_add + at, n, a.wide);
             }
             Pair square = 0, product = 0;
 #pragma unroll
@@ -448,7 +533,12 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) dx.p[j] = add2(dx.p[j], more.p[j]);
                 }
-                if (n) store_raw8(a.dx + t * a.ld_dx + at, rounded8<T>(dx), n, a.wide);
+                if (!WHOLE && a.dx_room) to_room(smem + a.dx_room + at * (int)sizeof(T), rounded8<T>(dx).w);
+                else if (n) store_raw8(a.dx + t * a.ld_dx + at, rounded8<T>(dx), n, a.wide_dx);
+            }
+            if (!WHOLE && a.dx_room) {   // (written again behind the next row's barrier)
+                __syncthreads();
+                room_to(a.dx + t * a.ld_dx, smem + a.dx_room, a.d * (int)sizeof(T));
             }
         }
 #pragma unroll
@@ -489,7 +579,7 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
                     if (a.add) dx.v[j] += add.v[j];
                     if (part && j < n) part[c + j] = fmaf(dy.v[j], nrm, first ? 0.f : part[c + j]);
                 }
-                store8(a.dx + t * a.ld_dx + c, dx, n, a.wide);
+                store8(a.dx + t * a.ld_dx + c, dx, n, a.wide_dx);
             }
             first = false;
         }
