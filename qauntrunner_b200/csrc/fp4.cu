@@ -39,7 +39,22 @@ void release(qrm_fp4* m) {
     delete m;
 }
 
-size_t fit_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4FitStages * kFp4FitStage + 2 * kFp4FitRoom; }
+// room for rows of x in a stage, stages, shared memory of a CTA
+struct Fit {
+    static constexpr int kMost = kSmemMost - 256;   // (the kernel has some of its own)
+    int rows, stages;
+    size_t smem;
+    Fit(int groups, int64_t T) {
+        // a third more rows in a tile than a group has on average: smaller stages leave room for more of them
+        const int64_t used = std::min<int64_t>(T, groups), each = (T + used - 1) / used;
+        int64_t most = groups > 1 ? each * 3 / 2 : each;
+        if (const char* e = getenv("FITCAP")) most = atoi(e);
+        rows = (int)std::max<int64_t>(64, std::min<int64_t>(kFp4FitRows, (most + 31) / 32 * 32));
+        const int rest = 1024 + fp4_pair_stage_off(groups) + 2 * kFp4FitRoom;
+        stages = std::min(kFp4FitMaxStages, (kMost - rest) / fp4_fit_stage(rows));
+        smem = rest + (size_t)stages * fp4_fit_stage(rows);
+    }
+};
 size_t pair_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4PairStages * kFp4PairStage + 8 * kFp4PairOut; }
 
 template <int MODE>
@@ -48,7 +63,7 @@ cudaError_t prepare_kernels() {
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(fp4_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(kFp4MaxGroups));
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(fp4_fit_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)fit_smem(kFp4MaxGroups));
+        e = cudaFuncSetAttribute(fp4_fit_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fit::kMost);
     return e;
 }
 // registers a thread that the pair kernels were built with: their split may not pass what a launch has
@@ -56,7 +71,7 @@ template <int MODE>
 bool enough_regs() {
     cudaFuncAttributes pair{}, fit{};
     return cudaFuncGetAttributes(&pair, fp4_pair_kernel<MODE>) == cudaSuccess && pair.numRegs * kFp4PairThreads >= kFp4PairRegs &&
-           cudaFuncGetAttributes(&fit, fp4_fit_kernel<MODE>) == cudaSuccess && fit.numRegs * kFp4PairThreads >= kFp4FitRegs;
+           cudaFuncGetAttributes(&fit, fp4_fit_kernel<MODE>) == cudaSuccess && fit.numRegs * kFp4FitThreads >= kFp4FitRegs;
 }
 
 int create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes, const void* scales,
@@ -167,9 +182,11 @@ Fp4Form form_of(int64_t T, int groups) {
 template <int MODE>
 cudaError_t launch(const qrm_fp4* m, const Fp4RowMaps& x_maps, Fp4Params& p, Fp4Form form, int wide_out, int64_t T, cudaStream_t s) {
     const CUtensorMap& w_map = MODE == kFp4Plain ? m->map : m->gated_map;
-    if (form == kFit)
-        return launch_ahead(fp4_fit_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, fit_smem(m->groups), s, w_map,
-                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps, p, wide_out);
+    if (form == kFit) {
+        const Fit fit(m->groups, T);
+        return launch_ahead(fp4_fit_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4FitThreads, fit.smem, s, w_map,
+                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps, p, wide_out, fit.stages, fit.rows);
+    }
     if (form == kPair)
         return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, w_map,
                             MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps.rows[3], p, wide_out);

@@ -113,21 +113,41 @@ __device__ __forceinline__ void load_weights_pair(uint32_t dst, const CUtensorMa
 // what this thread wrote to shared memory is there for copies and MMAs
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// the eight scales of a row from block b on (0 for those past the last)
-__device__ __forceinline__ uint2 eight_scales(const uint8_t* __restrict__ row, int b, int blocks, bool wide) {
-    if (wide && b + 8 <= blocks) return __ldg(reinterpret_cast<const uint2*>(row + b));
-    uint32_t w[2] = {0, 0};
+// 4 N scales of a row from block b on (0 for those past the last).  Rows start
+// anywhere, so the whole words around the bytes are read and shifted; a word that
+// holds none of the row's bytes is not touched.
+template <int N>
+__device__ __forceinline__ void some_scales(const uint8_t* __restrict__ row, int b, int blocks, uint32_t (&out)[N]) {
+    const uint8_t* at = row + b;
+    const int in = (int)(reinterpret_cast<uintptr_t>(at) & 3), have = blocks - b;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(at - in);
+    uint32_t w[N + 1];
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (b + i < blocks) w[i >> 2] |= (uint32_t)__ldg(row + b + i) << (8 * (i & 3));
+    for (int i = 0; i <= N; i++) w[i] = 4 * i - in < have ? __ldg(words + i) : 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        out[i] = __funnelshift_r(w[i], w[i + 1], 8 * in);
+        const int left = have - 4 * i;
+        if (left < 4) out[i] = left > 0 ? out[i] & ((1u << (8 * left)) - 1) : 0;
+    }
+}
+// eight of them; wide: 2 when rows start on 16 bytes, 1 on 8
+__device__ __forceinline__ uint2 eight_scales(const uint8_t* __restrict__ row, int b, int blocks, int wide) {
+    if (wide && b + 8 <= blocks) return __ldg(reinterpret_cast<const uint2*>(row + b));
+    uint32_t w[2];
+    some_scales(row, b, blocks, w);
     return make_uint2(w[0], w[1]);
 }
-
-// sixteen of them; wide: 2 when rows start on 16 bytes, 1 on 8
+// sixteen, b a multiple of 16
 __device__ __forceinline__ uint4 sixteen_scales(const uint8_t* __restrict__ row, int b, int blocks, int wide) {
-    if (wide == 2 && b + 16 <= blocks) return __ldg(reinterpret_cast<const uint4*>(row + b));
-    const uint2 lo = eight_scales(row, b, blocks, wide), hi = eight_scales(row, b + 8, blocks, wide);
-    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    if (wide && b + 16 <= blocks) {
+        if (wide == 2) return __ldg(reinterpret_cast<const uint4*>(row + b));
+        const uint2 lo = __ldg(reinterpret_cast<const uint2*>(row + b)), hi = __ldg(reinterpret_cast<const uint2*>(row + b + 8));
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+    uint32_t w[4];
+    some_scales(row, b, blocks, w);
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 __device__ __forceinline__ float2 gated2(float2 gate, float2 up, float limit) {
@@ -808,26 +828,39 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
 
 // ------------------------------------------------------------ pairs with weights on the MMA's M side
 // The same pair of SMs with the operands' places changed: 256 outputs (gated: 128
-// features) on the M side, up to 256 rows of x on the N side, rounded up to 32
+// features) on the M side, up to 384 rows of x on the N side, rounded up to 32
 // only and shared evenly among a group's tiles.  Groups whose rows are no
-// multiple of 256 cost what their rows cost.
+// multiple of 256 cost what their rows cost, and the weights of a group of up to
+// 384 rows are loaded once.  Past 256 rows a step takes two MMAs, of 128 rows and
+// of the others.
 //
 // A lane of tensor memory is an output, so rows go out by way of shared memory:
 // 32 rows of x at a time, [row][output] in f32, written by the lanes' columns and
 // read along the rows.  For the gated product the lanes of gate and of up
 // exchange half of their columns first, so that each has both sums of 16 rows.
 //
+// Two accumulators where two neighbouring tiles have 224 rows at most; else a
+// tile's MMAs wait for the one before to be read.
+//
+// The scales of x go through registers, and a fence between what they write to
+// shared memory and the copy to tensor memory waits for loads of the same warp
+// that are on their way (a quarter of the time went there).  So the warps that
+// load and write them do not fence: they tell another one, which does.
+//
 // Warps: 0 loads codes and the weights' scales, 1 issues the MMAs (in the
-// pair's first CTA), 2 and 3 bring the scales of x (128 rows each, in both CTAs),
-// 4-7 and 8-11 write the output, every second 32 rows each.
-constexpr int kFp4FitStages = 5;
-constexpr int kFp4FitScalesW = 2 * kFp4Tile;                         // in a stage: codes of the weights, of x, scales
-constexpr int kFp4FitScalesX = kFp4FitScalesW + kFp4Scales;
-constexpr int kFp4FitStage = kFp4FitScalesX + 2 * kFp4Scales;
+// pair's first CTA), 2 fences, 4-7 bring the scales of x (in both CTAs), 8-11 and
+// 12-15 write the output, every second 32 rows each.
+constexpr int kFp4FitThreads = 512;
+constexpr int kFp4FitMaxStages = 8;
+constexpr int kFp4FitRows = 384;
+constexpr int kFp4FitSecond = 224, kFp4FitTmemScales = 448, kFp4FitScaleCols = 32;
 constexpr int kFp4FitRoom = 32 * 132 * 4;      // four warps' room for 32 rows on their way out
-constexpr int kFp4FitRegsFew = 104, kFp4FitRegsMany = 200;
-constexpr int kFp4FitRegs = 128 * kFp4FitRegsFew + 256 * kFp4FitRegsMany;
-static_assert(kFp4FitRegs <= kFp4PairThreads * 168, "register split");
+constexpr int kFp4FitRegsFew = 56, kFp4FitRegsMany = 200;
+constexpr int kFp4FitRegs = 256 * kFp4FitRegsFew + 256 * kFp4FitRegsMany;
+static_assert(kFp4FitRegs <= kFp4FitThreads * 128, "register split");
+// a stage: codes of the weights, of x (a CTA's half of up to `rows`, the most that a tile has), scales of the weights, of x
+__host__ __device__ inline int fp4_fit_codes(int rows) { return kFp4Tile + rows / 2 * 128; }
+__host__ __device__ inline int fp4_fit_stage(int rows) { return fp4_fit_codes(rows) + kFp4Scales + (rows + 127) / 128 * kFp4Scales; }
 
 struct Fp4RowMaps {
     CUtensorMap rows[4];   // x in boxes of 256 columns x 16, 32, 64 and 128 rows
@@ -904,35 +937,39 @@ __device__ __forceinline__ void room_out(const Fp4Params& p, const float* room, 
 }
 
 template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp4PairThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp4FitThreads, 1)
 fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap s_map,
-               const __grid_constant__ Fp4RowMaps x_maps, const __grid_constant__ Fp4Params p, int wide_out) {
+               const __grid_constant__ Fp4RowMaps x_maps, const __grid_constant__ Fp4Params p, int wide_out, int stages,
+               int x_rows /* most rows of x in a tile */) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // first CTA: both CTAs' copies are there
-    uint64_t* x_full = full + kFp4FitStages;            // first CTA: both CTAs' scales of x are there
-    uint64_t* done = x_full + kFp4FitStages;            // both: the stage's MMAs are done
-    uint64_t* tile_done = done + kFp4FitStages;         // [2] both: a tile's are
+    uint64_t* x_full = full + kFp4FitMaxStages;         // first CTA: both CTAs' scales of x are there
+    uint64_t* x_written = x_full + kFp4FitMaxStages;    // its own are written
+    uint64_t* done = x_written + kFp4FitMaxStages;      // both: the stage's MMAs are done
+    uint64_t* tile_done = done + kFp4FitMaxStages;         // [2] both: a tile's are
     uint64_t* tile_read = tile_done + 2;                // [2] first CTA: both epilogues have read an accumulator
     uint64_t* done_bar = tile_read + 2;
     uint64_t* left_bar = done_bar + 1;                  // both, when the first CTA gave up: its commits are through
     __shared__ volatile int given_up;
     __shared__ volatile uint32_t from_peer, issued;     // issued: stages, once their warp is through
-    __shared__ volatile uint32_t bytes[kFp4FitStages];
+    __shared__ volatile uint32_t bytes[kFp4FitMaxStages];
     volatile int* abort_flag = &given_up;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 776);
     int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp4PairTableOff);
     int32_t* start = first_tile + p.groups + 1;
     int32_t* rows = start + p.groups + 1;
     uint8_t* ring = sm + fp4_pair_stage_off(p.groups);
+    const uint32_t stage_bytes = fp4_fit_stage(x_rows), ws_off = fp4_fit_codes(x_rows), xs_off = ws_off + kFp4Scales;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = blockIdx.x & 1;   // in the pair: the cluster is two CTAs along x
     constexpr int kHalf = MODE == kFp4Plain ? 128 : 64;   // outputs of a CTA in a tile
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kFp4FitStages; i++) {
+        for (int i = 0; i < stages; i++) {
             mbar_init(&full[i], 1);
-            mbar_init(&x_full[i], 4);
+            mbar_init(&x_full[i], 2);
+            mbar_init(&x_written[i], 4);
             mbar_init(&done[i], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -950,7 +987,7 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     pdl_start();   // nothing before this reads or writes global memory
-    if (warp == 2) group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows, 256, (p.M + 2 * kHalf - 1) / (2 * kHalf), blockIdx.x == 0);
+    if (warp == 2) group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows, x_rows, (p.M + 2 * kHalf - 1) / (2 * kHalf), blockIdx.x == 0);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();   // the peer's barriers are ready
@@ -973,12 +1010,14 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             if (first_tile[mid] <= i) lo = mid;
             else hi = mid;
         }
-        const int blocks = (rows[lo] + 255) >> 8, in = i - first_tile[lo], m = in / blocks;
+        const int blocks = (rows[lo] + x_rows - 1) / x_rows, in = i - first_tile[lo], m = in / blocks;
         const int per = ((rows[lo] + blocks - 1) / blocks + 31) & ~31, at = (in - m * blocks) * per, n = min(per, rows[lo] - at);
         return Tile{lo, m * 2 * kHalf, start[lo] + at, n, (n + 31) & ~31};
     };
 
-    if (warp < 4) {
+    // where in tensor memory a pair's n-th tile is
+    auto place = [](uint32_t n, int cols) { return (n & 1) && cols <= kFp4FitSecond ? kFp4FitSecond : 0; };
+    if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp4FitRegsFew));
         if (warp == 0) {
             // -------------------------------------------- codes and the weights' scales
@@ -988,26 +1027,32 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
                 const Tile t = tile_at(i);
-                const int m = t.m + kHalf * (int)rank, mine = t.cols >> 1, pos = t.pos + mine * (int)rank;
-                const int s0 = (t.group * p.units + m / kHalf) * steps * 4;
-                const uint32_t share = kFp4Tile + mine * 128 + kFp4Scales;
+                const int m = t.m + kHalf * (int)rank, first = t.cols > 256 ? 128 : t.cols;
+                const uint32_t share = kFp4Tile + (t.cols >> 1) * 128 + kFp4Scales;
+                // A copy for each lane: 0 the weights', 1 their scales, 2-5 and 6-9 this CTA's halves of the MMAs' rows of x,
+                // a box for each power of two in their number.  (One thread with a loop over the boxes took up to 0.5 us a
+                // stage; boxes of 16 rows cost more to issue than to load.)
+                const int part = lane >= 6, box = (lane - 2) & 3, rows_of = (part ? t.cols - first : first) >> 1;
+                const bool copies = lane < 2 || (lane < 10 && rows_of >> box & 16);
+                const int below = rows_of & ((16 << box) - 1);   // rows of the boxes before
+                const CUtensorMap* map = lane == 1 ? &s_map : &x_maps.rows[box];
+                const uint32_t offset = lane == 1 ? ws_off : kFp4Tile + 128 * ((part ? first >> 1 : 0) + below);
+                int x = 0, y = lane == 1 ? (t.group * p.units + m / kHalf) * steps * 4 : t.pos + (part ? first : 0) + rows_of * (int)rank + below;
+                const int x_step = lane == 1 ? 0 : 128, y_step = lane == 1 ? 4 : 0;
                 for (int k = 0; k < steps; k++) {
                     if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
-                    if (elect_one()) {
-                        const uint32_t st = ring0 + r.i * kFp4FitStage, bar = full0 + 8 * r.i;
+                    const uint32_t st = ring0 + r.i * stage_bytes, bar = full0 + 8 * r.i;
+                    if (lane == 0) {
                         bytes[r.i] = share;
                         if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * share);
                         load_weights_pair<MODE != kFp4Plain>(st, &w_map, k * 128, m, t.group, bar);
-                        tma_pair_2d(st + kFp4FitScalesW, &s_map, 0, s0 + 4 * k, bar);
-                        // (a box for each power of two in the number of rows: 16 rows a box cost more to issue than to load)
-                        for (int b = 0, at = 0; b < 4; b++)
-                            if (mine >> b & 16) {
-                                tma_pair_2d(st + kFp4Tile + 128 * at, &x_maps.rows[b], k * 128, pos + at, bar);
-                                at += 16 << b;
-                            }
+                    } else if (copies) {
+                        tma_pair_2d(st + offset, map, x, y, bar);
                     }
+                    x += x_step;
+                    y += y_step;
                     __syncwarp();
-                    r.next(kFp4FitStages);
+                    r.next(stages);
                     n_issued++;
                 }
             }
@@ -1017,39 +1062,45 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             bool ok = true;
             Ring r;
             uint32_t n = 0, buffer = 0;   // tiles; of scales
-            int before = 0;               // columns of the tile before
+            int before = 0, before_end = 0;   // the columns of the tile before
             const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), ring0 = smem_u32(ring), read0 = smem_u32(tile_read);
             const uint64_t w_desc = sw128_desc(ring0), x_desc = sw128_desc(ring0 + kFp4Tile);
-            const uint64_t ws_desc = scale_desc(ring0 + kFp4FitScalesW), xs_desc = scale_desc(ring0 + kFp4FitScalesX);
+            const uint64_t ws_desc = scale_desc(ring0 + ws_off), xs_desc = scale_desc(ring0 + xs_off);
             const uint32_t odd = umma_idesc_mxf4(0, 0, 2) & ~umma_idesc_mxf4(0, 0, 0);
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs, n++) {
                 const Tile t = tile_at(i);
-                const uint32_t a = n & 1, d = tmem + (a ? kFp4PairSecond : 0), idesc = umma_idesc_mxf4(256, t.cols, 0);
-                // this accumulator has been read, and the other one where the two overlap
+                const uint32_t a = n & 1;
+                const int at_col = place(n, t.cols), first = t.cols > 256 ? 128 : t.cols;
+                const uint32_t d = tmem + at_col, idesc = umma_idesc_mxf4(256, first, 0), idesc2 = umma_idesc_mxf4(256, t.cols - first, 0);
+                // the columns have been read: of the tile two before, and of the one before where they are the same
                 if (n > 1 && !bar_wait(read0 + 8 * a, ((n >> 1) - 1) & 1u, ctl)) break;
-                if (n > 0 && (a ? before : t.cols) > kFp4PairSecond && !bar_wait(read0 + 8 * (a ^ 1), ((n - 1) >> 1) & 1u, ctl)) break;
-                before = t.cols;
+                if (n > 0 && before < at_col + t.cols && at_col < before_end && !bar_wait(read0 + 8 * (a ^ 1), ((n - 1) >> 1) & 1u, ctl)) break;
+                before = at_col;
+                before_end = at_col + t.cols;
                 for (int k = 0; k < steps; k++) {
                     if (!bar_wait(full0 + 8 * r.i, r.phase, ctl) || !bar_wait(x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
                     tc_fence_after();
                     if (elect_one()) {
-                        const uint32_t at = r.i * (kFp4FitStage >> 4);
-                        const uint32_t ws = tmem + kFp4PairTmemScales + kFp4ScaleCols * buffer, xs = ws + 8;
+                        const uint32_t at = r.i * stage_bytes >> 4;
+                        const uint32_t ws = tmem + kFp4FitTmemScales + kFp4FitScaleCols * buffer, xs = ws + 8;   // of x: 12 columns a half
 #pragma unroll
                         for (int u = 0; u < 2; u++) {   // half of the stage's contracted values
                             scales_to_tmem<2>(ws + 4 * u, ws_desc + at + u * (512 >> 4));
-                            scales_to_tmem<2>(xs + 8 * u, xs_desc + at + u * (512 >> 4));
-                            if (t.cols > 128) scales_to_tmem<2>(xs + 8 * u + 4, xs_desc + at + (kFp4Scales + u * 512 >> 4));
+                            for (int v = 0; 128 * v < t.cols; v++) scales_to_tmem<2>(xs + 12 * u + 4 * v, xs_desc + at + (v * kFp4Scales + u * 512 >> 4));
                         }
 #pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            umma_mxf4<2>(d, w_desc + at + 2 * j, x_desc + at + 2 * j, j & 1 ? idesc | odd : idesc, ws + 4 * (j >> 1),
-                                         xs + 8 * (j >> 1), k > 0 || j > 0);
+                        for (int j = 0; j < 4; j++) {
+                            const uint32_t half = j & 1 ? odd : 0;
+                            umma_mxf4<2>(d, w_desc + at + 2 * j, x_desc + at + 2 * j, idesc | half, ws + 4 * (j >> 1), xs + 12 * (j >> 1), k > 0 || j > 0);
+                            if (t.cols > 256)
+                                umma_mxf4<2>(d + 128, w_desc + at + 2 * j, x_desc + at + (64 * 128 >> 4) + 2 * j, idesc2 | half, ws + 4 * (j >> 1),
+                                             xs + 12 * (j >> 1) + 4, k > 0 || j > 0);
+                        }
                         umma_commit_pair(done0 + 8 * r.i);
                         if (k + 1 == steps) umma_commit_pair(smem_u32(tile_done) + 8 * a);
                     }
                     __syncwarp();
-                    r.next(kFp4FitStages);
+                    r.next(stages);
                     buffer ^= 1;
                 }
             }
@@ -1059,55 +1110,65 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                 mbar_wait(done_bar, 0u);
             }
             __syncwarp();
-        } else if (warp >= 2) {
-            // -------------------------------------------- scales of x: rows 128 (warp - 2) + lane, + 32, + 64, + 96 of the tile
-            // (as in fp4_pair_kernel: four stages' at a time, the next four's asked for behind the last of these)
+        } else if (warp == 2) {
+            // -------------------------------------------- what the others wrote, handed over
             bool ok = true;
             Ring r;
-            const int first = 128 * (warp - 2) + lane;
-            const uint32_t x_full0 = map_to_rank0(smem_u32(x_full));
-            uint4 four[4][2];   // [row][half]
+            const uint32_t x_full0 = map_to_rank0(smem_u32(x_full)), x_written0 = smem_u32(x_written);
+            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
+                for (int k = 0; k < steps; k++) {
+                    if (!bar_wait(x_written0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
+                    fence_async();
+                    if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
+                    r.next(stages);
+                }
+            }
+        } else if (warp >= 4) {
+            // -------------------------------------------- scales of x: rows 32 (warp - 4) + lane, + 128, + 256 of the tile
+            // (two stages' at a time, the next two's on their way)
+            bool ok = true;
+            Ring r;
+            const int first = 32 * (warp - 4) + lane;
+            const uint32_t x_written0 = smem_u32(x_written);
+            uint4 next[3];
             auto load = [&](const Tile& t, int k) {
                 const uint8_t* row = p.x_scales + (long long)(t.pos + first) * p.ld_xs;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const bool in = first + 32 * c < t.n;
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        four[c][h] = in ? sixteen_scales(row + 32 * c * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
-                }
+                for (int v = 0; v < 3; v++)
+                    next[v] = first + 128 * v < t.n ? sixteen_scales(row + 128 * v * p.ld_xs, 8 * k, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
             };
             int i = blockIdx.x >> 1;
             if (i < tiles) load(tile_at(i), 0);
             for (; i < tiles && ok; i += pairs) {
                 const Tile t = tile_at(i);
-                for (int k4 = 0; k4 < steps && ok; k4 += 4) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (k4 + j >= steps) break;
-                        if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
-                        if (t.cols > 128 * (warp - 2)) {
-                            uint4* to = reinterpret_cast<uint4*>(ring + r.i * kFp4FitStage + kFp4FitScalesX + kFp4Scales * (warp - 2)) + lane;
-                            const uint4 a = four[0][j >> 1], b = four[1][j >> 1], c = four[2][j >> 1], d = four[3][j >> 1];
-                            to[0] = j & 1 ? make_uint4(a.z, b.z, c.z, d.z) : make_uint4(a.x, b.x, c.x, d.x);
-                            to[32] = j & 1 ? make_uint4(a.w, b.w, c.w, d.w) : make_uint4(a.y, b.y, c.y, d.y);
-                            fence_async();
-                        }
-                        __syncwarp();
-                        if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
-                        r.next(kFp4FitStages);
-                    }
-                    if (k4 + 4 < steps) load(t, k4 + 4);
+                for (int k2 = 0; k2 < steps && ok; k2 += 2) {
+                    const uint4 now[3] = {next[0], next[1], next[2]};
+                    if (k2 + 2 < steps) load(t, k2 + 2);
                     else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        if (k2 + j >= steps) break;
+                        if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                        uint32_t* to = reinterpret_cast<uint32_t*>(ring + r.i * stage_bytes + xs_off) + 4 * lane + (warp - 4);
+#pragma unroll
+                        for (int v = 0; v < 3; v++)
+                            if (128 * v < t.cols) {
+                                to[256 * v] = j ? now[v].z : now[v].x;
+                                to[256 * v + 128] = j ? now[v].w : now[v].y;
+                            }
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(x_written0 + 8 * r.i);
+                        r.next(stages);
+                    }
                 }
             }
         }
     } else {
         // ------------------------------------------------ output
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp4FitRegsMany));
-        const int half = (warp - 4) >> 2, quarter = warp & 3, id = 32 * quarter + lane;   // (warps 4-7, 8-11: quarters 0-3)
+        const int half = (warp - 8) >> 2, quarter = warp & 3, id = 32 * quarter + lane;   // (warps 8-11, 12-15: quarters 0-3)
         const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16), read0 = map_to_rank0(smem_u32(tile_read));
-        float* room = reinterpret_cast<float*>(ring + kFp4FitStages * kFp4FitStage + half * kFp4FitRoom);
+        float* room = reinterpret_cast<float*>(ring + stages * stage_bytes + half * kFp4FitRoom);
         constexpr int kPitch = MODE == kFp4Plain ? 132 : 80;   // floats of a row there (the lanes' banks differ)
         uint32_t n = 0;
         for (int i = blockIdx.x >> 1; i < tiles; i += pairs, n++) {
@@ -1115,19 +1176,27 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             // (one of the four warps that gives up takes the others along: they meet at barriers from here on)
             if (!all_of(1 + half, 128, bar_wait(smem_u32(tile_done) + 8 * (n & 1), (n >> 1) & 1u, ctl))) break;
             tc_fence_after();
-            const uint32_t from = taddr + (n & 1 ? kFp4PairSecond : 0);
-            float acc[4][32];   // 32 rows of x of this lane's output, every second 32
+            const uint32_t from = taddr + place(n, t.cols);
+            const int m = t.m + kHalf * (int)rank, left = p.M - m;
+            // Every second 32 rows of x are this half's, `mine` of them: all but four, and the last four, whose columns are
+            // in registers when the accumulator is handed back.
+            const int mine = (t.cols + 32 - 32 * half) >> 6;
+#pragma unroll 1
+            for (int last = mine > 4 ? 0 : 1; last < 2; last++) {
+            const int c0 = last ? max(mine - 4, 0) : 0, count = last ? min(mine, 4) : mine - 4;
+            float acc[4][32];
 #pragma unroll
             for (int h = 0; h < 4; h++)
-                if (64 * h + 32 * half < t.cols) tmem_ld32(from + 64 * h + 32 * half, acc[h]);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) bar_arrive_cluster(read0 + 8 * (n & 1));
-            const int m = t.m + kHalf * (int)rank, left = p.M - m;
+                if (h < count) tmem_ld32(from + 64 * (c0 + h) + 32 * half, acc[h]);
+            if (last) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive_cluster(read0 + 8 * (n & 1));
+            }
 #pragma unroll
             for (int h = 0; h < 4; h++) {
-                const int at = 64 * h + 32 * half, have = t.n - at;   // (the same for all four warps)
-                if (have <= 0) break;
+                const int at = 64 * (c0 + h) + 32 * half, have = t.n - at;   // (the same for all four warps)
+                if (h >= count || have <= 0) break;
                 float (&v)[32] = acc[h];
                 named_barrier(1 + half, 128);   // what was in the room is out
                 if (MODE == kFp4Plain) {
@@ -1178,6 +1247,7 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
                     room_out<kHalf, __nv_bfloat16>(p, room, kPitch, row, have, m, left, id, wide_out);
                 }
             }
+            }
         }
     }
     // ---------------- teardown: every role of both CTAs is done (or gave up); free tensor memory
@@ -1191,7 +1261,7 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
     if (rank == 0 ? given_up != 0 : from_peer != 0) {
         if (rank == 0 && threadIdx.x == 0) {
             Fp4FitBars bars{full, bytes};
-            drain_pair(issued, from_peer, kFp4FitStages, bars);
+            drain_pair(issued, from_peer, stages, bars);
         }
         if (warp == 1) {
             if (rank == 0 && elect_one()) umma_commit_pair(smem_u32(left_bar));

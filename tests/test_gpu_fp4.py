@@ -146,7 +146,7 @@ def form(request, monkeypatch):
 
 SIZES = [(1, 1, 1, 1), (1, 1, 128, 32), (2, 1, 16, 256), (1, 1, 300, 2048), (3, 1, 257, 96), (17, 1, 130, 70), (16, 4, 128, 512),
          (64, 2, 384, 500), (65, 1, 256, 320), (200, 3, 304, 1000), (129, 7, 72, 1056), (257, 1, 520, 288), (530, 5, 640, 768),
-         (5, 40, 40, 64), (300, 33, 136, 4096)]
+         (5, 40, 40, 64), (300, 33, 136, 4096), (385, 1, 264, 544), (800, 3, 130, 300), (1500, 2, 72, 800)]
 
 
 def check(got, want, inside, type, untouched):
@@ -185,7 +185,7 @@ def test_product_of_wide_scales(rows, groups, n, k, form):
 
 
 GATED = [(1, 1, 1, 32), (1, 1, 16, 256), (1, 1, 128, 2048), (3, 1, 33, 96), (17, 1, 100, 70), (16, 4, 128, 512), (64, 2, 200, 500),
-         (200, 3, 152, 1000), (257, 1, 384, 288), (530, 5, 320, 768), (5, 40, 40, 64)]
+         (200, 3, 152, 1000), (257, 1, 384, 288), (530, 5, 320, 768), (5, 40, 40, 64), (700, 2, 80, 544)]
 
 
 @pytest.mark.parametrize("rows,groups,f,k", GATED)
