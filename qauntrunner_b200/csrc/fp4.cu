@@ -185,7 +185,7 @@ cudaError_t launch(const qrm_fp4* m, const Fp4RowMaps& x_maps, Fp4Params& p, Fp4
     if (form == kFit) {
         const Fit fit(m->groups, T);
         return launch_ahead(fp4_fit_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4FitThreads, fit.smem, s, w_map,
-                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps, p, wide_out, fit.stages, fit.rows);
+                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps, p, fit.stages, fit.rows);
     }
     if (form == kPair)
         return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, w_map,
@@ -269,7 +269,7 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     p.ld_xs = ld_xs;
     p.ld_out = ld_out;
     p.ld_os = ld_os;
-    p.limit = limit;
+    p.limit = limit > 0.f ? limit : INFINITY;
     p.T = (int)T;
     p.groups = m->groups;
     p.M = (int)M;

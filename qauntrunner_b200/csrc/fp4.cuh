@@ -41,7 +41,7 @@ struct Fp4Params {
     uint8_t* out_scales;       // [T][ld_os]
     int32_t* err;
     long long ld_xs, ld_out, ld_os;
-    float limit;
+    float limit;               // infinite: none
     int T, groups;
     int M;                     // outputs (gated: f)
     int units;                 // of 128 rows in w_scales, of one matrix (gated: 64 features)
@@ -110,6 +110,20 @@ __device__ __forceinline__ void load_weights_pair(uint32_t dst, const CUtensorMa
             "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(m >> 4), "r"(group), "r"(0), "r"(bar)
             : "memory");
 }
+// a value that is the same in all lanes, so that it may be kept in a register of the warp
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+// both barriers; one vote where both are ready
+__device__ __forceinline__ bool bar_wait_both(uint32_t a, uint32_t a_parity, uint32_t b, uint32_t b_parity, const WaitCtl& c) {
+    const bool first = bar_try(a, a_parity), second = bar_try(b, b_parity);
+    if (__all_sync(0xffffffffu, first && second)) return true;
+    return bar_wait(a, a_parity, c) && bar_wait(b, b_parity, c);
+}
+// The high words of the descriptors, which are constants: of operands in the
+// 128-byte swizzle, of units of scales.
+constexpr uint32_t kSw128High = (1024 >> 4) | (1u << 14) | (2u << 29), kScaleHigh = (128 >> 4) | (1u << 14);
+__device__ __forceinline__ uint32_t sw128_low(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t scale_low(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4; }
+__device__ __forceinline__ uint64_t wide_desc(uint32_t low, uint32_t high) { return (uint64_t)high << 32 | low; }
 // what this thread wrote to shared memory is there for copies and MMAs
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -150,8 +164,9 @@ __device__ __forceinline__ uint4 sixteen_scales(const uint8_t* __restrict__ row,
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// limit: infinite when there is none (a branch for each pair of values kept them from overlapping: 140 cycles a value)
 __device__ __forceinline__ float2 gated2(float2 gate, float2 up, float limit) {
-    const Swiglu2 s = limit > 0.f ? swiglu2<true>(gate, up, limit) : swiglu2<false>(gate, up, 0.f);
+    const Swiglu2 s = swiglu2<true>(gate, up, limit);
     return unpair(mul2(mul2(s.g, s.sig), s.u));
 }
 
@@ -834,10 +849,10 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
 // 384 rows are loaded once.  Past 256 rows a step takes two MMAs, of 128 rows and
 // of the others.
 //
-// A lane of tensor memory is an output, so rows go out by way of shared memory:
-// 32 rows of x at a time, [row][output] in f32, written by the lanes' columns and
-// read along the rows.  For the gated product the lanes of gate and of up
-// exchange half of their columns first, so that each has both sums of 16 rows.
+// A lane of tensor memory is an output.  For the gated product the lanes of gate
+// and of up exchange half of their columns, so that each has both sums of 16 rows;
+// on their way into 4-bit rows, whose blocks are two warps', they meet in shared
+// memory, 32 rows of x at a time, [row][feature] in f32.
 //
 // Two accumulators where two neighbouring tiles have 224 rows at most; else a
 // tile's MMAs wait for the one before to be read.
@@ -854,7 +869,7 @@ constexpr int kFp4FitThreads = 512;
 constexpr int kFp4FitMaxStages = 8;
 constexpr int kFp4FitRows = 384;
 constexpr int kFp4FitSecond = 224, kFp4FitTmemScales = 448, kFp4FitScaleCols = 32;
-constexpr int kFp4FitRoom = 32 * 132 * 4;      // four warps' room for 32 rows on their way out
+constexpr int kFp4FitRoom = 32 * 80 * 4;       // four warps' room for 32 rows on their way into 4 bits
 constexpr int kFp4FitRegsFew = 56, kFp4FitRegsMany = 200;
 constexpr int kFp4FitRegs = 256 * kFp4FitRegsFew + 256 * kFp4FitRegsMany;
 static_assert(kFp4FitRegs <= kFp4FitThreads * 128, "register split");
@@ -892,54 +907,55 @@ __device__ __forceinline__ bool all_of(int barrier, int threads, bool holds) {
                  : "memory");
     return r != 0;
 }
-// eight outputs of a row, v, to out, of which `left` exist; wide: rows start on 16 bytes
-template <typename T>
-__device__ __forceinline__ void store_eight(T* out, int left, const float (&v)[8], bool wide) {
-    if (wide && left >= 8) {
-        uint4* to = reinterpret_cast<uint4*>(out);
-        if constexpr (sizeof(T) == 4) {
-            to[0] = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-            to[1] = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
-        } else {
-            uint32_t w[4];
+// 32 columns of this warp's lanes of tensor memory, which are there after loaded()
+__device__ __forceinline__ void tmem_ld32_later(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const T h[2] = {round_to<T>(v[2 * i]), round_to<T>(v[2 * i + 1])};
-                memcpy(&w[i], h, 4);
-            }
-            *to = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-    } else {
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+template <int N>
+__device__ __forceinline__ void loaded(float (&v)[N][32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-            if (i < left) out[i] = round_to<T>(v[i]);
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 32; j++) asm volatile("" : "+f"(v[i][j]));   // (no use of the registers before the wait)
+}
+// Output m of rows first, first + step, ..., of which `have` count from row t on,
+// by a lane; a warp's lanes write neighbouring outputs.  No way through shared
+// memory: copies and MMAs leave its ports little time (32 rows of 128 outputs
+// took 1900 cycles that way).
+template <typename T, int N>
+__device__ __forceinline__ void store_outputs(const Fp4Params& p, long long t, int first, int step, int have, int m, const float (&v)[N]) {
+    if (m >= p.M) return;
+    T* out = reinterpret_cast<T*>(p.out) + (t + first) * p.ld_out + m;
+    const long long ahead = step * p.ld_out;
+#pragma unroll
+    for (int c = 0; c < N; c++) {
+        if (first + c * step < have) *out = round_to<T>(v[c]);
+        out += ahead;
     }
 }
-// 32 rows of W outputs each (room: [row][pitch] f32) from output m of row t on, by 128 threads, of which `rows` and
-// `left` exist
-template <int W, typename T>
-__device__ __forceinline__ void room_out(const Fp4Params& p, const float* room, int pitch, long long t, int rows, int m, int left, int id,
-                                         bool wide) {
-    T* out = reinterpret_cast<T*>(p.out) + t * p.ld_out + m;
-    if (wide) {
-#pragma unroll
-        for (int j = 0; j < 32 * W / 8 / 128; j++) {
-            const int row = (id + 128 * j) / (W / 8), o = (id + 128 * j) % (W / 8) * 8;
-            const float4* from = reinterpret_cast<const float4*>(room + row * pitch + o);
-            const float4 a = from[0], b = from[1];
-            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            if (row < rows) store_eight(out + row * p.ld_out + o, left - o, v, true);
-        }
-    } else {   // neighbouring lanes write neighbouring outputs
-        for (int j = id; j < W * min(rows, 32); j += 128)
-            if (j % W < left) out[j / W * p.ld_out + j % W] = round_to<T>(room[j / W * pitch + j % W]);
-    }
+template <int N>
+__device__ __forceinline__ void store_outputs(const Fp4Params& p, long long t, int first, int step, int have, int m, const float (&v)[N]) {
+    if (p.type == 0) store_outputs<float>(p, t, first, step, have, m, v);
+    else if (p.type == 1) store_outputs<__half>(p, t, first, step, have, m, v);
+    else store_outputs<__nv_bfloat16>(p, t, first, step, have, m, v);
 }
 
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp4FitThreads, 1)
 fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap s_map,
-               const __grid_constant__ Fp4RowMaps x_maps, const __grid_constant__ Fp4Params p, int wide_out, int stages,
+               const __grid_constant__ Fp4RowMaps x_maps, const __grid_constant__ Fp4Params p, int stages,
                int x_rows /* most rows of x in a tile */) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -1064,37 +1080,41 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             uint32_t n = 0, buffer = 0;   // tiles; of scales
             int before = 0, before_end = 0;   // the columns of the tile before
             const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), ring0 = smem_u32(ring), read0 = smem_u32(tile_read);
-            const uint64_t w_desc = sw128_desc(ring0), x_desc = sw128_desc(ring0 + kFp4Tile);
-            const uint64_t ws_desc = scale_desc(ring0 + ws_off), xs_desc = scale_desc(ring0 + xs_off);
+            const uint32_t w_low = sw128_low(ring0), x_low = sw128_low(ring0 + kFp4Tile);
+            const uint32_t ws_low = scale_low(ring0 + ws_off), xs_low = scale_low(ring0 + xs_off), base = uniform(tmem);
             const uint32_t odd = umma_idesc_mxf4(0, 0, 2) & ~umma_idesc_mxf4(0, 0, 0);
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs, n++) {
                 const Tile t = tile_at(i);
                 const uint32_t a = n & 1;
-                const int at_col = place(n, t.cols), first = t.cols > 256 ? 128 : t.cols;
-                const uint32_t d = tmem + at_col, idesc = umma_idesc_mxf4(256, first, 0), idesc2 = umma_idesc_mxf4(256, t.cols - first, 0);
+                const int cols = uniform(t.cols);
+                const int at_col = place(n, cols), first = cols > 256 ? 128 : cols;
+                const uint32_t d = base + at_col, idesc = umma_idesc_mxf4(256, first, 0), idesc2 = umma_idesc_mxf4(256, cols - first, 0);
                 // the columns have been read: of the tile two before, and of the one before where they are the same
                 if (n > 1 && !bar_wait(read0 + 8 * a, ((n >> 1) - 1) & 1u, ctl)) break;
-                if (n > 0 && before < at_col + t.cols && at_col < before_end && !bar_wait(read0 + 8 * (a ^ 1), ((n - 1) >> 1) & 1u, ctl)) break;
+                if (n > 0 && before < at_col + cols && at_col < before_end && !bar_wait(read0 + 8 * (a ^ 1), ((n - 1) >> 1) & 1u, ctl)) break;
                 before = at_col;
-                before_end = at_col + t.cols;
+                before_end = at_col + cols;
                 for (int k = 0; k < steps; k++) {
-                    if (!bar_wait(full0 + 8 * r.i, r.phase, ctl) || !bar_wait(x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
+                    if (!bar_wait_both(full0 + 8 * r.i, r.phase, x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
                     tc_fence_after();
+                    const uint32_t at = r.i * stage_bytes >> 4, wl = w_low + at, xl = x_low + at, wsl = ws_low + at, xsl = xs_low + at;
+                    const uint32_t ws = base + kFp4FitTmemScales + kFp4FitScaleCols * buffer, xs = ws + 8;   // of x: 12 columns a half
+                    const uint32_t more = k > 0;
                     if (elect_one()) {
-                        const uint32_t at = r.i * stage_bytes >> 4;
-                        const uint32_t ws = tmem + kFp4FitTmemScales + kFp4FitScaleCols * buffer, xs = ws + 8;   // of x: 12 columns a half
 #pragma unroll
                         for (int u = 0; u < 2; u++) {   // half of the stage's contracted values
-                            scales_to_tmem<2>(ws + 4 * u, ws_desc + at + u * (512 >> 4));
-                            for (int v = 0; 128 * v < t.cols; v++) scales_to_tmem<2>(xs + 12 * u + 4 * v, xs_desc + at + (v * kFp4Scales + u * 512 >> 4));
+                            scales_to_tmem<2>(ws + 4 * u, wide_desc(wsl + u * (512 >> 4), kScaleHigh));
+                            scales_to_tmem<2>(xs + 12 * u, wide_desc(xsl + u * (512 >> 4), kScaleHigh));
+                            if (cols > 128) scales_to_tmem<2>(xs + 12 * u + 4, wide_desc(xsl + (kFp4Scales + u * 512 >> 4), kScaleHigh));
+                            if (cols > 256) scales_to_tmem<2>(xs + 12 * u + 8, wide_desc(xsl + (2 * kFp4Scales + u * 512 >> 4), kScaleHigh));
                         }
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            const uint32_t half = j & 1 ? odd : 0;
-                            umma_mxf4<2>(d, w_desc + at + 2 * j, x_desc + at + 2 * j, idesc | half, ws + 4 * (j >> 1), xs + 12 * (j >> 1), k > 0 || j > 0);
-                            if (t.cols > 256)
-                                umma_mxf4<2>(d + 128, w_desc + at + 2 * j, x_desc + at + (64 * 128 >> 4) + 2 * j, idesc2 | half, ws + 4 * (j >> 1),
-                                             xs + 12 * (j >> 1) + 4, k > 0 || j > 0);
+                            const uint64_t wd = wide_desc(wl + 2 * j, kSw128High);
+                            umma_mxf4<2>(d, wd, wide_desc(xl + 2 * j, kSw128High), j & 1 ? idesc | odd : idesc, ws + 4 * (j >> 1), xs + 12 * (j >> 1), j > 0 ? 1 : more);
+                            if (cols > 256)
+                                umma_mxf4<2>(d + 128, wd, wide_desc(xl + (64 * 128 >> 4) + 2 * j, kSw128High), j & 1 ? idesc2 | odd : idesc2,
+                                             ws + 4 * (j >> 1), xs + 12 * (j >> 1) + 4, j > 0 ? 1 : more);
                         }
                         umma_commit_pair(done0 + 8 * r.i);
                         if (k + 1 == steps) umma_commit_pair(smem_u32(tile_done) + 8 * a);
@@ -1169,7 +1189,7 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
         const int half = (warp - 8) >> 2, quarter = warp & 3, id = 32 * quarter + lane;   // (warps 8-11, 12-15: quarters 0-3)
         const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16), read0 = map_to_rank0(smem_u32(tile_read));
         float* room = reinterpret_cast<float*>(ring + stages * stage_bytes + half * kFp4FitRoom);
-        constexpr int kPitch = MODE == kFp4Plain ? 132 : 80;   // floats of a row there (the lanes' banks differ)
+        constexpr int kPitch = 80;   // floats of a row there (the lanes' banks differ)
         uint32_t n = 0;
         for (int i = blockIdx.x >> 1; i < tiles; i += pairs, n++) {
             const Tile t = tile_at(i);
@@ -1177,76 +1197,78 @@ fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant_
             if (!all_of(1 + half, 128, bar_wait(smem_u32(tile_done) + 8 * (n & 1), (n >> 1) & 1u, ctl))) break;
             tc_fence_after();
             const uint32_t from = taddr + place(n, t.cols);
-            const int m = t.m + kHalf * (int)rank, left = p.M - m;
+            const int m = t.m + kHalf * (int)rank;
             // Every second 32 rows of x are this half's, `mine` of them: all but four, and the last four, whose columns are
             // in registers when the accumulator is handed back.
             const int mine = (t.cols + 32 - 32 * half) >> 6;
 #pragma unroll 1
             for (int last = mine > 4 ? 0 : 1; last < 2; last++) {
-            const int c0 = last ? max(mine - 4, 0) : 0, count = last ? min(mine, 4) : mine - 4;
-            float acc[4][32];
+                const int c0 = last ? max(mine - 4, 0) : 0, count = last ? min(mine, 4) : mine - 4;
+                float acc[4][32];
 #pragma unroll
-            for (int h = 0; h < 4; h++)
-                if (h < count) tmem_ld32(from + 64 * (c0 + h) + 32 * half, acc[h]);
-            if (last) {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive_cluster(read0 + 8 * (n & 1));
-            }
+                for (int h = 0; h < 4; h++)
+                    if (h < count) tmem_ld32_later(from + 64 * (c0 + h) + 32 * half, acc[h]);
+                loaded(acc);
+                if (last) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive_cluster(read0 + 8 * (n & 1));
+                }
 #pragma unroll
-            for (int h = 0; h < 4; h++) {
-                const int at = 64 * (c0 + h) + 32 * half, have = t.n - at;   // (the same for all four warps)
-                if (h >= count || have <= 0) break;
-                float (&v)[32] = acc[h];
-                named_barrier(1 + half, 128);   // what was in the room is out
-                if (MODE == kFp4Plain) {
+                for (int h = 0; h < 4; h++) {
+                    const int at = 64 * (c0 + h) + 32 * half, have = t.n - at;   // (the same for all four warps)
+                    if (h >= count || have <= 0) break;
+                    const float (&v)[32] = acc[h];
+                    const long long row = t.pos + at;
+                    if (MODE == kFp4Plain) {
+                        store_outputs(p, row, 0, 1, have, m + id, v);
+                    } else {
+                        // gate's lanes get both sums of the even rows, up's of the odd ones
+                        const bool up = lane & 16;
+                        float y[16];
 #pragma unroll
-                    for (int c = 0; c < 32; c++) room[c * kPitch + id] = v[c];
-                } else {
-                    const bool up = lane & 16;
-                    float* to = room + (up ? kPitch : 0) + 16 * quarter + (lane & 15);
+                        for (int c = 0; c < 32; c += 4) {
+                            const float g0 = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 16);
+                            const float g1 = __shfl_xor_sync(0xffffffffu, up ? v[c + 2] : v[c + 3], 16);
+                            const float2 own = up ? make_float2(v[c + 1], v[c + 3]) : make_float2(v[c], v[c + 2]);
+                            const float2 other = make_float2(g0, g1);
+                            const float2 f = gated2(up ? other : own, up ? own : other, p.limit);
+                            y[c / 2] = f.x;
+                            y[c / 2 + 1] = f.y;
+                        }
+                        const int feature = 16 * quarter + (lane & 15);
+                        if (MODE == kFp4Gated) {
+                            store_outputs(p, row, up, 2, have, m + feature, y);
+                        } else {
+                            named_barrier(1 + half, 128);   // what was in the room is out
+                            float* to = room + (up ? kPitch : 0) + feature;
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {   // gate's lanes take rows c and c + 2, up's c + 1 and c + 3
-                        const float g0 = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 16);
-                        const float g1 = __shfl_xor_sync(0xffffffffu, up ? v[c + 2] : v[c + 3], 16);
-                        const float2 mine = up ? make_float2(v[c + 1], v[c + 3]) : make_float2(v[c], v[c + 2]);
-                        const float2 other = make_float2(g0, g1);
-                        const float2 y = gated2(up ? other : mine, up ? mine : other, p.limit);
-                        to[c * kPitch] = y.x;
-                        to[(c + 2) * kPitch] = y.y;
+                            for (int c = 0; c < 16; c++) to[2 * c * kPitch] = y[c];
+                            named_barrier(1 + half, 128);   // 32 rows are there
+                            const int left = p.M - m;
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {   // eight features a lane, four lanes a block
+                                const int r = (id + 128 * j) >> 3, o = (id & 7) * 8;
+                                const float4* f = reinterpret_cast<const float4*>(room + r * kPitch + o);
+                                const float4 a = f[0], b = f[1];
+                                float e[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                                uint32_t top = 0;
+#pragma unroll
+                                for (int k = 0; k < 8; k++) {
+                                    if (o + k >= left) e[k] = 0.f;
+                                    top = max(top, magnitude(e[k]));
+                                }
+                                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                                const uint32_t scale = fp4_scale(top), q = e2m1x8(e, scale);
+                                if (r < have && o / kFp4Block * kFp4Block < left) {
+                                    *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (row + r) * p.ld_out + (m + o) / 2) = q;
+                                    if ((id & 3) == 0) p.out_scales[(row + r) * p.ld_os + (m + o) / kFp4Block] = (uint8_t)scale;
+                                }
+                            }
+                        }
                     }
                 }
-                named_barrier(1 + half, 128);   // 32 rows are there
-                const long long row = t.pos + at;
-                if (MODE == kFp4GatedRows) {
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {   // eight features a lane, four lanes a block
-                        const int r = (id + 128 * j) >> 3, o = (id & 7) * 8;
-                        const float4* f = reinterpret_cast<const float4*>(room + r * kPitch + o);
-                        const float4 a = f[0], b = f[1];
-                        float e[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                        uint32_t top = 0;
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            if (o + k >= left) e[k] = 0.f;
-                            top = max(top, magnitude(e[k]));
-                        }
-                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        const uint32_t scale = fp4_scale(top), q = e2m1x8(e, scale);
-                        if (r < have && o / kFp4Block * kFp4Block < left) {
-                            *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (row + r) * p.ld_out + (m + o) / 2) = q;
-                            if ((id & 3) == 0) p.out_scales[(row + r) * p.ld_os + (m + o) / kFp4Block] = (uint8_t)scale;
-                        }
-                    }
-                } else if (p.type == 0) {
-                    room_out<kHalf, float>(p, room, kPitch, row, have, m, left, id, wide_out);
-                } else if (p.type == 1) {
-                    room_out<kHalf, __half>(p, room, kPitch, row, have, m, left, id, wide_out);
-                } else {
-                    room_out<kHalf, __nv_bfloat16>(p, room, kPitch, row, have, m, left, id, wide_out);
-                }
-            }
             }
         }
     }
