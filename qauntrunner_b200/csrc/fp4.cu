@@ -14,7 +14,7 @@ using namespace qrm;
 
 struct qrm_fp4 {
     int device = 0, sms = 0, groups = 0;
-    int form = -1;                       // QRM_FP4_FORM: the kernel of every product (Fp4Form)
+    int form = -1;                       // QRM_FP4_PAIR: 1 always / 0 never rows of x on the MMA's M side
     int64_t rows = 0, cols = 0;
     int units = 0, gated_units = 0;      // of 128 rows; of 64 features, if there are two halves
     int steps = 0;                       // of 256 columns
@@ -39,22 +39,6 @@ void release(qrm_fp4* m) {
     delete m;
 }
 
-// room for rows of x in a stage, stages, shared memory of a CTA
-struct Fit {
-    static constexpr int kMost = kSmemMost - 256;   // (the kernel has some of its own)
-    int rows, stages;
-    size_t smem;
-    Fit(int groups, int64_t T) {
-        // a third more rows in a tile than a group has on average: smaller stages leave room for more of them
-        const int64_t used = std::min<int64_t>(T, groups), each = (T + used - 1) / used;
-        int64_t most = groups > 1 ? each * 3 / 2 : each;
-        if (const char* e = getenv("FITCAP")) most = atoi(e);
-        rows = (int)std::max<int64_t>(64, std::min<int64_t>(kFp4FitRows, (most + 31) / 32 * 32));
-        const int rest = 1024 + fp4_pair_stage_off(groups) + 2 * kFp4FitRoom;
-        stages = std::min(kFp4FitMaxStages, (kMost - rest) / fp4_fit_stage(rows));
-        smem = rest + (size_t)stages * fp4_fit_stage(rows);
-    }
-};
 size_t pair_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4PairStages * kFp4PairStage + 8 * kFp4PairOut; }
 
 template <int MODE>
@@ -62,16 +46,13 @@ cudaError_t prepare_kernels() {
     cudaError_t e = cudaFuncSetAttribute(fp4_split_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(fp4_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(kFp4MaxGroups));
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(fp4_fit_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Fit::kMost);
     return e;
 }
 // registers a thread that the pair kernels were built with: their split may not pass what a launch has
 template <int MODE>
 bool enough_regs() {
-    cudaFuncAttributes pair{}, fit{};
-    return cudaFuncGetAttributes(&pair, fp4_pair_kernel<MODE>) == cudaSuccess && pair.numRegs * kFp4PairThreads >= kFp4PairRegs &&
-           cudaFuncGetAttributes(&fit, fp4_fit_kernel<MODE>) == cudaSuccess && fit.numRegs * kFp4FitThreads >= kFp4FitRegs;
+    cudaFuncAttributes pair{};
+    return cudaFuncGetAttributes(&pair, fp4_pair_kernel<MODE>) == cudaSuccess && pair.numRegs * kFp4PairThreads >= kFp4PairRegs;
 }
 
 int create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes, const void* scales,
@@ -105,7 +86,7 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
         release(m);
         return rc;
     };
-    if (const char* e = getenv("QRM_FP4_FORM")) m->form = std::max(0, std::min(2, atoi(e)));
+    if (const char* e = getenv("QRM_FP4_PAIR")) m->form = atoi(e) != 0;
     m->device = device;
     m->sms = sms;
     m->groups = groups;
@@ -171,38 +152,48 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
     return QRM_OK;
 }
 
-enum Fp4Form { kSplit = 0, kPair = 1, kFit = 2 };
-
-// Which kernel a product takes.
-Fp4Form form_of(int64_t T, int groups) {
-    const double used = (double)std::min<int64_t>(T, groups), rows = T / used;
-    return rows < 64 ? kSplit : rows < 1024 ? kFit : kPair;
+// Which kernel a product takes, by an estimate of what both would cost with all
+// T rows held and spread evenly over the groups.  Measured (us; weights / rows of
+// x on the MMA's M side), outputs x contracted:
+//   1 x 4096 x 7168:   1 row 7.6 / 13.8, 16 rows 9.1 / 13.4, 64 rows 12.9 / 13.8, 128 rows 16.3 / 14.4
+//   1 x 28672 x 4096:  1 row 13.6 / 23.0, 32 rows 19.1 / 20.3, 64 rows 21.8 / 20.4
+//   1 x 1024 x 2816:   1 row 5.8 / 8.0, 32 rows 7.7 / 8.4, 64 rows 9.6 / 8.8
+//   1 x 7168 x 2048:   16 rows 7.0 / 7.8, 32 rows 8.2 / 8.0, 64 rows 10.6 / 8.3
+//   8 x 5632 x 1024:   8 rows each 8.3 / 11.2, 16 rows each 9.8 / 11.3, 32 rows each 12.6 / 11.3
+//   32 x 4096 x 7168:  2 rows each 69 / 78, 16 rows each 86 / 90, 32 rows each 92 / 91, 64 rows each 113 / 94
+//   32 x 7168 x 2048:  4 rows each 48 / 48, 16 rows each 56 / 50, 64 rows each 85 / 53
+// The first takes what reading the weights takes, and something for each row of a
+// tile and all tiles' rows; the second a time for each stage of whole tiles of 256
+// rows x 256 outputs, in waves over the pairs of SMs, longer where most pairs are
+// at work.  The worst choices among 67 measured sizes take 1.15 times as long as
+// the other kernel.
+bool pair_is_faster(int64_t T, int64_t used, int64_t tiles_across, int steps, int tile_rows, int sms) {
+    const double rows = (double)T / used, row_tiles = std::ceil(rows / tile_rows), tiles = used * tiles_across * row_tiles;
+    const double read = (double)used * tiles_across * steps * 34816 / 6.4e6;   // us, of a stage's 256 x 256 codes and scales
+    const double one = 5 + read * (1 + (row_tiles - 1) / 2) + std::min<double>(rows, tile_rows) * (0.06 + 0.0006 * tiles);
+    const double pairs = sms / 2, wide = used * tiles_across * std::ceil(rows / 256);
+    const double two = 5 + std::ceil(wide / pairs) * steps * (wide <= pairs / 2 ? 0.30 : 0.45);
+    return two < one;
 }
 
 template <int MODE>
-cudaError_t launch(const qrm_fp4* m, const Fp4RowMaps& x_maps, Fp4Params& p, Fp4Form form, int wide_out, int64_t T, cudaStream_t s) {
+cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const Fp4Params& p, bool pair, int wide_out, int64_t T, cudaStream_t s) {
     const CUtensorMap& w_map = MODE == kFp4Plain ? m->map : m->gated_map;
-    if (form == kFit) {
-        const Fit fit(m->groups, T);
-        return launch_ahead(fp4_fit_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4FitThreads, fit.smem, s, w_map,
-                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps, p, fit.stages, fit.rows);
-    }
-    if (form == kPair)
+    if (pair)
         return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, w_map,
-                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_maps.rows[3], p, wide_out);
+                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_map, p, wide_out);
     const int64_t across = MODE == kFp4Plain ? (p.M + 255) / 256 : (p.M + 127) / 128;
-    const int64_t used = std::min<int64_t>(T, m->groups), per = (T / used + kFp4Rows - 1) / kFp4Rows;
+    const int64_t used = std::min<int64_t>(T, m->groups), per = (T / used + p.tile_rows - 1) / p.tile_rows;
     const int64_t tiles = used * per * across;
     int ranks = 1;
     while (ranks < 8 && tiles * ranks * 2 <= 2 * m->sms && p.steps >= 4 * ranks) ranks *= 2;
-    const int x_rows = (int)std::min<int64_t>(kFp4Rows, (T + 15) / 16 * 16);
     const int64_t ctas = (int64_t)p.row_tiles * across * ranks;
     // two CTAs on an SM, 1 KB of it kept for each: of one launch, or the next one's first
-    const int stages = std::min(kFp4MaxStages, (kSmemMost / 2 - 512 - 1024 - kFp4Header) / fp4_stage_bytes(x_rows));
+    const int stages = std::min(kFp4MaxStages, (kSmemMost / 2 - 512 - 1024 - kFp4Header) / fp4_stage_bytes(p.tile_rows));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kFp4Threads);
-    cfg.dynamicSmemBytes = 1024 + kFp4Header + (size_t)stages * fp4_stage_bytes(x_rows);
+    cfg.dynamicSmemBytes = 1024 + kFp4Header + (size_t)stages * fp4_stage_bytes(p.tile_rows);
     cfg.stream = s;
     cudaLaunchAttribute at[2] = {};
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -212,7 +203,7 @@ cudaError_t launch(const qrm_fp4* m, const Fp4RowMaps& x_maps, Fp4Params& p, Fp4
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, fp4_split_kernel<MODE>, w_map, x_maps.rows[0], p, stages, x_rows);
+    return cudaLaunchKernelEx(&cfg, fp4_split_kernel<MODE>, w_map, x_map, p, stages);
 }
 
 int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x, const uint8_t* xs, int64_t ld_xs,
@@ -225,7 +216,11 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     if (!b) return failf(QRM_E_FORMAT, "%s: type %d is not F32, F16 or BF16", what, type);
     if (!(limit >= 0.f)) return failf(QRM_E_INVALID, "%s: limit %g", what, (double)limit);
     if (T < 0 || T > INT_MAX) return failf(QRM_E_INVALID, "%s: %lld rows", what, (long long)T);
-    const int64_t across = (M + 127) / 128, row_tiles = T / kFp4Rows + std::min<int64_t>(T, m->groups);
+    // rows of x in a tile of the kernel with weights on the M side: a third more than a group has on average, so that most
+    // groups take one tile and a stage stays small
+    const int64_t used = std::max<int64_t>(1, std::min<int64_t>(T, m->groups)), each = (T + used - 1) / used;
+    const int tile_rows = (int)std::max<int64_t>(16, std::min<int64_t>(kFp4Rows, ((m->groups > 1 ? each * 4 / 3 : each) + 15) / 16 * 16));
+    const int64_t across = (M + 127) / 128, row_tiles = T / tile_rows + used;
     if (row_tiles * across > INT_MAX / 8)
         return failf(QRM_E_CAPACITY, "%s: %lld rows in %d groups are too many tiles", what, (long long)T, m->groups);
     if (T == 0) return QRM_OK;
@@ -249,16 +244,13 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     DeviceGuard here;
     cudaError_t e = here.enter(m->device);
     if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    const Fp4Form form = m->form >= 0 ? (Fp4Form)m->form : form_of(T, m->groups);
+    const bool pair = m->form >= 0 ? m->form : pair_is_faster(T, used, mode == kFp4Plain ? (M + 255) / 256 : across, m->steps, tile_rows, m->sms);
     const int wide_out = aligned(out, 16) && ld_out * b % 16 == 0;
-    Fp4RowMaps x_maps;
+    CUtensorMap x_map;
     const cuuint64_t dims[2] = {(cuuint64_t)(16 * blocks), (cuuint64_t)T};
     const cuuint64_t strides[1] = {(cuuint64_t)ld_x};
-    for (int i = 0; i < 4; i++) {   // the boxes that the kernel loads
-        const cuuint32_t box[2] = {128, 16u << i};
-        if ((form == kFit || i == (form == kPair ? 3 : 0)) && !encode(&x_maps.rows[i], x, 2, dims, strides, box))
-            return failf(QRM_E_CUDA, "%s: tensor map", what);
-    }
+    const cuuint32_t box[2] = {128, pair ? 128u : 16u};
+    if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
     Fp4Params p{};
     p.w_scales = mode == kFp4Plain ? m->scales : m->gated_scales;
     p.x_scales = xs;
@@ -277,12 +269,13 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     p.steps = m->steps;
     p.blocks = (int)blocks;
     p.type = type;
-    p.row_tiles = (int)(offsets ? row_tiles : (T + kFp4Rows - 1) / kFp4Rows);
+    p.tile_rows = tile_rows;
+    p.row_tiles = (int)(offsets ? row_tiles : (T + tile_rows - 1) / tile_rows);
     p.wide_xs = aligned(xs, 16) && ld_xs % 16 == 0 ? 2 : aligned(xs, 8) && ld_xs % 8 == 0 ? 1 : 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_maps, p, form, wide_out, T, s)
-        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_maps, p, form, wide_out, T, s)
-                            : launch<kFp4GatedRows>(m, x_maps, p, form, wide_out, T, s);
+    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, p, pair, wide_out, T, s)
+        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_map, p, pair, wide_out, T, s)
+                            : launch<kFp4GatedRows>(m, x_map, p, pair, wide_out, T, s);
     return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
 }
 

@@ -48,7 +48,7 @@ struct Fp4Params {
     int steps;                 // stages of the contracted dimension
     int blocks;                // of 32 in it
     int type;                  // of out
-    int row_tiles;             // room for tiles of rows in the grid (weights on the M side)
+    int row_tiles, tile_rows;  // weights on the M side: room for tiles of rows in the grid, most rows of one
     int wide_xs;               // rows of scales start on 16 bytes: 2, on 8: 1
 };
 
@@ -57,11 +57,6 @@ struct Fp4Params {
 __device__ __forceinline__ constexpr uint32_t umma_idesc_mxf4(int m, int n, int part) {
     return ((uint32_t)part << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) |
            ((uint32_t)part << 29);
-}
-// Descriptor of a unit of scales in shared memory for tcgen05.cp: 32 rows of 16
-// bytes one after the other, no swizzle (8-row groups 128 bytes apart).
-__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
 template <int CTAS>
 __device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t a_scales,
@@ -118,8 +113,11 @@ __device__ __forceinline__ bool bar_wait_both(uint32_t a, uint32_t a_parity, uin
     if (__all_sync(0xffffffffu, first && second)) return true;
     return bar_wait(a, a_parity, c) && bar_wait(b, b_parity, c);
 }
-// The high words of the descriptors, which are constants: of operands in the
-// 128-byte swizzle, of units of scales.
+// Descriptors in two words, of which the high ones are constants: of operands in
+// the 128-byte swizzle (as sw128_desc), and of units of scales for tcgen05.cp, 32
+// rows of 16 bytes one after the other without a swizzle (8-row groups 128 bytes
+// apart).  With that, and with what goes into them in registers of the warp, a
+// stage's instructions take the issuing thread 420 cycles in place of 620.
 constexpr uint32_t kSw128High = (1024 >> 4) | (1u << 14) | (2u << 29), kScaleHigh = (128 >> 4) | (1u << 14);
 __device__ __forceinline__ uint32_t sw128_low(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4 | 1u << 16; }
 __device__ __forceinline__ uint32_t scale_low(uint32_t saddr) { return (saddr & 0x3FFFFu) >> 4; }
@@ -199,7 +197,7 @@ struct Fp4Tile {
 // in group_tables; `report`: look at all of them and raise an error for offsets
 // that make no sense.
 __device__ inline Fp4Tile fp4_find(const Fp4Params& p, int at, bool report) {
-    if (!p.offsets) return {0, at * kFp4Rows, min(max(p.T - at * kFp4Rows, 0), kFp4Rows)};
+    if (!p.offsets) return {0, at * p.tile_rows, min(max(p.T - at * p.tile_rows, 0), p.tile_rows)};
     const int lane = threadIdx.x & 31;
     Fp4Tile r{0, 0, 0};
     int before = 0, top = 0;
@@ -220,7 +218,7 @@ __device__ inline Fp4Tile fp4_find(const Fp4Params& p, int at, bool report) {
             bad |= g < p.groups;
             a = b = 0;
         }
-        const int tiles = (b - a + kFp4Rows - 1) / kFp4Rows;
+        const int tiles = (b - a + p.tile_rows - 1) / p.tile_rows;
         int scan = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -232,8 +230,8 @@ __device__ inline Fp4Tile fp4_find(const Fp4Params& p, int at, bool report) {
         if (here && !found) {
             const int from = __ffs(here) - 1;
             r.group = g0 + from;
-            r.pos = __shfl_sync(0xffffffffu, a + in * kFp4Rows, from);
-            r.n = __shfl_sync(0xffffffffu, min(b - a - in * kFp4Rows, kFp4Rows), from);
+            r.pos = __shfl_sync(0xffffffffu, a + in * p.tile_rows, from);
+            r.n = __shfl_sync(0xffffffffu, min(b - a - in * p.tile_rows, p.tile_rows), from);
             found = true;
         }
         before += __shfl_sync(0xffffffffu, scan, 31);
@@ -281,7 +279,7 @@ __device__ __forceinline__ void store_lane4(const Fp4Params& p, long long t, int
 template <int MODE>
 __global__ void __launch_bounds__(kFp4Threads, 2)
 fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
-                 const __grid_constant__ Fp4Params p, int stages, int x_rows /* room for rows of x in a stage */) {
+                 const __grid_constant__ Fp4Params p, int stages) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // [stages] copies are there: the weights', those of x
@@ -292,9 +290,9 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 516);
     volatile uint32_t* issued = reinterpret_cast<volatile uint32_t*>(sm + 520);   // stages, once their warp is through
     Fp4Tile* found = reinterpret_cast<Fp4Tile*>(sm + 528);
-    const uint32_t stage_bytes = fp4_stage_bytes(x_rows);
+    const uint32_t stage_bytes = fp4_stage_bytes(p.tile_rows);
     // a stage: codes of x, codes of both blocks, their scales, scales of x
-    const uint32_t w_off = x_rows * 128, ws_off = w_off + 2 * kFp4Tile, xs_off = ws_off + 2 * kFp4Scales;
+    const uint32_t w_off = p.tile_rows * 128, ws_off = w_off + 2 * kFp4Tile, xs_off = ws_off + 2 * kFp4Scales;
     uint8_t* ring = sm + kFp4Header;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -378,25 +376,25 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         // ------------------------------------------------ MMAs (one thread issues)
         Ring r;
         const uint32_t ring0 = smem_u32(ring);
-        const uint64_t x_desc = sw128_desc(ring0), w_desc = sw128_desc(ring0 + w_off);
-        const uint64_t ws_desc = scale_desc(ring0 + ws_off), xs_desc = scale_desc(ring0 + xs_off);
-        const uint32_t idesc = umma_idesc_mxf4(128, (t.n + 15) & ~15, 0), odd = umma_idesc_mxf4(0, 0, 2) & ~umma_idesc_mxf4(0, 0, 0);
+        const uint32_t x_low = sw128_low(ring0), w_low = sw128_low(ring0 + w_off);
+        const uint32_t ws_low = scale_low(ring0 + ws_off), xs_low = scale_low(ring0 + xs_off), base = uniform(tmem);
+        const uint32_t idesc = umma_idesc_mxf4(128, uniform(t.n + 15) & ~15, 0), odd = umma_idesc_mxf4(0, 0, 2) & ~umma_idesc_mxf4(0, 0, 0);
         for (int k = k0; k < k1; k++) {
-            if (!bar_wait(full0 + 8 * r.i, r.phase, ctl) || !bar_wait(x_full0 + 8 * r.i, r.phase, ctl)) break;
+            if (!bar_wait_both(full0 + 8 * r.i, r.phase, x_full0 + 8 * r.i, r.phase, ctl)) break;
             tc_fence_after();
+            const uint32_t at = r.i * stage_bytes >> 4, wl = w_low + at, xl = x_low + at, wsl = ws_low + at, xsl = xs_low + at;
+            const uint32_t ws = base + kFp4TmemScales + kFp4ScaleCols * ((k - k0) & 1), xs = ws + 16, more = k > k0;
             if (elect_one()) {
-                const uint32_t at = r.i * stage_bytes >> 4;
-                const uint32_t ws = tmem + kFp4TmemScales + kFp4ScaleCols * ((k - k0) & 1), xs = ws + 16;
 #pragma unroll
-                for (int u = 0; u < 4; u++) scales_to_tmem<1>(ws + 4 * u, ws_desc + at + u * (512 >> 4));   // block u / 2, half u % 2
+                for (int u = 0; u < 4; u++) scales_to_tmem<1>(ws + 4 * u, wide_desc(wsl + u * (512 >> 4), kScaleHigh));   // block u / 2, half u % 2
 #pragma unroll
-                for (int u = 0; u < 2; u++) scales_to_tmem<1>(xs + 4 * u, xs_desc + at + u * (512 >> 4));
+                for (int u = 0; u < 2; u++) scales_to_tmem<1>(xs + 4 * u, wide_desc(xsl + u * (512 >> 4), kScaleHigh));
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
                     for (int b = 0; b < 2; b++)
-                        umma_mxf4<1>(tmem + 64 * b, w_desc + at + b * (kFp4Tile >> 4) + 2 * j, x_desc + at + 2 * j,
-                                     j & 1 ? idesc | odd : idesc, ws + 8 * b + 4 * (j >> 1), xs + 4 * (j >> 1), k > k0 || j > 0);
+                        umma_mxf4<1>(base + 64 * b, wide_desc(wl + b * (kFp4Tile >> 4) + 2 * j, kSw128High), wide_desc(xl + 2 * j, kSw128High),
+                                     j & 1 ? idesc | odd : idesc, ws + 8 * b + 4 * (j >> 1), xs + 4 * (j >> 1), j > 0 ? 1 : more);
                 umma_commit(&done[r.i]);
             }
             __syncwarp();
@@ -453,26 +451,49 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     cluster_sync_all();
     if (warp == 1) tmem_dealloc(tmem, kFp4TmemCols);
     // ---------------- this CTA's share of (row, 32 outputs), over all of the cluster
-    constexpr int per_row = MODE == kFp4Plain ? 8 : 4;
+    constexpr int per_row = MODE == kFp4Plain ? 8 : 4, kAtOnce = 4;
     const uint32_t mine = smem_u32(sums);
-    for (int i = rank + ranks * warp; i < t.n * per_row && !*abort_flag; i += ranks * (kFp4Threads / 32)) {
-        const int row = i / per_row, o = 32 * (i % per_row), j = o + lane;
-        // (gated: 16 of gate, 16 of up, and so on)
-        const uint32_t at = mine + 4 * (row * 256 + (MODE == kFp4Plain ? j : 2 * j - (j & 15)));
-        float y = 0.f, up = 0.f;
+    const int items = *abort_flag ? 0 : t.n * per_row, step = ranks * (kFp4Threads / 32);
+    for (int i0 = rank + ranks * warp; i0 < items; i0 += kAtOnce * step) {   // kAtOnce of them, whose loads are on their way together
+        const int now = min((items - i0 + step - 1) / step, kAtOnce);
+        float y[kAtOnce], up[kAtOnce];
+        uint32_t at[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+            const int i = i0 + u * step, j = 32 * (i % per_row) + lane;
+            // (gated: 16 of gate, 16 of up, and so on)
+            at[u] = mine + 4 * (i / per_row * 256 + (MODE == kFp4Plain ? j : 2 * j - (j & 15)));
+            y[u] = up[u] = 0.f;
+        }
 #pragma unroll
         for (int q = 0; q < 8; q++) {
             if (q >= (int)ranks) break;
-            y += load_peer(at, q);
-            if (MODE != kFp4Plain) up += load_peer(at + 64, q);
+            float a[kAtOnce], b[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++) {
+                a[u] = b[u] = 0.f;
+                if (u >= now) break;
+                a[u] = load_peer(at[u], q);
+                if (MODE != kFp4Plain) b[u] = load_peer(at[u] + 64, q);
+            }
+#pragma unroll
+            for (int u = 0; u < kAtOnce; u++) {
+                y[u] += a[u];
+                if (MODE != kFp4Plain) up[u] += b[u];
+            }
         }
-        const long long to = t.pos + row;
-        if (MODE == kFp4Plain) {
-            store_lane(p, to, m0 + o + lane, y);
-        } else {
-            const float h = gated2(make_float2(y, y), make_float2(up, up), p.limit).x;
-            if (MODE == kFp4Gated) store_lane(p, to, m0 + o + lane, h);
-            else store_lane4(p, to, m0 + o, h);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; u++) {
+            const int i = i0 + u * step, o = 32 * (i % per_row);
+            if (u >= now) break;
+            const long long to = t.pos + i / per_row;
+            if (MODE == kFp4Plain) {
+                store_lane(p, to, m0 + o + lane, y[u]);
+            } else {
+                const float h = gated2(make_float2(y[u], y[u]), make_float2(up[u], up[u]), p.limit).x;
+                if (MODE == kFp4Gated) store_lane(p, to, m0 + o + lane, h);
+                else store_lane4(p, to, m0 + o, h);
+            }
         }
     }
     cluster_sync_all();   // the others may still read this CTA's sums
@@ -687,28 +708,29 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             Ring r;
             uint32_t n = 0, buffer = 0;   // tiles; of scales
             const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), ring0 = smem_u32(ring);
-            const uint64_t x_desc = sw128_desc(ring0), w_desc = sw128_desc(ring0 + kFp4Tile);
-            const uint64_t ws_desc = scale_desc(ring0 + 2 * kFp4Tile), xs_desc = scale_desc(ring0 + kFp4PairTx);
+            const uint32_t x_low = sw128_low(ring0), w_low = sw128_low(ring0 + kFp4Tile);
+            const uint32_t ws_low = scale_low(ring0 + 2 * kFp4Tile), xs_low = scale_low(ring0 + kFp4PairTx), base = uniform(tmem);
             constexpr uint32_t idesc[2] = {umma_idesc_mxf4(256, 256, 0), umma_idesc_mxf4(256, 256, 2)};
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs, n++) {
                 // the accumulator of the tile before has been read
                 if (n > 0 && !bar_wait(smem_u32(tile_read), (n - 1) & 1u, ctl)) break;
-                const uint32_t d = tmem + (n & 1 ? kFp4PairSecond : 0);
+                const uint32_t d = base + (n & 1 ? kFp4PairSecond : 0);
                 for (int k = 0; k < steps; k++) {
-                    if (!bar_wait(full0 + 8 * r.i, r.phase, ctl) || !bar_wait(x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
+                    if (!bar_wait_both(full0 + 8 * r.i, r.phase, x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
                     tc_fence_after();
+                    const uint32_t at = r.i * (kFp4PairStage >> 4), wl = w_low + at, xl = x_low + at, wsl = ws_low + at, xsl = xs_low + at;
+                    const uint32_t xs = base + kFp4PairTmemScales + kFp4ScaleCols * buffer, ws = xs + 8, more = k > 0;
                     if (elect_one()) {
-                        const uint32_t at = r.i * (kFp4PairStage >> 4);
-                        const uint32_t xs = tmem + kFp4PairTmemScales + kFp4ScaleCols * buffer, ws = xs + 8;
 #pragma unroll
                         for (int u = 0; u < 2; u++) {   // half of the stage's contracted values
-                            scales_to_tmem<2>(xs + 4 * u, xs_desc + at + u * (512 >> 4));
-                            scales_to_tmem<2>(ws + 8 * u, ws_desc + at + u * (512 >> 4));
-                            scales_to_tmem<2>(ws + 8 * u + 4, ws_desc + at + (kFp4Scales + u * 512 >> 4));
+                            scales_to_tmem<2>(xs + 4 * u, wide_desc(xsl + u * (512 >> 4), kScaleHigh));
+                            scales_to_tmem<2>(ws + 8 * u, wide_desc(wsl + u * (512 >> 4), kScaleHigh));
+                            scales_to_tmem<2>(ws + 8 * u + 4, wide_desc(wsl + (kFp4Scales + u * 512 >> 4), kScaleHigh));
                         }
 #pragma unroll
                         for (int j = 0; j < 4; j++)
-                            umma_mxf4<2>(d, x_desc + at + 2 * j, w_desc + at + 2 * j, idesc[j & 1], xs + 4 * (j >> 1), ws + 8 * (j >> 1), k > 0 || j > 0);
+                            umma_mxf4<2>(d, wide_desc(xl + 2 * j, kSw128High), wide_desc(wl + 2 * j, kSw128High), idesc[j & 1], xs + 4 * (j >> 1),
+                                         ws + 8 * (j >> 1), j > 0 ? 1 : more);
                         umma_commit_pair(done0 + 8 * r.i);
                         if (k + 1 == steps) umma_commit_pair(smem_u32(tile_done) + 8 * (n & 1));
                     }
@@ -829,461 +851,6 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
         if (rank == 0 && threadIdx.x == 0) {
             Fp4PairBars bars{full};
             drain_pair(issued, from_peer, kFp4PairStages, bars);
-        }
-        if (warp == 1) {
-            if (rank == 0 && elect_one()) umma_commit_pair(smem_u32(left_bar));
-            __syncwarp();
-            if (lane == 0) mbar_wait(left_bar, 0u);
-        }
-        __syncwarp();
-        cluster_sync_all();
-    }
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
-}
-
-// ------------------------------------------------------------ pairs with weights on the MMA's M side
-// The same pair of SMs with the operands' places changed: 256 outputs (gated: 128
-// features) on the M side, up to 384 rows of x on the N side, rounded up to 32
-// only and shared evenly among a group's tiles.  Groups whose rows are no
-// multiple of 256 cost what their rows cost, and the weights of a group of up to
-// 384 rows are loaded once.  Past 256 rows a step takes two MMAs, of 128 rows and
-// of the others.
-//
-// A lane of tensor memory is an output.  For the gated product the lanes of gate
-// and of up exchange half of their columns, so that each has both sums of 16 rows;
-// on their way into 4-bit rows, whose blocks are two warps', they meet in shared
-// memory, 32 rows of x at a time, [row][feature] in f32.
-//
-// Two accumulators where two neighbouring tiles have 224 rows at most; else a
-// tile's MMAs wait for the one before to be read.
-//
-// The scales of x go through registers, and a fence between what they write to
-// shared memory and the copy to tensor memory waits for loads of the same warp
-// that are on their way (a quarter of the time went there).  So the warps that
-// load and write them do not fence: they tell another one, which does.
-//
-// Warps: 0 loads codes and the weights' scales, 1 issues the MMAs (in the
-// pair's first CTA), 2 fences, 4-7 bring the scales of x (in both CTAs), 8-11 and
-// 12-15 write the output, every second 32 rows each.
-constexpr int kFp4FitThreads = 512;
-constexpr int kFp4FitMaxStages = 8;
-constexpr int kFp4FitRows = 384;
-constexpr int kFp4FitSecond = 224, kFp4FitTmemScales = 448, kFp4FitScaleCols = 32;
-constexpr int kFp4FitRoom = 32 * 80 * 4;       // four warps' room for 32 rows on their way into 4 bits
-constexpr int kFp4FitRegsFew = 56, kFp4FitRegsMany = 200;
-constexpr int kFp4FitRegs = 256 * kFp4FitRegsFew + 256 * kFp4FitRegsMany;
-static_assert(kFp4FitRegs <= kFp4FitThreads * 128, "register split");
-// a stage: codes of the weights, of x (a CTA's half of up to `rows`, the most that a tile has), scales of the weights, of x
-__host__ __device__ inline int fp4_fit_codes(int rows) { return kFp4Tile + rows / 2 * 128; }
-__host__ __device__ inline int fp4_fit_stage(int rows) { return fp4_fit_codes(rows) + kFp4Scales + (rows + 127) / 128 * kFp4Scales; }
-
-struct Fp4RowMaps {
-    CUtensorMap rows[4];   // x in boxes of 256 columns x 16, 32, 64 and 128 rows
-};
-// the first CTA's barriers, as drain_pair moves them on; the tiles' stages have different numbers of bytes
-struct Fp4FitBars {
-    uint64_t* full;
-    volatile uint32_t* bytes;   // a CTA's share of the stage that it issued last in each slot
-    __device__ uint32_t peer_bytes(uint32_t slot) const {
-        uint32_t a, v;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(a) : "r"(smem_u32(const_cast<uint32_t*>(&bytes[slot]))));
-        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-        return v;
-    }
-    __device__ void expect(uint32_t slot) { mbar_arrive_expect_tx(&full[slot], peer_bytes(slot)); }
-    __device__ void complete(uint32_t slot) {
-        asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[slot])), "r"(bytes[slot])
-                     : "memory");
-    }
-    __device__ void wait(uint32_t slot, uint32_t parity) { mbar_wait(&full[slot], parity); }
-};
-
-// whether it holds for all of `threads`, which meet here
-__device__ __forceinline__ bool all_of(int barrier, int threads, bool holds) {
-    uint32_t r;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-                 : "=r"(r)
-                 : "r"((uint32_t)holds), "r"(barrier), "r"(threads)
-                 : "memory");
-    return r != 0;
-}
-// 32 columns of this warp's lanes of tensor memory, which are there after loaded()
-__device__ __forceinline__ void tmem_ld32_later(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
-}
-template <int N>
-__device__ __forceinline__ void loaded(float (&v)[N][32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < N; i++)
-#pragma unroll
-        for (int j = 0; j < 32; j++) asm volatile("" : "+f"(v[i][j]));   // (no use of the registers before the wait)
-}
-// Output m of rows first, first + step, ..., of which `have` count from row t on,
-// by a lane; a warp's lanes write neighbouring outputs.  No way through shared
-// memory: copies and MMAs leave its ports little time (32 rows of 128 outputs
-// took 1900 cycles that way).
-template <typename T, int N>
-__device__ __forceinline__ void store_outputs(const Fp4Params& p, long long t, int first, int step, int have, int m, const float (&v)[N]) {
-    if (m >= p.M) return;
-    T* out = reinterpret_cast<T*>(p.out) + (t + first) * p.ld_out + m;
-    const long long ahead = step * p.ld_out;
-#pragma unroll
-    for (int c = 0; c < N; c++) {
-        if (first + c * step < have) *out = round_to<T>(v[c]);
-        out += ahead;
-    }
-}
-template <int N>
-__device__ __forceinline__ void store_outputs(const Fp4Params& p, long long t, int first, int step, int have, int m, const float (&v)[N]) {
-    if (p.type == 0) store_outputs<float>(p, t, first, step, have, m, v);
-    else if (p.type == 1) store_outputs<__half>(p, t, first, step, have, m, v);
-    else store_outputs<__nv_bfloat16>(p, t, first, step, have, m, v);
-}
-
-template <int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp4FitThreads, 1)
-fp4_fit_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap s_map,
-               const __grid_constant__ Fp4RowMaps x_maps, const __grid_constant__ Fp4Params p, int stages,
-               int x_rows /* most rows of x in a tile */) {
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-    uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // first CTA: both CTAs' copies are there
-    uint64_t* x_full = full + kFp4FitMaxStages;         // first CTA: both CTAs' scales of x are there
-    uint64_t* x_written = x_full + kFp4FitMaxStages;    // its own are written
-    uint64_t* done = x_written + kFp4FitMaxStages;      // both: the stage's MMAs are done
-    uint64_t* tile_done = done + kFp4FitMaxStages;         // [2] both: a tile's are
-    uint64_t* tile_read = tile_done + 2;                // [2] first CTA: both epilogues have read an accumulator
-    uint64_t* done_bar = tile_read + 2;
-    uint64_t* left_bar = done_bar + 1;                  // both, when the first CTA gave up: its commits are through
-    __shared__ volatile int given_up;
-    __shared__ volatile uint32_t from_peer, issued;     // issued: stages, once their warp is through
-    __shared__ volatile uint32_t bytes[kFp4FitMaxStages];
-    volatile int* abort_flag = &given_up;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 776);
-    int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp4PairTableOff);
-    int32_t* start = first_tile + p.groups + 1;
-    int32_t* rows = start + p.groups + 1;
-    uint8_t* ring = sm + fp4_pair_stage_off(p.groups);
-    const uint32_t stage_bytes = fp4_fit_stage(x_rows), ws_off = fp4_fit_codes(x_rows), xs_off = ws_off + kFp4Scales;
-
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = blockIdx.x & 1;   // in the pair: the cluster is two CTAs along x
-    constexpr int kHalf = MODE == kFp4Plain ? 128 : 64;   // outputs of a CTA in a tile
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < stages; i++) {
-            mbar_init(&full[i], 1);
-            mbar_init(&x_full[i], 2);
-            mbar_init(&x_written[i], 4);
-            mbar_init(&done[i], 1);
-        }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&tile_done[i], 1);
-            mbar_init(&tile_read[i], 16);
-        }
-        mbar_init(done_bar, 1);
-        mbar_init(left_bar, 1);
-        *abort_flag = 0;
-        issued = 0;
-        fence_barrier_init();
-    }
-    if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    }
-    pdl_start();   // nothing before this reads or writes global memory
-    if (warp == 2) group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows, x_rows, (p.M + 2 * kHalf - 1) / (2 * kHalf), blockIdx.x == 0);
-    tc_fence_before();
-    __syncthreads();
-    cluster_sync_all();   // the peer's barriers are ready
-    tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
-    const WaitCtl ctl{abort_flag, p.err};
-    const uint32_t done0 = smem_u32(done);
-    const int tiles = first_tile[p.groups], pairs = gridDim.x >> 1, steps = p.steps;
-
-    struct Tile {
-        int group, m;      // matrix, first output of the pair
-        int pos, n;        // first row of x, rows
-        int cols;          // n in whole 32s: columns of the accumulator
-    };
-    // the tiles of one block of outputs follow each other, so its weights come from HBM once
-    auto tile_at = [&](int i) {
-        int lo = 0, hi = p.groups;   // the last group with first_tile <= i has rows
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (first_tile[mid] <= i) lo = mid;
-            else hi = mid;
-        }
-        const int blocks = (rows[lo] + x_rows - 1) / x_rows, in = i - first_tile[lo], m = in / blocks;
-        const int per = ((rows[lo] + blocks - 1) / blocks + 31) & ~31, at = (in - m * blocks) * per, n = min(per, rows[lo] - at);
-        return Tile{lo, m * 2 * kHalf, start[lo] + at, n, (n + 31) & ~31};
-    };
-
-    // where in tensor memory a pair's n-th tile is
-    auto place = [](uint32_t n, int cols) { return (n & 1) && cols <= kFp4FitSecond ? kFp4FitSecond : 0; };
-    if (warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp4FitRegsFew));
-        if (warp == 0) {
-            // -------------------------------------------- codes and the weights' scales
-            bool ok = true;
-            Ring r;
-            uint32_t n_issued = 0;
-            const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
-            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
-                const Tile t = tile_at(i);
-                const int m = t.m + kHalf * (int)rank, first = t.cols > 256 ? 128 : t.cols;
-                const uint32_t share = kFp4Tile + (t.cols >> 1) * 128 + kFp4Scales;
-                // A copy for each lane: 0 the weights', 1 their scales, 2-5 and 6-9 this CTA's halves of the MMAs' rows of x,
-                // a box for each power of two in their number.  (One thread with a loop over the boxes took up to 0.5 us a
-                // stage; boxes of 16 rows cost more to issue than to load.)
-                const int part = lane >= 6, box = (lane - 2) & 3, rows_of = (part ? t.cols - first : first) >> 1;
-                const bool copies = lane < 2 || (lane < 10 && rows_of >> box & 16);
-                const int below = rows_of & ((16 << box) - 1);   // rows of the boxes before
-                const CUtensorMap* map = lane == 1 ? &s_map : &x_maps.rows[box];
-                const uint32_t offset = lane == 1 ? ws_off : kFp4Tile + 128 * ((part ? first >> 1 : 0) + below);
-                int x = 0, y = lane == 1 ? (t.group * p.units + m / kHalf) * steps * 4 : t.pos + (part ? first : 0) + rows_of * (int)rank + below;
-                const int x_step = lane == 1 ? 0 : 128, y_step = lane == 1 ? 4 : 0;
-                for (int k = 0; k < steps; k++) {
-                    if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
-                    const uint32_t st = ring0 + r.i * stage_bytes, bar = full0 + 8 * r.i;
-                    if (lane == 0) {
-                        bytes[r.i] = share;
-                        if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * share);
-                        load_weights_pair<MODE != kFp4Plain>(st, &w_map, k * 128, m, t.group, bar);
-                    } else if (copies) {
-                        tma_pair_2d(st + offset, map, x, y, bar);
-                    }
-                    x += x_step;
-                    y += y_step;
-                    __syncwarp();
-                    r.next(stages);
-                    n_issued++;
-                }
-            }
-            if (lane == 0) issued = n_issued;
-        } else if (warp == 1 && rank == 0) {
-            // -------------------------------------------- MMAs (one thread issues for both CTAs)
-            bool ok = true;
-            Ring r;
-            uint32_t n = 0, buffer = 0;   // tiles; of scales
-            int before = 0, before_end = 0;   // the columns of the tile before
-            const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), ring0 = smem_u32(ring), read0 = smem_u32(tile_read);
-            const uint32_t w_low = sw128_low(ring0), x_low = sw128_low(ring0 + kFp4Tile);
-            const uint32_t ws_low = scale_low(ring0 + ws_off), xs_low = scale_low(ring0 + xs_off), base = uniform(tmem);
-            const uint32_t odd = umma_idesc_mxf4(0, 0, 2) & ~umma_idesc_mxf4(0, 0, 0);
-            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs, n++) {
-                const Tile t = tile_at(i);
-                const uint32_t a = n & 1;
-                const int cols = uniform(t.cols);
-                const int at_col = place(n, cols), first = cols > 256 ? 128 : cols;
-                const uint32_t d = base + at_col, idesc = umma_idesc_mxf4(256, first, 0), idesc2 = umma_idesc_mxf4(256, cols - first, 0);
-                // the columns have been read: of the tile two before, and of the one before where they are the same
-                if (n > 1 && !bar_wait(read0 + 8 * a, ((n >> 1) - 1) & 1u, ctl)) break;
-                if (n > 0 && before < at_col + cols && at_col < before_end && !bar_wait(read0 + 8 * (a ^ 1), ((n - 1) >> 1) & 1u, ctl)) break;
-                before = at_col;
-                before_end = at_col + cols;
-                for (int k = 0; k < steps; k++) {
-                    if (!bar_wait_both(full0 + 8 * r.i, r.phase, x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t at = r.i * stage_bytes >> 4, wl = w_low + at, xl = x_low + at, wsl = ws_low + at, xsl = xs_low + at;
-                    const uint32_t ws = base + kFp4FitTmemScales + kFp4FitScaleCols * buffer, xs = ws + 8;   // of x: 12 columns a half
-                    const uint32_t more = k > 0;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int u = 0; u < 2; u++) {   // half of the stage's contracted values
-                            scales_to_tmem<2>(ws + 4 * u, wide_desc(wsl + u * (512 >> 4), kScaleHigh));
-                            scales_to_tmem<2>(xs + 12 * u, wide_desc(xsl + u * (512 >> 4), kScaleHigh));
-                            if (cols > 128) scales_to_tmem<2>(xs + 12 * u + 4, wide_desc(xsl + (kFp4Scales + u * 512 >> 4), kScaleHigh));
-                            if (cols > 256) scales_to_tmem<2>(xs + 12 * u + 8, wide_desc(xsl + (2 * kFp4Scales + u * 512 >> 4), kScaleHigh));
-                        }
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const uint64_t wd = wide_desc(wl + 2 * j, kSw128High);
-                            umma_mxf4<2>(d, wd, wide_desc(xl + 2 * j, kSw128High), j & 1 ? idesc | odd : idesc, ws + 4 * (j >> 1), xs + 12 * (j >> 1), j > 0 ? 1 : more);
-                            if (cols > 256)
-                                umma_mxf4<2>(d + 128, wd, wide_desc(xl + (64 * 128 >> 4) + 2 * j, kSw128High), j & 1 ? idesc2 | odd : idesc2,
-                                             ws + 4 * (j >> 1), xs + 12 * (j >> 1) + 4, j > 0 ? 1 : more);
-                        }
-                        umma_commit_pair(done0 + 8 * r.i);
-                        if (k + 1 == steps) umma_commit_pair(smem_u32(tile_done) + 8 * a);
-                    }
-                    __syncwarp();
-                    r.next(stages);
-                    buffer ^= 1;
-                }
-            }
-            // every MMA has completed before tensor memory is released
-            if (elect_one()) {
-                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done_bar)) : "memory");
-                mbar_wait(done_bar, 0u);
-            }
-            __syncwarp();
-        } else if (warp == 2) {
-            // -------------------------------------------- what the others wrote, handed over
-            bool ok = true;
-            Ring r;
-            const uint32_t x_full0 = map_to_rank0(smem_u32(x_full)), x_written0 = smem_u32(x_written);
-            for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
-                for (int k = 0; k < steps; k++) {
-                    if (!bar_wait(x_written0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
-                    fence_async();
-                    if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
-                    r.next(stages);
-                }
-            }
-        } else if (warp >= 4) {
-            // -------------------------------------------- scales of x: rows 32 (warp - 4) + lane, + 128, + 256 of the tile
-            // (two stages' at a time, the next two's on their way)
-            bool ok = true;
-            Ring r;
-            const int first = 32 * (warp - 4) + lane;
-            const uint32_t x_written0 = smem_u32(x_written);
-            uint4 next[3];
-            auto load = [&](const Tile& t, int k) {
-                const uint8_t* row = p.x_scales + (long long)(t.pos + first) * p.ld_xs;
-#pragma unroll
-                for (int v = 0; v < 3; v++)
-                    next[v] = first + 128 * v < t.n ? sixteen_scales(row + 128 * v * p.ld_xs, 8 * k, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
-            };
-            int i = blockIdx.x >> 1;
-            if (i < tiles) load(tile_at(i), 0);
-            for (; i < tiles && ok; i += pairs) {
-                const Tile t = tile_at(i);
-                for (int k2 = 0; k2 < steps && ok; k2 += 2) {
-                    const uint4 now[3] = {next[0], next[1], next[2]};
-                    if (k2 + 2 < steps) load(t, k2 + 2);
-                    else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        if (k2 + j >= steps) break;
-                        if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
-                        uint32_t* to = reinterpret_cast<uint32_t*>(ring + r.i * stage_bytes + xs_off) + 4 * lane + (warp - 4);
-#pragma unroll
-                        for (int v = 0; v < 3; v++)
-                            if (128 * v < t.cols) {
-                                to[256 * v] = j ? now[v].z : now[v].x;
-                                to[256 * v + 128] = j ? now[v].w : now[v].y;
-                            }
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(x_written0 + 8 * r.i);
-                        r.next(stages);
-                    }
-                }
-            }
-        }
-    } else {
-        // ------------------------------------------------ output
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp4FitRegsMany));
-        const int half = (warp - 8) >> 2, quarter = warp & 3, id = 32 * quarter + lane;   // (warps 8-11, 12-15: quarters 0-3)
-        const uint32_t taddr = tmem + ((uint32_t)(32 * quarter) << 16), read0 = map_to_rank0(smem_u32(tile_read));
-        float* room = reinterpret_cast<float*>(ring + stages * stage_bytes + half * kFp4FitRoom);
-        constexpr int kPitch = 80;   // floats of a row there (the lanes' banks differ)
-        uint32_t n = 0;
-        for (int i = blockIdx.x >> 1; i < tiles; i += pairs, n++) {
-            const Tile t = tile_at(i);
-            // (one of the four warps that gives up takes the others along: they meet at barriers from here on)
-            if (!all_of(1 + half, 128, bar_wait(smem_u32(tile_done) + 8 * (n & 1), (n >> 1) & 1u, ctl))) break;
-            tc_fence_after();
-            const uint32_t from = taddr + place(n, t.cols);
-            const int m = t.m + kHalf * (int)rank;
-            // Every second 32 rows of x are this half's, `mine` of them: all but four, and the last four, whose columns are
-            // in registers when the accumulator is handed back.
-            const int mine = (t.cols + 32 - 32 * half) >> 6;
-#pragma unroll 1
-            for (int last = mine > 4 ? 0 : 1; last < 2; last++) {
-                const int c0 = last ? max(mine - 4, 0) : 0, count = last ? min(mine, 4) : mine - 4;
-                float acc[4][32];
-#pragma unroll
-                for (int h = 0; h < 4; h++)
-                    if (h < count) tmem_ld32_later(from + 64 * (c0 + h) + 32 * half, acc[h]);
-                loaded(acc);
-                if (last) {
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) bar_arrive_cluster(read0 + 8 * (n & 1));
-                }
-#pragma unroll
-                for (int h = 0; h < 4; h++) {
-                    const int at = 64 * (c0 + h) + 32 * half, have = t.n - at;   // (the same for all four warps)
-                    if (h >= count || have <= 0) break;
-                    const float (&v)[32] = acc[h];
-                    const long long row = t.pos + at;
-                    if (MODE == kFp4Plain) {
-                        store_outputs(p, row, 0, 1, have, m + id, v);
-                    } else {
-                        // gate's lanes get both sums of the even rows, up's of the odd ones
-                        const bool up = lane & 16;
-                        float y[16];
-#pragma unroll
-                        for (int c = 0; c < 32; c += 4) {
-                            const float g0 = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 16);
-                            const float g1 = __shfl_xor_sync(0xffffffffu, up ? v[c + 2] : v[c + 3], 16);
-                            const float2 own = up ? make_float2(v[c + 1], v[c + 3]) : make_float2(v[c], v[c + 2]);
-                            const float2 other = make_float2(g0, g1);
-                            const float2 f = gated2(up ? other : own, up ? own : other, p.limit);
-                            y[c / 2] = f.x;
-                            y[c / 2 + 1] = f.y;
-                        }
-                        const int feature = 16 * quarter + (lane & 15);
-                        if (MODE == kFp4Gated) {
-                            store_outputs(p, row, up, 2, have, m + feature, y);
-                        } else {
-                            named_barrier(1 + half, 128);   // what was in the room is out
-                            float* to = room + (up ? kPitch : 0) + feature;
-#pragma unroll
-                            for (int c = 0; c < 16; c++) to[2 * c * kPitch] = y[c];
-                            named_barrier(1 + half, 128);   // 32 rows are there
-                            const int left = p.M - m;
-#pragma unroll
-                            for (int j = 0; j < 2; j++) {   // eight features a lane, four lanes a block
-                                const int r = (id + 128 * j) >> 3, o = (id & 7) * 8;
-                                const float4* f = reinterpret_cast<const float4*>(room + r * kPitch + o);
-                                const float4 a = f[0], b = f[1];
-                                float e[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                                uint32_t top = 0;
-#pragma unroll
-                                for (int k = 0; k < 8; k++) {
-                                    if (o + k >= left) e[k] = 0.f;
-                                    top = max(top, magnitude(e[k]));
-                                }
-                                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                                const uint32_t scale = fp4_scale(top), q = e2m1x8(e, scale);
-                                if (r < have && o / kFp4Block * kFp4Block < left) {
-                                    *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (row + r) * p.ld_out + (m + o) / 2) = q;
-                                    if ((id & 3) == 0) p.out_scales[(row + r) * p.ld_os + (m + o) / kFp4Block] = (uint8_t)scale;
-                                }
-                            }
-                        }
-                    }
-                }
-            }
-        }
-    }
-    // ---------------- teardown: every role of both CTAs is done (or gave up); free tensor memory
-    tc_fence_before();
-    __syncthreads();
-    // (as in fp8_pair_kernel: the first CTA learns how many stages the other has issued, which learns whether to stay)
-    if (threadIdx.x == 0) store_peer(const_cast<uint32_t*>(&from_peer), rank ^ 1, rank == 0 ? (uint32_t)given_up : issued);
-    __syncwarp();
-    cluster_sync_all();
-    tc_fence_after();
-    if (rank == 0 ? given_up != 0 : from_peer != 0) {
-        if (rank == 0 && threadIdx.x == 0) {
-            Fp4FitBars bars{full, bytes};
-            drain_pair(issued, from_peer, stages, bars);
         }
         if (warp == 1) {
             if (rank == 0 && elect_one()) umma_commit_pair(smem_u32(left_bar));

@@ -135,12 +135,12 @@ class Case:
         return Q.Fp4Matrix(self.n, self.k, self.w[0].cuda(), self.w[1].cuda(), groups=self.groups)
 
 
-@pytest.fixture(params=["0", "1", "2", None], ids=["split", "pair", "fit", "chosen"])
+@pytest.fixture(params=["0", "1", None], ids=["split", "pair", "chosen"])
 def form(request, monkeypatch):
     if request.param is None:
-        monkeypatch.delenv("QRM_FP4_FORM", raising=False)
+        monkeypatch.delenv("QRM_FP4_PAIR", raising=False)
     else:
-        monkeypatch.setenv("QRM_FP4_FORM", request.param)
+        monkeypatch.setenv("QRM_FP4_PAIR", request.param)
     return request.param
 
 
