@@ -46,9 +46,9 @@ class Fp8Experts:
                                stream=torch.cuda.current_stream().cuda_stream)
         return Q.Fp8Matrix(rows, cols, codes, scales, groups=groups, device=w.device.index or 0)
 
-    def forward(self, x, topk_idx, topk_w):
+    def forward(self, x, topk_idx, topk_w, add=None):
         """x [T, d] bf16, topk_idx [T, k] int32 (-1: none), topk_w [T, k] f32 ->
-        (x + the experts' weighted outputs, what the backward needs)."""
+        (x, or add, + the experts' weighted outputs, what the backward needs)."""
         stream = torch.cuda.current_stream().cuda_stream
         T, k = topk_idx.shape
         n = T * k
@@ -65,11 +65,12 @@ class Fp8Experts:
         self.gate_up.product(BF16, *x8, n, gu, offsets, stream=stream)
         Q.swiglu_fp8(BF16, gu, n, self.ffn, *h8, limit=self.limit, n_rows=held, stream=stream)
         self.down.product(BF16, *h8, n, y, offsets, stream=stream)
-        Q.combine_rows(BF16, y, n, pos, topk_w, T, k, self.d, out, add=x, stream=stream)
+        Q.combine_rows(BF16, y, n, pos, topk_w, T, k, self.d, out, add=x if add is None else add, stream=stream)
         return out, (pos, offsets, gu, y, topk_w)
 
-    def backward(self, dout, kept):
-        """dout [T, d] bf16 -> (dx, dw)."""
+    def backward(self, dout, kept, through=True):
+        """dout [T, d] bf16 -> (dx, dw); through: with dout itself, the gradient of
+        the x that forward added."""
         stream = torch.cuda.current_stream().cuda_stream
         pos, offsets, gu, y, w = kept
         T, k = w.shape
@@ -85,7 +86,7 @@ class Fp8Experts:
         Q.swiglu_fp8_grad(BF16, gu, dh, n, self.ffn, *dgu8, limit=self.limit, n_rows=held, stream=stream)
         self.gate_up.product_t(BF16, *dgu8, n, dxr, offsets, stream=stream)
         # the gradient of the gather, on top of the residual stream's own
-        Q.combine_rows(BF16, dxr, n, pos, None, T, k, self.d, dx, add=dout, stream=stream)
+        Q.combine_rows(BF16, dxr, n, pos, None, T, k, self.d, dx, add=dout if through else None, stream=stream)
         return dx, dw
 
     def sync(self):
@@ -96,6 +97,31 @@ class Fp8Experts:
     def close(self):
         self.gate_up.close()
         self.down.close()
+
+
+class PreNormExperts:
+    """s = x + residual, out = s + experts(norm(s)); norm_w [d] f32."""
+
+    def __init__(self, experts, norm_w, eps=1e-5):
+        self.experts, self.w, self.eps = experts, norm_w, eps
+
+    def forward(self, x, residual, topk_idx, topk_w):
+        stream = torch.cuda.current_stream().cuda_stream
+        total, y = torch.empty_like(x), torch.empty_like(x)
+        Q.rms_norm(BF16, x, *x.shape, self.w, self.eps, y, add=residual, sum=total, stream=stream)
+        out, kept = self.experts.forward(y, topk_idx, topk_w, add=total)
+        return out, (total, kept)
+
+    def backward(self, dout, kept):
+        """(the gradient of x and of the residual, which is the same, of the
+        norm's weight and of the routing weights)"""
+        stream = torch.cuda.current_stream().cuda_stream
+        total, inner = kept
+        dy, dtopk = self.experts.backward(dout, inner, through=False)
+        dx, dw = torch.empty_like(dout), torch.empty_like(self.w)
+        work = torch.empty(Q.rms_norm_grad_work(*dout.shape), device=dout.device)
+        Q.rms_norm_grad(BF16, dy, total, *dout.shape, self.w, self.eps, dx, dw=dw, work=work, add=dout, stream=stream)
+        return dx, dw, dtopk
 
 
 def plain(x, idx, w, w_gate_up, w_down, limit=0.0):

@@ -303,6 +303,26 @@ def test_offsets_that_make_no_sense(offsets, bad, form):
     m.close()
 
 
+@pytest.mark.parametrize("offsets,bad", [([3, 9], False), ([4, 4], False), ([0, 11], True), ([6, 2], True), ([-1, 5], True)])
+def test_one_group_of_some_rows(offsets, bad, form):
+    """One matrix, whose weights are asked for before the offsets are known."""
+    c = Case(10, 1, 96, 2100)
+    m = c.matrix()
+    y = torch.full((10, 96), 5.0).cuda()
+    m.product(0, c.x[0].cuda(), c.x[1].cuda(), 10, y, offsets=torch.tensor(offsets, dtype=torch.int32).cuda())
+    want = torch.full((10, 96), 5.0)
+    if bad:
+        with pytest.raises(Q.QrmError) as e:
+            m.sync()
+        assert e.value.code == Q.E_INVALID
+    else:
+        m.sync()
+        a, b = offsets
+        want[a:b] = c.want.float()[a:b]
+    assert torch.equal(y.cpu(), want)
+    m.close()
+
+
 def test_many_groups():
     """1024 matrices, most without rows."""
     c = Case(40, 1024, 32, 64)

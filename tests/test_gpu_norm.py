@@ -40,7 +40,7 @@ def near(got, want, bound, type):
     assert bool((off <= slack).all()), float((off / slack).max())
 
 
-SHAPES = [(1, 1), (1, 7), (2, 8), (3, 33), (5, 130), (4, 1024), (3, 2049), (2, 2816), (400, 300), (3, 2820), (3, 7168), (2, 8193), (2, 16385),
+SHAPES = [(1, 1), (1, 7), (2, 8), (3, 33), (5, 130), (4, 1024), (3, 2049), (2, 2816), (400, 300), (3, 2820), (3, 7168), (2, 8193), (2, 12288), (2, 16385),
           (300, 64)]
 
 
