@@ -170,19 +170,26 @@ __device__ __forceinline__ float2 gated2(float2 gate, float2 up, float limit) {
 
 // ------------------------------------------------------------ weights on the MMA's M side
 // For groups of few rows, which reading the weights bounds.  A tile is 256
-// outputs (two blocks of 128; gated: 128 of gate and the same of up) x up to 64
-// rows of x, the MMA's N, rounded up to 16 only.  A cluster of CTAs shares a
-// tile's contracted dimension, so that one token through one matrix is read by
-// most SMs; each leaves its f32 sums in its shared memory, and then each adds up
-// its share of the outputs over all of them, in their order.  No partial sums in
-// global memory, so calls need no workspace and may overlap; two CTAs fit on an
-// SM, and one's start and end go on behind the other's loads.
+// outputs (two blocks of 128; gated: 128 features) x up to tile_rows <= 64 rows
+// of x, the MMA's N, rounded up to 16 only.  A cluster of CTAs shares a tile's
+// contracted dimension, so that one token through one matrix is read by most
+// SMs; each leaves its f32 sums in its shared memory, and then each adds up its
+// share of the outputs over all of them, in their order.  No partial sums in
+// global memory, so calls need no workspace and may overlap.
+//
+// Two CTAs fit on an SM, so one's start and end, or the next launch's start, go on
+// behind the other's loads; where there is one matrix, its first stages are asked
+// for before the launch before has ended.  Together that took one row through
+// 4096 x 7168 (15.6 MB) from 12.2 to 7.1 us, the rest of which is latencies: the
+// first loads, the MMAs, two cluster barriers and reads of other SMs between them.
+// 256 rows over 32 x 4096 x 7168 (499 MB): 80 us, 6.3 TB/s; 16 rows, which 12.7 of
+// the 32 have on average: 36 us (floor 30).
 //
 // Warps: 0 loads codes and the weights' scales, 1 issues the MMAs, 2 finds the
 // tile and brings the scales of x; all eight write the output.
 constexpr int kFp4Threads = 256;
 constexpr int kFp4Rows = 64;                 // most rows of x in a tile
-constexpr int kFp4MaxStages = 6;
+constexpr int kFp4MaxStages = 4;
 constexpr int kFp4TmemCols = 256;            // two accumulators of 64 columns, scales behind them
 constexpr int kFp4TmemScales = 128;
 constexpr int kFp4ScaleCols = 24;            // of one stage: weights 2 x 2 x 4, x 2 x 4
@@ -502,17 +509,27 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // ------------------------------------------------------------ rows of x on the MMA's M side
 // For groups of many rows, which the tensor cores bound.  A pair of SMs
 // (cta_group::2) shares a tile of 256 rows of x times 256 outputs (gated: 128
-// features): each CTA loads 128 rows of x and 128 of the weights, 32 KB of codes for 256 contracted values, 64 bytes a
-// cycle at the full MMA rate.
+// features): each CTA loads 128 rows of x and 128 of the weights, 32 KB of codes
+// for 256 contracted values, and the MMA reads both halves of the weights.
+//
+// 4096 rows, 28672 x 4096: 174 us, 5.5 PFLOP/s, and 207 under sustained load: the
+// power cap bounds it (the same launch on an idle GPU takes 415 cycles a stage,
+// as many as its four MMAs).  What took it there from 310 us: the scales of x
+// handed over without a cluster-scope release (a full memory barrier with every
+// stage) and asked for four stages at a time, rows out by way of shared memory,
+// descriptors with constant high words.  8192 rows over 32 x 4096 x 7168: 141 us,
+// of which a third goes to rows that a group's last tile does not have.  The
+// places of the operands changed (rows of x as the MMA's N, rounded up to 32 only,
+// 384 a tile) it took 137 us there, and more everywhere else.
 //
 // Tensor memory holds two accumulators of 256 columns but for the scales' 48
 // columns: the second begins 48 before the first ends, and a tile's MMAs wait
-// for the epilogue of the one before to have read its accumulator (a few hundred
+// for the epilogue of the one before to have read its accumulator (some 1000
 // cycles, in which the ring of stages fills up).
 //
 // Warps: 0 loads codes and the weights' scales, 1 issues the MMAs (in the
-// pair's first CTA), 2 and 3 bring the scales of x, 4-11
-// write the output: lane quarter (warp & 3), half of the columns (warp >= 8).
+// pair's first CTA), 2 and 3 bring the scales of x, 4-11 write the output: lane
+// quarter (warp & 3), half of the columns (warp >= 8).
 constexpr int kFp4PairThreads = 384;
 constexpr int kFp4PairStages = 5;
 constexpr int kFp4PairTx = 2 * kFp4Tile + 2 * kFp4Scales;            // bytes of a CTA's copies of a stage

@@ -1,4 +1,4 @@
-// host_util.h -- what the operator units (rows.cu, fp8.cu) share on the host:
+// host_util.h -- what the operator units (rows.cu, norm.cu, fp8.cu, fp4.cu) share on the host:
 // error texts, checks of types, pitches and pointers, the device check.
 #pragma once
 #include <cuda_runtime.h>

@@ -1,5 +1,5 @@
 // pair_drain.h -- how a pair of CTAs whose copies complete on barriers of the
-// first one leaves when a wait gave up (fp8.cuh).  Host code too: the order of
+// first one leaves when a wait gave up (fp8.cuh, fp4.cuh).  Host code too: the order of
 // the steps is checked on the CPU.
 #pragma once
 #include <stdint.h>

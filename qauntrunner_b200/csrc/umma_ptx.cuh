@@ -1,6 +1,6 @@
 // umma_ptx.cuh -- the tcgen05, tensor-memory and TMA instructions that the
-// tensor-core kernels (umma.cuh, fp8.cuh) issue, and the descriptors of their
-// operands.
+// tensor-core kernels (umma.cuh, fp8.cuh, fp4.cuh) issue, and the descriptors of
+// their operands.
 #pragma once
 #include <cuda.h>
 
