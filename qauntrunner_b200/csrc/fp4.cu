@@ -43,7 +43,8 @@ size_t pair_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) 
 
 template <int MODE>
 cudaError_t prepare_kernels() {
-    cudaError_t e = cudaFuncSetAttribute(fp4_split_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    cudaError_t e = cudaFuncSetAttribute(fp4_split_kernel<MODE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp4_split_kernel<MODE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(fp4_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(kFp4MaxGroups));
     return e;
@@ -182,7 +183,7 @@ cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const Fp4Params& 
     if (pair)
         return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, w_map,
                             MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_map, p, wide_out);
-    const int64_t across = MODE == kFp4Plain ? (p.M + 255) / 256 : (p.M + 127) / 128;
+    const int64_t across = p.across;
     const int64_t used = std::min<int64_t>(T, m->groups), per = (T / used + p.tile_rows - 1) / p.tile_rows;
     const int64_t tiles = used * per * across;
     int ranks = 1;
@@ -203,7 +204,7 @@ cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const Fp4Params& 
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, fp4_split_kernel<MODE>, w_map, x_map, p, stages);
+    return cudaLaunchKernelEx(&cfg, p.groups > 1 ? fp4_split_kernel<MODE, true> : fp4_split_kernel<MODE, false>, w_map, x_map, p, stages);
 }
 
 int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x, const uint8_t* xs, int64_t ld_xs,
@@ -270,7 +271,8 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     p.blocks = (int)blocks;
     p.type = type;
     p.tile_rows = tile_rows;
-    p.row_tiles = (int)(offsets ? row_tiles : (T + tile_rows - 1) / tile_rows);
+    p.across = (int)(mode == kFp4Plain ? (M + 255) / 256 : across);
+    p.row_tiles = (int)(m->groups > 1 ? row_tiles : (T + tile_rows - 1) / tile_rows);
     p.wide_xs = aligned(xs, 16) && ld_xs % 16 == 0 ? 2 : aligned(xs, 8) && ld_xs % 8 == 0 ? 1 : 0;
     const cudaStream_t s = (cudaStream_t)stream;
     e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, p, pair, wide_out, T, s)
