@@ -199,70 +199,51 @@ __host__ __device__ inline int fp4_stage_bytes(int x_rows) { return x_rows * 128
 
 struct Fp4Tile {
     int group, pos, n;   // matrix, first row of x, rows (none: no such tile)
-    int block;           // 256 outputs
 };
 
-// Tile number `unit` of a grouped product, by one warp, in all its lanes.  Groups
-// count as in group_tables; the first CTA raises an error for offsets that make no
-// sense.  Only tiles that have rows are counted: their CTAs are the grid's first,
-// and do not wait for those that find nothing to do (16 tokens of a rank with 32
-// of 256 experts, 6 of which have rows: 36 us in place of 42).
-__device__ inline Fp4Tile fp4_find(const Fp4Params& p, uint32_t unit) {
+// The tile of rows number `at`, by one warp, in all its lanes.  Groups count as
+// in group_tables; `report`: look at all of them and raise an error for offsets
+// that make no sense.
+__device__ inline Fp4Tile fp4_find(const Fp4Params& p, int at, bool report) {
     const int lane = threadIdx.x & 31;
-    Fp4Tile r{0, 0, 0, 0};
-    int a = 0, rows = 0, tiles = 0, scan = 0, before = 0, top = 0, at = 0;
-    bool bad = false, counted = false;
-    for (int g0 = 0; g0 < p.groups;) {
-        if (!counted || p.groups > 32) {   // 32 groups, a lane each: first row, rows, tiles, tiles up to it and with it
-            const int g = g0 + lane;
-            int b = 0;
-            a = 0;
-            if (g < p.groups) {
-                a = p.offsets[g];
-                b = p.offsets[g + 1];
-            }
-            int most = a;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) most = max(most, __shfl_up_sync(0xffffffffu, most, o));
-            most = max(most, top);
-            top = __shfl_sync(0xffffffffu, most, 31);
-            if (a < most || a < 0 || b < a || b > p.T) {
-                bad |= g < p.groups;
-                a = b = 0;
-            }
-            rows = b - a;
-            scan = tiles = (rows + p.tile_rows - 1) / p.tile_rows;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, scan, o);
-                if (lane >= o) scan += v;
-            }
+    Fp4Tile r{0, 0, 0};
+    int before = 0, top = 0;
+    bool bad = false, found = false;
+    for (int g0 = 0; g0 < p.groups && (report || !found); g0 += 32) {
+        const int g = g0 + lane;
+        int a = 0, b = 0;
+        if (g < p.groups) {
+            a = p.offsets[g];
+            b = p.offsets[g + 1];
         }
-        if (!counted) {
-            before += __shfl_sync(0xffffffffu, scan, 31);
-            g0 += 32;
-            if (g0 < p.groups) continue;
-            if (blockIdx.x == 0 && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.err, (int)ERR_BOUNDS);
-            if (before == 0) break;
-            r.block = unit / (uint32_t)before;
-            at = unit - (uint32_t)r.block * before;
-            if (r.block >= p.across) break;
-            counted = true;
-            g0 = before = top = 0;
-            if (p.groups > 32) continue;
+        int most = a;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) most = max(most, __shfl_up_sync(0xffffffffu, most, o));
+        most = max(most, top);
+        top = __shfl_sync(0xffffffffu, most, 31);
+        if (a < most || a < 0 || b < a || b > p.T) {
+            bad |= g < p.groups;
+            a = b = 0;
+        }
+        const int tiles = (b - a + p.tile_rows - 1) / p.tile_rows;
+        int scan = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += v;
         }
         const int in = at - (before + scan - tiles);
         const uint32_t here = __ballot_sync(0xffffffffu, in >= 0 && in < tiles);
-        if (here) {
+        if (here && !found) {
             const int from = __ffs(here) - 1;
             r.group = g0 + from;
             r.pos = __shfl_sync(0xffffffffu, a + in * p.tile_rows, from);
-            r.n = __shfl_sync(0xffffffffu, min(rows - in * p.tile_rows, p.tile_rows), from);
-            break;
+            r.n = __shfl_sync(0xffffffffu, min(b - a - in * p.tile_rows, p.tile_rows), from);
+            found = true;
         }
         before += __shfl_sync(0xffffffffu, scan, 31);
-        g0 += 32;
     }
+    if (report && __any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.err, (int)ERR_BOUNDS);
     return r;
 }
 
@@ -326,16 +307,18 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     uint32_t rank, ranks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
-    const uint32_t unit = blockIdx.x / ranks;
+    // The outputs of a tile of rows are neighbours in the grid, so the CTAs of tiles that have rows come first and do not
+    // wait for those that find none (16 tokens of a rank with 32 of 256 experts, 6 of which have rows: 36 us in place of 42)
+    const int tile = blockIdx.x / ranks, row_tile = tile / p.across, block = tile % p.across;
     constexpr int kBlock = MODE == kFp4Plain ? 128 : 64;   // outputs of a block
+    const int m0 = block * 2 * kBlock;
     const int k0 = (int)((long long)p.steps * rank / ranks), k1 = (int)((long long)p.steps * (rank + 1) / ranks);
     // one matrix: the tile's outputs are known, and its first stages are asked for before the kernel before has ended, which
     // does not write them
-    Fp4Tile t{0, 0, 0, GROUPED ? 0 : (int)unit / p.row_tiles};
+    Fp4Tile t{0, 0, 0};
     const int early = GROUPED ? 0 : min(stages, k1 - k0);
     // a stage's copies of the weights, by one thread
     auto load_stage = [&](uint32_t slot, int k) {
-        const int m0 = t.block * 2 * kBlock;
         uint8_t* st = ring + slot * stage_bytes;
         mbar_arrive_expect_tx(&full[slot], (uint32_t)(2 * kFp4Tile + 2 * kFp4Scales));
 #pragma unroll
@@ -362,7 +345,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     if (warp == 1) tmem_alloc(smem_u32(tmem_slot), kFp4TmemCols);
     pdl_start();   // nothing before this reads or writes global memory, but for the weights
     if (GROUPED && warp == 2) {
-        const Fp4Tile mine = fp4_find(p, unit);
+        const Fp4Tile mine = fp4_find(p, row_tile, blockIdx.x == 0);
         if (lane == 0) *found = mine;
     }
     if (!GROUPED) {   // its rows (see fp4_find)
@@ -375,7 +358,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
                 if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(p.err, (int)ERR_BOUNDS);
             }
         }
-        const int in = ((int)unit - t.block * p.row_tiles) * p.tile_rows;
+        const int in = row_tile * p.tile_rows;
         t.pos = a + in;
         t.n = max(0, min(b - a - in, p.tile_rows));
     }
@@ -395,7 +378,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     }
     const WaitCtl ctl{abort_flag, p.err};
     const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), done0 = smem_u32(done);
-    const int boxes = (t.n + 15) >> 4, m0 = t.block * 2 * kBlock;
+    const int boxes = (t.n + 15) >> 4;
 
     if (warp == 0) {
         // ------------------------------------------------ codes and the weights' scales
