@@ -156,24 +156,24 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
 // Which kernel a product takes, by an estimate of what both would cost with all
 // T rows held and spread evenly over the groups.  Measured (us; weights / rows of
 // x on the MMA's M side), outputs x contracted:
-//   1 x 4096 x 7168:   1 row 7.6 / 13.8, 16 rows 9.1 / 13.4, 64 rows 12.9 / 13.8, 128 rows 16.3 / 14.4
-//   1 x 28672 x 4096:  1 row 13.6 / 23.0, 32 rows 19.1 / 20.3, 64 rows 21.8 / 20.4
-//   1 x 1024 x 2816:   1 row 5.8 / 8.0, 32 rows 7.7 / 8.4, 64 rows 9.6 / 8.8
-//   1 x 7168 x 2048:   16 rows 7.0 / 7.8, 32 rows 8.2 / 8.0, 64 rows 10.6 / 8.3
-//   8 x 5632 x 1024:   8 rows each 8.3 / 11.2, 16 rows each 9.8 / 11.3, 32 rows each 12.6 / 11.3
-//   32 x 4096 x 7168:  2 rows each 69 / 78, 16 rows each 86 / 90, 32 rows each 92 / 91, 64 rows each 113 / 94
-//   32 x 7168 x 2048:  4 rows each 48 / 48, 16 rows each 56 / 50, 64 rows each 85 / 53
+//   1 x 4096 x 7168:   1 row 7.4 / 13.8, 16 rows 8.4 / 13.5, 64 rows 12.7 / 13.9, 128 rows 14.4 / 14.5, 256 rows 14.8 / 14.5
+//   1 x 28672 x 4096:  1 row 13.6 / 22.9, 32 rows 17.2 / 20.4, 64 rows 20.6 / 20.4, 128 rows 27.8 / 21.7
+//   1 x 1024 x 2816:   1 row 5.7 / 8.1, 32 rows 7.9 / 8.4, 64 rows 10.2 / 8.8
+//   1 x 7168 x 2048:   16 rows 7.1 / 7.8, 32 rows 8.3 / 8.1, 64 rows 10.7 / 8.4
+//   8 x 5632 x 1024:   8 rows each 8.4 / 11.1, 16 rows each 9.9 / 11.4, 32 rows each 12.2 / 11.4
+//   32 x 4096 x 7168:  2 rows each 71 / 81, 16 rows each 87 / 94, 32 rows each 93 / 96, 64 rows each 112 / 98
+//   32 x 7168 x 2048:  4 rows each 49 / 49, 16 rows each 58 / 51, 64 rows each 82 / 55
 // The first takes what reading the weights takes, and something for each row of a
 // tile and all tiles' rows; the second a time for each stage of whole tiles of 256
 // rows x 256 outputs, in waves over the pairs of SMs, longer where most pairs are
-// at work.  The worst choices among 67 measured sizes take 1.15 times as long as
+// at work.  The worst choice among 70 measured sizes takes 1.08 times as long as
 // the other kernel.
 bool pair_is_faster(int64_t T, int64_t used, int64_t tiles_across, int steps, int tile_rows, int sms) {
     const double rows = (double)T / used, row_tiles = std::ceil(rows / tile_rows), tiles = used * tiles_across * row_tiles;
     const double read = (double)used * tiles_across * steps * 34816 / 6.4e6;   // us, of a stage's 256 x 256 codes and scales
-    const double one = 5 + read * (1 + (row_tiles - 1) / 2) + std::min<double>(rows, tile_rows) * (0.06 + 0.0006 * tiles);
+    const double one = 4 + read * (1 + (row_tiles - 1) / 2) + std::min<double>(rows, tile_rows) * (0.07 + 0.0004 * tiles);
     const double pairs = sms / 2, wide = used * tiles_across * std::ceil(rows / 256);
-    const double two = 5 + std::ceil(wide / pairs) * steps * (wide <= pairs / 2 ? 0.30 : 0.45);
+    const double two = 5 + std::ceil(wide / pairs) * steps * (wide <= pairs / 2 ? 0.28 : 0.43);
     return two < one;
 }
 

@@ -180,11 +180,12 @@ __device__ __forceinline__ float2 gated2(float2 gate, float2 up, float limit) {
 //
 // Two CTAs fit on an SM, so one's start and end, or the next launch's start, go on
 // behind the other's loads; where there is one matrix, its first stages are asked
-// for before the launch before has ended.  Together that took one row through
-// 4096 x 7168 (15.6 MB) from 12.2 to 7.1 us, the rest of which is latencies: the
-// first loads, the MMAs, two cluster barriers and reads of other SMs between them.
-// 256 rows over 32 x 4096 x 7168 (499 MB): 80 us, 6.3 TB/s; 16 rows, which 12.7 of
-// the 32 have on average: 36 us (floor 30).
+// for before the launch before has ended.  Together with a search for the tile that
+// one matrix does not need, that took one row through 4096 x 7168 (15.6 MB) from
+// 12.2 to 7.4 us, the rest of which is latencies: the first loads, the MMAs, two
+// cluster barriers and reads of other SMs between them.  256 rows over 32 x 4096 x
+// 7168 (499 MB): 81 us, 6.2 TB/s; 16 rows, which 12.7 of the 32 have on average: 37
+// us (floor 30).
 //
 // Warps: 0 loads codes and the weights' scales, 1 issues the MMAs, 2 finds the
 // tile and brings the scales of x; all eight write the output.
@@ -308,7 +309,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
     // The outputs of a tile of rows are neighbours in the grid, so the CTAs of tiles that have rows come first and do not
-    // wait for those that find none (16 tokens of a rank with 32 of 256 experts, 6 of which have rows: 36 us in place of 42)
+    // wait for those that find none (16 tokens of a rank with 32 of 256 experts, 6 of which have rows: 37 us in place of 42)
     const int tile = blockIdx.x / ranks, row_tile = tile / p.across, block = tile % p.across;
     constexpr int kBlock = MODE == kFp4Plain ? 128 : 64;   // outputs of a block
     const int m0 = block * 2 * kBlock;
@@ -531,15 +532,15 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // features): each CTA loads 128 rows of x and 128 of the weights, 32 KB of codes
 // for 256 contracted values, and the MMA reads both halves of the weights.
 //
-// 4096 rows, 28672 x 4096: 174 us, 5.5 PFLOP/s, and 207 under sustained load: the
-// power cap bounds it (the same launch on an idle GPU takes 415 cycles a stage,
-// as many as its four MMAs).  What took it there from 310 us: the scales of x
-// handed over without a cluster-scope release (a full memory barrier with every
-// stage) and asked for four stages at a time, rows out by way of shared memory,
-// descriptors with constant high words.  8192 rows over 32 x 4096 x 7168: 141 us,
-// of which a third goes to rows that a group's last tile does not have.  The
-// places of the operands changed (rows of x as the MMA's N, rounded up to 32 only,
-// 384 a tile) it took 137 us there, and more everywhere else.
+// 4096 rows, 28672 x 4096: 176 us, 5.5 PFLOP/s, and 207 under sustained load: the
+// power cap bounds it (a launch by itself takes 415 cycles a stage).  What took it
+// there from 310 us: the scales of x handed over without a cluster-scope release
+// (a full memory barrier with every stage) and asked for four stages at a time,
+// rows out by way of shared memory, descriptors with constant high words.  8192
+// rows over 32 x 4096 x 7168: 144 us, of which a third goes to rows that a group's
+// last tile does not have.  The places of the operands changed (rows of x as the
+// MMA's N, rounded up to 32 only, 384 a tile) it took 137 us there where this one
+// took 141, but 217 in place of 176 and 91 in place of 81 with 7168 x 2048.
 //
 // Tensor memory holds two accumulators of 256 columns but for the scales' 48
 // columns: the second begins 48 before the first ends, and a tile's MMAs wait
