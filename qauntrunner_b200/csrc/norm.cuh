@@ -375,6 +375,11 @@ __device__ __forceinline__ float norm_factor(float total, float per_d, float eps
 // may be x or add, y any of them: a thread has read a column before it writes it,
 // and a row is copied ahead of others only.  WHOLE: all rows start and end on 16
 // bytes (the code for others costs these a tenth of their time).
+//
+// 4096 x 7168 bf16 with the residual, the sum written, into 8 bits (206 MB): 39 us,
+// 5.3 TB/s (a copy of as many bytes 35), 62 with loads of its own in place of the
+// ring, one f32 at a time and 8 columns a thread.  One row of 7168 f32 columns 4.3.
+// 4000 x 7001, whose rows start anywhere: 59, and 251 with loads of single values.
 template <typename T, int OUT, int V, bool WHOLE>
 __global__ void __launch_bounds__(kNormThreads)
 rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
@@ -471,7 +476,13 @@ struct NormGradArgs {
 };
 
 // A thread keeps its 8 V columns' weights and their sums over the rows in
-// registers.
+// registers, so the rows' products for dw are added up without atomics and in a
+// fixed order: first a CTA's rows, then the CTAs' parts (rms_norm_dw_kernel).
+//
+// 4096 x 7168 bf16 with the residual's gradient and dw (235 MB): 48 us, 4.9 TB/s (a
+// copy of as many bytes 40), 4 of them for dw.  4000 x 7001: 75, of single values
+// 265.  1021 x 2816 f32: 11.  Two rows between two barriers and two CTAs an SM were
+// no faster.
 template <typename T, int V, bool WHOLE>
 __global__ void __launch_bounds__(kNormThreads)
 rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {

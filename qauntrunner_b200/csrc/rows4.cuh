@@ -76,7 +76,11 @@ __device__ __forceinline__ Fp4Half quantize4_16(const T* __restrict__ x, int n, 
 }
 
 // rows[pos[a]] = x[t] in 4 bits: a token's row is quantised once for all its
-// slots, as gather_rows_fp8_kernel does in 8 bits
+// slots, as gather_rows_fp8_kernel does in 8 bits.  Memory bounds both kernels:
+// 1024 rows of 7168 bf16 columns to 8 places each (46 MB) 9.3 us, 4.9 TB/s; below,
+// 4096 x 4096 bf16 (42 MB) 8.8 us, 4.8 TB/s, cold.  A thread takes half a block, so
+// that its loads and stores are 16 and 8 bytes and a block's largest magnitude
+// needs one exchange.
 template <typename T>
 __global__ void __launch_bounds__(256)
 gather_rows_fp4_kernel(const T* __restrict__ x, long long ld_x, const int32_t* __restrict__ pos, int k, int d,

@@ -323,6 +323,51 @@ def test_one_group_of_some_rows(offsets, bad, form):
     m.close()
 
 
+@pytest.mark.parametrize("offsets", [[5, 140], [0, 150], [149, 150], [70, 70], [0, 64], [16, 81]])
+def test_one_group_of_many_rows(offsets, form):
+    """Several tiles of rows and of outputs, some of them empty; the product and the gated one."""
+    c = Case(150, 1, 700, 1300)
+    assert float(c.size.max()) < 2 ** 18
+    m = c.matrix()
+    off = torch.tensor(offsets, dtype=torch.int32).cuda()
+    y = torch.full((150, 700), 5.0).cuda()
+    m.product(0, c.x[0].cuda(), c.x[1].cuda(), 150, y, offsets=off)
+    h, every = torch.full((150, 350), 5.0).cuda(), torch.empty(150, 350).cuda()
+    m.swiglu(0, c.x[0].cuda(), c.x[1].cuda(), 150, h, offsets=off)
+    m.swiglu(0, c.x[0].cuda(), c.x[1].cuda(), 150, every)
+    m.sync()
+    inside = torch.zeros(150, dtype=torch.bool)
+    inside[offsets[0]:offsets[1]] = True
+    check(y, c.want.float(), inside, 0, 5.0)
+    h, every = h.cpu(), every.cpu()
+    want = P.gate(c.want, 0.0)
+    slack = 16 * U * want.abs() + 4 * 2.0 ** -149 * (c.want[:, :350] * c.want[:, 350:]).abs()
+    slack = slack + F.ROUND[0] * (want.abs() + slack) + F.HALF_STEP[0]   # (as in test_gated)
+    assert bool(((every.double() - want).abs() <= slack).all())
+    assert torch.equal(h[inside], every[inside]) and bool((h[~inside] == 5).all())
+    m.close()
+
+
+@pytest.mark.parametrize("first,second", [(0, 1), (3, 37), (31, 32), (38, 39)])
+@pytest.mark.parametrize("type", TYPES)
+def test_two_groups_of_forty(first, second, type, form):
+    """Room for 120 rows, 50 of them held, the rest and the other groups without any."""
+    c = Case(120, 40, 300, 520)
+    w, x = P.values(*c.w, 520).reshape(40, 300, 520), P.values(*c.x, 520)
+    offsets = torch.zeros(41, dtype=torch.int32)
+    offsets[first + 1:] = 33
+    offsets[second + 1:] = 50
+    want = torch.full((120, 300), 5.0, dtype=torch.float64)
+    want[:33], want[33:50] = x[:33] @ w[first].T, x[33:50] @ w[second].T
+    assert float((x[:50].abs() @ w[[first, second]].abs().reshape(600, 520).T).max()) < 2 ** 18
+    m = c.matrix()
+    y = torch.full((120, 300), 5.0, dtype=F.DTYPE[type]).cuda()
+    m.product(type, c.x[0].cuda(), c.x[1].cuda(), 120, y, offsets=offsets.cuda())
+    m.sync()
+    assert torch.equal(y.cpu(), want.float().to(F.DTYPE[type]))   # (sums are exact in f32: see test_product_is_exact)
+    m.close()
+
+
 def test_many_groups():
     """1024 matrices, most without rows."""
     c = Case(40, 1024, 32, 64)
