@@ -40,20 +40,26 @@ void release(qrm_fp4* m) {
 }
 
 size_t pair_smem(int groups) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)kFp4PairStages * kFp4PairStage + 8 * kFp4PairOut; }
+size_t tail_smem(int groups, int stages) { return 1024 + (size_t)fp4_pair_stage_off(groups) + (size_t)stages * kFp4TailStage + kFp4TailRoom; }
+constexpr int kSmemStatic = 512;   // more than the kernels' own
+int tail_stages(int groups) { return tail_smem(groups, kFp4TailStages) <= kSmemMost - kSmemStatic ? kFp4TailStages : kFp4TailStages - 1; }
 
 template <int MODE>
 cudaError_t prepare_kernels() {
     cudaError_t e = cudaFuncSetAttribute(fp4_split_kernel<MODE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(fp4_split_kernel<MODE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(fp4_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(kFp4MaxGroups));
+        e = cudaFuncSetAttribute(fp4_pair_kernel<MODE, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pair_smem(kFp4MaxGroups));
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(fp4_pair_kernel<MODE, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost - kSmemStatic);
     return e;
 }
 // registers a thread that the pair kernels were built with: their split may not pass what a launch has
 template <int MODE>
 bool enough_regs() {
-    cudaFuncAttributes pair{};
-    return cudaFuncGetAttributes(&pair, fp4_pair_kernel<MODE>) == cudaSuccess && pair.numRegs * kFp4PairThreads >= kFp4PairRegs;
+    cudaFuncAttributes pair{}, tails{};
+    return cudaFuncGetAttributes(&pair, fp4_pair_kernel<MODE, false>) == cudaSuccess && pair.numRegs * kFp4PairThreads >= kFp4PairRegs &&
+           cudaFuncGetAttributes(&tails, fp4_pair_kernel<MODE, true>) == cudaSuccess && tails.numRegs * kFp4PairThreads >= kFp4PairRegs;
 }
 
 int create(int device, int groups, int64_t rows, int64_t cols, const void* codes, size_t code_bytes, const void* scales,
@@ -178,11 +184,18 @@ bool pair_is_faster(int64_t T, int64_t used, int64_t tiles_across, int steps, in
 }
 
 template <int MODE>
-cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const Fp4Params& p, bool pair, int wide_out, int64_t T, cudaStream_t s) {
+cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const CUtensorMap& few_map, const Fp4Params& p, bool pair, int wide_out, int64_t T, cudaStream_t s) {
     const CUtensorMap& w_map = MODE == kFp4Plain ? m->map : m->gated_map;
-    if (pair)
-        return launch_ahead(fp4_pair_kernel<MODE>, dim3(m->sms / 2 * 2), kFp4PairThreads, pair_smem(m->groups), s, w_map,
-                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_map, p, wide_out);
+    if (pair) {
+        // Tails (a third more shared memory a stage, smaller pieces on the way out) where groups are likely to have one and a
+        // tile has stages enough.  With and without, us: 32 x 4096 x 7168, 8192 rows 124 / 147, 4096 rows 106 / 104, 12000 rows
+        // 187 / 185; 32 x 7168 x 2048, 8192 rows 76 / 84; 8 x 5632 x 1024, 2048 rows 17.0 / 16.2, 512 rows 13.7 / 11.7.
+        const bool tails = m->groups > 1 && T > (int64_t)128 * m->groups && p.steps >= 8;
+        const int stages = tails ? tail_stages(m->groups) : kFp4PairStages;
+        return launch_ahead(tails ? fp4_pair_kernel<MODE, true> : fp4_pair_kernel<MODE, false>, dim3(m->sms / 2 * 2), kFp4PairThreads,
+                            tails ? tail_smem(m->groups, stages) : pair_smem(m->groups), s, w_map,
+                            MODE == kFp4Plain ? m->scales_map : m->gated_scales_map, x_map, few_map, p, wide_out, stages);
+    }
     const int64_t across = p.across;
     const int64_t used = std::min<int64_t>(T, m->groups), per = (T / used + p.tile_rows - 1) / p.tile_rows;
     const int64_t tiles = used * per * across;
@@ -204,7 +217,7 @@ cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const Fp4Params& 
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, p.groups > 1 ? fp4_split_kernel<MODE, true> : fp4_split_kernel<MODE, false>, w_map, x_map, p, stages);
+    return cudaLaunchKernelEx(&cfg, p.groups > 1 ? fp4_split_kernel<MODE, true> : fp4_split_kernel<MODE, false>, w_map, few_map, p, stages);
 }
 
 int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x, const uint8_t* xs, int64_t ld_xs,
@@ -247,11 +260,11 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     if (e != cudaSuccess) return failf(QRM_E_CUDA, "%s: %s", what, cudaGetErrorString(e));
     const bool pair = m->form >= 0 ? m->form : pair_is_faster(T, used, mode == kFp4Plain ? (M + 255) / 256 : across, m->steps, tile_rows, m->sms);
     const int wide_out = aligned(out, 16) && ld_out * b % 16 == 0;
-    CUtensorMap x_map;
+    CUtensorMap x_map, few_map;   // in boxes of 128 rows; of half a tail's, or (weights on the M side) of 16
     const cuuint64_t dims[2] = {(cuuint64_t)(16 * blocks), (cuuint64_t)T};
     const cuuint64_t strides[1] = {(cuuint64_t)ld_x};
-    const cuuint32_t box[2] = {128, pair ? 128u : 16u};
-    if (!encode(&x_map, x, 2, dims, strides, box)) return failf(QRM_E_CUDA, "%s: tensor map", what);
+    const cuuint32_t box[2] = {128, 128}, few[2] = {128, pair ? kFp4TailRows / 2u : 16u};
+    if ((pair && !encode(&x_map, x, 2, dims, strides, box)) || !encode(&few_map, x, 2, dims, strides, few)) return failf(QRM_E_CUDA, "%s: tensor map", what);
     Fp4Params p{};
     p.w_scales = mode == kFp4Plain ? m->scales : m->gated_scales;
     p.x_scales = xs;
@@ -275,9 +288,9 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     p.row_tiles = (int)(m->groups > 1 ? row_tiles : (T + tile_rows - 1) / tile_rows);
     p.wide_xs = aligned(xs, 16) && ld_xs % 16 == 0 ? 2 : aligned(xs, 8) && ld_xs % 8 == 0 ? 1 : 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, p, pair, wide_out, T, s)
-        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_map, p, pair, wide_out, T, s)
-                            : launch<kFp4GatedRows>(m, x_map, p, pair, wide_out, T, s);
+    e = mode == kFp4Plain   ? launch<kFp4Plain>(m, x_map, few_map, p, pair, wide_out, T, s)
+        : mode == kFp4Gated ? launch<kFp4Gated>(m, x_map, few_map, p, pair, wide_out, T, s)
+                            : launch<kFp4GatedRows>(m, x_map, few_map, p, pair, wide_out, T, s);
     return e == cudaSuccess ? QRM_OK : failf(QRM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
 }
 

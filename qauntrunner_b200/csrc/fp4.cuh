@@ -536,11 +536,16 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // power cap bounds it (a launch by itself takes 415 cycles a stage).  What took it
 // there from 310 us: the scales of x handed over without a cluster-scope release
 // (a full memory barrier with every stage) and asked for four stages at a time,
-// rows out by way of shared memory, descriptors with constant high words.  8192
-// rows over 32 x 4096 x 7168: 144 us, of which a third goes to rows that a group's
-// last tile does not have.  The places of the operands changed (rows of x as the
-// MMA's N, rounded up to 32 only, 384 a tile) it took 137 us there where this one
-// took 141, but 217 in place of 176 and 91 in place of 81 with 7168 x 2048.
+// rows out by way of shared memory, descriptors with constant high words.
+//
+// Groups of uneven numbers of rows leave most of their last tile empty.  So up to
+// 64 rows behind a group's last whole tile, its tail, go with that tile: each stage
+// brings half of them to each CTA, and a second MMA takes them against the weights
+// that are there already, with the operands' places changed (weights on the M
+// side, the tail's rows, rounded up to 32, on the N side).  8192 rows over 32 x 4096
+// x 7168: 147 -> 124 us (floor 91).  Tiles of their own in that form gained
+// nothing (their weights come from L2 once more), nor did a kernel with all rows on
+// the N side, 384 a tile (137 us there, but 217 in place of 176 for one matrix).
 //
 // Tensor memory holds two accumulators of 256 columns but for the scales' 48
 // columns: the second begins 48 before the first ends, and a tile's MMAs wait
@@ -555,38 +560,72 @@ constexpr int kFp4PairStages = 5;
 constexpr int kFp4PairTx = 2 * kFp4Tile + 2 * kFp4Scales;            // bytes of a CTA's copies of a stage
 constexpr int kFp4PairStage = kFp4PairTx + kFp4Scales;               // and the scales of x
 constexpr int kFp4PairSecond = 208, kFp4PairTmemScales = 464;
+// With tails: half of the tail's rows, this CTA's weights' scales once more, the
+// tail's scales; tensor memory for a second accumulator, and 16 columns of scales a stage
+constexpr int kFp4TailRows = 64;
+constexpr int kFp4TailTx = kFp4TailRows / 2 * 128 + kFp4Scales;
+constexpr int kFp4TailStages = 5;             // where they fit (up to 84 matrices), 4 of them else
+constexpr int kFp4TailStage = kFp4PairStage + kFp4TailTx + kFp4Scales;
+constexpr int kFp4TailSecond = 176, kFp4TailTmemScales = 432, kFp4TailScaleCols = 40;
+// rows of x that a group's tiles are, by its rows: a rest of few rows goes with the last whole tile
+__host__ __device__ inline int fp4_tail(int rows) { return rows > 256 && (rows & 255) <= kFp4TailRows ? rows & 255 : 0; }
 constexpr int kFp4PairOut = 32 * 144;          // a warp's room for rows on their way out: 32 of 128 bytes, 16 apart
+constexpr int kFp4TailOut = 32 * 64;           // with tails: 32 of 64 bytes; gated into 4 bits, of two warps: 32 of 36 floats
+constexpr int kFp4TailBlocks = 32 * 144;
 constexpr int kFp4PairTableOff = 1024;
 constexpr int kFp4PairRegsFew = 72, kFp4PairRegsMany = 216;
 constexpr int kFp4PairRegs = 128 * kFp4PairRegsFew + 256 * kFp4PairRegsMany;
 static_assert(kFp4PairRegs <= kFp4PairThreads * 168, "register split");
+constexpr int kFp4TailRoom = 4 * kFp4TailBlocks;   // at least 8 kFp4TailOut
+static_assert(kFp4TailRoom >= 8 * kFp4TailOut, "room");
 __host__ __device__ inline int fp4_pair_stage_off(int groups) { return (kFp4PairTableOff + 12 * (groups + 1) + 1023) / 1024 * 1024; }
 
-// the first CTA's barriers, as drain_pair moves them on
+// the first CTA's barriers, as drain_pair moves them on; the tiles' stages have different numbers of bytes
 struct Fp4PairBars {
     uint64_t* full;
-    __device__ void expect(uint32_t slot) { mbar_arrive_expect_tx(&full[slot], kFp4PairTx); }
+    volatile uint32_t* bytes;   // a CTA's share of the stage that it issued last in each slot
+    __device__ uint32_t peer_bytes(uint32_t slot) const {
+        uint32_t a, v;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, 1;" : "=r"(a) : "r"(smem_u32(const_cast<uint32_t*>(&bytes[slot]))));
+        asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+        return v;
+    }
+    __device__ void expect(uint32_t slot) { mbar_arrive_expect_tx(&full[slot], peer_bytes(slot)); }
     __device__ void complete(uint32_t slot) {
-        asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[slot])),
-                     "r"((uint32_t)kFp4PairTx)
+        asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[slot])), "r"(bytes[slot])
                      : "memory");
     }
     __device__ void wait(uint32_t slot, uint32_t parity) { mbar_wait(&full[slot], parity); }
 };
+// whether it holds for all of `threads`, which meet here
+__device__ __forceinline__ bool all_of(int barrier, int threads, bool holds) {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(r)
+                 : "r"((uint32_t)holds), "r"(barrier), "r"(threads)
+                 : "memory");
+    return r != 0;
+}
+
 // A warp's 32 rows of 2 N outputs each (a lane holds a row) to out, by way of
-// shared memory, so that a store's lanes write neighbouring outputs, of four
-// rows at once.  left: how many of a row's exist; rows: how many rows do.
-template <typename T, int N>
+// shared memory, so that a store's lanes write neighbouring outputs, PIECE bytes of
+// each of several rows at once.  left: how many of a row's exist; rows: how many rows
+// do.  The room has 32 rows of a piece, 16 bytes apart or (of 64) their four parts in
+// another order for every two rows: eight lanes' parts are in eight places.
+template <int PIECE>
+__device__ __forceinline__ int part_at(int row, int part) {
+    return PIECE == 128 ? 144 * row + 16 * part : 64 * row + 16 * (part ^ ((row >> 1) & 3));
+}
+template <int PIECE, typename T, int N>
 __device__ __forceinline__ void store_rows(T* out, long long ld, int left, int rows, const float2 (&v)[N], uint8_t* room, bool wide) {
-    constexpr int C = 128 / sizeof(T);   // outputs of a row in one go
+    constexpr int C = PIECE / sizeof(T), P = PIECE / 16;   // outputs of a row in one go, parts of 16 bytes
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int c = 0; c < 2 * N; c += C) {
         if (c >= left) break;
         __syncwarp();
-        uint4* to = reinterpret_cast<uint4*>(room + 144 * lane);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {   // 16 bytes each
+        for (int i = 0; i < P; i++) {
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -599,20 +638,23 @@ __device__ __forceinline__ void store_rows(T* out, long long ld, int left, int r
                     memcpy(&w[k], h, 4);
                 }
             }
-            to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(room + part_at<PIECE>(lane, i)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
         __syncwarp();
         if (wide && c + C <= left) {
-            const int r0 = lane >> 3, at = 16 * (lane & 7);
-            uint8_t* o = reinterpret_cast<uint8_t*>(out + r0 * ld + c) + at;
+            const int r0 = lane / P, part = lane % P;
+            uint8_t* o = reinterpret_cast<uint8_t*>(out + r0 * ld + c) + 16 * part;
 #pragma unroll
-            for (int r = 0; r < 32; r += 4)
-                if (r + r0 < rows) *reinterpret_cast<uint4*>(o + r * ld * (long long)sizeof(T)) = *reinterpret_cast<const uint4*>(room + 144 * (r + r0) + at);
+            for (int r = 0; r < 32; r += 32 / P)
+                if (r + r0 < rows)
+                    *reinterpret_cast<uint4*>(o + r * ld * (long long)sizeof(T)) = *reinterpret_cast<const uint4*>(room + part_at<PIECE>(r + r0, part));
         } else {   // one output a lane
             for (int r = 0; r < min(rows, 32); r++)
 #pragma unroll
-                for (int k = 0; k < C; k += 32)
-                    if (c + k + lane < left) out[r * ld + c + k + lane] = reinterpret_cast<const T*>(room + 144 * r)[k + lane];
+                for (int k = 0; k < C; k += 32) {
+                    const int o = k + lane;
+                    if (o < C && c + o < left) out[r * ld + c + o] = *reinterpret_cast<const T*>(room + part_at<PIECE>(r, o * (int)sizeof(T) / 16) + o * (int)sizeof(T) % 16);
+                }
         }
     }
 }
@@ -637,21 +679,100 @@ __device__ __forceinline__ void store_row4(uint8_t* codes, uint8_t* scales, int 
     }
 }
 
+// Output m of rows first, first + step, ..., of which `have` count from row t on,
+// by a lane; a warp's lanes write neighbouring outputs
+template <typename T, int N>
+__device__ __forceinline__ void store_outputs(const Fp4Params& p, long long t, int first, int step, int have, int m, const float (&v)[N]) {
+    if (m >= p.M) return;
+    T* out = reinterpret_cast<T*>(p.out) + (t + first) * p.ld_out + m;
+    const long long ahead = step * p.ld_out;
+#pragma unroll
+    for (int c = 0; c < N; c++) {
+        if (first + c * step < have) *out = round_to<T>(v[c]);
+        out += ahead;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_outputs(const Fp4Params& p, long long t, int first, int step, int have, int m, const float (&v)[N]) {
+    if (p.type == 0) store_outputs<float>(p, t, first, step, have, m, v);
+    else if (p.type == 1) store_outputs<__half>(p, t, first, step, have, m, v);
+    else store_outputs<__nv_bfloat16>(p, t, first, step, have, m, v);
+}
+// 32 rows of a tail from row t on, of which `have` exist: the lane's output
+// of each, number `id` of the CTA's 128 (gated: a row of the MMA's A, gate's and up's in
+// turns of 16), which begin at m.  room: gated into 4 bits, of two warps, whose 32
+// features are a block.
 template <int MODE>
+__device__ __forceinline__ void tail_rows(const Fp4Params& p, long long t, int have, int m, int id, const float (&v)[32], float* room,
+                                            int barrier) {
+    if constexpr (MODE == kFp4Plain) {
+        store_outputs(p, t, 0, 1, have, m + id, v);
+    } else {
+        const int lane = threadIdx.x & 31;
+        // gate's lanes get both sums of the even rows, up's of the odd ones
+        const bool up = lane & 16;
+        float y[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+            const float g0 = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 16);
+            const float g1 = __shfl_xor_sync(0xffffffffu, up ? v[c + 2] : v[c + 3], 16);
+            const float2 own = up ? make_float2(v[c + 1], v[c + 3]) : make_float2(v[c], v[c + 2]), other = make_float2(g0, g1);
+            const float2 f = gated2(up ? other : own, up ? own : other, p.limit);
+            y[c / 2] = f.x;
+            y[c / 2 + 1] = f.y;
+        }
+        const int feature = (id >> 5) * 16 + (lane & 15);   // of the CTA's 64
+        if constexpr (MODE == kFp4Gated) {
+            store_outputs(p, t, up, 2, have, m + feature, y);
+        } else {
+            constexpr int kPitch = 36;   // floats of a row in the room
+            named_barrier(barrier, 64);  // what was in the room is out
+#pragma unroll
+            for (int c = 0; c < 16; c++) room[(2 * c + (up ? 1 : 0)) * kPitch + (feature & 31)] = y[c];
+            named_barrier(barrier, 64);  // 32 rows of 32 features are there: a thread takes half of one
+            const int r = (id & 63) >> 1, o = 16 * (id & 1), first = m + (feature & 32), left = p.M - first;
+            float e[16];
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                e[k] = o + k < left ? room[r * kPitch + o + k] : 0.f;
+                top = max(top, magnitude(e[k]));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            const uint32_t scale = fp4_scale(top);
+            if (r < have && left > 0) {
+                const float lo[8] = {e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]}, hi[8] = {e[8], e[9], e[10], e[11], e[12], e[13], e[14], e[15]};
+                *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.out) + (t + r) * p.ld_out + (first + o) / 2) =
+                    make_uint2(e2m1x8(lo, scale), e2m1x8(hi, scale));
+                if (o == 0) p.out_scales[(t + r) * p.ld_os + first / kFp4Block] = (uint8_t)scale;
+            }
+        }
+    }
+}
+
+// TAILS: tiles may have a tail
+template <int MODE, bool TAILS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFp4PairThreads, 1)
 fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap s_map,
-                const __grid_constant__ CUtensorMap x_map, const __grid_constant__ Fp4Params p, int wide_out) {
+                const __grid_constant__ CUtensorMap x_map, const __grid_constant__ CUtensorMap tail_map,
+                const __grid_constant__ Fp4Params p, int wide_out, int stages) {
+    constexpr int kMost = TAILS ? kFp4TailStages : kFp4PairStages, kStage = TAILS ? kFp4TailStage : kFp4PairStage;
+    const int n_stages = TAILS ? stages : kFp4PairStages;
+    constexpr int kSecond = TAILS ? kFp4TailSecond : kFp4PairSecond, kTmemScales = TAILS ? kFp4TailTmemScales : kFp4PairTmemScales;
+    constexpr int kCols = TAILS ? kFp4TailScaleCols : kFp4ScaleCols;   // of scales in tensor memory, a stage's
+    constexpr int kTailX = kFp4PairStage, kTailW = kTailX + kFp4TailRows / 2 * 128, kTailS = kTailW + kFp4Scales;   // in a stage
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // first CTA: both CTAs' copies are there
-    uint64_t* x_full = full + kFp4PairStages;           // first CTA: both CTAs' scales of x are there
-    uint64_t* done = x_full + kFp4PairStages;           // both: the stage's MMAs are done
-    uint64_t* tile_done = done + kFp4PairStages;        // [2] both: a tile's are
+    uint64_t* x_full = full + kMost;           // first CTA: both CTAs' scales of x are there
+    uint64_t* done = x_full + kMost;           // both: the stage's MMAs are done
+    uint64_t* tile_done = done + kMost;        // [2] both: a tile's are
     uint64_t* tile_read = tile_done + 2;                // first CTA: both epilogues have read an accumulator
     uint64_t* done_bar = tile_read + 1;
     uint64_t* left_bar = done_bar + 1;                  // both, when the first CTA gave up: its commits are through
     __shared__ volatile int given_up;
     __shared__ volatile uint32_t from_peer, issued;     // issued: stages, once their warp is through
+    __shared__ volatile uint32_t bytes[kMost];
     volatile int* abort_flag = &given_up;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + 776);
     int32_t* first_tile = reinterpret_cast<int32_t*>(sm + kFp4PairTableOff);
@@ -663,7 +784,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     const uint32_t rank = blockIdx.x & 1;   // in the pair: the cluster is two CTAs along x
     constexpr int kOut = MODE == kFp4Plain ? 256 : 128;   // outputs of a tile
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kFp4PairStages; i++) {
+        for (int i = 0; i < n_stages; i++) {
             mbar_init(&full[i], 1);
             mbar_init(&x_full[i], 4);
             mbar_init(&done[i], 1);
@@ -682,7 +803,9 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     pdl_start();   // nothing before this reads or writes global memory
-    if (warp == 2) group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows, 256, (p.M + kOut - 1) / kOut, blockIdx.x == 0);
+    if (warp == 2)
+        group_tables(p.offsets, p.groups, p.T, p.err, first_tile, start, rows,
+                     [&](int n) { return ((n - (TAILS ? fp4_tail(n) : 0) + 255) >> 8) * ((p.M + kOut - 1) / kOut); }, blockIdx.x == 0);
     tc_fence_before();
     __syncthreads();
     cluster_sync_all();   // the peer's barriers are ready
@@ -695,6 +818,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     struct Tile {
         int group, m;      // matrix, first output
         int pos, rows;     // first row of x of this CTA, rows of the group from there on
+        int tail;          // rows behind the pair's 256 that go with them
     };
     // the tiles of one block of outputs follow each other, so its weights come from HBM once
     auto tile_at = [&](int i) {
@@ -704,9 +828,9 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             if (first_tile[mid] <= i) lo = mid;
             else hi = mid;
         }
-        const int blocks = (rows[lo] + 255) >> 8, in = i - first_tile[lo];
-        const int n = in / blocks, at = (in - n * blocks) * 256 + 128 * (int)rank;
-        return Tile{lo, n * kOut, start[lo] + at, rows[lo] - at};
+        const int tail = TAILS ? fp4_tail(rows[lo]) : 0, blocks = (rows[lo] - tail + 255) >> 8, in = i - first_tile[lo];
+        const int n = in / blocks, r = in - n * blocks, at = r * 256 + 128 * (int)rank;
+        return Tile{lo, n * kOut, start[lo] + at, rows[lo] - at, r + 1 == blocks ? tail : 0};
     };
 
     if (warp < 4) {
@@ -721,20 +845,28 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                 const Tile t = tile_at(i);
                 // this CTA's half of the weights; both have all scales
                 const int m = t.m + kOut / 2 * (int)rank;
-                const int s0 = (t.group * p.units + t.m / (kOut / 2)) * steps * 4, s1 = s0 + steps * 4;
+                const int s0 = (t.group * p.units + t.m / (kOut / 2)) * steps * 4, s1 = s0 + steps * 4, own = s0 + steps * 4 * (int)rank;
+                // half of the tail's rows, in whole 16s
+                const int tail_at = t.pos - 128 * (int)rank + 256 + ((t.tail + 31) >> 5 << 4) * (int)rank;
+                const uint32_t share = kFp4PairTx + (t.tail ? kFp4TailTx : 0);
                 for (int k = 0; k < steps; k++) {
                     if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
                     if (elect_one()) {
-                        const uint32_t st = ring0 + r.i * kFp4PairStage, bar = full0 + 8 * r.i;
-                        if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * kFp4PairTx);
+                        const uint32_t st = ring0 + r.i * kStage, bar = full0 + 8 * r.i;
+                        bytes[r.i] = share;
+                        if (rank == 0) mbar_arrive_expect_tx(&full[r.i], 2 * share);
                         // (no rows for this CTA: from past the end, which is zeros and no traffic)
                         tma_pair_2d(st, &x_map, k * 128, t.rows > 0 ? t.pos : p.T, bar);
                         load_weights_pair<MODE != kFp4Plain>(st + kFp4Tile, &w_map, k * 128, m, t.group, bar);
                         tma_pair_2d(st + 2 * kFp4Tile, &s_map, 0, s0 + 4 * k, bar);
                         tma_pair_2d(st + 2 * kFp4Tile + kFp4Scales, &s_map, 0, s1 + 4 * k, bar);
+                        if (TAILS && t.tail) {
+                            tma_pair_2d(st + kTailX, &tail_map, k * 128, tail_at, bar);
+                            tma_pair_2d(st + kTailW, &s_map, 0, own + 4 * k, bar);
+                        }
                     }
                     __syncwarp();
-                    r.next(kFp4PairStages);
+                    r.next(n_stages);
                     n_issued++;
                 }
             }
@@ -751,12 +883,14 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs, n++) {
                 // the accumulator of the tile before has been read
                 if (n > 0 && !bar_wait(smem_u32(tile_read), (n - 1) & 1u, ctl)) break;
-                const uint32_t d = base + (n & 1 ? kFp4PairSecond : 0);
+                const uint32_t d = base + (n & 1 ? kSecond : 0);
+                // the tail's: weights on the M side, its rows on the N side, beside the other accumulator
+                const uint32_t tail = TAILS ? uniform(tile_at(i).tail) : 0, tail_d = base + (n & 1 ? 0 : 256), tail_idesc = umma_idesc_mxf4(256, (tail + 31) & ~31u, 0);
                 for (int k = 0; k < steps; k++) {
                     if (!bar_wait_both(full0 + 8 * r.i, r.phase, x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
                     tc_fence_after();
-                    const uint32_t at = r.i * (kFp4PairStage >> 4), wl = w_low + at, xl = x_low + at, wsl = ws_low + at, xsl = xs_low + at;
-                    const uint32_t xs = base + kFp4PairTmemScales + kFp4ScaleCols * buffer, ws = xs + 8, more = k > 0;
+                    const uint32_t at = r.i * (kStage >> 4), wl = w_low + at, xl = x_low + at, wsl = ws_low + at, xsl = xs_low + at;
+                    const uint32_t xs = base + kTmemScales + kCols * buffer, ws = xs + 8, more = k > 0;
                     if (elect_one()) {
 #pragma unroll
                         for (int u = 0; u < 2; u++) {   // half of the stage's contracted values
@@ -768,11 +902,23 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                         for (int j = 0; j < 4; j++)
                             umma_mxf4<2>(d, wide_desc(xl + 2 * j, kSw128High), wide_desc(wl + 2 * j, kSw128High), idesc[j & 1], xs + 4 * (j >> 1),
                                          ws + 8 * (j >> 1), j > 0 ? 1 : more);
+                        if (TAILS && tail) {
+                            const uint32_t tws = xs + 24, txs = tws + 8;
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                scales_to_tmem<2>(tws + 4 * u, wide_desc(wsl + (kTailW - 2 * kFp4Tile + u * 512 >> 4), kScaleHigh));
+                                scales_to_tmem<2>(txs + 4 * u, wide_desc(wsl + (kTailS - 2 * kFp4Tile + u * 512 >> 4), kScaleHigh));
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                umma_mxf4<2>(tail_d, wide_desc(wl + 2 * j, kSw128High), wide_desc(xl + (kTailX >> 4) + 2 * j, kSw128High),
+                                             j & 1 ? tail_idesc | (idesc[1] & ~idesc[0]) : tail_idesc, tws + 4 * (j >> 1), txs + 4 * (j >> 1), j > 0 ? 1 : more);
+                        }
                         umma_commit_pair(done0 + 8 * r.i);
                         if (k + 1 == steps) umma_commit_pair(smem_u32(tile_done) + 8 * (n & 1));
                     }
                     __syncwarp();
-                    r.next(kFp4PairStages);
+                    r.next(n_stages);
                     buffer ^= 1;
                 }
             }
@@ -791,6 +937,8 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             const int first = 64 * (warp - 2) + lane;
             const uint32_t x_full0 = map_to_rank0(smem_u32(x_full));
             uint4 four[2][2];   // [row][half]
+            uint4 of_tail[2];   // of its row 32 (warp - 2) + lane
+            bool tail = false;
             auto load = [&](const Tile& t, int k) {
                 const uint8_t* row = p.x_scales + (long long)(t.pos + first) * p.ld_xs;
 #pragma unroll
@@ -799,6 +947,15 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
 #pragma unroll
                     for (int h = 0; h < 2; h++)
                         four[c][h] = in ? sixteen_scales(row + 32 * c * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs) : make_uint4(0, 0, 0, 0);
+                }
+                if (!TAILS) return;
+                tail = t.tail != 0;
+                if (tail) {
+                    const int r = 32 * (warp - 2) + lane;
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        of_tail[h] = r < t.tail ? sixteen_scales(p.x_scales + (long long)(t.pos - 128 * (int)rank + 256 + r) * p.ld_xs, 8 * k + 16 * h, p.blocks, p.wide_xs)
+                                                : make_uint4(0, 0, 0, 0);
                 }
             };
             int i = blockIdx.x >> 1;
@@ -811,13 +968,19 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                         if (k4 + j >= steps) break;
                         const uint4 a = four[0][j >> 1], b = four[1][j >> 1];
                         if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
-                        uint2* to = reinterpret_cast<uint2*>(ring + r.i * kFp4PairStage + kFp4PairTx) + 2 * lane + (warp - 2);
+                        uint2* to = reinterpret_cast<uint2*>(ring + r.i * kStage + kFp4PairTx) + 2 * lane + (warp - 2);
                         to[0] = j & 1 ? make_uint2(a.z, b.z) : make_uint2(a.x, b.x);
                         to[64] = j & 1 ? make_uint2(a.w, b.w) : make_uint2(a.y, b.y);
+                        if (TAILS && tail) {
+                            uint32_t* more = reinterpret_cast<uint32_t*>(ring + r.i * kStage + kTailS) + 4 * lane + (warp - 2);
+                            const uint4 c = of_tail[j >> 1];
+                            more[0] = j & 1 ? c.z : c.x;
+                            more[128] = j & 1 ? c.w : c.y;
+                        }
                         fence_async();
                         __syncwarp();
                         if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
-                        r.next(kFp4PairStages);
+                        r.next(n_stages);
                     }
                     if (k4 + 4 < steps) load(t, k4 + 4);
                     else if (i + pairs < tiles) load(tile_at(i + pairs), 0);
@@ -828,15 +991,27 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
         // ------------------------------------------------ output
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp4PairRegsMany));
         const int half = (warp - 4) >> 2;
-        uint8_t* room = ring + kFp4PairStages * kFp4PairStage + (warp - 4) * kFp4PairOut;
+        uint8_t* room = ring + n_stages * kStage + (warp - 4) * (TAILS ? kFp4TailOut : kFp4PairOut);
         const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t read0 = map_to_rank0(smem_u32(tile_read));
+        constexpr int kPiece = TAILS ? 64 : 128;
+        const int two = 1 + ((warp - 4) >> 1);
         uint32_t n = 0;
         for (int i = blockIdx.x >> 1; i < tiles; i += pairs, n++) {
             const Tile t = tile_at(i);
-            if (!bar_wait(smem_u32(tile_done) + 8 * (n & 1), (n >> 1) & 1u, ctl)) break;
+            bool there = bar_wait(smem_u32(tile_done) + 8 * (n & 1), (n >> 1) & 1u, ctl);
+            // (two warps share a tail's blocks of features: as one of them gives up, both do, since they meet at barriers)
+            if (TAILS && MODE == kFp4GatedRows) there = all_of(two, 64, there);
+            if (!there) break;
             tc_fence_after();
-            const uint32_t from = taddr + (n & 1 ? kFp4PairSecond : 0);
+            const uint32_t from = taddr + (n & 1 ? kSecond : 0);
+            if (TAILS && t.tail > 32 * half) {   // its lanes are outputs, its columns rows of x, 32 for each half
+                float v[32];
+                tmem_ld32(taddr + (n & 1 ? 0 : 256) + 32 * half, v);
+                tail_rows<MODE>(p, (long long)t.pos - 128 * (int)rank + 256 + 32 * half, t.tail - 32 * half, t.m + kOut / 2 * (int)rank,
+                                32 * (warp & 3) + lane, v, reinterpret_cast<float*>(ring + n_stages * kStage + ((warp - 4) >> 1) * kFp4TailBlocks), two);
+                __syncwarp();
+            }
             float2 acc[64];   // 128 columns
             if (t.rows > 32 * (warp & 3)) {
 #pragma unroll
@@ -852,9 +1027,9 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                 if (MODE == kFp4Plain) {
                     const int m = t.m + 128 * half;
                     const long long o = at * p.ld_out + m;
-                    if (p.type == 0) store_rows(reinterpret_cast<float*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
-                    else if (p.type == 1) store_rows(reinterpret_cast<__half*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
-                    else store_rows(reinterpret_cast<__nv_bfloat16*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
+                    if (p.type == 0) store_rows<kPiece>(reinterpret_cast<float*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
+                    else if (p.type == 1) store_rows<kPiece>(reinterpret_cast<__half*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
+                    else store_rows<kPiece>(reinterpret_cast<__nv_bfloat16*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, acc, room, wide_out);
                 } else {
                     float2 h[32];
 #pragma unroll
@@ -865,11 +1040,11 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                         if (lane < t.rows - r0)
                             store_row4(reinterpret_cast<uint8_t*>(p.out) + (at + lane) * p.ld_out + m / 2, p.out_scales + (at + lane) * p.ld_os + m / kFp4Block, p.M - m, h);
                     } else if (p.type == 0) {
-                        store_rows(reinterpret_cast<float*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
+                        store_rows<kPiece>(reinterpret_cast<float*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
                     } else if (p.type == 1) {
-                        store_rows(reinterpret_cast<__half*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
+                        store_rows<kPiece>(reinterpret_cast<__half*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
                     } else {
-                        store_rows(reinterpret_cast<__nv_bfloat16*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
+                        store_rows<kPiece>(reinterpret_cast<__nv_bfloat16*>(p.out) + o, p.ld_out, p.M - m, t.rows - r0, h, room, wide_out);
                     }
                 }
             }
@@ -886,8 +1061,8 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     tc_fence_after();
     if (rank == 0 ? given_up != 0 : from_peer != 0) {
         if (rank == 0 && threadIdx.x == 0) {
-            Fp4PairBars bars{full};
-            drain_pair(issued, from_peer, kFp4PairStages, bars);
+            Fp4PairBars bars{full, bytes};
+            drain_pair(issued, from_peer, n_stages, bars);
         }
         if (warp == 1) {
             if (rank == 0 && elect_one()) umma_commit_pair(smem_u32(left_bar));

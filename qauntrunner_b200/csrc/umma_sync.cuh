@@ -209,9 +209,10 @@ __device__ __forceinline__ void store_row(T* out, int left, const float2 (&acc)[
 // error, and so does a start below any offset before it: no row outside x or
 // out is ever touched, and none belongs to two groups (whose CTAs would both
 // write it, and whose tiles together could be more than a count of them holds).
-// tile_rows rows of x a tile, `across` tiles along the outputs.
+// tiles_of: a group's tiles (or what they cost) by its rows; none for no rows.
+template <typename Tiles>
 __device__ inline void group_tables(const int32_t* offsets, int groups, int T, int32_t* err, int32_t* first_tile, int32_t* start,
-                                    int32_t* rows, int tile_rows, int across, bool report) {
+                                    int32_t* rows, Tiles tiles_of, bool report) {
     const int lane = threadIdx.x & 31;
     int before = 0, top = 0;   // tiles, largest offset so far
     bool bad = false;
@@ -233,7 +234,7 @@ __device__ inline void group_tables(const int32_t* offsets, int groups, int T, i
             bad |= g < groups;
             a = b = 0;
         }
-        const int tiles = (b - a + tile_rows - 1) / tile_rows * across;
+        const int tiles = tiles_of(b - a);
         int scan = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -249,6 +250,12 @@ __device__ inline void group_tables(const int32_t* offsets, int groups, int T, i
     }
     if (lane == 0) first_tile[groups] = before;
     if (__any_sync(0xffffffffu, bad) && report && lane == 0) atomicOr(err, (int)ERR_BOUNDS);
+}
+
+// the same for tiles of tile_rows rows of x, `across` of them along the outputs
+__device__ inline void group_tables(const int32_t* offsets, int groups, int T, int32_t* err, int32_t* first_tile, int32_t* start,
+                                    int32_t* rows, int tile_rows, int across, bool report) {
+    group_tables(offsets, groups, T, err, first_tile, start, rows, [&](int n) { return (n + tile_rows - 1) / tile_rows * across; }, report);
 }
 
 }  // namespace qrm

@@ -368,6 +368,67 @@ def test_two_groups_of_forty(first, second, type, form):
     m.close()
 
 
+# groups of whole tiles of 256 rows and a few more, of tiles without more, of one row, of none
+TAILS = [[257, 288, 256, 320], [321, 0, 576, 1, 577], [300, 300], [64, 1000, 319]]
+
+
+@pytest.mark.parametrize("sizes", TAILS, ids=str)
+@pytest.mark.parametrize("odd", [0, 1], ids=["aligned", "odd"])
+@pytest.mark.parametrize("n,k", [(300, 1900), (256, 2304), (130, 4100)])
+def test_few_rows_behind_a_tile(sizes, odd, n, k, form):
+    """Products and gated ones; odd: rows of scales and outputs that start anywhere."""
+    T, f = sum(sizes), n // 2
+    c = Case(T, len(sizes), n, k, spread=1)
+    offsets = torch.tensor([0] + sizes).cumsum(0)
+    w, x = P.values(*c.w, k).reshape(len(sizes), n, k), P.values(*c.x, k)
+    want = torch.cat([x[offsets[i]:offsets[i + 1]] @ w[i].T for i in range(len(sizes))])
+    assert max(float((x[offsets[i]:offsets[i + 1]].abs() @ w[i].abs().T).max()) for i in range(len(sizes)) if sizes[i]) < 2 ** 18
+    off, m = offsets.int().cuda(), c.matrix()
+    codes, scales = c.x[0].cuda(), torch.zeros(T, c.x[1].shape[1] + odd, dtype=torch.uint8).cuda()
+    scales[:, :c.x[1].shape[1]] = c.x[1].cuda()
+    ld = scales.shape[1]
+    for type in TYPES:
+        y = torch.full((T + 1, n + odd), 5.0, dtype=F.DTYPE[type]).cuda()
+        m.product(type, codes, scales, T, y, offsets=off, ld_scales=ld, ld_y=n + odd)
+        m.sync()
+        assert torch.equal(y[:T, :n].cpu(), want.float().to(F.DTYPE[type]))
+        assert bool((y[T] == 5).all()) and bool((y[:, n:] == 5).all())
+    # (gates of up to some tens, so that a rounding of the product is within the test's slack)
+    scales = (scales.int() - 4).to(torch.uint8)
+    want = want / 16
+    h = torch.full((T + 1, f + odd), 5.0).cuda()
+    m.swiglu(0, codes, scales, T, h, offsets=off, limit=7.0, ld_scales=ld, ld_h=f + odd)
+    c4, s4 = rows4(T + 1, f)
+    m.swiglu_fp4(codes, scales, T, c4, s4, offsets=off, limit=7.0, ld_xs=ld)
+    m.sync()
+    h, gated = h.cpu(), P.gate(want, 7.0)
+    slack = 16 * U * gated.abs() + 4 * 2.0 ** -149 * (want[:, :f] * want[:, f:2 * f]).abs()
+    slack = slack + F.ROUND[0] * (gated.abs() + slack) + F.HALF_STEP[0]   # (as in test_gated)
+    assert bool(((h[:T, :f].double() - gated).abs() <= slack).all())
+    assert bool((h[T] == 5).all()) and bool((h[:, f:] == 5).all())
+    qc, qs = P.quantize(h[:T, :f].contiguous())
+    assert torch.equal(c4[:T].cpu(), qc) and torch.equal(s4[:T].cpu(), qs)
+    assert bool((c4[T] == 0x77).all()) and bool((s4[T] == 0x77).all())
+    m.close()
+
+
+def test_a_hundred_groups_with_a_few_rows_behind_a_tile(form):
+    """(a table of groups that leaves less shared memory for the products' stages)"""
+    sizes = [257 + i % 70 if i % 2 else i for i in range(100)]
+    T, n, k = sum(sizes), 48, 1800
+    c = Case(T, 100, n, k, spread=1)
+    w, x = P.values(*c.w, k).reshape(100, n, k), P.values(*c.x, k)
+    offsets = torch.tensor([0] + sizes).cumsum(0)
+    want = torch.cat([x[offsets[i]:offsets[i + 1]] @ w[i].T for i in range(100)])
+    assert T > 128 * 100 and float((x.abs() @ w.abs().amax(0).T).max()) < 2 ** 18
+    m = c.matrix()
+    y = torch.empty(T, n).cuda()
+    m.product(0, c.x[0].cuda(), c.x[1].cuda(), T, y, offsets=offsets.int().cuda())
+    m.sync()
+    assert torch.equal(y.cpu(), want.float())
+    m.close()
+
+
 def test_many_groups():
     """1024 matrices, most without rows."""
     c = Case(40, 1024, 32, 64)
