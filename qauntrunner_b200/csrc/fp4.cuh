@@ -570,14 +570,14 @@ constexpr int kFp4TailSecond = 176, kFp4TailTmemScales = 432, kFp4TailScaleCols 
 // rows of x that a group's tiles are, by its rows: a rest of few rows goes with the last whole tile
 __host__ __device__ inline int fp4_tail(int rows) { return rows > 256 && (rows & 255) <= kFp4TailRows ? rows & 255 : 0; }
 constexpr int kFp4PairOut = 32 * 144;          // a warp's room for rows on their way out: 32 of 128 bytes, 16 apart
-constexpr int kFp4TailOut = 32 * 64;           // with tails: 32 of 64 bytes; gated into 4 bits, of two warps: 32 of 36 floats
-constexpr int kFp4TailBlocks = 32 * 144;
+constexpr int kFp4TailOut = 32 * 64;           // with tails: 32 of 64 bytes
+constexpr int kFp4TailBlocks = 16 * 144;       // gated into 4 bits, of two warps: 16 of 36 floats
 constexpr int kFp4PairTableOff = 1024;
 constexpr int kFp4PairRegsFew = 72, kFp4PairRegsMany = 216;
 constexpr int kFp4PairRegs = 128 * kFp4PairRegsFew + 256 * kFp4PairRegsMany;
 static_assert(kFp4PairRegs <= kFp4PairThreads * 168, "register split");
-constexpr int kFp4TailRoom = 4 * kFp4TailBlocks;   // at least 8 kFp4TailOut
-static_assert(kFp4TailRoom >= 8 * kFp4TailOut, "room");
+constexpr int kFp4TailRoom = 8 * kFp4TailOut;
+static_assert(kFp4TailRoom >= 4 * kFp4TailBlocks, "room");
 __host__ __device__ inline int fp4_pair_stage_off(int groups) { return (kFp4PairTableOff + 12 * (groups + 1) + 1023) / 1024 * 1024; }
 
 // the first CTA's barriers, as drain_pair moves them on; the tiles' stages have different numbers of bytes
@@ -698,22 +698,22 @@ __device__ __forceinline__ void store_outputs(const Fp4Params& p, long long t, i
     else if (p.type == 1) store_outputs<__half>(p, t, first, step, have, m, v);
     else store_outputs<__nv_bfloat16>(p, t, first, step, have, m, v);
 }
-// 32 rows of a tail from row t on, of which `have` exist: the lane's output
-// of each, number `id` of the CTA's 128 (gated: a row of the MMA's A, gate's and up's in
+// 16 rows of a tail from row t on, of which `have` exist: the lane's output of
+// each, number `id` of the CTA's 128 (gated: a row of the MMA's A, gate's and up's in
 // turns of 16), which begin at m.  room: gated into 4 bits, of two warps, whose 32
 // features are a block.
 template <int MODE>
-__device__ __forceinline__ void tail_rows(const Fp4Params& p, long long t, int have, int m, int id, const float (&v)[32], float* room,
-                                            int barrier) {
+__device__ __forceinline__ void tail_rows(const Fp4Params& p, long long t, int have, int m, int id, const float (&v)[16], float* room,
+                                          int barrier) {
     if constexpr (MODE == kFp4Plain) {
         store_outputs(p, t, 0, 1, have, m + id, v);
     } else {
         const int lane = threadIdx.x & 31;
         // gate's lanes get both sums of the even rows, up's of the odd ones
         const bool up = lane & 16;
-        float y[16];
+        float y[8];
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
+        for (int c = 0; c < 16; c += 4) {
             const float g0 = __shfl_xor_sync(0xffffffffu, up ? v[c] : v[c + 1], 16);
             const float g1 = __shfl_xor_sync(0xffffffffu, up ? v[c + 2] : v[c + 3], 16);
             const float2 own = up ? make_float2(v[c + 1], v[c + 3]) : make_float2(v[c], v[c + 2]), other = make_float2(g0, g1);
@@ -728,22 +728,23 @@ __device__ __forceinline__ void tail_rows(const Fp4Params& p, long long t, int h
             constexpr int kPitch = 36;   // floats of a row in the room
             named_barrier(barrier, 64);  // what was in the room is out
 #pragma unroll
-            for (int c = 0; c < 16; c++) room[(2 * c + (up ? 1 : 0)) * kPitch + (feature & 31)] = y[c];
-            named_barrier(barrier, 64);  // 32 rows of 32 features are there: a thread takes half of one
-            const int r = (id & 63) >> 1, o = 16 * (id & 1), first = m + (feature & 32), left = p.M - first;
-            float e[16];
+            for (int c = 0; c < 8; c++) room[(2 * c + (up ? 1 : 0)) * kPitch + (feature & 31)] = y[c];
+            named_barrier(barrier, 64);  // 16 rows of 32 features are there: a thread takes a quarter of one
+            const int r = (id & 63) >> 2, o = 8 * (id & 3), first = m + (feature & 32), left = p.M - first;
+            const float4* from = reinterpret_cast<const float4*>(room + r * kPitch + o);
+            const float4 a = from[0], b = from[1];
+            float e[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
             uint32_t top = 0;
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                e[k] = o + k < left ? room[r * kPitch + o + k] : 0.f;
+            for (int k = 0; k < 8; k++) {
+                if (o + k >= left) e[k] = 0.f;
                 top = max(top, magnitude(e[k]));
             }
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const uint32_t scale = fp4_scale(top);
             if (r < have && left > 0) {
-                const float lo[8] = {e[0], e[1], e[2], e[3], e[4], e[5], e[6], e[7]}, hi[8] = {e[8], e[9], e[10], e[11], e[12], e[13], e[14], e[15]};
-                *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(p.out) + (t + r) * p.ld_out + (first + o) / 2) =
-                    make_uint2(e2m1x8(lo, scale), e2m1x8(hi, scale));
+                *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + (t + r) * p.ld_out + (first + o) / 2) = e2m1x8(e, scale);
                 if (o == 0) p.out_scales[(t + r) * p.ld_os + first / kFp4Block] = (uint8_t)scale;
             }
         }
@@ -1005,13 +1006,15 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             if (!there) break;
             tc_fence_after();
             const uint32_t from = taddr + (n & 1 ? kSecond : 0);
-            if (TAILS && t.tail > 32 * half) {   // its lanes are outputs, its columns rows of x, 32 for each half
-                float v[32];
-                tmem_ld32(taddr + (n & 1 ? 0 : 256) + 32 * half, v);
-                tail_rows<MODE>(p, (long long)t.pos - 128 * (int)rank + 256 + 32 * half, t.tail - 32 * half, t.m + kOut / 2 * (int)rank,
+            // a tail's lanes are outputs, its columns rows of x, every second 16 of them for this half
+#pragma unroll 1
+            for (int c = 16 * half; TAILS && c < t.tail; c += 32) {
+                float v[16];
+                tmem_ld16_now(taddr + (n & 1 ? 0 : 256) + c, v);
+                tail_rows<MODE>(p, (long long)t.pos - 128 * (int)rank + 256 + c, t.tail - c, t.m + kOut / 2 * (int)rank,
                                 32 * (warp & 3) + lane, v, reinterpret_cast<float*>(ring + n_stages * kStage + ((warp - 4) >> 1) * kFp4TailBlocks), two);
-                __syncwarp();
             }
+            __syncwarp();
             float2 acc[64];   // 128 columns
             if (t.rows > 32 * (warp & 3)) {
 #pragma unroll
