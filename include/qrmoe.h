@@ -414,7 +414,8 @@ int qrm_gather_rows_fp4(int type, const void* x_dev, int64_t ld_x, const int32_t
 /* groups matrices [rows x cols] in 4 bits, kept in HBM: codes
  * [groups][rows][16 ceil(cols/32)] and scales [groups][rows][ceil(cols/32)],
  * bytes both, are copied, from the host or (_device) from any device, after a
- * synchronise of it.  At most 1024 groups (QRM_E_CAPACITY).
+ * synchronise of it (the scales twice where rows is even: gate's and up's lie
+ * side by side for the gated product).  At most 1024 groups (QRM_E_CAPACITY).
  * qrm_fp4_product: y[t] = W_g x[t] for the rows t in [offsets[g], offsets[g+1])
  * of each group g (offsets NULL: one group, all T rows), x [T][cols] in 4 bits
  * and y [T][rows]; rows outside every group are not written.

@@ -187,9 +187,10 @@ template <int MODE>
 cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const CUtensorMap& few_map, const Fp4Params& p, bool pair, int wide_out, int64_t T, cudaStream_t s) {
     const CUtensorMap& w_map = MODE == kFp4Plain ? m->map : m->gated_map;
     if (pair) {
-        // Tails (a third more shared memory a stage, smaller pieces on the way out) where groups are likely to have one and a
-        // tile has stages enough.  With and without, us: 32 x 4096 x 7168, 8192 rows 124 / 147, 4096 rows 106 / 104, 12000 rows
-        // 187 / 185; 32 x 7168 x 2048, 8192 rows 76 / 84; 8 x 5632 x 1024, 2048 rows 17.0 / 16.2, 512 rows 13.7 / 11.7.
+        // Tails (a sixth more shared memory a stage, smaller pieces on the way out) where groups are likely to have one and a
+        // tile has stages enough.  With and without, us: 32 x 4096 x 7168, 8192 rows 120 / 145, 9000 rows 137 / 180, 12000 rows
+        // 187 / 183; 32 x 7168 x 2048, 8192 rows 72 / 83; 64 x 4096 x 2048, 20000 rows 114 / 128; 20 x 3584 x 2816, 7000 rows 52 / 48;
+        // 8 x 5632 x 2048, 2560 rows 27 / 25; 8 x 5632 x 1024, 512 rows 13.7 / 11.7.
         const bool tails = m->groups > 1 && T > (int64_t)128 * m->groups && p.steps >= 8;
         const int stages = tails ? tail_stages(m->groups) : kFp4PairStages;
         return launch_ahead(tails ? fp4_pair_kernel<MODE, true> : fp4_pair_kernel<MODE, false>, dim3(m->sms / 2 * 2), kFp4PairThreads,

@@ -543,7 +543,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // brings half of them to each CTA, and a second MMA takes them against the weights
 // that are there already, with the operands' places changed (weights on the M
 // side, the tail's rows, rounded up to 32, on the N side).  8192 rows over 32 x 4096
-// x 7168: 147 -> 124 us (floor 91).  Tiles of their own in that form gained
+// x 7168: 145 -> 120 us (floor 91).  Tiles of their own in that form gained
 // nothing (their weights come from L2 once more), nor did a kernel with all rows on
 // the N side, 384 a tile (137 us there, but 217 in place of 176 for one matrix).
 //
@@ -564,7 +564,7 @@ constexpr int kFp4PairSecond = 208, kFp4PairTmemScales = 464;
 // tail's scales; tensor memory for a second accumulator, and 16 columns of scales a stage
 constexpr int kFp4TailRows = 64;
 constexpr int kFp4TailTx = kFp4TailRows / 2 * 128 + kFp4Scales;
-constexpr int kFp4TailStages = 5;             // where they fit (up to 84 matrices), 4 of them else
+constexpr int kFp4TailStages = 5;             // where they fit (up to 255 matrices), 4 of them else
 constexpr int kFp4TailStage = kFp4PairStage + kFp4TailTx + kFp4Scales;
 constexpr int kFp4TailSecond = 176, kFp4TailTmemScales = 432, kFp4TailScaleCols = 40;
 // rows of x that a group's tiles are, by its rows: a rest of few rows goes with the last whole tile
@@ -882,11 +882,12 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             const uint32_t ws_low = scale_low(ring0 + 2 * kFp4Tile), xs_low = scale_low(ring0 + kFp4PairTx), base = uniform(tmem);
             constexpr uint32_t idesc[2] = {umma_idesc_mxf4(256, 256, 0), umma_idesc_mxf4(256, 256, 2)};
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs, n++) {
+                const uint32_t tail = TAILS ? uniform(tile_at(i).tail) : 0;   // (looked up while the epilogue is at work)
                 // the accumulator of the tile before has been read
                 if (n > 0 && !bar_wait(smem_u32(tile_read), (n - 1) & 1u, ctl)) break;
                 const uint32_t d = base + (n & 1 ? kSecond : 0);
                 // the tail's: weights on the M side, its rows on the N side, beside the other accumulator
-                const uint32_t tail = TAILS ? uniform(tile_at(i).tail) : 0, tail_d = base + (n & 1 ? 0 : 256), tail_idesc = umma_idesc_mxf4(256, (tail + 31) & ~31u, 0);
+                const uint32_t tail_d = base + (n & 1 ? 0 : 256), tail_idesc = umma_idesc_mxf4(256, (tail + 31) & ~31u, 0);
                 for (int k = 0; k < steps; k++) {
                     if (!bar_wait_both(full0 + 8 * r.i, r.phase, x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
                     tc_fence_after();

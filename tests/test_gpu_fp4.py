@@ -412,15 +412,16 @@ def test_few_rows_behind_a_tile(sizes, odd, n, k, form):
     m.close()
 
 
-def test_a_hundred_groups_with_a_few_rows_behind_a_tile(form):
-    """(a table of groups that leaves less shared memory for the products' stages)"""
-    sizes = [257 + i % 70 if i % 2 else i for i in range(100)]
+@pytest.mark.parametrize("groups", [100, 300])
+def test_many_groups_with_a_few_rows_behind_a_tile(groups, form):
+    """(300: a table of groups that leaves less shared memory for the products' stages)"""
+    sizes = [257 + i % 70 if i % 2 else i % 100 for i in range(groups)]
     T, n, k = sum(sizes), 48, 1800
-    c = Case(T, 100, n, k, spread=1)
-    w, x = P.values(*c.w, k).reshape(100, n, k), P.values(*c.x, k)
+    c = Case(T, groups, n, k, spread=1)
+    w, x = P.values(*c.w, k).reshape(groups, n, k), P.values(*c.x, k)
     offsets = torch.tensor([0] + sizes).cumsum(0)
-    want = torch.cat([x[offsets[i]:offsets[i + 1]] @ w[i].T for i in range(100)])
-    assert T > 128 * 100 and float((x.abs() @ w.abs().amax(0).T).max()) < 2 ** 18
+    want = torch.cat([x[offsets[i]:offsets[i + 1]] @ w[i].T for i in range(groups)])
+    assert T > 128 * groups and float((x.abs() @ w.abs().amax(0).T).max()) < 2 ** 18
     m = c.matrix()
     y = torch.empty(T, n).cuda()
     m.product(0, c.x[0].cuda(), c.x[1].cuda(), T, y, offsets=offsets.int().cuda())
