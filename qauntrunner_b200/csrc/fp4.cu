@@ -221,6 +221,8 @@ cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const CUtensorMap
     return cudaLaunchKernelEx(&cfg, p.groups > 1 ? fp4_split_kernel<MODE, true> : fp4_split_kernel<MODE, false>, w_map, few_map, p, stages);
 }
 
+constexpr int64_t kMostRows = INT_MAX - 1023;   // the end of the last one's tile fits in 32 bits
+
 int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x, const uint8_t* xs, int64_t ld_xs,
             const int32_t* offsets, int64_t T, float limit, int type, void* out, int64_t ld_out, uint8_t* out_scales,
             int64_t ld_os, void* stream) {
@@ -230,7 +232,7 @@ int product(const char* what, int mode, qrm_fp4* m, const void* x, int64_t ld_x,
     const int b = mode == kFp4GatedRows ? 1 : type_bytes(type);
     if (!b) return failf(QRM_E_FORMAT, "%s: type %d is not F32, F16 or BF16", what, type);
     if (!(limit >= 0.f)) return failf(QRM_E_INVALID, "%s: limit %g", what, (double)limit);
-    if (T < 0 || T > INT_MAX) return failf(QRM_E_INVALID, "%s: %lld rows", what, (long long)T);
+    if (T < 0 || T > kMostRows) return failf(QRM_E_INVALID, "%s: %lld rows", what, (long long)T);
     // rows of x in a tile of the kernel with weights on the M side: a third more than a group has on average, so that most
     // groups take one tile and a stage stays small
     const int64_t used = std::max<int64_t>(1, std::min<int64_t>(T, m->groups)), each = (T + used - 1) / used;

@@ -567,7 +567,7 @@ constexpr int kFp4TailTx = kFp4TailRows / 2 * 128 + kFp4Scales;
 constexpr int kFp4TailStages = 5;             // where they fit (up to 255 matrices), 4 of them else
 constexpr int kFp4TailStage = kFp4PairStage + kFp4TailTx + kFp4Scales;
 constexpr int kFp4TailSecond = 176, kFp4TailTmemScales = 432, kFp4TailScaleCols = 40;
-// rows of x that a group's tiles are, by its rows: a rest of few rows goes with the last whole tile
+// a group's tail, by its rows: few rows behind its last whole tile of 256
 __host__ __device__ inline int fp4_tail(int rows) { return rows > 256 && (rows & 255) <= kFp4TailRows ? rows & 255 : 0; }
 constexpr int kFp4PairOut = 32 * 144;          // a warp's room for rows on their way out: 32 of 128 bytes, 16 apart
 constexpr int kFp4TailOut = 32 * 64;           // with tails: 32 of 64 bytes

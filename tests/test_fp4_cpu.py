@@ -181,6 +181,8 @@ def test_product_arguments(fake):
     assert refused(m.product, 3, A, A, 8, A, **ok) == Q.E_FORMAT
     assert refused(m.product, 0, A, A, -1, A, **ok) == Q.E_INVALID
     assert refused(m.product, 0, A, A, 1 << 31, A, **ok) == Q.E_INVALID
+    assert refused(m.product, 0, A, A, (1 << 31) - 1, A, **ok) == Q.E_INVALID   # (tiles' ends would pass 32 bits)
+    assert refused(m.swiglu, 0, A, A, (1 << 31) - 500, A, **ok) == Q.E_INVALID
     assert refused(m.product, 0, A, A, 8, A) == Q.E_INVALID                    # two matrices need offsets
     assert refused(m.product, 0, A + 8, A, 8, A, **ok) == Q.E_INVALID
     assert refused(m.product, 0, A, A, 8, A, ld_x=168, **ok) == Q.E_INVALID

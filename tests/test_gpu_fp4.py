@@ -456,13 +456,15 @@ def test_host_arrays_give_the_same_matrix():
 
 def test_calls_on_two_streams_and_captured(form):
     """Calls of one matrix at the same time, on two streams and in two graphs."""
-    cases = [Case(rows, 3, 512, 2048, seed=s, even=True) for s, rows in enumerate((40, 300))]
+    cases = [Case(rows, 3, 512, 2048, spread=1, seed=s, even=True) for s, rows in enumerate((40, 300, 1000))]
+    cases[2].offsets = torch.tensor([0, 300, 620, 1000], dtype=torch.int32)   # (with a few rows behind a tile)
     m = cases[0].matrix()
     for c in cases[1:]:   # the same matrix
         x, w = P.values(*c.x, c.k), P.values(*cases[0].w, c.k).reshape(3, 512, c.k)
         for i in range(3):
             a, b = int(c.offsets[i]), int(c.offsets[i + 1])
             c.want[a:b] = x[a:b] @ w[i].T
+            assert a == b or float((x[a:b].abs() @ w[i].abs().T).max()) < 2 ** 18
     ins = [(c.x[0].cuda(), c.x[1].cuda(), c.offsets.cuda()) for c in cases]
     outs = [torch.zeros(c.rows, c.n).cuda() for c in cases]
     streams, graphs = [torch.cuda.Stream() for _ in cases], [torch.cuda.CUDAGraph() for _ in cases]
