@@ -538,6 +538,14 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // (a full memory barrier with every stage) and asked for four stages at a time,
 // rows out by way of shared memory, descriptors with constant high words.
 //
+// The MMAs of both CTAs are issued by a thread of the first, which has to know
+// that the other's scales of x, written by its own warps, are there.  They go
+// first: a CTA's copies of a stage are issued by a thread that has waited for the
+// stage's scales, so what completes on the first CTA's barrier, the copies' bytes
+// (a release of cluster scope), comes behind them.  An arrive of those warps on
+// that barrier would need such a release of its own: 396 us in place of 217 under
+// sustained load, 370 with a warp that does nothing else.
+//
 // Groups of uneven numbers of rows leave most of their last tile empty.  So up to
 // 64 rows behind a group's last whole tile, its tail, go with that tile: each stage
 // brings half of them to each CTA, and a second MMA takes them against the weights
@@ -552,8 +560,8 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // for the epilogue of the one before to have read its accumulator (some 1000
 // cycles, in which the ring of stages fills up).
 //
-// Warps: 0 loads codes and the weights' scales, 1 issues the MMAs (in the
-// pair's first CTA), 2 and 3 bring the scales of x, 4-11 write the output: lane
+// Warps: 2 and 3 bring the scales of x, 0 then loads codes and the weights'
+// scales, 1 issues the MMAs (in the pair's first CTA), 4-11 write the output: lane
 // quarter (warp & 3), half of the columns (warp >= 8).
 constexpr int kFp4PairThreads = 384;
 constexpr int kFp4PairStages = 5;
@@ -765,7 +773,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint64_t* full = reinterpret_cast<uint64_t*>(sm);   // first CTA: both CTAs' copies are there
-    uint64_t* x_full = full + kMost;           // first CTA: both CTAs' scales of x are there
+    uint64_t* x_full = full + kMost;           // both: the stage is free and this CTA's scales of x are in it
     uint64_t* done = x_full + kMost;           // both: the stage's MMAs are done
     uint64_t* tile_done = done + kMost;        // [2] both: a tile's are
     uint64_t* tile_read = tile_done + 2;                // first CTA: both epilogues have read an accumulator
@@ -787,7 +795,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
     if (threadIdx.x == 0) {
         for (int i = 0; i < n_stages; i++) {
             mbar_init(&full[i], 1);
-            mbar_init(&x_full[i], 4);
+            mbar_init(&x_full[i], 2);
             mbar_init(&done[i], 1);
         }
         mbar_init(&tile_done[0], 1);
@@ -841,7 +849,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             bool ok = true;
             Ring r;
             uint32_t n_issued = 0;
-            const uint32_t full0 = map_to_rank0(smem_u32(full)), ring0 = smem_u32(ring);
+            const uint32_t full0 = map_to_rank0(smem_u32(full)), x_full0 = smem_u32(x_full), ring0 = smem_u32(ring);
             for (int i = blockIdx.x >> 1; i < tiles && ok; i += pairs) {
                 const Tile t = tile_at(i);
                 // this CTA's half of the weights; both have all scales
@@ -851,7 +859,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                 const int tail_at = t.pos - 128 * (int)rank + 256 + ((t.tail + 31) >> 5 << 4) * (int)rank;
                 const uint32_t share = kFp4PairTx + (t.tail ? kFp4TailTx : 0);
                 for (int k = 0; k < steps; k++) {
-                    if (!bar_wait(done0 + 8 * r.i, r.phase ^ 1u, ctl)) { ok = false; break; }
+                    if (!bar_wait(x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
                     if (elect_one()) {
                         const uint32_t st = ring0 + r.i * kStage, bar = full0 + 8 * r.i;
                         bytes[r.i] = share;
@@ -877,7 +885,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             bool ok = true;
             Ring r;
             uint32_t n = 0, buffer = 0;   // tiles; of scales
-            const uint32_t full0 = smem_u32(full), x_full0 = smem_u32(x_full), ring0 = smem_u32(ring);
+            const uint32_t full0 = smem_u32(full), ring0 = smem_u32(ring);
             const uint32_t x_low = sw128_low(ring0), w_low = sw128_low(ring0 + kFp4Tile);
             const uint32_t ws_low = scale_low(ring0 + 2 * kFp4Tile), xs_low = scale_low(ring0 + kFp4PairTx), base = uniform(tmem);
             constexpr uint32_t idesc[2] = {umma_idesc_mxf4(256, 256, 0), umma_idesc_mxf4(256, 256, 2)};
@@ -889,7 +897,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                 // the tail's: weights on the M side, its rows on the N side, beside the other accumulator
                 const uint32_t tail_d = base + (n & 1 ? 0 : 256), tail_idesc = umma_idesc_mxf4(256, (tail + 31) & ~31u, 0);
                 for (int k = 0; k < steps; k++) {
-                    if (!bar_wait_both(full0 + 8 * r.i, r.phase, x_full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
+                    if (!bar_wait_cluster(full0 + 8 * r.i, r.phase, ctl)) { ok = false; break; }
                     tc_fence_after();
                     const uint32_t at = r.i * (kStage >> 4), wl = w_low + at, xl = x_low + at, wsl = ws_low + at, xsl = xs_low + at;
                     const uint32_t xs = base + kTmemScales + kCols * buffer, ws = xs + 8, more = k > 0;
@@ -937,7 +945,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             bool ok = true;
             Ring r;
             const int first = 64 * (warp - 2) + lane;
-            const uint32_t x_full0 = map_to_rank0(smem_u32(x_full));
+            const uint32_t x_full0 = smem_u32(x_full);
             uint4 four[2][2];   // [row][half]
             uint4 of_tail[2];   // of its row 32 (warp - 2) + lane
             bool tail = false;
@@ -981,7 +989,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
                         }
                         fence_async();
                         __syncwarp();
-                        if (lane == 0) bar_arrive_cluster(x_full0 + 8 * r.i);
+                        if (lane == 0) bar_arrive(x_full0 + 8 * r.i);
                         r.next(n_stages);
                     }
                     if (k4 + 4 < steps) load(t, k4 + 4);

@@ -118,11 +118,28 @@ __device__ __forceinline__ uint32_t map_to_rank0(uint32_t addr) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
     return r;
 }
-// (What it hands over was read from tensor memory and is ordered by the
-// tcgen05 fence before it; with cluster scope here a full memory barrier came
-// with every block: 1010 us in place of 560 at 4096 x 28672 x 4096, then.)
+// That this warp has read an accumulator, and no more: its loads from tensor
+// memory are waited for and the tcgen05 fence is before it.  Without a scope an
+// arrive releases to threads of its own CTA, so nothing that was written goes
+// with this one.  (With cluster scope here a full memory barrier came with every
+// block: 1010 us in place of 560 at 4096 x 28672 x 4096, then.)
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// bar_wait for a barrier that copies of both CTAs complete on
+__device__ __forceinline__ bool bar_try_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait_cluster(uint32_t bar, uint32_t parity, const WaitCtl& c) {
+    if (__all_sync(0xffffffffu, bar_try_cluster(bar, parity))) return true;
+    if (!bar_wait_slow(bar, parity, c.abort_flag, c.err)) return false;
+    return __all_sync(0xffffffffu, bar_try_cluster(bar, parity));   // (this phase is over, and the next one is not)
 }
 // loads of a pair's CTA that complete on a barrier of its first CTA
 __device__ __forceinline__ void tma_pair_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
