@@ -368,7 +368,9 @@ int  qrm_fp8_sync(qrm_fp8* m);
  * s = x + add, rounded to type (add NULL: x), inv = 1 / sqrt(mean(s^2) + eps),
  * y = s inv w; w is f32 [d] (NULL: 1).  The norm is that of the sum as it is
  * stored; sum_dev (NULL: not wanted) receives it.  Squares are summed in f32: a
- * row whose sum of squares passes 2^128 gives zeros.
+ * row whose sum of squares passes 2^128 gives zeros.  Waits for copies into shared
+ * memory are bounded (2 s); where one gave up, what those threads write, here and
+ * in the gradient, is NaN (8-bit and 4-bit rows: their scales).
  * qrm_rms_norm writes y in type, _fp8 in 8-bit rows, _fp4 in 4-bit rows; the
  * latter two also write it in type where y_dev is not NULL (the router's
  * input).  sum may be x or add, y any of them, in the same place and pitch.

@@ -13,7 +13,9 @@
 // holds a row in registers, 8 neighbouring columns to a load, so that each row is
 // read once.  Rows come by bulk copies into a ring of `slots` rows in shared
 // memory, several ahead of the one that is worked on: a slot is free again once
-// all threads have its row in registers, which the row's barrier says.  A copy
+// all threads have its row in registers, which the row's barrier says.  The wait
+// for a copy is bounded; a CTA in which one gave up writes NaN to all its rows in
+// the end (ring_walk.h).  A copy
 // starts and ends on 16 bytes, so a row that does not is copied with the bytes
 // around it and shifted into place on its way to registers; such a row goes out
 // by way of shared memory, in words.  Where a CTA has one row, loads of its own
@@ -23,6 +25,7 @@
 #include <type_traits>
 
 #include "gemv_tma.cuh"
+#include "ring_walk.h"
 #include "rows4.cuh"
 
 namespace qrm {
@@ -118,18 +121,23 @@ __device__ __forceinline__ Raw8<T> load8_again(const T* p, int n) {
 
 // A ring of rows in shared memory: slot i % slots holds the CTA's i-th row of
 // each of N arrays (NULL: none), `bytes` of it, with up to 15 bytes in front of it
-// and behind it.  (Those bytes share 16 aligned ones with the row's own.)
+// and behind it.  (Those bytes share 16 aligned ones with the row's own.)  How it is
+// walked: ring_walk.h.
 template <int N>
 struct RowRing {
     const char* from[N];
     long long pitch[N];   // bytes
     uint32_t at;          // address in shared memory
     uint64_t* full;
-    int slots, bytes, room;   // room: bytes of a row there
+    volatile int* given_up;   // [0]: a wait did, [1]: behind how many rows that were loaded
+    uint32_t slots, rows;
+    int bytes, room;          // room: bytes of a row there
     uint32_t i = 0, parity = 0, here = at;   // of the row that is worked on
     __device__ void init() {
         if (threadIdx.x == 0) {
-            for (int k = 0; k < slots; k++) mbar_init(&full[k], 1);
+            for (uint32_t k = 0; k < slots; k++) mbar_init(&full[k], 1);
+            given_up[0] = 0;
+            given_up[1] = -1;
             fence_barrier_init();
         }
         __syncthreads();
@@ -138,7 +146,9 @@ struct RowRing {
         return ((uint32_t)reinterpret_cast<uintptr_t>(from[j]) + t * (uint32_t)pitch[j]) & 15;
     }
     // row t into slot k, by one thread
-    __device__ void load(uint32_t k, uint32_t t) {
+    __device__ void load(uint32_t k, unsigned long long row) {
+        if (row >= rows) return;
+        const uint32_t t = (uint32_t)row;
         uint32_t total = 0;
 #pragma unroll
         for (int j = 0; j < N; j++)
@@ -152,22 +162,29 @@ struct RowRing {
                     "l"(from[j] + (long long)t * pitch[j] - offset(j, t)), "r"((offset(j, t) + bytes + 15) & ~15u), "r"(smem_u32(&full[k]))
                     : "memory");
     }
-    __device__ void start(uint32_t rows) {
+    __device__ void start() {
         if (threadIdx.x == 0)
-            for (uint32_t k = 0, t = blockIdx.x; k < (uint32_t)slots && t < rows; k++, t += gridDim.x) load(k, t);
+            for (uint32_t k = 0, t = blockIdx.x; k < slots && t < rows; k++, t += gridDim.x) load(k, t);
     }
-    // the row that is worked on is there (its copies were issued, so they come; the wait is bounded all the same)
-    __device__ void wait() { mbar_wait(&full[i], parity); }
-    // its slot takes the row `slots` turns on; all threads have read it
-    __device__ void next(uint32_t t, uint32_t rows) {
-        const unsigned long long ahead = t + (unsigned long long)slots * gridDim.x;
-        if (threadIdx.x == 0 && ahead < rows) load(i, (uint32_t)ahead);
-        here += N * room;
-        if (++i == (uint32_t)slots) {
-            i = 0;
-            parity ^= 1;
-            here = at;
+    __device__ bool wait(uint32_t slot, uint32_t phase) {
+        if (mbar_try_wait(&full[slot], phase)) return true;
+        const uint64_t t0 = global_ns();
+        for (;;) {
+            for (int k = 0; k < 64; k++)
+                if (mbar_try_wait(&full[slot], phase)) return true;
+            if (failed() || global_ns() - t0 > kWaitLimitNs) return mbar_try_wait(&full[slot], phase);
         }
+    }
+    __device__ void drain(uint32_t slot, uint32_t phase) { mbar_wait(&full[slot], phase); }
+    __device__ bool lead() const { return threadIdx.x == 0; }
+    __device__ void fail() { *given_up = 1; }
+    __device__ bool failed() const { return *given_up != 0; }
+    __device__ void stop(unsigned long long row) {
+        if (given_up[1] < 0) given_up[1] = (int)((min(row, (unsigned long long)rows + gridDim.x - 1) - blockIdx.x) / gridDim.x);
+    }
+    __device__ void next(uint32_t t) {
+        ring_next(*this, t + (unsigned long long)slots * gridDim.x);
+        here = i ? here + N * room : at;
     }
     // the n columns at c (the others are 0) of array j's row t; WHOLE: rows start and end on 16 bytes
     template <typename T, bool WHOLE>
@@ -371,6 +388,32 @@ __device__ __forceinline__ void norm_out(const NormArgs<T>& a, uint32_t smem, lo
 // 1 / sqrt(mean + eps), within 2 ulp
 __device__ __forceinline__ float norm_factor(float total, float per_d, float eps) { return rsqrtf(fmaf(total, per_d, eps)); }
 
+// Where a wait gave up: the copies land, and all that this CTA has written becomes NaN (out of line: it costs the
+// others no registers)
+struct RingEnd {
+    uint64_t* full;
+    uint32_t slots;
+    __device__ void drain(uint32_t slot, uint32_t phase) { mbar_wait(&full[slot], phase); }
+};
+__device__ __forceinline__ void leave_ring(uint64_t* full, int slots, int issued) {
+    RingEnd ring{full, (uint32_t)slots};
+    if (threadIdx.x == 0) ring_drain(ring, (uint32_t)issued);
+    __syncthreads();   // all of it is written
+}
+template <typename T, int OUT>
+__device__ __noinline__ void spoil(const NormArgs<T>& a, uint64_t* full, int issued) {
+    leave_ring(full, a.slots, issued);
+    const float nan = __uint_as_float(0x7fffffffu);
+    for (long long t = blockIdx.x; t < a.rows; t += gridDim.x) {
+        for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+            if (a.sum) a.sum[t * a.ld_sum + c] = from_f32<T>(nan);
+            if (a.y) a.y[t * a.ld_y + c] = from_f32<T>(nan);
+            if (OUT == kNorm8 && c % kFp8Block == 0) static_cast<float*>(a.scales)[t * a.ld_s + c / kFp8Block] = nan;
+            if (OUT == kNorm4 && c % kFp4Block == 0) static_cast<uint8_t*>(a.scales)[t * a.ld_s + c / kFp4Block] = 255;
+        }
+    }
+}
+
 // A row of 8 V neighbouring columns a thread (0: of any length, read twice).  sum
 // may be x or add, y any of them: a thread has read a column before it writes it,
 // and a row is copied ahead of others only.  WHOLE: all rows start and end on 16
@@ -385,15 +428,17 @@ __global__ void __launch_bounds__(kNormThreads)
 rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
     extern __shared__ __align__(16) char ring_mem[];
     __shared__ uint64_t full[kNormSlots];
+    __shared__ int given_up[2];
     __shared__ float scratch[2][1][32];   // two rows' turns
     const uint32_t smem = smem_u32(ring_mem);
     if constexpr (V > 0) {
         const int c = 8 * V * threadIdx.x;
         RowRing<2> ring{{reinterpret_cast<const char*>(a.x), reinterpret_cast<const char*>(a.add)},
-                        {a.ld_x * (long long)sizeof(T), a.ld_add * (long long)sizeof(T)}, smem, full, a.slots, a.d * (int)sizeof(T), a.room};
+                        {a.ld_x * (long long)sizeof(T), a.ld_add * (long long)sizeof(T)}, smem, full, given_up, (uint32_t)a.slots,
+                        (uint32_t)a.rows, a.d * (int)sizeof(T), a.room};
         if (a.slots) ring.init();
         pdl_start();
-        if (a.slots) ring.start(a.rows);
+        if (a.slots) ring.start();
         int turn = 0;
         Pairs8 w[V];
 #pragma unroll
@@ -401,7 +446,7 @@ rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
         for (uint32_t t = blockIdx.x; t < (uint32_t)a.rows; t += gridDim.x, turn ^= 1) {   // (unsigned, as in combine_rows_kernel)
             Raw8<T> raw[V], more[V];
             Pairs8 s[V];
-            if (a.slots) ring.wait();
+            if (a.slots) ring_wait(ring);
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const int at = c + 8 * i, n = columns_at(at, a.d);
@@ -420,7 +465,7 @@ rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
             }
             float total[1] = {joined(part)};
             cta_sum(total, scratch[turn]);   // (one barrier a row: the turns keep a row's sum from the next one's)
-            if (a.slots) ring.next(t, a.rows);
+            if (a.slots) ring.next(t);
             if (!WHOLE && a.sum_room) room_to(a.sum + t * a.ld_sum, smem + a.sum_room, a.d * (int)sizeof(T));
             norm_out<T, OUT, V, WHOLE>(a, smem, t, s, w, norm_factor(total[0], a.per_d, a.eps), c);
             if (!WHOLE && (a.sum_room | a.y_room | a.c_room)) {
@@ -431,6 +476,7 @@ rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
                 if (a.c_room) room_to(a.codes + t * a.ld_c, smem + a.c_room, a.d);
             }
         }
+        if (a.slots && ring.failed()) spoil<T, OUT>(a, full, given_up[1]);   // (what is said before the last row's barrier is seen by all)
     } else {
         pdl_start();
         const int step = 8 * blockDim.x, c0 = 8 * threadIdx.x;
@@ -475,6 +521,17 @@ struct NormGradArgs {
     bool wide, wide_dx, wide_w, wide_part;
 };
 
+// as the norm's
+template <typename T>
+__device__ __noinline__ void spoil(const NormGradArgs<T>& a, uint64_t* full, int issued) {
+    leave_ring(full, a.slots, issued);
+    const float nan = __uint_as_float(0x7fffffffu);
+    for (int c = threadIdx.x; c < a.d; c += blockDim.x) {
+        for (long long t = blockIdx.x; t < a.rows; t += gridDim.x) a.dx[t * a.ld_dx + c] = from_f32<T>(nan);
+        if (a.part) a.part[(size_t)blockIdx.x * a.d + c] = nan;
+    }
+}
+
 // A thread keeps its 8 V columns' weights and their sums over the rows in
 // registers, so the rows' products for dw are added up without atomics and in a
 // fixed order: first a CTA's rows, then the CTAs' parts (rms_norm_dw_kernel).
@@ -488,16 +545,17 @@ __global__ void __launch_bounds__(kNormThreads)
 rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
     extern __shared__ __align__(16) char ring_mem[];
     __shared__ uint64_t full[kNormSlots];
+    __shared__ int given_up[2];
     __shared__ float scratch[2][2][32];   // two rows' turns
     int turn = 0;
     if constexpr (V > 0) {
         const uint32_t smem = smem_u32(ring_mem);
         RowRing<3> ring{{reinterpret_cast<const char*>(a.x), reinterpret_cast<const char*>(a.dy), reinterpret_cast<const char*>(a.add)},
                         {a.ld_x * (long long)sizeof(T), a.ld_dy * (long long)sizeof(T), a.ld_add * (long long)sizeof(T)},
-                        smem, full, a.slots, a.d * (int)sizeof(T), a.room};
+                        smem, full, given_up, (uint32_t)a.slots, (uint32_t)a.rows, a.d * (int)sizeof(T), a.room};
         if (a.slots) ring.init();
         pdl_start();
-        if (a.slots) ring.start(a.rows);
+        if (a.slots) ring.start();
         const int c = 8 * V * threadIdx.x;
         Pairs8 w[V], dw[V];
 #pragma unroll
@@ -509,7 +567,7 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
         for (uint32_t t = blockIdx.x; t < (uint32_t)a.rows; t += gridDim.x, turn ^= 1) {   // (unsigned, as in combine_rows_kernel)
             Raw8<T> add[V];
             Pairs8 x[V], dy[V];
-            if (a.slots) ring.wait();
+            if (a.slots) ring_wait(ring);
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const int at = c + 8 * i, n = columns_at(at, a.d);
@@ -526,7 +584,7 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
             }
             float sums[2] = {joined(square), joined(product)};
             cta_sum(sums, scratch[turn]);
-            if (a.slots) ring.next(t, a.rows);
+            if (a.slots) ring.next(t);
             const float inv = norm_factor(sums[0], a.per_d, a.eps);
             const Pair f = both(inv), minus = both(-(sums[1] * a.per_d * inv));   // - mean(g n)
 #pragma unroll
@@ -557,6 +615,7 @@ rms_norm_grad_kernel(const __grid_constant__ NormGradArgs<T> a) {
             const int at = c + 8 * i, n = columns_at(at, a.d);
             if (a.part && n) store_raw8(a.part + (size_t)blockIdx.x * a.d + at, rounded8<float>(dw[i]), n, a.wide_part);
         }
+        if (a.slots && ring.failed()) spoil(a, full, given_up[1]);   // (as in rms_norm_kernel)
     } else {
         pdl_start();
         float* part = a.part ? a.part + (size_t)blockIdx.x * a.d : nullptr;
