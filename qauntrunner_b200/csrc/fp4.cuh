@@ -372,7 +372,7 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
         if (threadIdx.x == 0)
             for (int i = 0; i < early; i++) {   // copies land before the CTA exits
                 mbar_arrive(&full[i]);
-                mbar_wait(&full[i], 0u);
+                if (!mbar_wait(&full[i], 0u)) atomicOr(p.err, (int)ERR_TIMEOUT);
             }
         if (warp == 1) tmem_dealloc(tmem, kFp4TmemCols);
         return;
@@ -459,7 +459,10 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
     }
     __syncwarp();
     // ---------------- every warp: the sums into shared memory, [row of x][output], where the ring was
-    mbar_wait(done_bar, 0u);   // (of MMAs that were issued: it comes)
+    if (!mbar_wait(done_bar, 0u)) {   // (of MMAs that were issued: it comes; if not, this CTA writes nothing)
+        *abort_flag = 1;
+        atomicOr(p.err, (int)ERR_TIMEOUT);
+    }
     tc_fence_after();
     __syncthreads();           // no role still waits on the ring
     float* sums = reinterpret_cast<float*>(ring);
@@ -603,7 +606,7 @@ struct Fp4PairBars {
         asm volatile("mbarrier.complete_tx.relaxed.cluster.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&full[slot])), "r"(bytes[slot])
                      : "memory");
     }
-    __device__ void wait(uint32_t slot, uint32_t parity) { mbar_wait(&full[slot], parity); }
+    __device__ void wait(uint32_t slot, uint32_t parity) { (void)mbar_wait(&full[slot], parity); }   // (an error is raised already)
 };
 // whether it holds for all of `threads`, which meet here
 __device__ __forceinline__ bool all_of(int barrier, int threads, bool holds) {
@@ -935,7 +938,10 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
             // every MMA has completed before tensor memory is released
             if (elect_one()) {
                 asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(done_bar)) : "memory");
-                mbar_wait(done_bar, 0u);
+                if (!mbar_wait(done_bar, 0u)) {
+                    *abort_flag = 1;
+                    atomicOr(p.err, (int)ERR_TIMEOUT);
+                }
             }
             __syncwarp();
         } else if (warp >= 2) {
@@ -1079,7 +1085,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant
         if (warp == 1) {
             if (rank == 0 && elect_one()) umma_commit_pair(smem_u32(left_bar));
             __syncwarp();
-            if (lane == 0) mbar_wait(left_bar, 0u);
+            if (lane == 0) (void)mbar_wait(left_bar, 0u);
         }
         __syncwarp();
         cluster_sync_all();
