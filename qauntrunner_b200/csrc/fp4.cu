@@ -160,26 +160,30 @@ int create(int device, int groups, int64_t rows, int64_t cols, const void* codes
 }
 
 // Which kernel a product takes, by an estimate of what both would cost with all
-// T rows held and spread evenly over the groups.  Measured (us; weights / rows of
-// x on the MMA's M side), outputs x contracted:
-//   1 x 4096 x 7168:   1 row 7.4 / 13.8, 16 rows 8.4 / 13.5, 64 rows 12.7 / 13.9, 128 rows 14.4 / 14.5, 256 rows 14.8 / 14.5
-//   1 x 28672 x 4096:  1 row 13.6 / 22.9, 32 rows 17.2 / 20.4, 64 rows 20.6 / 20.4, 128 rows 27.8 / 21.7
-//   1 x 1024 x 2816:   1 row 5.7 / 8.1, 32 rows 7.9 / 8.4, 64 rows 10.2 / 8.8
-//   1 x 7168 x 2048:   16 rows 7.1 / 7.8, 32 rows 8.3 / 8.1, 64 rows 10.7 / 8.4
-//   8 x 5632 x 1024:   8 rows each 8.4 / 11.1, 16 rows each 9.9 / 11.4, 32 rows each 12.2 / 11.4
-//   32 x 4096 x 7168:  2 rows each 71 / 81, 16 rows each 87 / 94, 32 rows each 93 / 96, 64 rows each 112 / 98
-//   32 x 7168 x 2048:  4 rows each 49 / 49, 16 rows each 58 / 51, 64 rows each 82 / 55
-// The first takes what reading the weights takes, and something for each row of a
-// tile and all tiles' rows; the second a time for each stage of whole tiles of 256
-// rows x 256 outputs, in waves over the pairs of SMs, longer where most pairs are
-// at work.  The worst choice among 70 measured sizes takes 1.08 times as long as
-// the other kernel.
+// T rows held and spread evenly over the groups: a call that passes room for more
+// rows than its groups have is judged by the room, which the host knows, not by
+// the offsets.  Measured (us, graphs of ten calls in bursts, matrices that no cache
+// holds; weights / rows of x on the MMA's M side), outputs x contracted:
+//   1 x 4096 x 7168:   1 row 8.4 / 15.4, 16 rows 9.7 / 15.2, 64 rows 13.1 / 15.8, 128 rows 14.7 / 16.2, 256 rows 15.4 / 16.6
+//   1 x 28672 x 4096:  1 row 12.9 / 26.4, 32 rows 16.4 / 20.7, 64 rows 19.9 / 20.7, 128 rows 27.6 / 21.7
+//   1 x 1024 x 2816:   1 row 5.5 / 8.3, 32 rows 7.7 / 8.8, 64 rows 10.0 / 9.2
+//   1 x 7168 x 2048:   16 rows 6.8 / 8.8, 32 rows 8.0 / 9.0, 64 rows 10.4 / 9.0
+//   8 x 5632 x 1024:   8 rows each 10.6 / 12.5, 16 rows each 12.3 / 13.1, 32 rows each 14.9 / 13.7
+//   32 x 4096 x 7168:  2 rows each 73 / 90, 16 rows each 87 / 100, 32 rows each 101 / 102, 64 rows each 112 / 105
+//   32 x 7168 x 2048:  4 rows each 48 / 53, 16 rows each 59 / 57, 64 rows each 79 / 60
+// (Grouped, under sustained load: 32 x 4096 x 7168 75 / 105, 89 / 117, 104 / 120,
+// 119 / 123; 32 x 7168 x 2048 48 / 63, 59 / 68, 79 / 72.)  The first takes what
+// reading the weights takes, and something for each row of a tile and all tiles'
+// rows; the second a time for each stage of whole tiles of 256 rows x 256 outputs,
+// in waves over the pairs of SMs, longer where most pairs are at work.  The worst
+// choice among these sizes takes 1.08 times as long as the other kernel in bursts
+// and 1.09 times under load (256 rows through 4096 x 7168, both).
 bool pair_is_faster(int64_t T, int64_t used, int64_t tiles_across, int steps, int tile_rows, int sms) {
     const double rows = (double)T / used, row_tiles = std::ceil(rows / tile_rows), tiles = used * tiles_across * row_tiles;
     const double read = (double)used * tiles_across * steps * 34816 / 6.4e6;   // us, of a stage's 256 x 256 codes and scales
     const double one = 4 + read * (1 + (row_tiles - 1) / 2) + std::min<double>(rows, tile_rows) * (0.07 + 0.0004 * tiles);
     const double pairs = sms / 2, wide = used * tiles_across * std::ceil(rows / 256);
-    const double two = 5 + std::ceil(wide / pairs) * steps * (wide <= pairs / 2 ? 0.28 : 0.43);
+    const double two = 5.5 + std::ceil(wide / pairs) * steps * (wide <= pairs / 2 ? 0.3 : 0.45);
     return two < one;
 }
 
@@ -188,9 +192,11 @@ cudaError_t launch(const qrm_fp4* m, const CUtensorMap& x_map, const CUtensorMap
     const CUtensorMap& w_map = MODE == kFp4Plain ? m->map : m->gated_map;
     if (pair) {
         // Tails (a sixth more shared memory a stage, smaller pieces on the way out) where groups are likely to have one and a
-        // tile has stages enough.  With and without, us: 32 x 4096 x 7168, 8192 rows 120 / 145, 9000 rows 137 / 180, 12000 rows
-        // 187 / 183; 32 x 7168 x 2048, 8192 rows 72 / 83; 64 x 4096 x 2048, 20000 rows 114 / 128; 20 x 3584 x 2816, 7000 rows 52 / 48;
-        // 8 x 5632 x 2048, 2560 rows 27 / 25; 8 x 5632 x 1024, 512 rows 13.7 / 11.7.
+        // tile has stages enough.  With and without, us in bursts, the mean of three draws of uneven groups: 32 x 4096 x 7168,
+        // 8192 rows 142 / 148, 9000 rows 149 / 164, 12000 rows 188 / 202; 32 x 7168 x 2048, 8192 rows 85 / 87; 64 x 4096 x 2048,
+        // 20000 rows 113 / 120; 20 x 3584 x 2816, 7000 rows 50.1 / 50.0; 8 x 5632 x 2048, 2560 rows 26.1 / 25.7; where the rule
+        // takes none, 8 x 5632 x 1024, 512 rows 15.2 / 13.8, 20 x f 1536 x 6144 gated, 2559 rows 54.9 / 52.9.  A single draw may go the other way, since what counts is whether the tiles saved are a wave over the pairs: the worst one seen
+        // took 1.08 times as long with tails (7000 rows over 20 x 3584 x 2816).
         const bool tails = m->groups > 1 && T > (int64_t)128 * m->groups && p.steps >= 8;
         const int stages = tails ? tail_stages(m->groups) : kFp4PairStages;
         return launch_ahead(tails ? fp4_pair_kernel<MODE, true> : fp4_pair_kernel<MODE, false>, dim3(m->sms / 2 * 2), kFp4PairThreads,
