@@ -421,7 +421,8 @@ int qrm_gather_rows_fp4(int type, const void* x_dev, int64_t ld_x, const int32_t
  * qrm_fp4_product: y[t] = W_g x[t] for the rows t in [offsets[g], offsets[g+1])
  * of each group g (offsets NULL: one group, all T rows), x [T][cols] in 4 bits
  * and y [T][rows], T below 2^31 - 1023; rows outside every group are not
- * written.
+ * written.  T is the room: which of two kernels runs goes by it, not by how many
+ * rows the groups have.
  * qrm_fp4_swiglu: the matrix holds gate's f rows, then up's (rows = 2 f);
  * h[t] = silu(W_gate x[t]) (W_up x[t]) [T][f], in one kernel; limit > 0: gate is
  * cut off above it and up to [-limit, limit] first.  _fp4 writes h in 4-bit

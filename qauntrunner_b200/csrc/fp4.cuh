@@ -535,9 +535,8 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // features): each CTA loads 128 rows of x and 128 of the weights, 32 KB of codes
 // for 256 contracted values, and the MMA reads both halves of the weights.
 //
-// 4096 rows, 28672 x 4096: 176 us, 5.5 PFLOP/s, and 207 under sustained load: the
-// power cap bounds it (a launch by itself takes 415 cycles a stage).  What took it
-// there from 310 us: the scales of x handed over without a cluster-scope release
+// 4096 rows, 28672 x 4096: 186 us in bursts, 5.2 PFLOP/s, and 217 under sustained
+// load: the power cap bounds it.  What took it from 310 us to 176 in bursts: the scales of x handed over without a cluster-scope release
 // (a full memory barrier with every stage) and asked for four stages at a time,
 // rows out by way of shared memory, descriptors with constant high words.
 //
@@ -547,14 +546,17 @@ fp4_split_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constan
 // stage's scales, so what completes on the first CTA's barrier, the copies' bytes
 // (a release of cluster scope), comes behind them.  An arrive of those warps on
 // that barrier would need such a release of its own: 396 us in place of 217 under
-// sustained load, 370 with a warp that does nothing else.
+// sustained load, 370 with a warp that does nothing else.  The copies wait some
+// hundred cycles for it, which a tile by itself shows: 256 rows through 4096 x 7168
+// take 16.4 us.
 //
 // Groups of uneven numbers of rows leave most of their last tile empty.  So up to
 // 64 rows behind a group's last whole tile, its tail, go with that tile: each stage
 // brings half of them to each CTA, and a second MMA takes them against the weights
 // that are there already, with the operands' places changed (weights on the M
 // side, the tail's rows, rounded up to 32, on the N side).  8192 rows over 32 x 4096
-// x 7168: 145 -> 120 us (floor 91).  Tiles of their own in that form gained
+// x 7168, one draw of groups in bursts: 145 -> 120 us (floor 91; 148 -> 142 over
+// three draws).  Tiles of their own in that form gained
 // nothing (their weights come from L2 once more), nor did a kernel with all rows on
 // the N side, 384 a tile (137 us there, but 217 in place of 176 for one matrix).
 //

@@ -104,8 +104,9 @@ int norm(const char* what, int out, int type, const void* x, int64_t ld_x, const
 // twice), its CTAs, and so many parts of dw: about 700 threads an SM.  With 512
 // (or 1024) and 16 columns a thread from 1024 on, 4096 x 2816 bf16 takes 29 (21)
 // us in place of 21, 4096 x 7168 48 (52) in place of 48, 1021 x 2816 f32 17 (11)
-// in place of 11.  (148 SMs, a number of its own, so that the room for the parts
-// needs no device.)
+// in place of 11.  Other widths were not measured; from 2817 to 4096 columns a CTA
+// has 384 to 512 threads, and an SM one of them.  (148 SMs, a number of its own, so
+// that the room for the parts needs no device.)
 int grad_chunks(int64_t d) { return chunks_of(d) <= 512 ? 1 : chunks_of(d) <= 2 * kNormThreads ? 2 : 0; }
 int grad_threads(int64_t d) { return grad_chunks(d) ? whole_warps((chunks_of(d) + grad_chunks(d) - 1) / grad_chunks(d)) : kNormThreads; }
 int grad_ctas_an_sm(int64_t d) { return std::max(1, std::min(4, 704 / grad_threads(d))); }

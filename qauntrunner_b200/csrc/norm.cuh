@@ -419,10 +419,10 @@ __device__ __noinline__ void spoil(const NormArgs<T>& a, uint64_t* full, int iss
 // and a row is copied ahead of others only.  WHOLE: all rows start and end on 16
 // bytes (the code for others costs these a tenth of their time).
 //
-// 4096 x 7168 bf16 with the residual, the sum written, into 8 bits (206 MB): 39 us,
+// 4096 x 7168 bf16 with the residual, the sum written, into 8 bits (206 MB): 38 us,
 // 5.3 TB/s (a copy of as many bytes 35), 62 with loads of its own in place of the
 // ring, one f32 at a time and 8 columns a thread.  One row of 7168 f32 columns 4.3.
-// 4000 x 7001, whose rows start anywhere: 59, and 251 with loads of single values.
+// 4000 x 7001, whose rows start anywhere: 58, and 251 with loads of single values.
 template <typename T, int OUT, int V, bool WHOLE>
 __global__ void __launch_bounds__(kNormThreads)
 rms_norm_kernel(const __grid_constant__ NormArgs<T> a) {
@@ -536,9 +536,9 @@ __device__ __noinline__ void spoil(const NormGradArgs<T>& a, uint64_t* full, int
 // registers, so the rows' products for dw are added up without atomics and in a
 // fixed order: first a CTA's rows, then the CTAs' parts (rms_norm_dw_kernel).
 //
-// 4096 x 7168 bf16 with the residual's gradient and dw (235 MB): 48 us, 4.9 TB/s (a
-// copy of as many bytes 40), 4 of them for dw.  4000 x 7001: 75, of single values
-// 265.  1021 x 2816 f32: 11.  Two rows between two barriers and two CTAs an SM were
+// 4096 x 7168 bf16 with the residual's gradient and dw (235 MB): 49 us, 4.8 TB/s (a
+// copy of as many bytes 40), 4 of them for dw.  4000 x 7001: 76, of single values
+// 265.  1021 x 2816 f32: 11.5.  Two rows between two barriers and two CTAs an SM were
 // no faster.
 template <typename T, int V, bool WHOLE>
 __global__ void __launch_bounds__(kNormThreads)
